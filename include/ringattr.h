@@ -45,6 +45,15 @@ extern "C" {
 #define RINGATTR_ERR_WORKSPACE 2 /* workspace pointer null or too small */
 #define RINGATTR_ERR_HIP 3       /* a HIP runtime call or kernel launch failed */
 
+/* Types of what the sequence operators read and write. */
+#define RINGATTR_F32 0
+#define RINGATTR_BF16 1
+#define RINGATTR_F16 2
+/* Types of positions. */
+#define RINGATTR_POS_I64 0
+#define RINGATTR_POS_I32 1
+#define RINGATTR_POS_F32 2
+
 /* Library version (major*1000 + minor). */
 RINGATTR_API int ringattr_version(void);
 
@@ -270,6 +279,56 @@ RINGATTR_API int ringattr_clip_adam(int n_tensors, void* const* params, void* co
 RINGATTR_API int ringattr_clip_adam_counted(int n_tensors, void* const* params, void* const* grads, void* const* exp_avg,
                       void* const* exp_avg_sq, const size_t* numel, float lr, float beta1, float beta2, float eps,
                       float max_norm, void* step_counter, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Sequence operators beside the time loop; no counterpart in the reference.  `type` is RINGATTR_F32, _BF16 or _F16 and
+ * holds for every tensor that is not said to be fp32.  A tensor [B,T,heads,D] is given by its address and its strides (batch, token, head,
+ * in elements; a head's D values are neighbours), outputs are contiguous.
+ *
+ * Linear attention with a decay for each head, lambda_h = exp(log_decay[h]) (log_decay fp32 [heads]):
+ *   S_t = lambda_h S_(t-1) + k_t v_t^T,   o_t = scale * q_t S_t
+ * q [B,T,heads,dk], k [B,T,kv_heads,dk], v [B,T,kv_heads,dv] (head h uses head h / (heads / kv_heads) of k and v), dk and dv up to
+ * 256; states fp32 [B,heads,dk,dv].  initial_state NULL: zeros; final_state NULL: not wanted.  lengths (device int32 [B], NULL:
+ * seq_len) says how many tokens of each sequence count: outputs and gradients behind them are zero, nothing there is read, the
+ * final state is the one behind the last token that counts.  Values that are infinite or NaN do not reach rows that do not see
+ * them.  strides: host array, three for each of q, k, v (and grad_o), in that order. */
+#define RINGATTR_ATTENTION_MAX_DIM 256
+RINGATTR_API size_t ringattr_linear_attention_fwd_workspace_bytes(int type, int batch_size, int seq_len, int heads, int kv_heads,
+                      int dk, int dv);
+RINGATTR_API int ringattr_linear_attention_fwd(const void* q, const void* k, const void* v, const long long* strides,
+                      const void* log_decay, const void* initial_state, const void* lengths, void* o, void* final_state,
+                      float scale, int type, int batch_size, int seq_len, int heads, int kv_heads, int dk, int dv,
+                      void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients of q, k, v and (NULL: not wanted) of the initial state, from those of o and (NULL: zero) of the final state.
+ * The gradients of shared heads are summed in fp32 in a fixed order. */
+RINGATTR_API size_t ringattr_linear_attention_bwd_workspace_bytes(int type, int batch_size, int seq_len, int heads, int kv_heads,
+                      int dk, int dv);
+RINGATTR_API int ringattr_linear_attention_bwd(const void* q, const void* k, const void* v, const void* grad_o,
+                      const long long* strides, const void* log_decay, const void* initial_state, const void* lengths,
+                      const void* grad_final_state, void* grad_q, void* grad_k, void* grad_v, void* grad_initial_state,
+                      float scale, int type, int batch_size, int seq_len, int heads, int kv_heads, int dk, int dv,
+                      void* workspace, size_t workspace_bytes, void* stream);
+/* One token for each sequence: q [B,heads,dk], k [B,kv_heads,dk], v [B,kv_heads,dv] (strides: batch, head of each), the state
+ * [B,heads,dk,dv] updated in place, o [B,heads,dv].  active (device bytes [B], NULL: all): where it is zero the state is left as it
+ * is and o is zero. */
+RINGATTR_API int ringattr_linear_attention_step(const void* q, const void* k, const void* v, const long long* strides,
+                      const void* log_decay, void* state, const void* active, void* o, float scale, int type, int batch_size,
+                      int heads, int kv_heads, int dk, int dv, void* stream);
+
+/* Rotary positions of one tensor or two that share them (x1 NULL, heads1 0: one): pair m of the first rot values of a head,
+ * (m, m + rot / 2) or, interleaved, (2m, 2m + 1), is turned by position * frequencies[m] (fp64 [rot / 2]) and multiplied by scale;
+ * the other values are copied.  inverse: turned back (the gradient).  positions: device array of position_type (RINGATTR_POS_*), the
+ * one of (b, t) at b * pos_stride_b + t * pos_stride_t.  strides: host array, three for each tensor.  Outputs contiguous, not the
+ * inputs' own memory. */
+RINGATTR_API int ringattr_rotary(const void* x0, const void* x1, const long long* strides, const void* positions,
+                      long long pos_stride_b, long long pos_stride_t, int position_type, const void* frequencies, void* y0, void* y1,
+                      float scale, int interleaved, int inverse, int type, int batch_size, int seq_len, int heads0, int heads1,
+                      int dim, int rot, void* stream);
+
+/* y = residual + dropout(x) over n values (residual NULL: none).  Value i is kept, and multiplied by `scale`, where word i % 4 of block
+ * i / 4 of Philox (four words, seven rounds; counter: block, offset; key: seed) is at least `threshold`.  offset_ptr (device
+ * int64, or NULL) is added to offset: a recorded graph counts on by it.  y may be x or residual. */
+RINGATTR_API int ringattr_dropout(const void* x, const void* residual, void* y, size_t n, unsigned int threshold, float scale,
+                      unsigned long long seed, unsigned long long offset, const void* offset_ptr, int type, void* stream);
 
 /* Per-kernel timing for benchmarks; no counterpart in the reference.  ringattr_profile_enable(n): n = 0 switches it
  * off; n >= 1 brackets every n-th launch of each kernel (counted per kernel from this call on) by two HIP events

@@ -8,6 +8,10 @@ _EXPORTS = {
     "ring_rnn_loss_func": "loss_head", "RingRnnLossFunc": "loss_head",
     "generate_inputs": "device_aux", "FusedClipAdam": "device_aux",
     "ring_gain_func": "gain", "RingGainFunc": "gain", "pack_gain_nets": "gain",
+    "linear_attention_func": "linear_attention", "LinearAttentionFunc": "linear_attention",
+    "linear_attention_step": "linear_attention",
+    "rotary_func": "rotary", "RotaryFunc": "rotary", "rotary_frequencies": "rotary",
+    "dropout_func": "dropout", "DropoutFunc": "dropout",
 }
 
 

@@ -75,6 +75,18 @@ PROTOTYPES = {
                                            ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p), ctypes.POINTER(c_size_t),
                                            c_float, c_float, c_float, c_float, c_float, c_void_p, c_void_p, c_size_t,
                                            c_void_p]),
+    "ringattr_linear_attention_fwd_workspace_bytes": (c_size_t, [c_int] * 7),
+    "ringattr_linear_attention_fwd": (c_int, [c_void_p] * 3 + [ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 5 + [c_float] +
+                                      [c_int] * 7 + [c_void_p, c_size_t, c_void_p]),
+    "ringattr_linear_attention_bwd_workspace_bytes": (c_size_t, [c_int] * 7),
+    "ringattr_linear_attention_bwd": (c_int, [c_void_p] * 4 + [ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 8 + [c_float] +
+                                      [c_int] * 7 + [c_void_p, c_size_t, c_void_p]),
+    "ringattr_linear_attention_step": (c_int, [c_void_p] * 3 + [ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 4 + [c_float] +
+                                       [c_int] * 6 + [c_void_p]),
+    "ringattr_rotary": (c_int, [c_void_p] * 2 + [ctypes.POINTER(ctypes.c_longlong), c_void_p, ctypes.c_longlong, ctypes.c_longlong, c_int] +
+                        [c_void_p] * 3 + [c_float] + [c_int] * 9 + [c_void_p]),
+    "ringattr_dropout": (c_int, [c_void_p] * 3 + [c_size_t, ctypes.c_uint, c_float, ctypes.c_ulonglong, ctypes.c_ulonglong, c_void_p, c_int,
+                                 c_void_p]),
     "ringattr_profile_enable": (c_int, [c_int]),
     "ringattr_profile_read": (c_int, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_longlong)]),
     "ringattr_last_kernel_name": (c_int, [c_int, ctypes.c_char_p, ctypes.c_size_t]),
@@ -152,6 +164,24 @@ def profile_read():
     cnt = (ctypes.c_longlong * n)()
     check(load().ringattr_profile_read(ms, cnt))
     return {KERNEL_NAMES[i]: (ms[i], cnt[i]) for i in range(n)}
+
+
+SEQUENCE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # RINGATTR_F32, _BF16, _F16
+
+
+def check_sequence_tensor(name, t, shape=None, dtype=None, device=None) -> None:
+    """What the sequence operators ask of a tensor: one of their types (or the one given), on the GPU, and the shape."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if dtype is None:
+        if t.dtype not in SEQUENCE_TYPES:
+            raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    elif t.dtype != dtype:
+        raise TypeError(f"{name} must be {str(dtype)[6:]}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise RuntimeError(f"{name} must be on {device if device is not None else 'a GPU'} (got {t.device}); there is no CPU path")
 
 
 class _Here:

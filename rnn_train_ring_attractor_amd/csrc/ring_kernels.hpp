@@ -326,3 +326,71 @@ hipError_t ring_run_team_rows(const RingFwdArgs& a, const float* Wo, const float
 hipError_t ring_run_team_rows_bptt(const RingBpttArgs& a, const float* Wo, const float* Wa, void* ws, hipStream_t st);
 hipError_t ring_run_team_rebuild(const RingFwdArgs& a, bool folded, int cts, hipStream_t st);
 hipError_t ring_run_team_bptt(const RingBpttArgs& a, const float* Wo, const float* Wa, bool folded, int cts, void* ws, hipStream_t st);
+
+// Linear attention with a decay for each head (ring_linattn*.hip).  Types of what is in memory: RINGATTR_F32, _BF16, _F16.
+struct RingLinTensor {
+  const void* p;
+  long sb, st, sh;       // strides in elements: sequence, token, head; a head's values are neighbours
+  bool vec;              // every row starts at 16 bytes and is a whole number of them long
+};
+// One pass of the chunk kernel: rows X against rows Y (Da wide) weigh rows Z (Db wide); see ring_linattn.hpp
+struct RingLinArgs {
+  RingLinTensor X, Y, Z;
+  int xs, ys, zs;        // heads that share one of the tensor's
+  void* out;             // [B,T,H,Db] in the type of the rows, or in fp32 (out_f32)
+  bool out_vec, out_f32;
+  const float* log_decay;
+  const float* s_in;     // states [B,H,..]: element (a, b) at a * sa + b * sb; null: zeros
+  float* s_out;          // null: not wanted
+  long sa, sb;
+  float* seg;            // nseg > 1: [B,H,nseg,..] the states in front of the segments (written by the pass over states only)
+  const int* lengths;    // tokens of each sequence, null: T
+  float intra, inter, update;    // factors of the weights, of what the state gives, of what it takes in
+  int B, T, H, Da, Db, nseg, seg_tokens, slices;
+};
+struct RingLinShape { int B, T, H, G, Dk, Dv, type; float scale; };
+struct RingLinStep {
+  RingLinTensor q, k, v; // (st unused)
+  const float* log_decay;
+  float* state;
+  const unsigned char* active;
+  void* out;
+};
+int ring_linattn_segments(const RingLinShape& s);
+size_t ring_linattn_fwd_bytes(const RingLinShape& s);
+size_t ring_linattn_bwd_bytes(const RingLinShape& s);
+hipError_t ring_linattn_fwd(const RingLinShape& s, const RingLinTensor& q, const RingLinTensor& k, const RingLinTensor& v,
+                            const float* log_decay, const float* s_in, const int* lengths, void* o, float* s_out, void* ws, hipStream_t st);
+hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const RingLinTensor& k, const RingLinTensor& v,
+                            const float* log_decay, const float* s_in, const int* lengths, const RingLinTensor& go, const float* gs,
+                            void* gq, void* gk, void* gv, float* gs_in, void* ws, hipStream_t st);
+hipError_t ring_linattn_step(const RingLinShape& s, const RingLinStep& a, hipStream_t st);
+hipError_t ring_launch_linattn_f32(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st);
+hipError_t ring_launch_linattn_bf16(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st);
+hipError_t ring_launch_linattn_f16(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st);
+
+// Rotary positions (ring_rotary.hip) of one tensor or two ([B,T,heads,D], heads[1] = 0: one)
+struct RingRotaryArgs {
+  RingLinTensor in[2];
+  void* out[2];          // contiguous
+  int heads[2];
+  const void* positions; // element (b, t) at b * pos_b + t * pos_t
+  const double* frequencies;     // [rot / 2], radians per position
+  long pos_b, pos_t;
+  int position_type, B, T, D, rot, interleaved, inverse;
+  float scale;
+  int tokens, heads_per; // (the launcher's)
+};
+hipError_t ring_launch_rotary(const RingRotaryArgs& p, int type, hipStream_t st);
+
+// Dropout (ring_dropout.hip)
+struct RingDropoutArgs {
+  const void *x, *residual;      // residual: null if there is none
+  void* y;
+  size_t n;
+  unsigned long long seed, offset;
+  const long long* offset_ptr;   // device int64 added to the offset, or null
+  unsigned threshold;
+  float scale;
+};
+hipError_t ring_launch_dropout(const RingDropoutArgs& p, int type, hipStream_t st);

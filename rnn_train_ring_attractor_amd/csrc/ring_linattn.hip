@@ -1,0 +1,291 @@
+// Linear attention with a decay for each head: the passes of a forward and of a backward, and the single token.
+#include "ring_linattn.hpp"
+#include "ringattr.h"
+
+using namespace ring_lin;
+
+namespace {
+
+constexpr int kChunk = 32;
+
+size_t round_up(size_t x) { return (x + 255) / 256 * 256; }
+
+hipError_t launch_pass(int type, const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
+  if (type == RINGATTR_F32) return ring_launch_linattn_f32(a, rev, state_only, st);
+  if (type == RINGATTR_BF16) return ring_launch_linattn_bf16(a, rev, state_only, st);
+  return ring_launch_linattn_f16(a, rev, state_only, st);
+}
+
+int slices(int Db) { return Db <= 64 ? 1 : (Db + 127) / 128; }
+
+RingLinArgs base(const RingLinShape& s, const float* log_decay, const int* lengths, int nseg) {
+  RingLinArgs a = {};
+  a.log_decay = log_decay;
+  a.lengths = lengths;
+  a.B = s.B;
+  a.T = s.T;
+  a.H = s.H;
+  a.nseg = nseg;
+  const int chunks = (s.T + kChunk - 1) / kChunk;
+  a.seg_tokens = nseg > 1 ? (chunks + nseg - 1) / nseg * kChunk : (s.T > 0 ? s.T : 1);
+  a.intra = a.inter = a.update = 1.f;
+  return a;
+}
+
+}  // namespace
+
+// The states in front of the segments: seg[i] is what segment i adds to a state of zeros and becomes the state in front of it
+// (REV: behind it).  A thread walks one element through the segments.
+__global__ __launch_bounds__(256) void ring_linattn_scan_kernel(RingLinArgs p, bool rev) {
+  const int D = p.Da * p.Db;
+  const int per = (D + 255) / 256, e = (int)(blockIdx.x % per) * 256 + threadIdx.x;
+  const size_t bh = blockIdx.x / per;
+  if (e >= D) return;
+  const int b = (int)(bh / p.H), h = (int)(bh % p.H);
+  const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const float g2 = (float)((double)p.log_decay[h] * 1.4426950408889634);
+  float* seg = p.seg + bh * p.nseg * D + e;
+  float run = p.s_in ? p.s_in[bh * D + e] : 0.f;
+#pragma unroll 8
+  for (int i = 0; i < p.nseg; ++i) {
+    const int s = rev ? p.nseg - 1 - i : i;
+    const int n = min(max(len - s * p.seg_tokens, 0), min(p.seg_tokens, p.T - s * p.seg_tokens));
+    const float local = seg[(size_t)s * D];
+    seg[(size_t)s * D] = run;
+    if (n > 0) run = fmaf(power(g2, n), run, local);
+  }
+  if (p.s_out) p.s_out[bh * D + e] = run;
+}
+
+// out[row][g][d] = sum over the heads that share g
+template <typename T>
+__global__ __launch_bounds__(256) void ring_linattn_share_kernel(const float* __restrict__ in, T* __restrict__ out, int share, int D, size_t n) {
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+    const size_t row = i / D, d = i - row * D;                 // (row, shared head)
+    const float* p = in + row * share * D + d;
+    float sum = 0.f;
+    for (int s = 0; s < share; ++s) sum += p[(size_t)s * D];
+    out[i] = (T)sum;
+  }
+}
+
+static hipError_t launch_share(int type, const float* in, void* out, int share, int D, size_t n, hipStream_t st) {
+  const size_t blocks = (n + 255) / 256;
+  const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192)), block(256);
+  if (type == RINGATTR_F32) hipLaunchKernelGGL(ring_linattn_share_kernel<float>, grid, block, 0, st, in, (float*)out, share, D, n);
+  else if (type == RINGATTR_BF16) hipLaunchKernelGGL(ring_linattn_share_kernel<__bf16>, grid, block, 0, st, in, (__bf16*)out, share, D, n);
+  else hipLaunchKernelGGL(ring_linattn_share_kernel<_Float16>, grid, block, 0, st, in, (_Float16*)out, share, D, n);
+  return hipGetLastError();
+}
+
+// A single token: S = lambda S + k v^T in place, o = scale q S.  A workgroup takes `tc` lanes of V columns each of one state; its other
+// lanes share the rows.  Nothing but the state moves: read once, written once.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void ring_linattn_step_kernel(RingLinStep p, RingLinShape s, int tc) {
+  typedef float vec __attribute__((ext_vector_type(V)));
+  __shared__ vec part[256];
+  const int tid = threadIdx.x, lane = tid & (tc - 1), tr = tid / tc, nr = 256 / tc;
+  const int ns = (s.Dv + tc * V - 1) / (tc * V);
+  const int slice = blockIdx.x % ns;
+  const size_t bh = blockIdx.x / ns;
+  const int h = (int)(bh % s.H), b = (int)(bh / s.H), share = s.H / s.G;
+  const int c = (slice * tc + lane) * V;
+  T* out = (T*)p.out + bh * s.Dv + c;
+  if (p.active && !p.active[b]) {
+    if (tr == 0 && c < s.Dv)
+#pragma unroll
+      for (int e = 0; e < V; ++e) out[e] = (T)0.f;
+    return;
+  }
+  const T* q = rows_of<T>(p.q, b, h, 1);
+  const T* k = rows_of<T>(p.k, b, h, share);
+  const T* v = rows_of<T>(p.v, b, h, share);
+  const float lam = power((float)((double)p.log_decay[h] * 1.4426950408889634), 1);
+  vec o, x;
+#pragma unroll
+  for (int e = 0; e < V; ++e) o[e] = x[e] = 0.f;
+  if (c < s.Dv) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = (float)v[c + e];
+    float* S = p.state + bh * s.Dk * s.Dv + c;
+#pragma unroll 8
+    for (int a = tr; a < s.Dk; a += nr) {
+      vec* at = reinterpret_cast<vec*>(S + (size_t)a * s.Dv);
+      const float ka = (float)k[a], qa = (float)q[a];
+      vec y = *at;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        y[e] = fmaf(ka, x[e], lam * y[e]);
+        o[e] = fmaf(qa, y[e], o[e]);
+      }
+      *at = y;
+    }
+  }
+  part[tid] = o;
+  __syncthreads();
+  for (int half = nr / 2; half > 0; half /= 2) {
+    if (tr < half) part[tid] += part[tid + half * tc];
+    __syncthreads();
+  }
+  if (tr == 0 && c < s.Dv)
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = (T)(s.scale * part[tid][e]);
+}
+
+template <typename T> static hipError_t launch_step(const RingLinShape& s, const RingLinStep& a, hipStream_t st) {
+  const bool vec = s.Dv % 4 == 0 && (reinterpret_cast<uintptr_t>(a.state) & 15) == 0;
+  const int width = vec ? (s.Dv + 3) / 4 : s.Dv;               // lanes that a row of the state takes
+  const long heads = (long)s.B * s.H;
+  int tc = 8;
+  while (tc < width && tc < 64 && heads * ((width + tc - 1) / tc) > 1024) tc *= 2;
+  const dim3 grid((unsigned)(heads * ((width + tc - 1) / tc))), block(256);
+  if (vec) hipLaunchKernelGGL((ring_linattn_step_kernel<T, 4>), grid, block, 0, st, a, s, tc);
+  else hipLaunchKernelGGL((ring_linattn_step_kernel<T, 1>), grid, block, 0, st, a, s, tc);
+  return hipGetLastError();
+}
+
+hipError_t ring_linattn_step(const RingLinShape& s, const RingLinStep& a, hipStream_t st) {
+  if (s.type == RINGATTR_F32) return launch_step<float>(s, a, st);
+  if (s.type == RINGATTR_BF16) return launch_step<__bf16>(s, a, st);
+  return launch_step<_Float16>(s, a, st);
+}
+
+// Into how many segments the tokens are cut so that there is work for all compute units
+int ring_linattn_segments(const RingLinShape& s) {
+  const long groups = (long)s.B * s.H * slices(s.Dv);
+  const int chunks = (s.T + kChunk - 1) / kChunk;
+  long n = groups > 0 ? 512 / groups : 1;
+  if (n > chunks / 8) n = chunks / 8;
+  if (n <= 1) return 1;
+  const int per = (int)((chunks + n - 1) / n);
+  return (chunks + per - 1) / per;
+}
+
+static size_t states_bytes(const RingLinShape& s, int nseg) {
+  return nseg > 1 ? round_up((size_t)s.B * s.H * nseg * s.Dk * s.Dv * sizeof(float)) : 0;
+}
+
+size_t ring_linattn_fwd_bytes(const RingLinShape& s) { return states_bytes(s, ring_linattn_segments(s)); }
+
+size_t ring_linattn_bwd_bytes(const RingLinShape& s) {
+  size_t n = 2 * states_bytes(s, ring_linattn_segments(s));
+  if (s.G != s.H) n += round_up((size_t)s.B * s.T * s.H * s.Dk * sizeof(float)) + round_up((size_t)s.B * s.T * s.H * s.Dv * sizeof(float));
+  return n;
+}
+
+// The states in front of the segments of Y and Z (rows of natural states, [Dk][Dv]) into `seg`, the one behind them all into s_out.
+static hipError_t segment_states(const RingLinShape& s, RingLinArgs a, bool rev, hipStream_t st) {
+  a.Da = s.Dk;
+  a.Db = s.Dv;
+  a.sa = s.Dv;
+  a.sb = 1;
+  a.slices = slices(s.Dv);
+  hipError_t e = launch_pass(s.type, a, rev, true, st);
+  if (e != hipSuccess) return e;
+  const unsigned per = (unsigned)((s.Dk * s.Dv + 255) / 256);
+  hipLaunchKernelGGL(ring_linattn_scan_kernel, dim3((unsigned)((size_t)per * s.B * s.H)), dim3(256), 0, st, a, rev);
+  return hipGetLastError();
+}
+
+hipError_t ring_linattn_fwd(const RingLinShape& s, const RingLinTensor& q, const RingLinTensor& k, const RingLinTensor& v,
+                            const float* log_decay, const float* s_in, const int* lengths, void* o, float* s_out, void* ws, hipStream_t st) {
+  const int nseg = ring_linattn_segments(s);
+  RingLinArgs a = base(s, log_decay, lengths, nseg);
+  a.X = q;
+  a.Y = k;
+  a.Z = v;
+  a.xs = 1;
+  a.ys = a.zs = s.H / s.G;
+  a.s_in = s_in;
+  a.s_out = s_out;
+  a.seg = (float*)ws;
+  if (nseg > 1) {
+    hipError_t e = segment_states(s, a, false, st);
+    if (e != hipSuccess) return e;
+  }
+  a.Da = s.Dk;
+  a.Db = s.Dv;
+  a.sa = s.Dv;
+  a.sb = 1;
+  a.slices = slices(a.Db);
+  a.out = o;
+  a.out_vec = s.Dv % 8 == 0;
+  a.intra = a.inter = s.scale;
+  return launch_pass(s.type, a, false, false, st);
+}
+
+hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const RingLinTensor& k, const RingLinTensor& v,
+                            const float* log_decay, const float* s_in, const int* lengths, const RingLinTensor& go, const float* gs,
+                            void* gq, void* gk, void* gv, float* gs_in, void* ws, hipStream_t st) {
+  const int nseg = ring_linattn_segments(s), share = s.H / s.G;
+  unsigned char* w = (unsigned char*)ws;
+  float *seg_f = (float*)w, *seg_r = (float*)(w + states_bytes(s, nseg));
+  w += 2 * states_bytes(s, nseg);
+  float *part_k = (float*)w, *part_v = (float*)(w + round_up((size_t)s.B * s.T * s.H * s.Dk * sizeof(float)));
+  hipError_t e;
+  RingLinArgs f = base(s, log_decay, lengths, nseg), r = f;
+  f.s_in = s_in;
+  f.seg = seg_f;
+  f.Y = k;
+  f.Z = v;
+  f.ys = f.zs = share;
+  r.s_in = gs;
+  r.seg = seg_r;
+  r.Y = q;
+  r.Z = go;
+  r.ys = r.zs = 1;
+  r.update = s.scale;
+  r.s_out = gs_in;
+  if (nseg > 1) {
+    e = segment_states(s, f, false, st);
+    if (e != hipSuccess) return e;
+    e = segment_states(s, r, true, st);
+    if (e != hipSuccess) return e;
+  }
+  // dq: do against v weighs k, the state transposed
+  f.X = go;
+  f.xs = 1;
+  f.Y = v;
+  f.Z = k;
+  f.Da = s.Dv;
+  f.Db = s.Dk;
+  f.sa = 1;
+  f.sb = s.Dv;
+  f.slices = slices(f.Db);
+  f.out = gq;
+  f.out_vec = s.Dk % 8 == 0;
+  f.intra = f.inter = s.scale;
+  e = launch_pass(s.type, f, false, false, st);
+  if (e != hipSuccess) return e;
+  // dv: k against q weighs do
+  r.X = k;
+  r.xs = share;
+  r.Da = s.Dk;
+  r.Db = s.Dv;
+  r.sa = s.Dv;
+  r.sb = 1;
+  r.slices = slices(r.Db);
+  r.intra = s.scale;
+  r.out = share > 1 ? (void*)part_v : gv;
+  r.out_f32 = share > 1;
+  r.out_vec = s.Dv % 8 == 0;
+  e = launch_pass(s.type, r, true, false, st);
+  if (e != hipSuccess) return e;
+  // dk: v against do weighs q, the state transposed
+  r.X = v;
+  r.Y = go;
+  r.Z = q;
+  r.Da = s.Dv;
+  r.Db = s.Dk;
+  r.sa = 1;
+  r.sb = s.Dv;
+  r.slices = slices(r.Db);
+  r.s_out = nullptr;
+  r.out = share > 1 ? (void*)part_k : gk;
+  r.out_vec = s.Dk % 8 == 0;
+  e = launch_pass(s.type, r, true, false, st);
+  if (e != hipSuccess || share == 1) return e;
+  e = launch_share(s.type, part_k, gk, share, s.Dk, (size_t)s.B * s.T * s.G * s.Dk, st);
+  if (e != hipSuccess) return e;
+  return launch_share(s.type, part_v, gv, share, s.Dv, (size_t)s.B * s.T * s.G * s.Dv, st);
+}

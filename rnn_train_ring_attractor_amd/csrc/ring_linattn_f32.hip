@@ -1,0 +1,6 @@
+// The chunk kernels of linear attention for fp32 rows.
+#include "ring_linattn.hpp"
+
+hipError_t ring_launch_linattn_f32(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
+  return ring_lin::launch<float>(a, rev, state_only, st);
+}

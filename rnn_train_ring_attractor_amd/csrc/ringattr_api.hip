@@ -916,6 +916,181 @@ static int clip_adam_impl(int n_tensors, void* const* params, void* const* grads
   return RINGATTR_OK;
 }
 
+// ---- sequence operators ----
+
+static bool known_type(const char* who, int type) {
+  if (type == RINGATTR_F32 || type == RINGATTR_BF16 || type == RINGATTR_F16) return true;
+  fail(RINGATTR_ERR_INVALID, "%s: type %d is not one of 0 fp32, 1 bf16, 2 fp16", who, type);
+  return false;
+}
+
+// Workgroups are counted in one launch dimension and rows within a tensor in 64 bits.
+static bool linattn_shape(const char* who, int type, int B, int T, int H, int G, int Dk, int Dv, RingLinShape& s) {
+  if (!known_type(who, type)) return false;
+  if (B <= 0 || T <= 0 || H <= 0 || G <= 0 || Dk <= 0 || Dv <= 0) {
+    fail(RINGATTR_ERR_INVALID, "%s: batch_size, seq_len, heads, kv_heads, dk, dv must be positive (got %d, %d, %d, %d, %d, %d)", who, B,
+         T, H, G, Dk, Dv);
+    return false;
+  }
+  if (H % G != 0) {
+    fail(RINGATTR_ERR_INVALID, "%s: heads (%d) must be a multiple of kv_heads (%d)", who, H, G);
+    return false;
+  }
+  if (Dk > RINGATTR_ATTENTION_MAX_DIM || Dv > RINGATTR_ATTENTION_MAX_DIM) {
+    fail(RINGATTR_ERR_INVALID, "%s: dk and dv up to %d (got %d, %d)", who, RINGATTR_ATTENTION_MAX_DIM, Dk, Dv);
+    return false;
+  }
+  if ((double)B * H > 4e6 || T > (1 << 30)) {
+    fail(RINGATTR_ERR_INVALID, "%s: batch_size * heads up to 4000000, seq_len up to 2^30 (got %d * %d, %d)", who, B, H, T);
+    return false;
+  }
+  s = RingLinShape{B, T, H, G, Dk, Dv, type, 1.f};
+  return true;
+}
+
+static RingLinTensor rows_tensor(const void* p, const long long* strides, int dim, int type) {
+  const int per = type == RINGATTR_F32 ? 4 : 8;
+  RingLinTensor t = {p, (long)strides[0], (long)strides[1], (long)strides[2], false};
+  t.vec = dim % per == 0 && aligned16(p) && strides[0] % per == 0 && strides[1] % per == 0 && strides[2] % per == 0;
+  return t;
+}
+
+size_t ringattr_linear_attention_fwd_workspace_bytes(int type, int batch_size, int seq_len, int heads, int kv_heads, int dk, int dv) {
+  RingLinShape s;
+  if (!linattn_shape("ringattr_linear_attention", type, batch_size, seq_len, heads, kv_heads, dk, dv, s)) return 0;
+  return ring_linattn_fwd_bytes(s);
+}
+
+size_t ringattr_linear_attention_bwd_workspace_bytes(int type, int batch_size, int seq_len, int heads, int kv_heads, int dk, int dv) {
+  RingLinShape s;
+  if (!linattn_shape("ringattr_linear_attention", type, batch_size, seq_len, heads, kv_heads, dk, dv, s)) return 0;
+  return ring_linattn_bwd_bytes(s);
+}
+
+int ringattr_linear_attention_fwd(const void* q, const void* k, const void* v, const long long* strides, const void* log_decay,
+                                  const void* initial_state, const void* lengths, void* o, void* final_state, float scale, int type,
+                                  int batch_size, int seq_len, int heads, int kv_heads, int dk, int dv, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  const char* who = "ringattr_linear_attention_fwd";
+  RingLinShape s;
+  if (!linattn_shape(who, type, batch_size, seq_len, heads, kv_heads, dk, dv, s)) return RINGATTR_ERR_INVALID;
+  if (!q || !k || !v || !strides || !log_decay || !o) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  if (!aligned16(o) || !aligned16(initial_state) || !aligned16(final_state) || !aligned16(workspace))
+    return fail(RINGATTR_ERR_INVALID, "%s: outputs, states and workspace must be 16-byte aligned", who);
+  const size_t need = ring_linattn_fwd_bytes(s);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(RINGATTR_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
+  s.scale = scale;
+  hipError_t e = ring_linattn_fwd(s, rows_tensor(q, strides, dk, type), rows_tensor(k, strides + 3, dk, type),
+                                  rows_tensor(v, strides + 6, dv, type), (const float*)log_decay, (const float*)initial_state,
+                                  (const int*)lengths, o, (float*)final_state, workspace, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "linear attention forward launch");
+  return RINGATTR_OK;
+}
+
+int ringattr_linear_attention_bwd(const void* q, const void* k, const void* v, const void* grad_o, const long long* strides,
+                                  const void* log_decay, const void* initial_state, const void* lengths, const void* grad_final_state,
+                                  void* grad_q, void* grad_k, void* grad_v, void* grad_initial_state, float scale, int type,
+                                  int batch_size, int seq_len, int heads, int kv_heads, int dk, int dv, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  const char* who = "ringattr_linear_attention_bwd";
+  RingLinShape s;
+  if (!linattn_shape(who, type, batch_size, seq_len, heads, kv_heads, dk, dv, s)) return RINGATTR_ERR_INVALID;
+  if (!q || !k || !v || !grad_o || !strides || !log_decay || !grad_q || !grad_k || !grad_v)
+    return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  if (!aligned16(grad_q) || !aligned16(grad_k) || !aligned16(grad_v) || !aligned16(initial_state) || !aligned16(grad_final_state) ||
+      !aligned16(grad_initial_state) || !aligned16(workspace))
+    return fail(RINGATTR_ERR_INVALID, "%s: outputs, states and workspace must be 16-byte aligned", who);
+  const size_t need = ring_linattn_bwd_bytes(s);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(RINGATTR_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
+  s.scale = scale;
+  hipError_t e = ring_linattn_bwd(s, rows_tensor(q, strides, dk, type), rows_tensor(k, strides + 3, dk, type),
+                                  rows_tensor(v, strides + 6, dv, type), (const float*)log_decay, (const float*)initial_state,
+                                  (const int*)lengths, rows_tensor(grad_o, strides + 9, dv, type), (const float*)grad_final_state, grad_q,
+                                  grad_k, grad_v, (float*)grad_initial_state, workspace, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "linear attention backward launch");
+  return RINGATTR_OK;
+}
+
+int ringattr_linear_attention_step(const void* q, const void* k, const void* v, const long long* strides, const void* log_decay,
+                                   void* state, const void* active, void* o, float scale, int type, int batch_size, int heads,
+                                   int kv_heads, int dk, int dv, void* stream) {
+  const char* who = "ringattr_linear_attention_step";
+  RingLinShape s;
+  if (!linattn_shape(who, type, batch_size, 1, heads, kv_heads, dk, dv, s)) return RINGATTR_ERR_INVALID;
+  if (!q || !k || !v || !strides || !log_decay || !state || !o) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  s.scale = scale;
+  RingLinStep a = {};
+  a.q = RingLinTensor{q, (long)strides[0], 0, (long)strides[1], false};
+  a.k = RingLinTensor{k, (long)strides[2], 0, (long)strides[3], false};
+  a.v = RingLinTensor{v, (long)strides[4], 0, (long)strides[5], false};
+  a.log_decay = (const float*)log_decay;
+  a.state = (float*)state;
+  a.active = (const unsigned char*)active;
+  a.out = o;
+  hipError_t e = ring_linattn_step(s, a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "linear attention step launch");
+  return RINGATTR_OK;
+}
+
+int ringattr_rotary(const void* x0, const void* x1, const long long* strides, const void* positions, long long pos_stride_b,
+                    long long pos_stride_t, int position_type, const void* frequencies, void* y0, void* y1, float scale, int interleaved,
+                    int inverse, int type, int batch_size, int seq_len, int heads0, int heads1, int dim, int rot, void* stream) {
+  const char* who = "ringattr_rotary";
+  if (!known_type(who, type)) return RINGATTR_ERR_INVALID;
+  if (position_type < RINGATTR_POS_I64 || position_type > RINGATTR_POS_F32)
+    return fail(RINGATTR_ERR_INVALID, "%s: position_type %d is not one of 0 int64, 1 int32, 2 fp32", who, position_type);
+  if (batch_size <= 0 || seq_len <= 0 || heads0 <= 0 || heads1 < 0 || dim <= 0)
+    return fail(RINGATTR_ERR_INVALID, "%s: batch_size, seq_len, heads0, dim must be positive, heads1 not negative (got %d, %d, %d, %d, %d)", who,
+                batch_size, seq_len, heads0, dim, heads1);
+  if (rot < 2 || rot % 2 != 0 || rot > dim || rot > 2048)
+    return fail(RINGATTR_ERR_INVALID, "%s: rot must be even, between 2 and dim, and no more than 2048 (got %d of %d)", who, rot, dim);
+  if (((double)heads0 + heads1) * dim > (double)(1 << 22) || (double)batch_size * seq_len > 2e9)
+    return fail(RINGATTR_ERR_INVALID, "%s: up to 2^22 values a token and 2e9 tokens (got %ld heads of %d, %d * %d)", who,
+                (long)heads0 + heads1, dim, batch_size, seq_len);
+  if (!x0 || !y0 || (heads1 && (!x1 || !y1)) || !strides || !positions || !frequencies)
+    return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  RingRotaryArgs p = {};
+  p.in[0] = rows_tensor(x0, strides, dim, type);
+  p.in[0].vec = p.in[0].vec && aligned16(y0);
+  if (heads1) {
+    p.in[1] = rows_tensor(x1, strides + 3, dim, type);
+    p.in[1].vec = p.in[1].vec && aligned16(y1);
+  }
+  p.out[0] = y0;
+  p.out[1] = y1;
+  p.heads[0] = heads0;
+  p.heads[1] = heads1;
+  p.positions = positions;
+  p.frequencies = (const double*)frequencies;
+  p.pos_b = (long)pos_stride_b;
+  p.pos_t = (long)pos_stride_t;
+  p.position_type = position_type;
+  p.B = batch_size;
+  p.T = seq_len;
+  p.D = dim;
+  p.rot = rot;
+  p.interleaved = interleaved ? 1 : 0;
+  p.inverse = inverse ? 1 : 0;
+  p.scale = scale;
+  hipError_t e = ring_launch_rotary(p, type, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "rotary launch");
+  return RINGATTR_OK;
+}
+
+int ringattr_dropout(const void* x, const void* residual, void* y, size_t n, unsigned int threshold, float scale, unsigned long long seed,
+                     unsigned long long offset, const void* offset_ptr, int type, void* stream) {
+  const char* who = "ringattr_dropout";
+  if (!known_type(who, type)) return RINGATTR_ERR_INVALID;
+  if (n == 0 || n > ((size_t)1 << 48)) return fail(RINGATTR_ERR_INVALID, "%s: between 1 and 2^48 values (got %zu)", who, n);
+  if (!x || !y) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  hipError_t e = ring_launch_dropout(RingDropoutArgs{x, residual, y, n, seed, offset, (const long long*)offset_ptr, threshold, scale}, type,
+                                     static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "dropout launch");
+  return RINGATTR_OK;
+}
+
 int ringattr_profile_enable(int on) {
   ring_profile_set(on);
   return RINGATTR_OK;

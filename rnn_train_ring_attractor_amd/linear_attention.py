@@ -1,0 +1,167 @@
+"""Linear attention with a decay for each head: the leak of the ring's time loop on a matrix of associations.
+
+    S_t = exp(log_decay[h]) S_(t-1) + k_t v_t^T,   o_t = scale q_t S_t
+
+`linear_attention_func` takes whole sequences (training and prompts: the chunked form, differentiable with respect to q, k, v and the
+initial state, by the same kernels run over other operands), `linear_attention_step` one token for each sequence of a batch (serving:
+the recurrent form, the state updated in place).  What the one leaves as its state the other goes on from.
+
+The operands are float32, bfloat16 or float16; states are float32.  With bfloat16 only inputs and results are rounded to 8 bits:
+what is computed between them enters the matrix units as sums of two or three bfloat16 numbers."""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import SEQUENCE_TYPES, check_sequence_tensor
+
+_Strides9, _Strides12, _Strides6 = ctypes.c_longlong * 9, ctypes.c_longlong * 12, ctypes.c_longlong * 6
+
+
+def _rows(t):
+    """t with a head's values as neighbours (any other strides are taken as they are)."""
+    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _checked(q, k, v, log_decay, dims):
+    check_sequence_tensor("q", q)
+    if q.dim() != dims:
+        raise ValueError(f"q must have {dims} dimensions, got {tuple(q.shape)}")
+    lead, (H, Dk), dev = tuple(q.shape[:-2]), q.shape[-2:], q.device
+    check_sequence_tensor("k", k, dtype=q.dtype, device=dev)
+    check_sequence_tensor("v", v, dtype=q.dtype, device=dev)
+    if k.dim() != dims or tuple(k.shape[:-2]) != lead or k.shape[-1] != Dk:
+        raise ValueError(f"k must have shape {lead + ('kv_heads', Dk)}, got {tuple(k.shape)}")
+    G = k.shape[-2]
+    if v.dim() != dims or tuple(v.shape[:-1]) != lead + (G,):
+        raise ValueError(f"v must have shape {lead + (G, 'dv')}, got {tuple(v.shape)}")
+    Dv = v.shape[-1]
+    if H == 0 or G == 0 or Dk == 0 or Dv == 0 or H % G != 0:
+        raise ValueError(f"heads ({H}) must be a positive multiple of kv_heads ({G}), dk and dv positive ({Dk}, {Dv})")
+    check_sequence_tensor("log_decay", log_decay, (H,), torch.float32, dev)
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise ValueError("log_decay is a setting, as the time loop's alpha: it gets no gradient (detach it)")
+    return H, G, Dk, Dv, dev
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state):
+    B, T, H, Dk = q.shape
+    G, Dv, dev = k.shape[2], v.shape[3], q.device
+    lib, kind = _lib.load(), SEQUENCE_TYPES[q.dtype]
+    with _lib.on_device(dev):
+        o = torch.empty(B, T, H, Dv, dtype=q.dtype, device=dev)
+        state = torch.empty(B, H, Dk, Dv, dtype=torch.float32, device=dev) if want_state else None
+        if B == 0 or T == 0:
+            if want_state:
+                state.zero_() if initial_state is None else state.copy_(initial_state)
+            return o, state
+        nbytes = lib.ringattr_linear_attention_fwd_workspace_bytes(kind, B, T, H, G, Dk, Dv)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        strides = _Strides9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+        _lib.check(lib.ringattr_linear_attention_fwd(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, log_decay.data_ptr(), _ptr(initial_state), _ptr(lengths), o.data_ptr(),
+            _ptr(state), scale, kind, B, T, H, G, Dk, Dv, _ptr(ws), nbytes, _lib.stream_handle(dev)))
+    return o, state
+
+
+class LinearAttentionFunc(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale, want_state):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
+        ctx.scale = scale
+        return _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_o, grad_state):
+        q, k, v, log_decay, initial_state, lengths = ctx.saved_tensors
+        B, T, H, Dk = q.shape
+        G, Dv, dev = k.shape[2], v.shape[3], q.device
+        lib, kind = _lib.load(), SEQUENCE_TYPES[q.dtype]
+        with _lib.on_device(dev):
+            gq, gk, gv = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k, v))
+            want = initial_state is not None and ctx.needs_input_grad[4]
+            g0 = torch.empty(B, H, Dk, Dv, dtype=torch.float32, device=dev) if want else None
+            gs = None if grad_state is None else grad_state.to(torch.float32).contiguous()
+            if B == 0 or T == 0:
+                if want:
+                    g0.zero_() if gs is None else g0.copy_(gs)
+            else:
+                go = torch.zeros(B, T, H, Dv, dtype=q.dtype, device=dev) if grad_o is None else _rows(grad_o.to(q.dtype))
+                nbytes = lib.ringattr_linear_attention_bwd_workspace_bytes(kind, B, T, H, G, Dk, Dv)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+                strides = _Strides12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *go.stride()[:3])
+                _lib.check(lib.ringattr_linear_attention_bwd(
+                    q.data_ptr(), k.data_ptr(), v.data_ptr(), go.data_ptr(), strides, log_decay.data_ptr(), _ptr(initial_state),
+                    _ptr(lengths), _ptr(gs), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _ptr(g0), ctx.scale, kind, B, T, H, G, Dk, Dv,
+                    _ptr(ws), nbytes, _lib.stream_handle(dev)))
+        return gq, gk, gv, None, g0, None, None, None
+
+
+def linear_attention_func(q, k, v, log_decay, initial_state=None, lengths=None, scale=None, return_state=False):
+    """Linear attention over whole sequences.
+
+    q [B,T,H,dk], k [B,T,G,dk], v [B,T,G,dv], G a divisor of H (head h uses head h // (H // G) of k and v), dk and dv up to 256, of one
+    type; a head's values lie next to each other, all other strides are free (a ring history's [T,B,..] order, a slice of one
+    projection's output).  log_decay [H] float32, at most zero for a memory that fades (-inf: one that holds the last token only).
+    initial_state [B,H,dk,dv] float32 or None (zeros).  lengths [B] int32 (int64 is converted) or None: how many tokens of each sequence
+    count, none among the possibilities; outputs and gradients behind them are zero, nothing there is read and the state is the one
+    behind the last token that counts.  scale: dk ** -0.5 if None.
+
+    Returns o [B,T,H,dv], with return_state=True (o, the state behind the sequences).  Differentiable once with respect to q, k, v and
+    initial_state.  A value that is infinite or NaN reaches the rows that see it (as an infinity or as NaN) and no other."""
+    H, G, Dk, Dv, dev = _checked(q, k, v, log_decay, 4)
+    B, T = q.shape[:2]
+    if initial_state is not None:
+        check_sequence_tensor("initial_state", initial_state, (B, H, Dk, Dv), torch.float32, dev)
+        initial_state = initial_state.contiguous()
+    if lengths is not None:
+        if isinstance(lengths, torch.Tensor) and lengths.dtype == torch.int64:
+            lengths = lengths.clamp(0, T).to(torch.int32)
+        check_sequence_tensor("lengths", lengths, (B,), torch.int32, dev)
+        lengths = lengths.contiguous()
+    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
+    scale = Dk ** -0.5 if scale is None else float(scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                    (initial_state is not None and initial_state.requires_grad)):
+        o, state = LinearAttentionFunc.apply(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
+    else:
+        o, state = _forward(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
+    return (o, state) if return_state else o
+
+
+def linear_attention_step(q, k, v, log_decay, state, active=None, scale=None):
+    """One token for each sequence: q [B,H,dk], k [B,G,dk], v [B,G,dv] as in `linear_attention_func`; state [B,H,dk,dv] float32,
+    contiguous, is updated in place.  active [B] (bool or uint8) or None: where it is zero the state stays as it is and the output is
+    zero (a batch with places that wait).  Returns o [B,H,dv].  It has no gradient."""
+    H, G, Dk, Dv, dev = _checked(q, k, v, log_decay, 3)
+    B = q.shape[0]
+    check_sequence_tensor("state", state, (B, H, Dk, Dv), torch.float32, dev)
+    if not state.is_contiguous():
+        raise RuntimeError("state must be contiguous: it is updated in place")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+        raise RuntimeError("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention_func to train")
+    if active is not None:
+        check_sequence_tensor("active", active, (B,), torch.uint8 if getattr(active, "dtype", None) == torch.uint8 else torch.bool, dev)
+        active = active.contiguous()
+    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        o = torch.empty(B, H, Dv, dtype=q.dtype, device=dev)
+        if B == 0:
+            return o
+        strides = _Strides6(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
+        _lib.check(lib.ringattr_linear_attention_step(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, log_decay.data_ptr(), state.data_ptr(), _ptr(active), o.data_ptr(),
+            Dk ** -0.5 if scale is None else float(scale), SEQUENCE_TYPES[q.dtype], B, H, G, Dk, Dv, _lib.stream_handle(dev)))
+    torch.autograd.graph.increment_version(state)
+    return o
