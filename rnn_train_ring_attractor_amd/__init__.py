@@ -18,5 +18,6 @@ _EXPORTS = {
 def __getattr__(name):          # resolved on first use so `python -m ...build` does not import torch
     if name in _EXPORTS:
         import importlib
-        return getattr(importlib.import_module(f"{__name__}.{_EXPORTS[name]}"), name)
+        value = globals()[name] = getattr(importlib.import_module(f"{__name__}.{_EXPORTS[name]}"), name)      # (found directly from now on)
+        return value
     raise AttributeError(name)

@@ -331,14 +331,14 @@ hipError_t ring_run_team_bptt(const RingBpttArgs& a, const float* Wo, const floa
 struct RingLinTensor {
   const void* p;
   long sb, st, sh;       // strides in elements: sequence, token, head; a head's values are neighbours
-  bool vec;              // every row starts at 16 bytes and is a whole number of them long
+  bool vec;              // every row starts at 16 bytes and is a whole number of them long; the token stride is less than 16 MiB
 };
 // One pass of the chunk kernel: rows X against rows Y (Da wide) weigh rows Z (Db wide); see ring_linattn.hpp
 struct RingLinArgs {
   RingLinTensor X, Y, Z;
   int xs, ys, zs;        // heads that share one of the tensor's
   void* out;             // [B,T,H,Db] in the type of the rows, or in fp32 (out_f32)
-  bool out_vec, out_f32;
+  bool out_f32, out_vec; // out_vec: rows are whole numbers of 16 bytes, a token's less than 16 MiB
   const float* log_decay;
   const float* s_in;     // states [B,H,..]: element (a, b) at a * sa + b * sb; null: zeros
   float* s_out;          // null: not wanted

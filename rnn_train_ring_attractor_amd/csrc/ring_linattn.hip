@@ -32,6 +32,9 @@ RingLinArgs base(const RingLinShape& s, const float* log_decay, const int* lengt
   return a;
 }
 
+// a token's outputs of all heads are less than 16 MiB
+bool out_fits(const RingLinArgs& a) { return (long)a.H * a.Db < (1 << 22); }
+
 }  // namespace
 
 // The states in front of the segments: seg[i] is what segment i adds to a state of zeros and becomes the state in front of it
@@ -189,7 +192,7 @@ static hipError_t segment_states(const RingLinShape& s, RingLinArgs a, bool rev,
 
 hipError_t ring_linattn_fwd(const RingLinShape& s, const RingLinTensor& q, const RingLinTensor& k, const RingLinTensor& v,
                             const float* log_decay, const float* s_in, const int* lengths, void* o, float* s_out, void* ws, hipStream_t st) {
-  const int nseg = ring_linattn_segments(s);
+  const int nseg = ring_linattn_segments(s), epv = s.type == RINGATTR_F32 ? 4 : 8;
   RingLinArgs a = base(s, log_decay, lengths, nseg);
   a.X = q;
   a.Y = k;
@@ -209,7 +212,7 @@ hipError_t ring_linattn_fwd(const RingLinShape& s, const RingLinTensor& q, const
   a.sb = 1;
   a.slices = slices(a.Db);
   a.out = o;
-  a.out_vec = s.Dv % 8 == 0;
+  a.out_vec = a.Db % epv == 0 && out_fits(a);
   a.intra = a.inter = s.scale;
   return launch_pass(s.type, a, false, false, st);
 }
@@ -217,7 +220,7 @@ hipError_t ring_linattn_fwd(const RingLinShape& s, const RingLinTensor& q, const
 hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const RingLinTensor& k, const RingLinTensor& v,
                             const float* log_decay, const float* s_in, const int* lengths, const RingLinTensor& go, const float* gs,
                             void* gq, void* gk, void* gv, float* gs_in, void* ws, hipStream_t st) {
-  const int nseg = ring_linattn_segments(s), share = s.H / s.G;
+  const int nseg = ring_linattn_segments(s), share = s.H / s.G, epv = s.type == RINGATTR_F32 ? 4 : 8;
   unsigned char* w = (unsigned char*)ws;
   float *seg_f = (float*)w, *seg_r = (float*)(w + states_bytes(s, nseg));
   w += 2 * states_bytes(s, nseg);
@@ -253,7 +256,7 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
   f.sb = s.Dv;
   f.slices = slices(f.Db);
   f.out = gq;
-  f.out_vec = s.Dk % 8 == 0;
+  f.out_vec = f.Db % epv == 0 && out_fits(f);
   f.intra = f.inter = s.scale;
   e = launch_pass(s.type, f, false, false, st);
   if (e != hipSuccess) return e;
@@ -268,7 +271,7 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
   r.intra = s.scale;
   r.out = share > 1 ? (void*)part_v : gv;
   r.out_f32 = share > 1;
-  r.out_vec = s.Dv % 8 == 0;
+  r.out_vec = r.Db % epv == 0 && out_fits(r);
   e = launch_pass(s.type, r, true, false, st);
   if (e != hipSuccess) return e;
   // dk: v against do weighs q, the state transposed
@@ -282,7 +285,7 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
   r.slices = slices(r.Db);
   r.s_out = nullptr;
   r.out = share > 1 ? (void*)part_k : gk;
-  r.out_vec = s.Dk % 8 == 0;
+  r.out_vec = r.Db % epv == 0 && out_fits(r);
   e = launch_pass(s.type, r, true, false, st);
   if (e != hipSuccess || share == 1) return e;
   e = launch_share(s.type, part_k, gk, share, s.Dk, (size_t)s.B * s.T * s.G * s.Dk, st);

@@ -38,7 +38,12 @@ template <> struct Type<_Float16> { typedef float C; static constexpr int EPV = 
 
 __device__ __forceinline__ float power(float g2, int e) { return e == 0 ? 1.f : __builtin_amdgcn_exp2f(g2 * (float)e); }
 
-__device__ __forceinline__ f32x4 widen(bf16x4 x) { return __builtin_convertvector(x, f32x4); }
+// (by bits: left to itself the compiler converts the second of each pair once more instead)
+__device__ __forceinline__ f32x4 widen(bf16x4 x) {
+  const u32x2 b = __builtin_bit_cast(u32x2, x);
+  return f32x4{__builtin_bit_cast(float, b[0] << 16), __builtin_bit_cast(float, b[0] & 0xffff0000u), __builtin_bit_cast(float, b[1] << 16),
+               __builtin_bit_cast(float, b[1] & 0xffff0000u)};
+}
 __device__ __forceinline__ bf16x4 narrow(f32x4 x) { return __builtin_convertvector(x, bf16x4); }
 __device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
@@ -69,60 +74,98 @@ template <int LD> __device__ __forceinline__ f32x4 read_rows(const float* tile, 
 }
 
 __device__ __forceinline__ bool nonfinite(float x) { return (__builtin_bit_cast(unsigned, x) & 0x7f800000u) == 0x7f800000u; }
+template <typename T> __device__ constexpr unsigned exponent() { return sizeof(T) == 4 ? 0x7f800000u : (Type<T>::BF ? 0x7f80u : 0x7c00u); }
 template <typename T> __device__ __forceinline__ bool words_nonfinite(u32x4 w) {
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    constexpr unsigned E = sizeof(T) == 4 ? 0x7f800000u : (Type<T>::BF ? 0x7f80u : 0x7c00u);
+    constexpr unsigned E = exponent<T>();
     bad |= (w[i] & E) == E;
     if (sizeof(T) == 2) bad |= (w[i] & (E << 16)) == (E << 16);
   }
   return bad;
 }
 
-// One tile of ROWS x COLS values, global -> registers -> LDS.
-template <typename T, int ROWS, int COLS, int NT> struct Stage {
+// One tile of ROWS x COLS values, global -> registers -> LDS.  Rows from `n` on and columns from `cols` on become zero on the way into
+// LDS; until then their place is taken by the last row and columns that there are, so that no load hangs on a branch (a value that is
+// merged behind one is waited for there).  VEC: 16-byte loads (RingLinTensor::vec).
+template <typename T, int ROWS, int COLS, int NT, bool VEC> struct Stage {
   typedef typename Type<T>::C C;
   static constexpr int EPV = Type<T>::EPV, UPR = COLS / EPV, UNITS = ROWS * UPR, NU = (UNITS + NT - 1) / NT, LD = COLS + Type<T>::PAD;
+  static constexpr int RS = NT / UPR;                          // rows from a thread's unit to its next; its columns stay
+  static_assert(NT % UPR == 0, "");
   u32x4 r[NU];
 
-  // n rows of `cols` values from base on, token stride st
-  __device__ __forceinline__ void load(const T* base, long st, int n, int cols, bool vec, int tid) {
+  // rows 0..last from base on, token stride st
+  __device__ __forceinline__ void load(const T* base, long st, int last, int cols, int tid) {
+    const int row = tid / UPR, c = (tid % UPR) * EPV;
+    if constexpr (VEC) {
+      const unsigned stb = (unsigned)st * (unsigned)sizeof(T), cb = (unsigned)(min(c, cols - EPV) * (int)sizeof(T));
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const int idx = tid + u * NT, row = idx / UPR, c = (idx % UPR) * EPV;
-      r[u] = u32x4{0, 0, 0, 0};
-      if (row < n && c < cols) {
-        const T* p = base + (long)row * st + c;
-        if (vec) {
-          r[u] = *reinterpret_cast<const u32x4*>(p);
-        } else if constexpr (sizeof(T) == 4) {
+      for (int u = 0; u < NU; ++u)
+        r[u] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + (__umul24((unsigned)min(row + u * RS, last), stb) + cb));
+    } else {
 #pragma unroll
-          for (int e = 0; e < EPV; ++e)
-            if (c + e < cols) r[u][e] = __builtin_bit_cast(unsigned, p[e]);
+      for (int u = 0; u < NU; ++u) {
+        const T* p = base + (long)min(row + u * RS, last) * st;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int e = 0; e < EPV; ++e) r[u][e] = __builtin_bit_cast(unsigned, p[min(c + e, cols - 1)]);
         } else {
 #pragma unroll
-          for (int e = 0; e < EPV; ++e)
-            if (c + e < cols) r[u][e / 2] |= (unsigned)__builtin_bit_cast(unsigned short, p[e]) << (16 * (e & 1));
+          for (int e = 0; e < EPV; e += 2)
+            r[u][e / 2] = __builtin_bit_cast(unsigned short, p[min(c + e, cols - 1)]) |
+                          (unsigned)__builtin_bit_cast(unsigned short, p[min(c + e + 1, cols - 1)]) << 16;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void mask(int n, int cols, int tid) {
+    const int row = tid / UPR, c = (tid % UPR) * EPV;
+    if (n >= ROWS && cols >= COLS) return;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const bool in = row + u * RS < n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (VEC) {
+          r[u][e] = in && c < cols ? r[u][e] : 0u;
+        } else if constexpr (sizeof(T) == 4) {
+          r[u][e] = in && c + e < cols ? r[u][e] : 0u;
+        } else {
+          r[u][e] &= (in && c + 2 * e < cols ? 0xffffu : 0u) | (in && c + 2 * e + 1 < cols ? 0xffff0000u : 0u);
         }
       }
     }
   }
   __device__ __forceinline__ void store(C* tile, int tid) const {
+    const int row = tid / UPR, c = (tid % UPR) * EPV;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      const int idx = tid + u * NT, row = idx / UPR, c = (idx % UPR) * EPV;
-      if (UNITS % NT == 0 || idx < UNITS) {
-        C* p = tile + row * LD + c;
-        if constexpr (sizeof(C) == sizeof(T)) {
-          *reinterpret_cast<u32x4*>(p) = r[u];
-        } else {
-          const f16x8 h = __builtin_bit_cast(f16x8, r[u]);
-          *reinterpret_cast<f32x4*>(p) = f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
-          *reinterpret_cast<f32x4*>(p + 4) = f32x4{(float)h[4], (float)h[5], (float)h[6], (float)h[7]};
-        }
+      if (UNITS % NT != 0 && row + u * RS >= ROWS) continue;
+      C* p = tile + (row + u * RS) * LD + c;
+      if constexpr (sizeof(C) == sizeof(T)) {
+        *reinterpret_cast<u32x4*>(p) = r[u];
+      } else {
+        const f16x8 h = __builtin_bit_cast(f16x8, r[u]);
+        *reinterpret_cast<f32x4*>(p) = f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+        *reinterpret_cast<f32x4*>(p + 4) = f32x4{(float)h[4], (float)h[5], (float)h[6], (float)h[7]};
       }
     }
+  }
+  __device__ __forceinline__ void clean() {                    // values that are not finite become zero
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        constexpr unsigned E = exponent<T>();
+        if constexpr (sizeof(T) == 4) {
+          if ((r[u][e] & E) == E) r[u][e] = 0;
+        } else {
+          if ((r[u][e] & E) == E) r[u][e] &= 0xffff0000u;
+          if ((r[u][e] & (E << 16)) == (E << 16)) r[u][e] &= 0xffffu;
+        }
+      }
   }
   __device__ __forceinline__ bool bad() const {
     bool b = false;
@@ -141,13 +184,13 @@ template <typename T> __device__ __forceinline__ const T* rows_of(const RingLinT
 // rows 4g..4g+3 of column l into lane (g, l) and take them as contraction indices from there.  The weights are formed transposed
 // for the same reason, by every wave for itself (the kernel is bound by memory: a chunk of 128-wide bf16 rows moves in about four times what
 // its products take).
-template <typename T, int DA, int NC, int CT, bool REV, bool STATE_ONLY>
+template <typename T, int DA, int NC, int CT, bool VEC, bool REV, bool STATE_ONLY>
 __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(RingLinArgs p) {
   constexpr int NW = 4, NT = 64 * NW, WC = 16 * NC * NW, CH = 16 * CT, DT = DA / 16;
   constexpr bool BF = Type<T>::BF;
   typedef typename Type<T>::C C;
-  typedef Stage<T, CH, DA, NT> SA;
-  typedef Stage<T, CH, WC, NT> SZ;
+  typedef Stage<T, CH, DA, NT, VEC> SA;
+  typedef Stage<T, CH, WC, NT, VEC> SZ;
   __shared__ __align__(16) C ldsX[STATE_ONLY ? 8 : CH * SA::LD];
   __shared__ __align__(16) C ldsY[CH * SA::LD];
   __shared__ __align__(16) C ldsZ[CH * SZ::LD];
@@ -159,7 +202,8 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
   const int cw = 16 * NC * w;                                  // the wave's columns within the workgroup's
   const int T_ = p.T;
   const int len = p.lengths ? min(max(p.lengths[b], 0), T_) : T_;
-  const int t0 = seg * p.seg_tokens, t1 = min(T_, t0 + p.seg_tokens), nch = (t1 - t0 + CH - 1) / CH;
+  const int t0 = seg * p.seg_tokens, t1 = min(T_, t0 + p.seg_tokens), te = min(len, t1), nch = (t1 - t0 + CH - 1) / CH;
+  const int full = te > t0 ? (te - t0 + CH - 1) / CH : 0;      // chunks with tokens that count
   const float g2 = (float)((double)p.log_decay[h] * 1.4426950408889634);
   const size_t bh = (size_t)b * p.H + h;
 
@@ -194,290 +238,306 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
     }
   int n_now = -1;
 
-  SA rx, ry;
-  SZ rz;
-  auto fetch = [&](int c) {
-    const int t = t0 + c * CH, n = min(max(len - t, 0), min(CH, t1 - t));
-    if (n <= 0) return;
-    if (!STATE_ONLY) rx.load(X + (long)t * p.X.st, p.X.st, n, p.Da, p.X.vec, tid);
-    ry.load(Y + (long)t * p.Y.st, p.Y.st, n, p.Da, p.Y.vec, tid);
-    rz.load(Z + (long)t * p.Z.st, p.Z.st, n, cols, p.Z.vec, tid);
-  };
-  if (tid < 2) flag[tid] = 0;
-  __syncthreads();
-  fetch(REV ? nch - 1 : 0);
-  for (int i = 0; i < nch; ++i) {
-    const int c = REV ? nch - 1 - i : i, t = t0 + c * CH;
-    const int rows = min(CH, t1 - t), n = min(max(len - t, 0), rows);
-    f32x4 O[NC][CT];
+  // O = inner S X^T, what the state in front gives, and P = Y X^T, the weights
+  auto from_state = [&](f32x4 (&O)[NC][CT], f32x4 (&P)[CT][CT]) {
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
       for (int it = 0; it < CT; ++it) O[ct][it] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    if (n > 0) {
-      if (!STATE_ONLY) {
-        rx.store(ldsX, tid);
-        if (rz.bad()) flag[i & 1] = 1;
-        if (tid == 0) flag[(i + 1) & 1] = 0;
-      }
-      ry.store(ldsY, tid);
-      rz.store(ldsZ, tid);
-      __syncthreads();
-    }
-    if (i + 1 < nch) fetch(REV ? c - 1 : c + 1);
-    if (n > 0) {
-      if (n != n_now) {                                        // (whole chunks, but for the last of a sequence)
-        n_now = n;
-        whole = power(g2, n);
 #pragma unroll
-        for (int it = 0; it < CT; ++it) {
-          inner[it] = p.inter * power(g2, REV ? max(n - 1 - 16 * it - l, 0) : 16 * it + l + 1);
+    for (int s = 0; s < DT; s += 2) {
+      if constexpr (BF) {
+        bf16x8 x[CT];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = 16 * it + 4 * g + r;
-            outer[it][r] = p.update * power(g2, REV ? j + 1 : max(n - 1 - j, 0));
-          }
-        }
-      }
-      if constexpr (!STATE_ONLY) {
-        f32x4 P[CT][CT];                                       // [tile of Y's rows][tile of X's rows]
+        for (int it = 0; it < CT; ++it)
+          x[it] = join(read_rows<SA::LD>(ldsX, 16 * it, 16 * s, g, l), read_rows<SA::LD>(ldsX, 16 * it, 16 * s + 16, g, l));
 #pragma unroll
-        for (int jt = 0; jt < CT; ++jt)
-#pragma unroll
-          for (int it = 0; it < CT; ++it) P[jt][it] = f32x4{0.f, 0.f, 0.f, 0.f};
-        // weights, and what the state in front gives
-#pragma unroll
-        for (int s = 0; s < DT; s += 2) {
-          if constexpr (BF) {
-            bf16x8 x[CT];
+          for (int jt = 0; jt < CT; ++jt) {
+            const bf16x8 y = join(read_rows<SA::LD>(ldsY, 16 * jt, 16 * s, g, l), read_rows<SA::LD>(ldsY, 16 * jt, 16 * s + 16, g, l));
 #pragma unroll
             for (int it = 0; it < CT; ++it)
-              x[it] = join(read_rows<SA::LD>(ldsX, 16 * it, 16 * s, g, l), read_rows<SA::LD>(ldsX, 16 * it, 16 * s + 16, g, l));
-#pragma unroll
-            for (int ct = 0; ct < NC; ++ct) {
-              const bf16x4 a0 = narrow(S[s][ct]), a1 = narrow(S[s + 1][ct]);
-              const bf16x4 b0 = narrow(S[s][ct] - widen(a0)), b1 = narrow(S[s + 1][ct] - widen(a1));
-              const bf16x8 hi = join(a0, a1), lo = join(b0, b1);
-#pragma unroll
-              for (int it = 0; it < CT; ++it) {
-                O[ct][it] = mfma16(hi, x[it], O[ct][it]);
-                O[ct][it] = mfma16(lo, x[it], O[ct][it]);
-              }
-            }
-#pragma unroll
-            for (int jt = 0; jt < CT; ++jt) {
-              const bf16x8 y = join(read_rows<SA::LD>(ldsY, 16 * jt, 16 * s, g, l), read_rows<SA::LD>(ldsY, 16 * jt, 16 * s + 16, g, l));
-#pragma unroll
-              for (int it = 0; it < CT; ++it)
-                if (REV ? jt >= it : jt <= it) P[jt][it] = mfma16(y, x[it], P[jt][it]);
-            }
-          } else {
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              f32x4 x[CT];
-#pragma unroll
-              for (int it = 0; it < CT; ++it) x[it] = read_rows<SA::LD>(ldsX, 16 * it, 16 * (s + q), g, l);
-#pragma unroll
-              for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-                for (int it = 0; it < CT; ++it)
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) O[ct][it] = mfma4(S[s + q][ct][r], x[it][r], O[ct][it]);
-#pragma unroll
-              for (int jt = 0; jt < CT; ++jt) {
-                const f32x4 y = read_rows<SA::LD>(ldsY, 16 * jt, 16 * (s + q), g, l);
-#pragma unroll
-                for (int it = 0; it < CT; ++it)
-                  if (REV ? jt >= it : jt <= it)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) P[jt][it] = mfma4(y[r], x[it][r], P[jt][it]);
-              }
-            }
+              if (REV ? jt >= it : jt <= it) P[jt][it] = mfma16(y, x[it], P[jt][it]);
           }
-        }
-#pragma unroll
-        for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-          for (int it = 0; it < CT; ++it) O[ct][it] *= inner[it];
-        // what is not to be seen is left out, not multiplied by zero: it may be anything
-#pragma unroll
-        for (int jt = 0; jt < CT; ++jt)
-#pragma unroll
-          for (int it = 0; it < CT; ++it)
-            if (REV ? jt >= it : jt <= it)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float f = near[REV ? jt - it : it - jt][r];
-                P[jt][it][r] = jt == it && (REV ? 4 * g + r < l : 4 * g + r > l) ? 0.f : P[jt][it][r] * f;
-              }
-        // A row of Z with infinities or NaN must not reach rows that do not see it: there the products within tiles on the
-        // diagonal, which multiply it by zero, go without its non-finite values, which are added one by one.
-        const bool bad = flag[i & 1] != 0;
 #pragma unroll
         for (int ct = 0; ct < NC; ++ct) {
-          if constexpr (BF) {
+          const bf16x4 a0 = narrow(S[s][ct]), a1 = narrow(S[s + 1][ct]);
+          const bf16x8 hi = join(a0, a1), lo = join(narrow(S[s][ct] - widen(a0)), narrow(S[s + 1][ct] - widen(a1)));
 #pragma unroll
-            for (int jp = 0; jp < CT; jp += 2) {
-              bf16x4 z0 = read_columns<SZ::LD, NC>(ldsZ, 16 * jp, cw, ct, g, l), z1 = read_columns<SZ::LD, NC>(ldsZ, 16 * jp + 16, cw, ct, g, l);
-              if (bad)
+          for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(hi, x[it], O[ct][it]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  if (nonfinite((float)z0[e])) z0[e] = (__bf16)0.f;
-                  if (nonfinite((float)z1[e])) z1[e] = (__bf16)0.f;
-                }
-              const bf16x8 z = join(z0, z1);
+          for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(lo, x[it], O[ct][it]);
+        }
+      } else {
 #pragma unroll
-              for (int it = 0; it < CT; ++it)
-                if (REV ? jp + 1 >= it : jp <= it) {
-                  const bf16x4 a0 = narrow(P[jp][it]), a1 = narrow(P[jp + 1][it]);
-                  O[ct][it] = mfma16(z, join(a0, a1), O[ct][it]);
-                  O[ct][it] = mfma16(z, join(narrow(P[jp][it] - widen(a0)), narrow(P[jp + 1][it] - widen(a1))), O[ct][it]);
-                }
-            }
-          } else {
+        for (int q = 0; q < 2; ++q) {
+          f32x4 x[CT];
+#pragma unroll
+          for (int it = 0; it < CT; ++it) x[it] = read_rows<SA::LD>(ldsX, 16 * it, 16 * (s + q), g, l);
 #pragma unroll
             for (int jt = 0; jt < CT; ++jt) {
-              f32x4 z = read_columns<SZ::LD, NC>(ldsZ, 16 * jt, cw, ct, g, l);
-              if (bad)
+              const f32x4 y = read_rows<SA::LD>(ldsY, 16 * jt, 16 * (s + q), g, l);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (nonfinite(z[e])) z[e] = 0.f;
+              for (int r = 0; r < 4; ++r)
 #pragma unroll
-              for (int it = 0; it < CT; ++it)
-                if (REV ? jt >= it : jt <= it)
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) O[ct][it] = mfma4(z[r], P[jt][it][r], O[ct][it]);
+                for (int it = 0; it < CT; ++it)
+                  if (REV ? jt >= it : jt <= it) P[jt][it] = mfma4(y[r], x[it][r], P[jt][it]);
             }
-          }
-        }
-        if (bad) {
-          for (int j = 0; j < n; ++j) {
-            float z[NC][4];
-            bool any = false;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                z[ct][r] = (float)ldsZ[j * SZ::LD + cw + column<NC>(ct, 4 * g + r)];
-                any |= nonfinite(z[ct][r]);
-              }
-            if (!__any(any)) continue;
-#pragma unroll
-            for (int it = 0; it < CT; ++it) {
-              const int row = 16 * it + l, e = REV ? j - row : row - j;
-              float dot = 0.f;
-              for (int a = 0; a < DA; ++a) dot = fmaf((float)ldsX[row * SA::LD + a], (float)ldsY[j * SA::LD + a], dot);
-              if (e < 0) continue;
-              dot *= p.intra * power(g2, e);
-#pragma unroll
-              for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  if (nonfinite(z[ct][r])) O[ct][it][r] += dot * z[ct][r];
-            }
-          }
+              for (int it = 0; it < CT; ++it) O[ct][it] = mfma4(S[s + q][ct][r], x[it][r], O[ct][it]);
         }
       }
-      // the state behind the chunk
-      if constexpr (BF) {
-        bf16x8 z[NC][CT / 2][3];
+    }
 #pragma unroll
-        for (int ct = 0; ct < NC; ++ct)
+    for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
-          for (int jp = 0; jp < CT; jp += 2) {
-            bf16x4 part[2][3];
+      for (int it = 0; it < CT; ++it) O[ct][it] *= inner[it];
+  };
+  auto put = [&](const f32x4 (&O)[NC][CT], int t, int rows) {
+    const int c = cw + (NC == 2 ? 8 * g : 4 * g);
+    const size_t at = ((size_t)b * T_ + t) * p.H + h, size = p.out_f32 || sizeof(T) == 4 ? 4 : sizeof(T);
+    char* const base = (char*)p.out + (at * p.Db + c0) * size;
+    const unsigned step = (unsigned)(p.H * p.Db) * (unsigned)size, first = (unsigned)c * (unsigned)size;     // (VEC: within 24 bits)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              f32x4 v = widen(read_columns<SZ::LD, NC>(ldsZ, 16 * (jp + q), cw, ct, g, l));
+    for (int it = 0; it < CT; ++it) {
+      const int row = 16 * it + l;
+      if (row >= rows || c >= cols) continue;
+      char* const o = VEC ? base + (__umul24((unsigned)row, step) + first) : base + ((size_t)row * step + first);
+      if (p.out_f32 || sizeof(T) == 4) {
 #pragma unroll
-              for (int r = 0; r < 4; ++r) v[r] *= outer[jp + q][r];
+        for (int ct = 0; ct < NC; ++ct) {
+          if (VEC) {
+            if (c + 4 * ct < cols) reinterpret_cast<f32x4*>(o)[ct] = O[ct][it];
+          } else {
 #pragma unroll
-              for (int k = 0; k < 3; ++k) {
-                part[q][k] = narrow(v);
-                v -= widen(part[q][k]);
-              }
-            }
-#pragma unroll
-            for (int k = 0; k < 3; ++k) z[ct][jp / 2][k] = join(part[0][k], part[1][k]);
-          }
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-#pragma unroll
-          for (int ct = 0; ct < NC; ++ct) S[d][ct] *= whole;
-#pragma unroll
-          for (int jp = 0; jp < CT; jp += 2) {
-            const bf16x8 y = join(read_columns<SA::LD, 1>(ldsY, 16 * jp, 16 * d, 0, g, l), read_columns<SA::LD, 1>(ldsY, 16 * jp + 16, 16 * d, 0, g, l));
-#pragma unroll
-            for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-              for (int k = 0; k < 3; ++k) S[d][ct] = mfma16(y, z[ct][jp / 2][k], S[d][ct]);
+            for (int r = 0; r < 4; ++r)
+              if (c + 4 * ct + r < cols) reinterpret_cast<float*>(o)[4 * ct + r] = O[ct][it][r];
           }
         }
       } else {
-        f32x4 z[NC][CT];
+        typedef T vec_t __attribute__((ext_vector_type(4 * NC)));
+        vec_t q;
 #pragma unroll
-        for (int ct = 0; ct < NC; ++ct)
+        for (int e = 0; e < 4 * NC; ++e) q[e] = (T)O[e / 4][it][e % 4];
+        if (VEC) {
+          *reinterpret_cast<vec_t*>(o) = q;
+        } else {
 #pragma unroll
-          for (int jt = 0; jt < CT; ++jt) {
-            z[ct][jt] = read_columns<SZ::LD, NC>(ldsZ, 16 * jt, cw, ct, g, l);
+          for (int e = 0; e < 4 * NC; ++e)
+            if (c + e < cols) reinterpret_cast<T*>(o)[e] = q[e];
+        }
+      }
+    }
+  };
+
+  if constexpr (!STATE_ONLY) {                                 // chunks without tokens that count
+    f32x4 zero[NC][CT];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) z[ct][jt][r] *= outer[jt][r];
+    for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+      for (int it = 0; it < CT; ++it) zero[ct][it] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = full; c < nch; ++c) put(zero, t0 + c * CH, min(CH, t1 - t0 - c * CH));
+  }
+
+  SA rx, ry;
+  SZ rz;
+  auto fetch = [&](int c) {
+    const int t = t0 + c * CH, last = min(CH, te - t) - 1;
+    if (!STATE_ONLY) rx.load(X + (long)t * p.X.st, p.X.st, last, p.Da, tid);
+    ry.load(Y + (long)t * p.Y.st, p.Y.st, last, p.Da, tid);
+    rz.load(Z + (long)t * p.Z.st, p.Z.st, last, cols, tid);
+  };
+  if (tid < 2) flag[tid] = 0;
+  __syncthreads();
+  if (full > 0) fetch(REV ? full - 1 : 0);
+  for (int i = 0; i < full; ++i) {
+    const int c = REV ? full - 1 - i : i, t = t0 + c * CH, n = min(CH, te - t);
+    if (!STATE_ONLY) {
+      rx.mask(n, p.Da, tid);
+      rx.store(ldsX, tid);
+    }
+    ry.mask(n, p.Da, tid);
+    ry.store(ldsY, tid);
+    rz.mask(n, cols, tid);
+    if (!STATE_ONLY) {
+      if (rz.bad()) {
+        rz.clean();
+        flag[i & 1] = 1;
+      }
+      if (tid == 0) flag[(i + 1) & 1] = 0;
+    }
+    rz.store(ldsZ, tid);
+    lds_barrier();
+    fetch(i + 1 < full ? (REV ? c - 1 : c + 1) : c);           // (the last one's again: nothing reads it)
+    if (n != n_now) {                                          // (whole chunks, but for the last of a sequence)
+      n_now = n;
+      whole = power(g2, n);
+#pragma unroll
+      for (int it = 0; it < CT; ++it) {
+        inner[it] = p.inter * power(g2, REV ? max(n - 1 - 16 * it - l, 0) : 16 * it + l + 1);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = 16 * it + 4 * g + r;
+          outer[it][r] = p.update * power(g2, REV ? j + 1 : max(n - 1 - j, 0));
+        }
+      }
+    }
+    if constexpr (!STATE_ONLY) {
+      f32x4 O[NC][CT], P[CT][CT];                              // P: [tile of Y's rows][tile of X's rows]
+#pragma unroll
+      for (int jt = 0; jt < CT; ++jt)
+#pragma unroll
+        for (int it = 0; it < CT; ++it) P[jt][it] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const bool bad = flag[i & 1] != 0;
+      from_state(O, P);
+      // what is not to be seen is left out, not multiplied by zero: it may be anything
+#pragma unroll
+      for (int jt = 0; jt < CT; ++jt)
+#pragma unroll
+        for (int it = 0; it < CT; ++it)
+          if (REV ? jt >= it : jt <= it)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float f = near[REV ? jt - it : it - jt][r];
+              P[jt][it][r] = jt == it && (REV ? 4 * g + r < l : 4 * g + r > l) ? 0.f : P[jt][it][r] * f;
+            }
+      if constexpr (BF) {
+#pragma unroll
+        for (int jp = 0; jp < CT; jp += 2) {
+          bf16x8 z[NC];
+#pragma unroll
+          for (int ct = 0; ct < NC; ++ct)
+            z[ct] = join(read_columns<SZ::LD, NC>(ldsZ, 16 * jp, cw, ct, g, l), read_columns<SZ::LD, NC>(ldsZ, 16 * jp + 16, cw, ct, g, l));
+#pragma unroll
+          for (int it = 0; it < CT; ++it)
+            if (REV ? jp + 1 >= it : jp <= it) {
+              const bf16x4 a0 = narrow(P[jp][it]), a1 = narrow(P[jp + 1][it]);
+              const bf16x8 hi = join(a0, a1), lo = join(narrow(P[jp][it] - widen(a0)), narrow(P[jp + 1][it] - widen(a1)));
+#pragma unroll
+              for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma16(z[ct], hi, O[ct][it]);
+#pragma unroll
+              for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma16(z[ct], lo, O[ct][it]);
+            }
+        }
+      } else {
+#pragma unroll
+        for (int jt = 0; jt < CT; ++jt) {
+          f32x4 z[NC];
+#pragma unroll
+          for (int ct = 0; ct < NC; ++ct) z[ct] = read_columns<SZ::LD, NC>(ldsZ, 16 * jt, cw, ct, g, l);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int it = 0; it < CT; ++it)
+              if (REV ? jt >= it : jt <= it)
+#pragma unroll
+                for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma4(z[ct][r], P[jt][it][r], O[ct][it]);
+        }
+      }
+      // A value of Z that is infinite or NaN must not reach rows that do not see it, which the products within the tiles multiply by
+      // zero: such values are zero in LDS and what they give is added here, one by one.
+      if (bad)
+        for (int j = 0; j < n; ++j) {
+          float z[NC][4], zs[NC];                              // of the lane's columns of O, of its columns of S
+          const T* row = Z + (long)(t + j) * p.Z.st;
+          bool any = false;
+#pragma unroll
+          for (int ct = 0; ct < NC; ++ct) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int col = cw + column<NC>(ct, 4 * g + r);
+              z[ct][r] = col < cols ? (float)row[col] : 0.f;
+            }
+            const int col = cw + column<NC>(ct, l);
+            zs[ct] = col < cols ? (float)row[col] : 0.f;
+            any |= nonfinite(zs[ct]);
           }
+          if (!__any(any)) continue;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-#pragma unroll
-          for (int ct = 0; ct < NC; ++ct) S[d][ct] *= whole;
-#pragma unroll
-          for (int jt = 0; jt < CT; ++jt) {
-            const f32x4 y = read_columns<SA::LD, 1>(ldsY, 16 * jt, 16 * d, 0, g, l);
+          for (int it = 0; it < CT; ++it) {
+            const int i = 16 * it + l, e = REV ? j - i : i - j;
+            float dot = 0.f;
+            for (int a = 0; a < DA; ++a) dot = fmaf((float)ldsX[i * SA::LD + a], (float)ldsY[j * SA::LD + a], dot);
+            dot *= e < 0 ? 0.f : p.intra * power(g2, e);
 #pragma unroll
             for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) S[d][ct] = mfma4(y[r], z[ct][jt][r], S[d][ct]);
+              for (int r = 0; r < 4; ++r)
+                if (e >= 0 && i < n && nonfinite(z[ct][r])) O[ct][it][r] += dot * z[ct][r];
           }
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int ct = 0; ct < NC; ++ct)
+                if (nonfinite(zs[ct])) S[d][ct][r] = fmaf((float)ldsY[j * SA::LD + 16 * d + 4 * g + r], zs[ct], S[d][ct][r]);
+        }
+      put(O, t, min(CH, t1 - t));
+    }
+    // the state behind the chunk
+    if constexpr (BF) {
+      bf16x8 z[NC][CT / 2][3];
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int jp = 0; jp < CT; jp += 2) {
+          bf16x4 part[2][3];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            f32x4 v = widen(read_columns<SZ::LD, NC>(ldsZ, 16 * (jp + q), cw, ct, g, l));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] *= outer[jp + q][r];
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+              part[q][k] = narrow(v);
+              v -= widen(part[q][k]);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 3; ++k) z[ct][jp / 2][k] = join(part[0][k], part[1][k]);
+        }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+#pragma unroll
+        for (int ct = 0; ct < NC; ++ct) S[d][ct] *= whole;
+#pragma unroll
+        for (int jp = 0; jp < CT; jp += 2) {
+          const bf16x8 y = join(read_columns<SA::LD, 1>(ldsY, 16 * jp, 16 * d, 0, g, l), read_columns<SA::LD, 1>(ldsY, 16 * jp + 16, 16 * d, 0, g, l));
+#pragma unroll
+          for (int k = 0; k < 3; ++k)
+#pragma unroll
+            for (int ct = 0; ct < NC; ++ct) S[d][ct] = mfma16(y, z[ct][jp / 2][k], S[d][ct]);
         }
       }
-      __syncthreads();                                         // the tiles are free for the next chunk
-    }
-    if constexpr (!STATE_ONLY) {
-      const bool wide = p.out_vec;
+    } else {
+      f32x4 z[NC][CT];
 #pragma unroll
-      for (int it = 0; it < CT; ++it) {
-        const int row = 16 * it + l, c = cw + (NC == 2 ? 8 * g : 4 * g);
-        if (row >= rows || c >= cols) continue;
-        const size_t at = (((size_t)b * T_ + t + row) * p.H + h) * p.Db + c0 + c;
-        float v[4 * NC];
+      for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
-        for (int ct = 0; ct < NC; ++ct)
+        for (int jt = 0; jt < CT; ++jt) {
+          z[ct][jt] = read_columns<SZ::LD, NC>(ldsZ, 16 * jt, cw, ct, g, l);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[4 * ct + r] = O[ct][it][r];
-        if (p.out_f32 || sizeof(T) == 4) {
-          float* o = (float*)p.out + at;
-          if (wide) {
+          for (int r = 0; r < 4; ++r) z[ct][jt][r] *= outer[jt][r];
+        }
 #pragma unroll
-            for (int ct = 0; ct < NC; ++ct) *reinterpret_cast<f32x4*>(o + 4 * ct) = O[ct][it];
-          } else {
+      for (int d = 0; d < DT; ++d) {
 #pragma unroll
-            for (int e = 0; e < 4 * NC; ++e)
-              if (c + e < cols) o[e] = v[e];
-          }
-        } else {
-          T* o = (T*)p.out + at;
-          typedef T vec_t __attribute__((ext_vector_type(4 * NC)));
-          vec_t q;
+        for (int ct = 0; ct < NC; ++ct) S[d][ct] *= whole;
 #pragma unroll
-          for (int e = 0; e < 4 * NC; ++e) q[e] = (T)v[e];
-          if (wide) {
-            *reinterpret_cast<vec_t*>(o) = q;
-          } else {
+        for (int jt = 0; jt < CT; ++jt) {
+          const f32x4 y = read_columns<SA::LD, 1>(ldsY, 16 * jt, 16 * d, 0, g, l);
 #pragma unroll
-            for (int e = 0; e < 4 * NC; ++e)
-              if (c + e < cols) o[e] = q[e];
-          }
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int ct = 0; ct < NC; ++ct) S[d][ct] = mfma4(y[r], z[ct][jt][r], S[d][ct]);
         }
       }
     }
+    lds_barrier();                                             // the tiles are free for the next chunk
   }
 
   float* s = STATE_ONLY ? p.seg + (bh * p.nseg + seg) * p.Da * p.Db : (p.s_out ? p.s_out + bh * p.Da * p.Db : nullptr);
@@ -495,30 +555,33 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
   }
 }
 
-template <typename T, int DA, int NC> hipError_t launch_sized(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
+template <typename T, int DA, int NC, bool VEC> hipError_t launch_sized(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
   constexpr int CT = 2;
   const dim3 grid((unsigned)((long)a.nseg * a.slices * a.H * a.B)), block(256);
   if (state_only) {
-    if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, true, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, false, true>), grid, block, 0, st, a);
+    if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, true, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, false, true>), grid, block, 0, st, a);
   } else {
-    if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, true, false>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, false, false>), grid, block, 0, st, a);
+    if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, true, false>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, false, false>), grid, block, 0, st, a);
   }
   return hipGetLastError();
 }
 
-template <typename T> hipError_t launch(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
+template <typename T, bool VEC> hipError_t launch_access(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
   if (a.Db <= 64) {
-    if (a.Da <= 32) return launch_sized<T, 32, 1>(a, rev, state_only, st);
-    if (a.Da <= 64) return launch_sized<T, 64, 1>(a, rev, state_only, st);
-    if (a.Da <= 128) return launch_sized<T, 128, 1>(a, rev, state_only, st);
-    return launch_sized<T, 256, 1>(a, rev, state_only, st);
+    if (a.Da <= 64) return launch_sized<T, 64, 1, VEC>(a, rev, state_only, st);
+    if (a.Da <= 128) return launch_sized<T, 128, 1, VEC>(a, rev, state_only, st);
+    return launch_sized<T, 256, 1, VEC>(a, rev, state_only, st);
   }
-  if (a.Da <= 32) return launch_sized<T, 32, 2>(a, rev, state_only, st);
-  if (a.Da <= 64) return launch_sized<T, 64, 2>(a, rev, state_only, st);
-  if (a.Da <= 128) return launch_sized<T, 128, 2>(a, rev, state_only, st);
-  return launch_sized<T, 256, 2>(a, rev, state_only, st);
+  if (a.Da <= 64) return launch_sized<T, 64, 2, VEC>(a, rev, state_only, st);
+  if (a.Da <= 128) return launch_sized<T, 128, 2, VEC>(a, rev, state_only, st);
+  return launch_sized<T, 256, 2, VEC>(a, rev, state_only, st);
+}
+
+template <typename T> hipError_t launch(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
+  const bool vec = a.Y.vec && a.Z.vec && (state_only || (a.X.vec && a.out_vec));
+  return vec ? launch_access<T, true>(a, rev, state_only, st) : launch_access<T, false>(a, rev, state_only, st);
 }
 
 }  // namespace ring_lin

@@ -951,7 +951,8 @@ static bool linattn_shape(const char* who, int type, int B, int T, int H, int G,
 static RingLinTensor rows_tensor(const void* p, const long long* strides, int dim, int type) {
   const int per = type == RINGATTR_F32 ? 4 : 8;
   RingLinTensor t = {p, (long)strides[0], (long)strides[1], (long)strides[2], false};
-  t.vec = dim % per == 0 && aligned16(p) && strides[0] % per == 0 && strides[1] % per == 0 && strides[2] % per == 0;
+  t.vec = dim % per == 0 && aligned16(p) && strides[0] % per == 0 && strides[1] % per == 0 && strides[2] % per == 0 &&
+          strides[1] >= 0 && strides[1] < (1ll << 22);
   return t;
 }
 
