@@ -27,14 +27,13 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 namespace ring_lin {
 
-// What is in memory as T is multiplied as C.  bf16 operands go to the matrix units as they are; what is computed on the way (weights,
-// decayed rows, the state) enters as the sum of two or three bf16 numbers, 16 or 24 bits, so that only the results are rounded to
-// bf16 and the state, which is kept in 32 bits, stays as exact as fp32 sums are.  fp32 and fp16 go to the fp32 matrix units: fp16
-// because the weights and the state can pass its range.
+// bf16 operands go to the matrix units as they are; what is computed on the way (weights, decayed rows, the state) enters as the sum of
+// two or three bf16 numbers, 16 or 24 bits, so that only the results are rounded to bf16 and the state, which is kept in 32 bits, stays
+// as exact as fp32 sums are.  fp32 and fp16 go to the fp32 matrix units: fp16 because the weights and the state can pass its range.
 template <typename T> struct Type;
-template <> struct Type<__bf16> { typedef __bf16 C; static constexpr int EPV = 8, PAD = 16; static constexpr bool BF = true; };
-template <> struct Type<float> { typedef float C; static constexpr int EPV = 4, PAD = 4; static constexpr bool BF = false; };
-template <> struct Type<_Float16> { typedef float C; static constexpr int EPV = 8, PAD = 4; static constexpr bool BF = false; };
+template <> struct Type<__bf16> { static constexpr bool BF = true; static constexpr unsigned EXPONENT = 0x7f80u; typedef bf16x4 V4; };
+template <> struct Type<float> { static constexpr bool BF = false; static constexpr unsigned EXPONENT = 0x7f800000u; typedef f32x4 V4; };
+template <> struct Type<_Float16> { static constexpr bool BF = false; static constexpr unsigned EXPONENT = 0x7c00u; typedef f16x4 V4; };
 
 __device__ __forceinline__ float power(float g2, int e) { return e == 0 ? 1.f : __builtin_amdgcn_exp2f(g2 * (float)e); }
 
@@ -44,134 +43,115 @@ __device__ __forceinline__ f32x4 widen(bf16x4 x) {
   return f32x4{__builtin_bit_cast(float, b[0] << 16), __builtin_bit_cast(float, b[0] & 0xffff0000u), __builtin_bit_cast(float, b[1] << 16),
                __builtin_bit_cast(float, b[1] & 0xffff0000u)};
 }
+__device__ __forceinline__ f32x4 widen(f16x4 x) { return __builtin_convertvector(x, f32x4); }
+__device__ __forceinline__ f32x4 widen(f32x4 x) { return x; }
 __device__ __forceinline__ bf16x4 narrow(f32x4 x) { return __builtin_convertvector(x, bf16x4); }
 __device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
-// Column of operand row m (0..15) of column tile ct of a wave: with two tiles, a lane's four values of both are eight neighbours.
-template <int NC> __device__ __forceinline__ int column(int ct, int m) {
-  return NC == 2 ? 8 * (m >> 2) + 4 * ct + (m & 3) : m;
-}
-
-// Rows of a tile, columns col0..col0+15 in the order of `column`: element e of lane (g, l) is row 4g + e, the lane's own column.
-template <int LD, int NC>
-__device__ __forceinline__ bf16x4 read_columns(const __bf16* tile, int row0, int col0, int ct, int g, int l) {
-  const __bf16* p = tile + (row0 + 4 * g + (l >> 2)) * LD + col0 + (NC == 2 ? 8 * (l & 3) + 4 * ct : 4 * (l & 3));
-  return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
-}
-template <int LD, int NC>
-__device__ __forceinline__ f32x4 read_columns(const float* tile, int row0, int col0, int ct, int g, int l) {
-  const float* p = tile + (row0 + 4 * g) * LD + col0 + column<NC>(ct, l);
-  return f32x4{p[0], p[LD], p[2 * LD], p[3 * LD]};
-}
-// Element e of lane (g, l): row row0 + l, column col0 + 4g + e.
-template <int LD> __device__ __forceinline__ bf16x4 read_rows(const __bf16* tile, int row0, int col0, int g, int l) {
-  return *reinterpret_cast<const bf16x4*>(tile + (row0 + l) * LD + col0 + 4 * g);
-}
-template <int LD> __device__ __forceinline__ f32x4 read_rows(const float* tile, int row0, int col0, int g, int l) {
-  return *reinterpret_cast<const f32x4*>(tile + (row0 + l) * LD + col0 + 4 * g);
-}
-
 __device__ __forceinline__ bool nonfinite(float x) { return (__builtin_bit_cast(unsigned, x) & 0x7f800000u) == 0x7f800000u; }
-template <typename T> __device__ constexpr unsigned exponent() { return sizeof(T) == 4 ? 0x7f800000u : (Type<T>::BF ? 0x7f80u : 0x7c00u); }
-template <typename T> __device__ __forceinline__ bool words_nonfinite(u32x4 w) {
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    constexpr unsigned E = exponent<T>();
-    bad |= (w[i] & E) == E;
-    if (sizeof(T) == 2) bad |= (w[i] & (E << 16)) == (E << 16);
-  }
-  return bad;
+
+// Column of operand row m (0..15) of column tile ct of a wave.  Two tiles of 16-bit values: a lane's four of each are eight neighbours.
+template <typename T, int NC> __device__ __forceinline__ int column(int ct, int m) {
+  return NC == 2 && sizeof(T) == 2 ? 8 * (m >> 2) + 4 * ct + (m & 3) : 16 * ct + m;
 }
 
-// One tile of ROWS x COLS values, global -> registers -> LDS.  Rows from `n` on and columns from `cols` on become zero on the way into
-// LDS; until then their place is taken by the last row and columns that there are, so that no load hangs on a branch (a value that is
-// merged behind one is waited for there).  VEC: 16-byte loads (RingLinTensor::vec).
-template <typename T, int ROWS, int COLS, int NT, bool VEC> struct Stage {
-  typedef typename Type<T>::C C;
-  static constexpr int EPV = Type<T>::EPV, UPR = COLS / EPV, UNITS = ROWS * UPR, NU = (UNITS + NT - 1) / NT, LD = COLS + Type<T>::PAD;
-  static constexpr int RS = NT / UPR;                          // rows from a thread's unit to its next; its columns stay
-  static_assert(NT % UPR == 0, "");
-  u32x4 r[NU];
+// A tile of ROWS x COLS values in LDS, rows one behind the other.  A row's 16-byte granules change places by an exclusive or with a
+// function of the row, such that what one instruction reads lies in all banks: 16 rows at one place (`rows`), 8 rows at two
+// neighbouring places by the transposing read of 16-bit values, 4 rows at four by single words (`columns`).
+template <typename T, int ROWS, int COLS> struct Tile16 {
+  static constexpr int EPV = 16 / sizeof(T), GPR = COLS / EPV, RB = COLS * sizeof(T), BYTES = ROWS * RB, NU = ROWS * GPR / 256;
+  static_assert(ROWS * GPR % 256 == 0 && 256 % GPR == 0, "");
+  typedef typename Type<T>::V4 V4;
 
-  // rows 0..last from base on, token stride st
-  __device__ __forceinline__ void load(const T* base, long st, int last, int cols, int tid) {
-    const int row = tid / UPR, c = (tid % UPR) * EPV;
-    if constexpr (VEC) {
-      const unsigned stb = (unsigned)st * (unsigned)sizeof(T), cb = (unsigned)(min(c, cols - EPV) * (int)sizeof(T));
+  static __device__ __forceinline__ int turn(int row) {
+    if (sizeof(T) == 4) return row & 15;
+    if (GPR >= 16) return ((row << 1) | ((row >> 3) & 1)) & 15;
+    const int k = (row >> 1) & 7;
+    return ((k << 1) | (k >> 2)) & 7;
+  }
+  // byte address of (row, col)
+  static __device__ __forceinline__ int at(int row, int col) {
+    return row * RB + (((col / EPV) ^ turn(row)) * 16) + (col % EPV) * (int)sizeof(T);
+  }
+
+  // Element e of lane (g, l): row 16 t + l, column 16 s + 4 g + e.  first(): the address at t = 0, s = 0, the others follow from it.
+  static __device__ __forceinline__ int rows_first(int g, int l) { return at(l, 4 * g); }
+  static __device__ __forceinline__ V4 rows(const char* tile, int first, int t, int s) {
+    return *reinterpret_cast<const V4*>(tile + (first ^ (s * 16 * (int)sizeof(T))) + t * 16 * RB);
+  }
+  // Element e of lane (g, l): row 16 t + 4 g + e, column 16 s + l (PAIR: the columns of `column` from 32 s on, tile ct).
+  template <bool PAIR> static __device__ __forceinline__ int columns_first(int g, int l, int r) {
+    if (sizeof(T) == 2) return PAIR ? at(4 * g + (l >> 2), 8 * (l & 3)) : at(4 * g + (l >> 2), 4 * (l & 3));
+    return at(4 * g + r, l);
+  }
+  template <bool PAIR> static __device__ __forceinline__ V4 columns(const char* tile, const int (&first)[4], int t, int s, int ct) {
+    const int x = PAIR ? (sizeof(T) == 2 ? (s * 64) | (ct * 8) : (2 * s + ct) * 64) : s * 16 * (int)sizeof(T);
+    if constexpr (sizeof(T) == 2) {
+      const char* p = tile + (first[0] ^ x) + t * 16 * RB;
+      return __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+    } else {
+      V4 v;
 #pragma unroll
-      for (int u = 0; u < NU; ++u)
-        r[u] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + (__umul24((unsigned)min(row + u * RS, last), stb) + cb));
+      for (int r = 0; r < 4; ++r) v[r] = *reinterpret_cast<const float*>(tile + (first[r] ^ x) + t * 16 * RB);
+      return v;
+    }
+  }
+};
+
+// Global memory -> LDS without registers: a wave's instruction fills 64 granules one behind the other, each lane from where it likes.
+// What is loaded is there behind a wait for vmcnt and a barrier (nobody else keeps count: the compiler does not see these loads).
+__device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
+// Fills a tile: rows 0..n-1 of `cols` values from base on, token stride st; what is not loaded is left as it is.
+template <typename T, int ROWS, int COLS, bool VEC> struct Filler {
+  typedef Tile16<T, ROWS, COLS> Tl;
+  static constexpr int EPV = Tl::EPV, GPR = Tl::GPR, NU = Tl::NU, RS = 256 / GPR;
+  unsigned off[NU];                                            // byte offsets of the thread's granules in a whole chunk
+  bool in;                                                     // all columns are there
+
+  __device__ __forceinline__ void init(long st, int cols, int tid) {
+    in = cols >= COLS;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int row = tid / GPR + u * RS, c = ((tid % GPR) ^ Tl::turn(row)) * EPV;
+      off[u] = (unsigned)row * (unsigned)st * (unsigned)sizeof(T) + (unsigned)c * (unsigned)sizeof(T);
+    }
+  }
+  __device__ __forceinline__ void fill(char* tile, const T* base, long st, int n, int cols, int tid) const {
+    if constexpr (VEC) {
+      const unsigned lds = __builtin_amdgcn_readfirstlane(lds_address(tile) + (tid >> 6) * 1024);
+      if (in && n == ROWS) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) load_to_lds(base, off[u], lds + u * 4096);
+      } else {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          const int row = tid / GPR + u * RS, c = ((tid % GPR) ^ Tl::turn(row)) * EPV;
+          if (row < n && c < cols) load_to_lds(base, off[u], lds + u * 4096);
+        }
+      }
     } else {
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        const T* p = base + (long)min(row + u * RS, last) * st;
-        if constexpr (sizeof(T) == 4) {
+        const int row = tid / GPR + u * RS, c = ((tid % GPR) ^ Tl::turn(row)) * EPV;
+        T v[EPV];
 #pragma unroll
-          for (int e = 0; e < EPV; ++e) r[u][e] = __builtin_bit_cast(unsigned, p[min(c + e, cols - 1)]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < EPV; e += 2)
-            r[u][e / 2] = __builtin_bit_cast(unsigned short, p[min(c + e, cols - 1)]) |
-                          (unsigned)__builtin_bit_cast(unsigned short, p[min(c + e + 1, cols - 1)]) << 16;
-        }
+        for (int e = 0; e < EPV; ++e) v[e] = row < n && c + e < cols ? base[(long)row * st + c + e] : (T)0.f;
+        if (row < n) *reinterpret_cast<u32x4*>(tile + (tid + u * 256) * 16) = *reinterpret_cast<const u32x4*>(v);
       }
     }
   }
-  __device__ __forceinline__ void mask(int n, int cols, int tid) {
-    const int row = tid / UPR, c = (tid % UPR) * EPV;
-    if (n >= ROWS && cols >= COLS) return;
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const bool in = row + u * RS < n;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (VEC) {
-          r[u][e] = in && c < cols ? r[u][e] : 0u;
-        } else if constexpr (sizeof(T) == 4) {
-          r[u][e] = in && c + e < cols ? r[u][e] : 0u;
-        } else {
-          r[u][e] &= (in && c + 2 * e < cols ? 0xffffu : 0u) | (in && c + 2 * e + 1 < cols ? 0xffff0000u : 0u);
-        }
-      }
-    }
-  }
-  __device__ __forceinline__ void store(C* tile, int tid) const {
-    const int row = tid / UPR, c = (tid % UPR) * EPV;
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      if (UNITS % NT != 0 && row + u * RS >= ROWS) continue;
-      C* p = tile + (row + u * RS) * LD + c;
-      if constexpr (sizeof(C) == sizeof(T)) {
-        *reinterpret_cast<u32x4*>(p) = r[u];
-      } else {
-        const f16x8 h = __builtin_bit_cast(f16x8, r[u]);
-        *reinterpret_cast<f32x4*>(p) = f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
-        *reinterpret_cast<f32x4*>(p + 4) = f32x4{(float)h[4], (float)h[5], (float)h[6], (float)h[7]};
-      }
-    }
-  }
-  __device__ __forceinline__ void clean() {                    // values that are not finite become zero
+  static __device__ __forceinline__ void clear(char* tile, int from, int tid) {
 #pragma unroll
     for (int u = 0; u < NU; ++u)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        constexpr unsigned E = exponent<T>();
-        if constexpr (sizeof(T) == 4) {
-          if ((r[u][e] & E) == E) r[u][e] = 0;
-        } else {
-          if ((r[u][e] & E) == E) r[u][e] &= 0xffff0000u;
-          if ((r[u][e] & (E << 16)) == (E << 16)) r[u][e] &= 0xffffu;
-        }
-      }
-  }
-  __device__ __forceinline__ bool bad() const {
-    bool b = false;
-#pragma unroll
-    for (int u = 0; u < NU; ++u) b |= words_nonfinite<T>(r[u]);
-    return b;
+      if (tid / GPR + u * RS >= from) *reinterpret_cast<u32x4*>(tile + (tid + u * 256) * 16) = u32x4{0, 0, 0, 0};
   }
 };
 
@@ -179,22 +159,25 @@ template <typename T> __device__ __forceinline__ const T* rows_of(const RingLinT
   return reinterpret_cast<const T*>(t.p) + (long)b * t.sb + (long)(h / share) * t.sh;
 }
 
-// A workgroup: one head of one sequence, WC = 16 NC NW columns of Z and of the state, one segment of the tokens.  Its waves share the
-// chunk's rows in LDS; each keeps 16 NC columns of the state in registers, where they are an operand as they lie: the matrix units put
-// rows 4g..4g+3 of column l into lane (g, l) and take them as contraction indices from there.  The weights are formed transposed
-// for the same reason, by every wave for itself (the kernel is bound by memory: a chunk of 128-wide bf16 rows moves in about four times what
-// its products take).
+template <int N> __device__ __forceinline__ void wait_and_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// A workgroup: one head of one sequence, WC = 64 NC columns of Z and of the state, one segment of the tokens.  Its waves share the
+// chunk's rows in LDS (two buffers: the next chunk's are on their way while one is worked on); each keeps 16 NC columns of the state
+// in registers, where they are an operand as they lie: the matrix units put rows 4g..4g+3 of column l into lane (g, l) and take them
+// as contraction indices from there.  The weights are formed transposed for the same reason, by every wave for itself.
 template <typename T, int DA, int NC, int CT, bool VEC, bool REV, bool STATE_ONLY>
 __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(RingLinArgs p) {
-  constexpr int NW = 4, NT = 64 * NW, WC = 16 * NC * NW, CH = 16 * CT, DT = DA / 16;
+  constexpr int WC = 64 * NC, CH = 16 * CT, DT = DA / 16;
   constexpr bool BF = Type<T>::BF;
-  typedef typename Type<T>::C C;
-  typedef Stage<T, CH, DA, NT, VEC> SA;
-  typedef Stage<T, CH, WC, NT, VEC> SZ;
-  __shared__ __align__(16) C ldsX[STATE_ONLY ? 8 : CH * SA::LD];
-  __shared__ __align__(16) C ldsY[CH * SA::LD];
-  __shared__ __align__(16) C ldsZ[CH * SZ::LD];
-  __shared__ int flag[2];
+  typedef typename Type<T>::V4 V4;
+  typedef Tile16<T, CH, DA> TA;
+  typedef Tile16<T, CH, WC> TZ;
+  typedef Filler<T, CH, DA, VEC> FA;
+  typedef Filler<T, CH, WC, VEC> FZ;
+  constexpr int XB = STATE_ONLY ? 0 : TA::BYTES, BUF = XB + TA::BYTES + TZ::BYTES;
+  __shared__ __align__(16) char lds[2 * BUF];
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 15, g = (tid >> 4) & 3;
   const int seg = blockIdx.x % p.nseg, slice = blockIdx.x / p.nseg % p.slices, head = blockIdx.x / (p.nseg * p.slices);
@@ -222,7 +205,7 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
       for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int a = 16 * d + 4 * g + r, c = cw + column<NC>(ct, l);
+          const int a = 16 * d + 4 * g + r, c = cw + column<T, NC>(ct, l);
           S[d][ct][r] = s && a < p.Da && c < cols ? s[(size_t)a * p.sa + (size_t)(c0 + c) * p.sb] : 0.f;
         }
   }
@@ -238,83 +221,25 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
     }
   int n_now = -1;
 
-  // O = inner S X^T, what the state in front gives, and P = Y X^T, the weights
-  auto from_state = [&](f32x4 (&O)[NC][CT], f32x4 (&P)[CT][CT]) {
-#pragma unroll
-    for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-      for (int it = 0; it < CT; ++it) O[ct][it] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < DT; s += 2) {
-      if constexpr (BF) {
-        bf16x8 x[CT];
-#pragma unroll
-        for (int it = 0; it < CT; ++it)
-          x[it] = join(read_rows<SA::LD>(ldsX, 16 * it, 16 * s, g, l), read_rows<SA::LD>(ldsX, 16 * it, 16 * s + 16, g, l));
-#pragma unroll
-          for (int jt = 0; jt < CT; ++jt) {
-            const bf16x8 y = join(read_rows<SA::LD>(ldsY, 16 * jt, 16 * s, g, l), read_rows<SA::LD>(ldsY, 16 * jt, 16 * s + 16, g, l));
-#pragma unroll
-            for (int it = 0; it < CT; ++it)
-              if (REV ? jt >= it : jt <= it) P[jt][it] = mfma16(y, x[it], P[jt][it]);
-          }
-#pragma unroll
-        for (int ct = 0; ct < NC; ++ct) {
-          const bf16x4 a0 = narrow(S[s][ct]), a1 = narrow(S[s + 1][ct]);
-          const bf16x8 hi = join(a0, a1), lo = join(narrow(S[s][ct] - widen(a0)), narrow(S[s + 1][ct] - widen(a1)));
-#pragma unroll
-          for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(hi, x[it], O[ct][it]);
-#pragma unroll
-          for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(lo, x[it], O[ct][it]);
-        }
-      } else {
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          f32x4 x[CT];
-#pragma unroll
-          for (int it = 0; it < CT; ++it) x[it] = read_rows<SA::LD>(ldsX, 16 * it, 16 * (s + q), g, l);
-#pragma unroll
-            for (int jt = 0; jt < CT; ++jt) {
-              const f32x4 y = read_rows<SA::LD>(ldsY, 16 * jt, 16 * (s + q), g, l);
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int it = 0; it < CT; ++it)
-                  if (REV ? jt >= it : jt <= it) P[jt][it] = mfma4(y[r], x[it][r], P[jt][it]);
-            }
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-              for (int it = 0; it < CT; ++it) O[ct][it] = mfma4(S[s + q][ct][r], x[it][r], O[ct][it]);
-        }
-      }
-    }
-#pragma unroll
-    for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-      for (int it = 0; it < CT; ++it) O[ct][it] *= inner[it];
-  };
   auto put = [&](const f32x4 (&O)[NC][CT], int t, int rows) {
-    const int c = cw + (NC == 2 ? 8 * g : 4 * g);
     const size_t at = ((size_t)b * T_ + t) * p.H + h, size = p.out_f32 || sizeof(T) == 4 ? 4 : sizeof(T);
     char* const base = (char*)p.out + (at * p.Db + c0) * size;
-    const unsigned step = (unsigned)(p.H * p.Db) * (unsigned)size, first = (unsigned)c * (unsigned)size;     // (VEC: within 24 bits)
+    const unsigned step = (unsigned)(p.H * p.Db) * (unsigned)size;                                   // (VEC: within 24 bits)
 #pragma unroll
     for (int it = 0; it < CT; ++it) {
-      const int row = 16 * it + l;
+      const int row = 16 * it + l, c = cw + column<T, NC>(0, 4 * g);
       if (row >= rows || c >= cols) continue;
-      char* const o = VEC ? base + (__umul24((unsigned)row, step) + first) : base + ((size_t)row * step + first);
+      char* const o = (VEC ? base + __umul24((unsigned)row, step) : base + (size_t)row * p.H * p.Db * size) + c * (int)size;
       if (p.out_f32 || sizeof(T) == 4) {
 #pragma unroll
         for (int ct = 0; ct < NC; ++ct) {
+          const int more = column<T, NC>(ct, 0);
           if (VEC) {
-            if (c + 4 * ct < cols) reinterpret_cast<f32x4*>(o)[ct] = O[ct][it];
+            if (c + more < cols) *reinterpret_cast<f32x4*>(o + 4 * more) = O[ct][it];
           } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (c + 4 * ct + r < cols) reinterpret_cast<float*>(o)[4 * ct + r] = O[ct][it][r];
+              if (c + more + r < cols) reinterpret_cast<float*>(o)[more + r] = O[ct][it][r];
           }
         }
       } else {
@@ -342,37 +267,48 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
     for (int c = full; c < nch; ++c) put(zero, t0 + c * CH, min(CH, t1 - t0 - c * CH));
   }
 
-  SA rx, ry;
-  SZ rz;
-  auto fetch = [&](int c) {
-    const int t = t0 + c * CH, last = min(CH, te - t) - 1;
-    if (!STATE_ONLY) rx.load(X + (long)t * p.X.st, p.X.st, last, p.Da, tid);
-    ry.load(Y + (long)t * p.Y.st, p.Y.st, last, p.Da, tid);
-    rz.load(Z + (long)t * p.Z.st, p.Z.st, last, cols, tid);
+  FA fx, fy;
+  FZ fz;
+  if (!STATE_ONLY) fx.init(p.X.st, p.Da, tid);
+  fy.init(p.Y.st, p.Da, tid);
+  fz.init(p.Z.st, cols, tid);
+  auto fetch = [&](int c, int buf) {
+    const int t = t0 + c * CH, n = min(CH, te - t);
+    char* const tile = lds + buf * BUF;
+    if (!STATE_ONLY) fx.fill(tile, X + (long)t * p.X.st, p.X.st, n, p.Da, tid);
+    fy.fill(tile + XB, Y + (long)t * p.Y.st, p.Y.st, n, p.Da, tid);
+    fz.fill(tile + XB + TA::BYTES, Z + (long)t * p.Z.st, p.Z.st, n, cols, tid);
   };
-  if (tid < 2) flag[tid] = 0;
-  __syncthreads();
-  if (full > 0) fetch(REV ? full - 1 : 0);
-  for (int i = 0; i < full; ++i) {
-    const int c = REV ? full - 1 - i : i, t = t0 + c * CH, n = min(CH, te - t);
-    if (!STATE_ONLY) {
-      rx.mask(n, p.Da, tid);
-      rx.store(ldsX, tid);
-    }
-    ry.mask(n, p.Da, tid);
-    ry.store(ldsY, tid);
-    rz.mask(n, cols, tid);
-    if (!STATE_ONLY) {
-      if (rz.bad()) {
-        rz.clean();
-        flag[i & 1] = 1;
+  int rows1 = TA::rows_first(g, l), cols1[4], cz1[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    cols1[r] = TA::template columns_first<false>(g, l, r);
+    cz1[r] = TZ::template columns_first<NC == 2>(g, l, r);
+  }
+  if (full > 0) {
+    if (VEC && (p.Da < DA || cols < WC)) {                     // columns that no load fills
+#pragma unroll
+      for (int buf = 0; buf < 2; ++buf) {
+        if (!STATE_ONLY) FA::clear(lds + buf * BUF, 0, tid);
+        FA::clear(lds + buf * BUF + XB, 0, tid);
+        FZ::clear(lds + buf * BUF + XB + TA::BYTES, 0, tid);
       }
-      if (tid == 0) flag[(i + 1) & 1] = 0;
+      lds_barrier();
     }
-    rz.store(ldsZ, tid);
-    lds_barrier();
-    fetch(i + 1 < full ? (REV ? c - 1 : c + 1) : c);           // (the last one's again: nothing reads it)
-    if (n != n_now) {                                          // (whole chunks, but for the last of a sequence)
+    fetch(REV ? full - 1 : 0, 0);
+  }
+  for (int i = 0; i < full; ++i) {
+    const int c = REV ? full - 1 - i : i, t = t0 + c * CH, n = min(CH, te - t), buf = i & 1;
+    char *const lx = lds + buf * BUF, *const ly = lx + XB, *const lz = ly + TA::BYTES;
+    wait_and_barrier<0>();
+    if (n < CH) {                                              // (the last chunk of a sequence)
+      if (!STATE_ONLY) FA::clear(lx, n, tid);
+      FA::clear(ly, n, tid);
+      FZ::clear(lz, n, tid);
+      lds_barrier();
+    }
+    if (i + 1 < full) fetch(REV ? c - 1 : c + 1, buf ^ 1);
+    if (n != n_now) {
       n_now = n;
       whole = power(g2, n);
 #pragma unroll
@@ -385,14 +321,98 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
         }
       }
     }
+    // The rows Z.  A value there that is infinite or NaN must not reach rows that do not see it, which the products within the tiles
+    // multiply by zero: it is taken out, and what it gives is added at the end, one by one.
+    V4 z[NC][CT];
+    bool bad = false;
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+      for (int jt = 0; jt < CT; ++jt) {
+        z[ct][jt] = TZ::template columns<NC == 2>(lz, cz1, jt, w, ct);
+        if (!STATE_ONLY) {
+          typedef unsigned words __attribute__((ext_vector_type(sizeof(T))));
+          const words q = __builtin_bit_cast(words, z[ct][jt]);
+#pragma unroll
+          for (int e = 0; e < (int)sizeof(T); ++e) {
+            constexpr unsigned E = Type<T>::EXPONENT;
+            bad |= (q[e] & E) == E;
+            if (sizeof(T) == 2) bad |= (q[e] & (E << 16)) == (E << 16);
+          }
+        }
+      }
+    if (!STATE_ONLY) bad = __any(bad);
+    if (!STATE_ONLY && bad)
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int jt = 0; jt < CT; ++jt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (nonfinite((float)z[ct][jt][e])) z[ct][jt][e] = (T)0.f;
+
+    f32x4 O[NC][CT];
     if constexpr (!STATE_ONLY) {
-      f32x4 O[NC][CT], P[CT][CT];                              // P: [tile of Y's rows][tile of X's rows]
+      f32x4 P[CT][CT];                                         // [tile of Y's rows][tile of X's rows]
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int it = 0; it < CT; ++it) O[ct][it] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int jt = 0; jt < CT; ++jt)
 #pragma unroll
         for (int it = 0; it < CT; ++it) P[jt][it] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const bool bad = flag[i & 1] != 0;
-      from_state(O, P);
+      // O = S X^T, what the state in front gives, and P = Y X^T, the weights
+#pragma unroll
+      for (int s = 0; s < DT; s += 2) {
+        if constexpr (BF) {
+          bf16x8 x[CT];
+#pragma unroll
+          for (int it = 0; it < CT; ++it) x[it] = join(TA::rows(lx, rows1, it, s), TA::rows(lx, rows1, it, s + 1));
+#pragma unroll
+          for (int jt = 0; jt < CT; ++jt) {
+            const bf16x8 y = join(TA::rows(ly, rows1, jt, s), TA::rows(ly, rows1, jt, s + 1));
+#pragma unroll
+            for (int it = 0; it < CT; ++it)
+              if (REV ? jt >= it : jt <= it) P[jt][it] = mfma16(y, x[it], P[jt][it]);
+          }
+#pragma unroll
+          for (int ct = 0; ct < NC; ++ct) {
+            const bf16x4 a0 = narrow(S[s][ct]), a1 = narrow(S[s + 1][ct]);
+            const bf16x8 hi = join(a0, a1), lo = join(narrow(S[s][ct] - widen(a0)), narrow(S[s + 1][ct] - widen(a1)));
+#pragma unroll
+            for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(hi, x[it], O[ct][it]);
+#pragma unroll
+            for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(lo, x[it], O[ct][it]);
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            f32x4 x[CT];
+#pragma unroll
+            for (int it = 0; it < CT; ++it) x[it] = widen(TA::rows(lx, rows1, it, s + q));
+#pragma unroll
+            for (int jt = 0; jt < CT; ++jt) {
+              const f32x4 y = widen(TA::rows(ly, rows1, jt, s + q));
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int it = 0; it < CT; ++it)
+                  if (REV ? jt >= it : jt <= it) P[jt][it] = mfma4(y[r], x[it][r], P[jt][it]);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+                for (int it = 0; it < CT; ++it) O[ct][it] = mfma4(S[s + q][ct][r], x[it][r], O[ct][it]);
+          }
+        }
+      }
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int it = 0; it < CT; ++it) O[ct][it] *= inner[it];
       // what is not to be seen is left out, not multiplied by zero: it may be anything
 #pragma unroll
       for (int jt = 0; jt < CT; ++jt)
@@ -406,138 +426,131 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
             }
       if constexpr (BF) {
 #pragma unroll
-        for (int jp = 0; jp < CT; jp += 2) {
-          bf16x8 z[NC];
-#pragma unroll
-          for (int ct = 0; ct < NC; ++ct)
-            z[ct] = join(read_columns<SZ::LD, NC>(ldsZ, 16 * jp, cw, ct, g, l), read_columns<SZ::LD, NC>(ldsZ, 16 * jp + 16, cw, ct, g, l));
+        for (int jp = 0; jp < CT; jp += 2)
 #pragma unroll
           for (int it = 0; it < CT; ++it)
             if (REV ? jp + 1 >= it : jp <= it) {
               const bf16x4 a0 = narrow(P[jp][it]), a1 = narrow(P[jp + 1][it]);
               const bf16x8 hi = join(a0, a1), lo = join(narrow(P[jp][it] - widen(a0)), narrow(P[jp + 1][it] - widen(a1)));
 #pragma unroll
-              for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma16(z[ct], hi, O[ct][it]);
+              for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma16(join(z[ct][jp], z[ct][jp + 1]), hi, O[ct][it]);
 #pragma unroll
-              for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma16(z[ct], lo, O[ct][it]);
+              for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma16(join(z[ct][jp], z[ct][jp + 1]), lo, O[ct][it]);
             }
-        }
       } else {
 #pragma unroll
         for (int jt = 0; jt < CT; ++jt) {
-          f32x4 z[NC];
+          f32x4 v[NC];
 #pragma unroll
-          for (int ct = 0; ct < NC; ++ct) z[ct] = read_columns<SZ::LD, NC>(ldsZ, 16 * jt, cw, ct, g, l);
+          for (int ct = 0; ct < NC; ++ct) v[ct] = widen(z[ct][jt]);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int it = 0; it < CT; ++it)
               if (REV ? jt >= it : jt <= it)
 #pragma unroll
-                for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma4(z[ct][r], P[jt][it][r], O[ct][it]);
+                for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma4(v[ct][r], P[jt][it][r], O[ct][it]);
         }
       }
-      // A value of Z that is infinite or NaN must not reach rows that do not see it, which the products within the tiles multiply by
-      // zero: such values are zero in LDS and what they give is added here, one by one.
+    }
+    // the state behind the chunk
+    if constexpr (BF) {
+      bf16x8 part[NC][CT / 2][3];
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int jp = 0; jp < CT; jp += 2) {
+          bf16x4 k[2][3];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            f32x4 v = widen(z[ct][jp + q]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] *= outer[jp + q][r];
+#pragma unroll
+            for (int m = 0; m < 3; ++m) {
+              k[q][m] = narrow(v);
+              v -= widen(k[q][m]);
+            }
+          }
+#pragma unroll
+          for (int m = 0; m < 3; ++m) part[ct][jp / 2][m] = join(k[0][m], k[1][m]);
+        }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+#pragma unroll
+        for (int ct = 0; ct < NC; ++ct) S[d][ct] *= whole;
+#pragma unroll
+        for (int jp = 0; jp < CT; jp += 2) {
+          const bf16x8 y = join(TA::template columns<false>(ly, cols1, jp, d, 0), TA::template columns<false>(ly, cols1, jp + 1, d, 0));
+#pragma unroll
+          for (int m = 0; m < 3; ++m)
+#pragma unroll
+            for (int ct = 0; ct < NC; ++ct) S[d][ct] = mfma16(y, part[ct][jp / 2][m], S[d][ct]);
+        }
+      }
+    } else {
+      f32x4 v[NC][CT];
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int jt = 0; jt < CT; ++jt) {
+          v[ct][jt] = widen(z[ct][jt]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[ct][jt][r] *= outer[jt][r];
+        }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+#pragma unroll
+        for (int ct = 0; ct < NC; ++ct) S[d][ct] *= whole;
+#pragma unroll
+        for (int jt = 0; jt < CT; ++jt) {
+          const f32x4 y = widen(TA::template columns<false>(ly, cols1, jt, d, 0));
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int ct = 0; ct < NC; ++ct) S[d][ct] = mfma4(y[r], v[ct][jt][r], S[d][ct]);
+        }
+      }
+    }
+    if constexpr (!STATE_ONLY) {
       if (bad)
         for (int j = 0; j < n; ++j) {
-          float z[NC][4], zs[NC];                              // of the lane's columns of O, of its columns of S
-          const T* row = Z + (long)(t + j) * p.Z.st;
+          float zo[NC][4], zs[NC];                             // row j in the lane's columns of O, of S
           bool any = false;
 #pragma unroll
           for (int ct = 0; ct < NC; ++ct) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int col = cw + column<NC>(ct, 4 * g + r);
-              z[ct][r] = col < cols ? (float)row[col] : 0.f;
-            }
-            const int col = cw + column<NC>(ct, l);
-            zs[ct] = col < cols ? (float)row[col] : 0.f;
+            for (int r = 0; r < 4; ++r) zo[ct][r] = (float)*reinterpret_cast<const T*>(lz + TZ::at(j, cw + column<T, NC>(ct, 4 * g + r)));
+            zs[ct] = (float)*reinterpret_cast<const T*>(lz + TZ::at(j, cw + column<T, NC>(ct, l)));
             any |= nonfinite(zs[ct]);
           }
           if (!__any(any)) continue;
 #pragma unroll
           for (int it = 0; it < CT; ++it) {
-            const int i = 16 * it + l, e = REV ? j - i : i - j;
+            const int row = 16 * it + l, e = REV ? j - row : row - j;
             float dot = 0.f;
-            for (int a = 0; a < DA; ++a) dot = fmaf((float)ldsX[i * SA::LD + a], (float)ldsY[j * SA::LD + a], dot);
+            for (int a = 0; a < DA; ++a)
+              dot = fmaf((float)*reinterpret_cast<const T*>(lx + TA::at(row, a)), (float)*reinterpret_cast<const T*>(ly + TA::at(j, a)), dot);
             dot *= e < 0 ? 0.f : p.intra * power(g2, e);
 #pragma unroll
             for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
               for (int r = 0; r < 4; ++r)
-                if (e >= 0 && i < n && nonfinite(z[ct][r])) O[ct][it][r] += dot * z[ct][r];
+                if (e >= 0 && row < n && nonfinite(zo[ct][r])) O[ct][it][r] += dot * zo[ct][r];
           }
+          const float f = p.update * power(g2, REV ? j + 1 : n - 1 - j);
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 4; ++r) {
+              const float y = f * (float)*reinterpret_cast<const T*>(ly + TA::at(j, 16 * d + 4 * g + r));
 #pragma unroll
               for (int ct = 0; ct < NC; ++ct)
-                if (nonfinite(zs[ct])) S[d][ct][r] = fmaf((float)ldsY[j * SA::LD + 16 * d + 4 * g + r], zs[ct], S[d][ct][r]);
+                if (nonfinite(zs[ct])) S[d][ct][r] = fmaf(y, zs[ct], S[d][ct][r]);
+            }
         }
       put(O, t, min(CH, t1 - t));
     }
-    // the state behind the chunk
-    if constexpr (BF) {
-      bf16x8 z[NC][CT / 2][3];
-#pragma unroll
-      for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-        for (int jp = 0; jp < CT; jp += 2) {
-          bf16x4 part[2][3];
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            f32x4 v = widen(read_columns<SZ::LD, NC>(ldsZ, 16 * (jp + q), cw, ct, g, l));
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] *= outer[jp + q][r];
-#pragma unroll
-            for (int k = 0; k < 3; ++k) {
-              part[q][k] = narrow(v);
-              v -= widen(part[q][k]);
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < 3; ++k) z[ct][jp / 2][k] = join(part[0][k], part[1][k]);
-        }
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-#pragma unroll
-        for (int ct = 0; ct < NC; ++ct) S[d][ct] *= whole;
-#pragma unroll
-        for (int jp = 0; jp < CT; jp += 2) {
-          const bf16x8 y = join(read_columns<SA::LD, 1>(ldsY, 16 * jp, 16 * d, 0, g, l), read_columns<SA::LD, 1>(ldsY, 16 * jp + 16, 16 * d, 0, g, l));
-#pragma unroll
-          for (int k = 0; k < 3; ++k)
-#pragma unroll
-            for (int ct = 0; ct < NC; ++ct) S[d][ct] = mfma16(y, z[ct][jp / 2][k], S[d][ct]);
-        }
-      }
-    } else {
-      f32x4 z[NC][CT];
-#pragma unroll
-      for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-        for (int jt = 0; jt < CT; ++jt) {
-          z[ct][jt] = read_columns<SZ::LD, NC>(ldsZ, 16 * jt, cw, ct, g, l);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) z[ct][jt][r] *= outer[jt][r];
-        }
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-#pragma unroll
-        for (int ct = 0; ct < NC; ++ct) S[d][ct] *= whole;
-#pragma unroll
-        for (int jt = 0; jt < CT; ++jt) {
-          const f32x4 y = read_columns<SA::LD, 1>(ldsY, 16 * jt, 16 * d, 0, g, l);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int ct = 0; ct < NC; ++ct) S[d][ct] = mfma4(y[r], z[ct][jt][r], S[d][ct]);
-        }
-      }
-    }
-    lds_barrier();                                             // the tiles are free for the next chunk
   }
 
   float* s = STATE_ONLY ? p.seg + (bh * p.nseg + seg) * p.Da * p.Db : (p.s_out ? p.s_out + bh * p.Da * p.Db : nullptr);
@@ -549,14 +562,14 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
       for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int a = 16 * d + 4 * g + r, c = cw + column<NC>(ct, l);
+          const int a = 16 * d + 4 * g + r, c = cw + column<T, NC>(ct, l);
           if (a < p.Da && c < cols) s[(size_t)a * p.sa + (size_t)(c0 + c) * p.sb] = S[d][ct][r];
         }
   }
 }
 
 template <typename T, int DA, int NC, bool VEC> hipError_t launch_sized(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
-  constexpr int CT = 2;
+  constexpr int CT = sizeof(T) == 4 ? 1 : 2;
   const dim3 grid((unsigned)((long)a.nseg * a.slices * a.H * a.B)), block(256);
   if (state_only) {
     if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, true, true>), grid, block, 0, st, a);
