@@ -31,9 +31,9 @@ namespace ring_lin {
 // two or three bf16 numbers, 16 or 24 bits, so that only the results are rounded to bf16 and the state, which is kept in 32 bits, stays
 // as exact as fp32 sums are.  fp32 and fp16 go to the fp32 matrix units: fp16 because the weights and the state can pass its range.
 template <typename T> struct Type;
-template <> struct Type<__bf16> { static constexpr bool BF = true; static constexpr unsigned EXPONENT = 0x7f80u; typedef bf16x4 V4; };
-template <> struct Type<float> { static constexpr bool BF = false; static constexpr unsigned EXPONENT = 0x7f800000u; typedef f32x4 V4; };
-template <> struct Type<_Float16> { static constexpr bool BF = false; static constexpr unsigned EXPONENT = 0x7c00u; typedef f16x4 V4; };
+template <> struct Type<__bf16> { static constexpr bool BF = true; static constexpr unsigned EXPONENT = 0x7f80u; typedef bf16x4 V4; typedef unsigned short Bits; };
+template <> struct Type<float> { static constexpr bool BF = false; static constexpr unsigned EXPONENT = 0x7f800000u; typedef f32x4 V4; typedef unsigned Bits; };
+template <> struct Type<_Float16> { static constexpr bool BF = false; static constexpr unsigned EXPONENT = 0x7c00u; typedef f16x4 V4; typedef unsigned short Bits; };
 
 __device__ __forceinline__ float power(float g2, int e) { return e == 0 ? 1.f : __builtin_amdgcn_exp2f(g2 * (float)e); }
 
@@ -52,9 +52,24 @@ __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __bui
 
 __device__ __forceinline__ bool nonfinite(float x) { return (__builtin_bit_cast(unsigned, x) & 0x7f800000u) == 0x7f800000u; }
 
-// Column of operand row m (0..15) of column tile ct of a wave.  Two tiles of 16-bit values: a lane's four of each are eight neighbours.
-template <typename T, int NC> __device__ __forceinline__ int column(int ct, int m) {
-  return NC == 2 && sizeof(T) == 2 ? 8 * (m >> 2) + 4 * ct + (m & 3) : 16 * ct + m;
+// The largest magnitude of a number of values, by their bits
+template <typename T> struct Magnitude {
+  typedef typename Type<T>::Bits bits __attribute__((ext_vector_type(2)));
+  bits most = {0, 0};
+  __device__ __forceinline__ void add(typename Type<T>::V4 x) {
+    struct Two { bits b[2]; };
+    const Two two = __builtin_bit_cast(Two, x);
+    constexpr typename Type<T>::Bits M = (typename Type<T>::Bits)~((typename Type<T>::Bits)1 << (8 * sizeof(T) - 1));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) most = __builtin_elementwise_max(most, two.b[i] & M);
+  }
+  __device__ __forceinline__ bool nonfinite() const { return most[0] >= Type<T>::EXPONENT || most[1] >= Type<T>::EXPONENT; }
+};
+
+// Place of operand row m (0..15) of tile i among tiles of 16.  Two tiles of 16-bit values go together: a lane's four of each are eight
+// neighbours, 16 bytes of one read or store.
+template <typename T, bool PAIR> __device__ __forceinline__ int place(int i, int m) {
+  return PAIR && sizeof(T) == 2 ? 32 * (i >> 1) + 8 * (m >> 2) + 4 * (i & 1) + (m & 3) : 16 * i + m;
 }
 
 // A tile of ROWS x COLS values in LDS, rows one behind the other.  A row's 16-byte granules change places by an exclusive or with a
@@ -76,18 +91,20 @@ template <typename T, int ROWS, int COLS> struct Tile16 {
     return row * RB + (((col / EPV) ^ turn(row)) * 16) + (col % EPV) * (int)sizeof(T);
   }
 
-  // Element e of lane (g, l): row 16 t + l, column 16 s + 4 g + e.  first(): the address at t = 0, s = 0, the others follow from it.
-  static __device__ __forceinline__ int rows_first(int g, int l) { return at(l, 4 * g); }
-  static __device__ __forceinline__ V4 rows(const char* tile, int first, int t, int s) {
-    return *reinterpret_cast<const V4*>(tile + (first ^ (s * 16 * (int)sizeof(T))) + t * 16 * RB);
+  // Lane (g, l): row 16 t + l, the EPV columns from 4 EPV s + EPV g on.  first: the address at t = 0, s = 0, from which the others
+  // follow.
+  typedef T V16 __attribute__((ext_vector_type(16 / sizeof(T))));
+  static __device__ __forceinline__ int rows_first(int g, int l) { return at(l, EPV * g); }
+  static __device__ __forceinline__ V16 rows(const char* tile, int first, int t, int s) {
+    return *reinterpret_cast<const V16*>(tile + (first ^ (s * 64)) + t * 16 * RB);
   }
-  // Element e of lane (g, l): row 16 t + 4 g + e, column 16 s + l (PAIR: the columns of `column` from 32 s on, tile ct).
+  // Element e of lane (g, l): row 16 t + 4 g + e, column place(s, l).
   template <bool PAIR> static __device__ __forceinline__ int columns_first(int g, int l, int r) {
     if (sizeof(T) == 2) return PAIR ? at(4 * g + (l >> 2), 8 * (l & 3)) : at(4 * g + (l >> 2), 4 * (l & 3));
     return at(4 * g + r, l);
   }
-  template <bool PAIR> static __device__ __forceinline__ V4 columns(const char* tile, const int (&first)[4], int t, int s, int ct) {
-    const int x = PAIR ? (sizeof(T) == 2 ? (s * 64) | (ct * 8) : (2 * s + ct) * 64) : s * 16 * (int)sizeof(T);
+  template <bool PAIR> static __device__ __forceinline__ V4 columns(const char* tile, const int (&first)[4], int t, int s) {
+    const int x = PAIR && sizeof(T) == 2 ? ((s >> 1) * 64) | ((s & 1) * 8) : s * 16 * (int)sizeof(T);
     if constexpr (sizeof(T) == 2) {
       const char* p = tile + (first[0] ^ x) + t * 16 * RB;
       return __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
@@ -114,28 +131,22 @@ template <typename T, int ROWS, int COLS, bool VEC> struct Filler {
   typedef Tile16<T, ROWS, COLS> Tl;
   static constexpr int EPV = Tl::EPV, GPR = Tl::GPR, NU = Tl::NU, RS = 256 / GPR;
   unsigned off[NU];                                            // byte offsets of the thread's granules in a whole chunk
-  bool in;                                                     // all columns are there
 
-  __device__ __forceinline__ void init(long st, int cols, int tid) {
-    in = cols >= COLS;
+  __device__ __forceinline__ void init(long st, int tid) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int row = tid / GPR + u * RS, c = ((tid % GPR) ^ Tl::turn(row)) * EPV;
       off[u] = (unsigned)row * (unsigned)st * (unsigned)sizeof(T) + (unsigned)c * (unsigned)sizeof(T);
     }
   }
-  __device__ __forceinline__ void fill(char* tile, const T* base, long st, int n, int cols, int tid) const {
+  // WHOLE: all rows and columns are there
+  template <bool WHOLE> __device__ __forceinline__ void fill(char* tile, const T* base, long st, int n, int cols, int tid) const {
     if constexpr (VEC) {
       const unsigned lds = __builtin_amdgcn_readfirstlane(lds_address(tile) + (tid >> 6) * 1024);
-      if (in && n == ROWS) {
 #pragma unroll
-        for (int u = 0; u < NU; ++u) load_to_lds(base, off[u], lds + u * 4096);
-      } else {
-#pragma unroll
-        for (int u = 0; u < NU; ++u) {
-          const int row = tid / GPR + u * RS, c = ((tid % GPR) ^ Tl::turn(row)) * EPV;
-          if (row < n && c < cols) load_to_lds(base, off[u], lds + u * 4096);
-        }
+      for (int u = 0; u < NU; ++u) {
+        const int row = tid / GPR + u * RS, c = ((tid % GPR) ^ Tl::turn(row)) * EPV;
+        if (WHOLE || (row < n && c < cols)) load_to_lds(base, off[u], lds + u * 4096);
       }
     } else {
 #pragma unroll
@@ -205,7 +216,7 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
       for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int a = 16 * d + 4 * g + r, c = cw + column<T, NC>(ct, l);
+          const int a = place<T, true>(d, 4 * g + r), c = cw + place<T, NC == 2>(ct, l);
           S[d][ct][r] = s && a < p.Da && c < cols ? s[(size_t)a * p.sa + (size_t)(c0 + c) * p.sb] : 0.f;
         }
   }
@@ -227,13 +238,13 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
     const unsigned step = (unsigned)(p.H * p.Db) * (unsigned)size;                                   // (VEC: within 24 bits)
 #pragma unroll
     for (int it = 0; it < CT; ++it) {
-      const int row = 16 * it + l, c = cw + column<T, NC>(0, 4 * g);
+      const int row = 16 * it + l, c = cw + place<T, NC == 2>(0, 4 * g);
       if (row >= rows || c >= cols) continue;
       char* const o = (VEC ? base + __umul24((unsigned)row, step) : base + (size_t)row * p.H * p.Db * size) + c * (int)size;
       if (p.out_f32 || sizeof(T) == 4) {
 #pragma unroll
         for (int ct = 0; ct < NC; ++ct) {
-          const int more = column<T, NC>(ct, 0);
+          const int more = place<T, NC == 2>(ct, 0);
           if (VEC) {
             if (c + more < cols) *reinterpret_cast<f32x4*>(o + 4 * more) = O[ct][it];
           } else {
@@ -269,24 +280,32 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
 
   FA fx, fy;
   FZ fz;
-  if (!STATE_ONLY) fx.init(p.X.st, p.Da, tid);
-  fy.init(p.Y.st, p.Da, tid);
-  fz.init(p.Z.st, cols, tid);
+  if (!STATE_ONLY) fx.init(p.X.st, tid);
+  fy.init(p.Y.st, tid);
+  fz.init(p.Z.st, tid);
+  const bool wide = p.Da == DA && cols >= WC;                  // (no columns to leave out)
   auto fetch = [&](int c, int buf) {
     const int t = t0 + c * CH, n = min(CH, te - t);
     char* const tile = lds + buf * BUF;
-    if (!STATE_ONLY) fx.fill(tile, X + (long)t * p.X.st, p.X.st, n, p.Da, tid);
-    fy.fill(tile + XB, Y + (long)t * p.Y.st, p.Y.st, n, p.Da, tid);
-    fz.fill(tile + XB + TA::BYTES, Z + (long)t * p.Z.st, p.Z.st, n, cols, tid);
+    const T *x = STATE_ONLY ? nullptr : X + (long)t * p.X.st, *y = Y + (long)t * p.Y.st, *zz = Z + (long)t * p.Z.st;
+    if (VEC && wide && n == CH) {
+      if (!STATE_ONLY) fx.template fill<true>(tile, x, p.X.st, n, p.Da, tid);
+      fy.template fill<true>(tile + XB, y, p.Y.st, n, p.Da, tid);
+      fz.template fill<true>(tile + XB + TA::BYTES, zz, p.Z.st, n, cols, tid);
+    } else {
+      if (!STATE_ONLY) fx.template fill<false>(tile, x, p.X.st, n, p.Da, tid);
+      fy.template fill<false>(tile + XB, y, p.Y.st, n, p.Da, tid);
+      fz.template fill<false>(tile + XB + TA::BYTES, zz, p.Z.st, n, cols, tid);
+    }
   };
   int rows1 = TA::rows_first(g, l), cols1[4], cz1[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    cols1[r] = TA::template columns_first<false>(g, l, r);
+    cols1[r] = TA::template columns_first<true>(g, l, r);
     cz1[r] = TZ::template columns_first<NC == 2>(g, l, r);
   }
   if (full > 0) {
-    if (VEC && (p.Da < DA || cols < WC)) {                     // columns that no load fills
+    if (VEC && !wide) {                                        // columns that no load fills
 #pragma unroll
       for (int buf = 0; buf < 2; ++buf) {
         if (!STATE_ONLY) FA::clear(lds + buf * BUF, 0, tid);
@@ -297,10 +316,13 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
     }
     fetch(REV ? full - 1 : 0, 0);
   }
+  bool stored = false;
   for (int i = 0; i < full; ++i) {
     const int c = REV ? full - 1 - i : i, t = t0 + c * CH, n = min(CH, te - t), buf = i & 1;
     char *const lx = lds + buf * BUF, *const ly = lx + XB, *const lz = ly + TA::BYTES;
-    wait_and_barrier<0>();
+    // the chunk's rows are there; the outputs of the one before, stored behind the loads, need not be (a store for each of its tiles)
+    if (VEC && !STATE_ONLY && stored) wait_and_barrier<CT>();
+    else wait_and_barrier<0>();
     if (n < CH) {                                              // (the last chunk of a sequence)
       if (!STATE_ONLY) FA::clear(lx, n, tid);
       FA::clear(ly, n, tid);
@@ -329,19 +351,16 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
     for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
       for (int jt = 0; jt < CT; ++jt) {
-        z[ct][jt] = TZ::template columns<NC == 2>(lz, cz1, jt, w, ct);
-        if (!STATE_ONLY) {
-          typedef unsigned words __attribute__((ext_vector_type(sizeof(T))));
-          const words q = __builtin_bit_cast(words, z[ct][jt]);
-#pragma unroll
-          for (int e = 0; e < (int)sizeof(T); ++e) {
-            constexpr unsigned E = Type<T>::EXPONENT;
-            bad |= (q[e] & E) == E;
-            if (sizeof(T) == 2) bad |= (q[e] & (E << 16)) == (E << 16);
-          }
-        }
+        z[ct][jt] = TZ::template columns<NC == 2>(lz, cz1, jt, NC * w + ct);
       }
-    if (!STATE_ONLY) bad = __any(bad);
+    if (!STATE_ONLY) {
+      Magnitude<T> most;
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int jt = 0; jt < CT; ++jt) most.add(z[ct][jt]);
+      bad = __any(most.nonfinite());
+    }
     if (!STATE_ONLY && bad)
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct)
@@ -362,51 +381,57 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
       for (int jt = 0; jt < CT; ++jt)
 #pragma unroll
         for (int it = 0; it < CT; ++it) P[jt][it] = f32x4{0.f, 0.f, 0.f, 0.f};
-      // O = S X^T, what the state in front gives, and P = Y X^T, the weights
+      // O = S X^T, what the state in front gives, and P = Y X^T, the weights; rows are read a step ahead
+      constexpr int STEPS = DA / (64 / (int)sizeof(T)), TPS = DT / STEPS;      // steps of 64 bytes a row, tiles of the state in each
+      typename TA::V16 xr[2][CT], yr[2][CT];
+      auto read = [&](int s) {
 #pragma unroll
-      for (int s = 0; s < DT; s += 2) {
+        for (int it = 0; it < CT; ++it) {
+          xr[s & 1][it] = TA::rows(lx, rows1, it, s);
+          yr[s & 1][it] = TA::rows(ly, rows1, it, s);
+        }
+      };
+      read(0);
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        if (s + 1 < STEPS) read(s + 1);
+        __builtin_amdgcn_sched_barrier(0);
         if constexpr (BF) {
-          bf16x8 x[CT];
 #pragma unroll
-          for (int it = 0; it < CT; ++it) x[it] = join(TA::rows(lx, rows1, it, s), TA::rows(lx, rows1, it, s + 1));
-#pragma unroll
-          for (int jt = 0; jt < CT; ++jt) {
-            const bf16x8 y = join(TA::rows(ly, rows1, jt, s), TA::rows(ly, rows1, jt, s + 1));
+          for (int jt = 0; jt < CT; ++jt)
 #pragma unroll
             for (int it = 0; it < CT; ++it)
-              if (REV ? jt >= it : jt <= it) P[jt][it] = mfma16(y, x[it], P[jt][it]);
-          }
+              if (REV ? jt >= it : jt <= it) P[jt][it] = mfma16(yr[s & 1][jt], xr[s & 1][it], P[jt][it]);
 #pragma unroll
           for (int ct = 0; ct < NC; ++ct) {
-            const bf16x4 a0 = narrow(S[s][ct]), a1 = narrow(S[s + 1][ct]);
-            const bf16x8 hi = join(a0, a1), lo = join(narrow(S[s][ct] - widen(a0)), narrow(S[s + 1][ct] - widen(a1)));
+            const bf16x4 a0 = narrow(S[2 * s][ct]), a1 = narrow(S[2 * s + 1][ct]);
+            const bf16x8 hi = join(a0, a1), lo = join(narrow(S[2 * s][ct] - widen(a0)), narrow(S[2 * s + 1][ct] - widen(a1)));
 #pragma unroll
-            for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(hi, x[it], O[ct][it]);
+            for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(hi, xr[s & 1][it], O[ct][it]);
 #pragma unroll
-            for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(lo, x[it], O[ct][it]);
+            for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(lo, xr[s & 1][it], O[ct][it]);
           }
         } else {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            f32x4 x[CT];
+          for (int q = 0; q < TPS; ++q)
 #pragma unroll
-            for (int it = 0; it < CT; ++it) x[it] = widen(TA::rows(lx, rows1, it, s + q));
+            for (int r = 0; r < 4; ++r) {
+              float x[CT], y[CT];
 #pragma unroll
-            for (int jt = 0; jt < CT; ++jt) {
-              const f32x4 y = widen(TA::rows(ly, rows1, jt, s + q));
+              for (int it = 0; it < CT; ++it) {
+                x[it] = (float)xr[s & 1][it][4 * q + r];
+                y[it] = (float)yr[s & 1][it][4 * q + r];
+              }
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
+              for (int it = 0; it < CT; ++it)
 #pragma unroll
-                for (int it = 0; it < CT; ++it)
-                  if (REV ? jt >= it : jt <= it) P[jt][it] = mfma4(y[r], x[it][r], P[jt][it]);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
+                for (int jt = 0; jt < CT; ++jt)
+                  if (REV ? jt >= it : jt <= it) P[jt][it] = mfma4(y[jt], x[it], P[jt][it]);
 #pragma unroll
               for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
-                for (int it = 0; it < CT; ++it) O[ct][it] = mfma4(S[s + q][ct][r], x[it][r], O[ct][it]);
-          }
+                for (int it = 0; it < CT; ++it) O[ct][it] = mfma4(S[TPS * s + q][ct][r], x[it], O[ct][it]);
+            }
         }
       }
 #pragma unroll
@@ -453,7 +478,15 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
         }
       }
     }
-    // the state behind the chunk
+    // the state behind the chunk; Y's columns are read AHEAD tiles ahead
+    constexpr int AHEAD = 2;
+    V4 yc[AHEAD + 1][CT];
+    auto turned = [&](int d) {
+#pragma unroll
+      for (int jt = 0; jt < CT; ++jt) yc[d % (AHEAD + 1)][jt] = TA::template columns<true>(ly, cols1, jt, d);
+    };
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) turned(d);
     if constexpr (BF) {
       bf16x8 part[NC][CT / 2][3];
 #pragma unroll
@@ -479,14 +512,15 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
       for (int d = 0; d < DT; ++d) {
 #pragma unroll
         for (int ct = 0; ct < NC; ++ct) S[d][ct] *= whole;
+        if (d + AHEAD < DT) turned(d + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int jp = 0; jp < CT; jp += 2) {
-          const bf16x8 y = join(TA::template columns<false>(ly, cols1, jp, d, 0), TA::template columns<false>(ly, cols1, jp + 1, d, 0));
+        for (int jp = 0; jp < CT; jp += 2)
 #pragma unroll
           for (int m = 0; m < 3; ++m)
 #pragma unroll
-            for (int ct = 0; ct < NC; ++ct) S[d][ct] = mfma16(y, part[ct][jp / 2][m], S[d][ct]);
-        }
+            for (int ct = 0; ct < NC; ++ct)
+              S[d][ct] = mfma16(join(yc[d % (AHEAD + 1)][jp], yc[d % (AHEAD + 1)][jp + 1]), part[ct][jp / 2][m], S[d][ct]);
       }
     } else {
       f32x4 v[NC][CT];
@@ -502,9 +536,11 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
       for (int d = 0; d < DT; ++d) {
 #pragma unroll
         for (int ct = 0; ct < NC; ++ct) S[d][ct] *= whole;
+        if (d + AHEAD < DT) turned(d + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int jt = 0; jt < CT; ++jt) {
-          const f32x4 y = widen(TA::template columns<false>(ly, cols1, jt, d, 0));
+          const f32x4 y = widen(yc[d % (AHEAD + 1)][jt]);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -520,8 +556,8 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
 #pragma unroll
           for (int ct = 0; ct < NC; ++ct) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) zo[ct][r] = (float)*reinterpret_cast<const T*>(lz + TZ::at(j, cw + column<T, NC>(ct, 4 * g + r)));
-            zs[ct] = (float)*reinterpret_cast<const T*>(lz + TZ::at(j, cw + column<T, NC>(ct, l)));
+            for (int r = 0; r < 4; ++r) zo[ct][r] = (float)*reinterpret_cast<const T*>(lz + TZ::at(j, cw + place<T, NC == 2>(ct, 4 * g + r)));
+            zs[ct] = (float)*reinterpret_cast<const T*>(lz + TZ::at(j, cw + place<T, NC == 2>(ct, l)));
             any |= nonfinite(zs[ct]);
           }
           if (!__any(any)) continue;
@@ -543,13 +579,14 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float y = f * (float)*reinterpret_cast<const T*>(ly + TA::at(j, 16 * d + 4 * g + r));
+              const float y = f * (float)*reinterpret_cast<const T*>(ly + TA::at(j, place<T, true>(d, 4 * g + r)));
 #pragma unroll
               for (int ct = 0; ct < NC; ++ct)
                 if (nonfinite(zs[ct])) S[d][ct][r] = fmaf(y, zs[ct], S[d][ct][r]);
             }
         }
       put(O, t, min(CH, t1 - t));
+      stored = n == CH && cw + 16 * NC <= cols;
     }
   }
 
@@ -562,7 +599,7 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
       for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int a = 16 * d + 4 * g + r, c = cw + column<T, NC>(ct, l);
+          const int a = place<T, true>(d, 4 * g + r), c = cw + place<T, NC == 2>(ct, l);
           if (a < p.Da && c < cols) s[(size_t)a * p.sa + (size_t)(c0 + c) * p.sb] = S[d][ct][r];
         }
   }
