@@ -1,6 +1,7 @@
 // Linear attention with a decay for each head: the passes of a forward and of a backward, and the single token.
 #include "ring_linattn.hpp"
 #include "ringattr.h"
+#include <stdlib.h>
 
 using namespace ring_lin;
 
@@ -157,7 +158,7 @@ hipError_t ring_linattn_step(const RingLinShape& s, const RingLinStep& a, hipStr
 int ring_linattn_segments(const RingLinShape& s) {
   const long groups = (long)s.B * s.H * slices(s.Dv);
   const int chunks = (s.T + kChunk - 1) / kChunk;
-  long n = groups > 0 ? 512 / groups : 1;
+  long n = groups > 0 ? (getenv("LINSEG") ? atol(getenv("LINSEG")) : 512) / groups : 1;
   if (n > chunks / 8) n = chunks / 8;
   if (n <= 1) return 1;
   const int per = (int)((chunks + n - 1) / n);

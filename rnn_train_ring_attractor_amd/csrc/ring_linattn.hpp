@@ -118,9 +118,11 @@ template <typename T, int ROWS, int COLS> struct Tile16 {
 };
 
 // Global memory -> LDS without registers: a wave's instruction fills 64 granules one behind the other, each lane from where it likes.
-// What is loaded is there behind a wait for vmcnt and a barrier (nobody else keeps count: the compiler does not see these loads).
+// What is loaded is there behind a wait for vmcnt and a barrier (nobody else keeps count: the compiler does not see these loads).  It
+// says nothing about memory to the compiler, so that reads of the other buffer pass it by: every use of what it writes, and every
+// use of what was there, is on the other side of wait_and_barrier, which does.
 __device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0");
 }
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
@@ -178,7 +180,7 @@ template <int N> __device__ __forceinline__ void wait_and_barrier() {
 // chunk's rows in LDS (two buffers: the next chunk's are on their way while one is worked on); each keeps 16 NC columns of the state
 // in registers, where they are an operand as they lie: the matrix units put rows 4g..4g+3 of column l into lane (g, l) and take them
 // as contraction indices from there.  The weights are formed transposed for the same reason, by every wave for itself.
-template <typename T, int DA, int NC, int CT, bool VEC, bool REV, bool STATE_ONLY>
+template <typename T, int DA, int NC, int CT, bool VEC, bool REV, bool STATE_ONLY, bool EXACT>
 __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(RingLinArgs p) {
   constexpr int WC = 64 * NC, CH = 16 * CT, DT = DA / 16;
   constexpr bool BF = Type<T>::BF;
@@ -395,7 +397,6 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
         if (s + 1 < STEPS) read(s + 1);
-        __builtin_amdgcn_sched_barrier(0);
         if constexpr (BF) {
 #pragma unroll
           for (int jt = 0; jt < CT; ++jt)
@@ -404,12 +405,11 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
               if (REV ? jt >= it : jt <= it) P[jt][it] = mfma16(yr[s & 1][jt], xr[s & 1][it], P[jt][it]);
 #pragma unroll
           for (int ct = 0; ct < NC; ++ct) {
-            const bf16x4 a0 = narrow(S[2 * s][ct]), a1 = narrow(S[2 * s + 1][ct]);
-            const bf16x8 hi = join(a0, a1), lo = join(narrow(S[2 * s][ct] - widen(a0)), narrow(S[2 * s + 1][ct] - widen(a1)));
+            const bf16x8 state = join(narrow(S[2 * s][ct]), narrow(S[2 * s + 1][ct]));
+            S[2 * s][ct] *= whole;
+            S[2 * s + 1][ct] *= whole;
 #pragma unroll
-            for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(hi, xr[s & 1][it], O[ct][it]);
-#pragma unroll
-            for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(lo, xr[s & 1][it], O[ct][it]);
+            for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(state, xr[s & 1][it], O[ct][it]);
           }
         } else {
 #pragma unroll
@@ -432,6 +432,10 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
 #pragma unroll
                 for (int it = 0; it < CT; ++it) O[ct][it] = mfma4(S[TPS * s + q][ct][r], x[it], O[ct][it]);
             }
+#pragma unroll
+          for (int q = 0; q < TPS; ++q)
+#pragma unroll
+            for (int ct = 0; ct < NC; ++ct) S[TPS * s + q][ct] *= whole;
         }
       }
 #pragma unroll
@@ -455,12 +459,9 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
 #pragma unroll
           for (int it = 0; it < CT; ++it)
             if (REV ? jp + 1 >= it : jp <= it) {
-              const bf16x4 a0 = narrow(P[jp][it]), a1 = narrow(P[jp + 1][it]);
-              const bf16x8 hi = join(a0, a1), lo = join(narrow(P[jp][it] - widen(a0)), narrow(P[jp + 1][it] - widen(a1)));
+              const bf16x8 weights = join(narrow(P[jp][it]), narrow(P[jp + 1][it]));
 #pragma unroll
-              for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma16(join(z[ct][jp], z[ct][jp + 1]), hi, O[ct][it]);
-#pragma unroll
-              for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma16(join(z[ct][jp], z[ct][jp + 1]), lo, O[ct][it]);
+              for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma16(join(z[ct][jp], z[ct][jp + 1]), weights, O[ct][it]);
             }
       } else {
 #pragma unroll
@@ -475,76 +476,6 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
               if (REV ? jt >= it : jt <= it)
 #pragma unroll
                 for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma4(v[ct][r], P[jt][it][r], O[ct][it]);
-        }
-      }
-    }
-    // the state behind the chunk; Y's columns are read AHEAD tiles ahead
-    constexpr int AHEAD = 2;
-    V4 yc[AHEAD + 1][CT];
-    auto turned = [&](int d) {
-#pragma unroll
-      for (int jt = 0; jt < CT; ++jt) yc[d % (AHEAD + 1)][jt] = TA::template columns<true>(ly, cols1, jt, d);
-    };
-#pragma unroll
-    for (int d = 0; d < AHEAD; ++d) turned(d);
-    if constexpr (BF) {
-      bf16x8 part[NC][CT / 2][3];
-#pragma unroll
-      for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-        for (int jp = 0; jp < CT; jp += 2) {
-          bf16x4 k[2][3];
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            f32x4 v = widen(z[ct][jp + q]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] *= outer[jp + q][r];
-#pragma unroll
-            for (int m = 0; m < 3; ++m) {
-              k[q][m] = narrow(v);
-              v -= widen(k[q][m]);
-            }
-          }
-#pragma unroll
-          for (int m = 0; m < 3; ++m) part[ct][jp / 2][m] = join(k[0][m], k[1][m]);
-        }
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-#pragma unroll
-        for (int ct = 0; ct < NC; ++ct) S[d][ct] *= whole;
-        if (d + AHEAD < DT) turned(d + AHEAD);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int jp = 0; jp < CT; jp += 2)
-#pragma unroll
-          for (int m = 0; m < 3; ++m)
-#pragma unroll
-            for (int ct = 0; ct < NC; ++ct)
-              S[d][ct] = mfma16(join(yc[d % (AHEAD + 1)][jp], yc[d % (AHEAD + 1)][jp + 1]), part[ct][jp / 2][m], S[d][ct]);
-      }
-    } else {
-      f32x4 v[NC][CT];
-#pragma unroll
-      for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-        for (int jt = 0; jt < CT; ++jt) {
-          v[ct][jt] = widen(z[ct][jt]);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[ct][jt][r] *= outer[jt][r];
-        }
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-#pragma unroll
-        for (int ct = 0; ct < NC; ++ct) S[d][ct] *= whole;
-        if (d + AHEAD < DT) turned(d + AHEAD);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int jt = 0; jt < CT; ++jt) {
-          const f32x4 y = widen(yc[d % (AHEAD + 1)][jt]);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int ct = 0; ct < NC; ++ct) S[d][ct] = mfma4(y[r], v[ct][jt][r], S[d][ct]);
         }
       }
     }
@@ -588,6 +519,77 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
       put(O, t, min(CH, t1 - t));
       stored = n == CH && cw + 16 * NC <= cols;
     }
+    // the state behind the chunk; Y's columns are read AHEAD tiles ahead
+    constexpr int AHEAD = 2;
+    V4 yc[AHEAD + 1][CT];
+    auto turned = [&](int d) {
+#pragma unroll
+      for (int jt = 0; jt < CT; ++jt) yc[d % (AHEAD + 1)][jt] = TA::template columns<true>(ly, cols1, jt, d);
+    };
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) turned(d);
+    if constexpr (BF) {
+      constexpr int PARTS = EXACT ? 3 : 2;
+      bf16x8 part[NC][CT / 2][PARTS];
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int jp = 0; jp < CT; jp += 2) {
+          bf16x4 k[2][PARTS];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            f32x4 v = widen(z[ct][jp + q]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] *= outer[jp + q][r];
+#pragma unroll
+            for (int m = 0; m < PARTS; ++m) {
+              k[q][m] = narrow(v);
+              if (m + 1 < PARTS) v -= widen(k[q][m]);
+            }
+          }
+#pragma unroll
+          for (int m = 0; m < PARTS; ++m) part[ct][jp / 2][m] = join(k[0][m], k[1][m]);
+        }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+#pragma unroll
+        for (int ct = 0; ct < NC; ++ct)
+          if (STATE_ONLY) S[d][ct] *= whole;
+        if (d + AHEAD < DT) turned(d + AHEAD);
+#pragma unroll
+        for (int jp = 0; jp < CT; jp += 2)
+#pragma unroll
+          for (int m = 0; m < PARTS; ++m)
+#pragma unroll
+            for (int ct = 0; ct < NC; ++ct)
+              S[d][ct] = mfma16(join(yc[d % (AHEAD + 1)][jp], yc[d % (AHEAD + 1)][jp + 1]), part[ct][jp / 2][m], S[d][ct]);
+      }
+    } else {
+      f32x4 v[NC][CT];
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int jt = 0; jt < CT; ++jt) {
+          v[ct][jt] = widen(z[ct][jt]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[ct][jt][r] *= outer[jt][r];
+        }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+#pragma unroll
+        for (int ct = 0; ct < NC; ++ct)
+          if (STATE_ONLY) S[d][ct] *= whole;
+        if (d + AHEAD < DT) turned(d + AHEAD);
+#pragma unroll
+        for (int jt = 0; jt < CT; ++jt) {
+          const f32x4 y = widen(yc[d % (AHEAD + 1)][jt]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int ct = 0; ct < NC; ++ct) S[d][ct] = mfma4(y[r], v[ct][jt][r], S[d][ct]);
+        }
+      }
+    }
   }
 
   float* s = STATE_ONLY ? p.seg + (bh * p.nseg + seg) * p.Da * p.Db : (p.s_out ? p.s_out + bh * p.Da * p.Db : nullptr);
@@ -608,12 +610,17 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
 template <typename T, int DA, int NC, bool VEC> hipError_t launch_sized(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
   constexpr int CT = sizeof(T) == 4 ? 1 : 2;
   const dim3 grid((unsigned)((long)a.nseg * a.slices * a.H * a.B)), block(256);
+  // (only bf16 rows have another way to a state that nobody but this kernel sees)
+  constexpr bool SHORT = !Type<T>::BF;
   if (state_only) {
-    if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, true, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, false, true>), grid, block, 0, st, a);
+    if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, true, true, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, false, true, true>), grid, block, 0, st, a);
+  } else if (!SHORT && a.nseg == 1 && a.s_out) {
+    if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, true, false, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, false, false, true>), grid, block, 0, st, a);
   } else {
-    if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, true, false>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, false, false>), grid, block, 0, st, a);
+    if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, true, false, SHORT>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, false, false, SHORT>), grid, block, 0, st, a);
   }
   return hipGetLastError();
 }
