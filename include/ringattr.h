@@ -299,12 +299,14 @@ RINGATTR_API int ringattr_linear_attention_fwd(const void* q, const void* k, con
                       float scale, int type, int batch_size, int seq_len, int heads, int kv_heads, int dk, int dv,
                       void* workspace, size_t workspace_bytes, void* stream);
 /* Gradients of q, k, v and (NULL: not wanted) of the initial state, from those of o and (NULL: zero) of the final state.
- * The gradients of shared heads are summed in fp32 in a fixed order. */
+ * The gradients of shared heads are summed in fp32 in a fixed order.  states: the workspace that a forward of the same
+ * arguments left (its states along the sequences; a caller that keeps it spares the backward a pass), or NULL: they are
+ * formed again. */
 RINGATTR_API size_t ringattr_linear_attention_bwd_workspace_bytes(int type, int batch_size, int seq_len, int heads, int kv_heads,
-                      int dk, int dv);
+                      int dk, int dv, int have_states);
 RINGATTR_API int ringattr_linear_attention_bwd(const void* q, const void* k, const void* v, const void* grad_o,
                       const long long* strides, const void* log_decay, const void* initial_state, const void* lengths,
-                      const void* grad_final_state, void* grad_q, void* grad_k, void* grad_v, void* grad_initial_state,
+                      const void* states, const void* grad_final_state, void* grad_q, void* grad_k, void* grad_v, void* grad_initial_state,
                       float scale, int type, int batch_size, int seq_len, int heads, int kv_heads, int dk, int dv,
                       void* workspace, size_t workspace_bytes, void* stream);
 /* One token for each sequence: q [B,heads,dk], k [B,kv_heads,dk], v [B,kv_heads,dv] (strides: batch, head of each), the state

@@ -78,8 +78,8 @@ PROTOTYPES = {
     "ringattr_linear_attention_fwd_workspace_bytes": (c_size_t, [c_int] * 7),
     "ringattr_linear_attention_fwd": (c_int, [c_void_p] * 3 + [ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 5 + [c_float] +
                                       [c_int] * 7 + [c_void_p, c_size_t, c_void_p]),
-    "ringattr_linear_attention_bwd_workspace_bytes": (c_size_t, [c_int] * 7),
-    "ringattr_linear_attention_bwd": (c_int, [c_void_p] * 4 + [ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 8 + [c_float] +
+    "ringattr_linear_attention_bwd_workspace_bytes": (c_size_t, [c_int] * 8),
+    "ringattr_linear_attention_bwd": (c_int, [c_void_p] * 4 + [ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 9 + [c_float] +
                                       [c_int] * 7 + [c_void_p, c_size_t, c_void_p]),
     "ringattr_linear_attention_step": (c_int, [c_void_p] * 3 + [ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 4 + [c_float] +
                                        [c_int] * 6 + [c_void_p]),

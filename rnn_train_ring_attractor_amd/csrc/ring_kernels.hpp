@@ -343,7 +343,9 @@ struct RingLinArgs {
   const float* s_in;     // states [B,H,..]: element (a, b) at a * sa + b * sb; null: zeros
   float* s_out;          // null: not wanted
   long sa, sb;
-  float* seg;            // nseg > 1: [B,H,nseg,..] the states in front of the segments (written by the pass over states only)
+  float* seg;            // nseg > 1: [B,H,nseg - 1,..] what the segments but the last add to a state of zeros, natural states, by
+                         // the pass over states only; scanned: the states behind them
+  bool scanned;
   const int* lengths;    // tokens of each sequence, null: T
   float intra, inter, update;    // factors of the weights, of what the state gives, of what it takes in
   int B, T, H, Da, Db, nseg, seg_tokens, slices;
@@ -356,14 +358,13 @@ struct RingLinStep {
   const unsigned char* active;
   void* out;
 };
-int ring_linattn_segments(const RingLinShape& s);
 size_t ring_linattn_fwd_bytes(const RingLinShape& s);
-size_t ring_linattn_bwd_bytes(const RingLinShape& s);
+size_t ring_linattn_bwd_bytes(const RingLinShape& s, bool have_states);
 hipError_t ring_linattn_fwd(const RingLinShape& s, const RingLinTensor& q, const RingLinTensor& k, const RingLinTensor& v,
                             const float* log_decay, const float* s_in, const int* lengths, void* o, float* s_out, void* ws, hipStream_t st);
 hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const RingLinTensor& k, const RingLinTensor& v,
-                            const float* log_decay, const float* s_in, const int* lengths, const RingLinTensor& go, const float* gs,
-                            void* gq, void* gk, void* gv, float* gs_in, void* ws, hipStream_t st);
+                            const float* log_decay, const float* s_in, const int* lengths, const float* states,
+                            const RingLinTensor& go, const float* gs, void* gq, void* gk, void* gv, float* gs_in, void* ws, hipStream_t st);
 hipError_t ring_linattn_step(const RingLinShape& s, const RingLinStep& a, hipStream_t st);
 hipError_t ring_launch_linattn_f32(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st);
 hipError_t ring_launch_linattn_bf16(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st);

@@ -1,13 +1,15 @@
 // Linear attention with a decay for each head: the passes of a forward and of a backward, and the single token.
 #include "ring_linattn.hpp"
 #include "ringattr.h"
-#include <stdlib.h>
 
 using namespace ring_lin;
 
 namespace {
 
 constexpr int kChunk = 32;
+// Up to so many segments a workgroup adds up what those in front have added itself; past that a scan does, a launch more but less to read
+// (8 x 4096 tokens, 16 heads of 128 in four segments, us a pass of the chunk kernel: 165 adding up itself, 130 and a scan of 17).
+constexpr int kFold = 2;
 
 size_t round_up(size_t x) { return (x + 255) / 256 * 256; }
 
@@ -27,6 +29,7 @@ RingLinArgs base(const RingLinShape& s, const float* log_decay, const int* lengt
   a.T = s.T;
   a.H = s.H;
   a.nseg = nseg;
+  a.scanned = nseg > kFold;
   const int chunks = (s.T + kChunk - 1) / kChunk;
   a.seg_tokens = nseg > 1 ? (chunks + nseg - 1) / nseg * kChunk : (s.T > 0 ? s.T : 1);
   a.intra = a.inter = a.update = 1.f;
@@ -38,27 +41,24 @@ bool out_fits(const RingLinArgs& a) { return (long)a.H * a.Db < (1 << 22); }
 
 }  // namespace
 
-// The states in front of the segments: seg[i] is what segment i adds to a state of zeros and becomes the state in front of it
-// (REV: behind it).  A thread walks one element through the segments.
+// What the segments add to a state of zeros becomes the states behind them, in place.  A thread walks one element through them.
 __global__ __launch_bounds__(256) void ring_linattn_scan_kernel(RingLinArgs p, bool rev) {
-  const int D = p.Da * p.Db;
+  const int D = p.Da * p.Db, ns = p.nseg - 1;
   const int per = (D + 255) / 256, e = (int)(blockIdx.x % per) * 256 + threadIdx.x;
   const size_t bh = blockIdx.x / per;
   if (e >= D) return;
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
   const float g2 = (float)((double)p.log_decay[h] * 1.4426950408889634);
-  float* seg = p.seg + bh * p.nseg * D + e;
+  float* seg = p.seg + bh * ns * D + e;
   float run = p.s_in ? p.s_in[bh * D + e] : 0.f;
 #pragma unroll 8
-  for (int i = 0; i < p.nseg; ++i) {
-    const int s = rev ? p.nseg - 1 - i : i;
-    const int n = min(max(len - s * p.seg_tokens, 0), min(p.seg_tokens, p.T - s * p.seg_tokens));
-    const float local = seg[(size_t)s * D];
-    seg[(size_t)s * D] = run;
+  for (int u = 0; u < ns; ++u) {
+    const int ts = (rev ? p.nseg - 1 - u : u) * p.seg_tokens, n = min(max(len - ts, 0), p.seg_tokens);
+    const float local = seg[(size_t)u * D];
     if (n > 0) run = fmaf(power(g2, n), run, local);
+    seg[(size_t)u * D] = run;
   }
-  if (p.s_out) p.s_out[bh * D + e] = run;
 }
 
 // out[row][g][d] = sum over the heads that share g
@@ -154,38 +154,54 @@ hipError_t ring_linattn_step(const RingLinShape& s, const RingLinStep& a, hipStr
   return launch_step<_Float16>(s, a, st);
 }
 
-// Into how many segments the tokens are cut so that there is work for all compute units
-int ring_linattn_segments(const RingLinShape& s) {
+// Into how many segments the tokens are cut so that there is work for all compute units: the number with the least expected time, in
+// units of what a workgroup alone on its compute unit takes for a chunk of 32 tokens.  Two on one take 1.6 each (heads past 128 wide
+// fill the registers: one at a time).  More than one segment costs a pass over their states, at 0.45 of a chunk, a launch and what the
+// segments behind read of it.
+static int segments(const RingLinShape& s) {
   const long groups = (long)s.B * s.H * slices(s.Dv);
   const int chunks = (s.T + kChunk - 1) / kChunk;
-  long n = groups > 0 ? (getenv("LINSEG") ? atol(getenv("LINSEG")) : 512) / groups : 1;
-  if (n > chunks / 8) n = chunks / 8;
-  if (n <= 1) return 1;
-  const int per = (int)((chunks + n - 1) / n);
-  return (chunks + per - 1) / per;
+  const bool one = s.Dk > 128 || s.Dv > 128;
+  auto rounds = [&](long work) {
+    const long at_once = one ? 256 : 512, rest = work % at_once;
+    return (double)(work / at_once) * (one ? 1.0 : 1.6) + (rest == 0 ? 0.0 : (one || rest <= 256 ? 1.0 : 1.6));
+  };
+  int best = 1;
+  double least = rounds(groups) * chunks;
+  for (int n = 2; n <= 64 && 2 * n <= chunks; ++n) {
+    const int per = (chunks + n - 1) / n;
+    if ((chunks + per - 1) / per != n) continue;
+    const double t = per * (rounds(groups * n) + 0.45 * rounds(groups * (n - 1))) + 3.0 + (n > kFold ? 3.0 : 0.0);
+    if (t < least) {
+      least = t;
+      best = n;
+    }
+  }
+  return best;
 }
 
-static size_t states_bytes(const RingLinShape& s, int nseg) {
-  return nseg > 1 ? round_up((size_t)s.B * s.H * nseg * s.Dk * s.Dv * sizeof(float)) : 0;
+static size_t states_bytes(const RingLinShape& s) {
+  return round_up((size_t)s.B * s.H * (segments(s) - 1) * s.Dk * s.Dv * sizeof(float));
 }
 
-size_t ring_linattn_fwd_bytes(const RingLinShape& s) { return states_bytes(s, ring_linattn_segments(s)); }
+size_t ring_linattn_fwd_bytes(const RingLinShape& s) { return states_bytes(s); }
 
-size_t ring_linattn_bwd_bytes(const RingLinShape& s) {
-  size_t n = 2 * states_bytes(s, ring_linattn_segments(s));
+size_t ring_linattn_bwd_bytes(const RingLinShape& s, bool have_states) {
+  size_t n = (have_states ? 1 : 2) * states_bytes(s);
   if (s.G != s.H) n += round_up((size_t)s.B * s.T * s.H * s.Dk * sizeof(float)) + round_up((size_t)s.B * s.T * s.H * s.Dv * sizeof(float));
   return n;
 }
 
-// The states in front of the segments of Y and Z (rows of natural states, [Dk][Dv]) into `seg`, the one behind them all into s_out.
+// What the segments of Y and Z add to a state (natural states, [Dk][Dv]), or the states behind them, into a.seg
 static hipError_t segment_states(const RingLinShape& s, RingLinArgs a, bool rev, hipStream_t st) {
+  if (a.nseg == 1) return hipSuccess;
   a.Da = s.Dk;
   a.Db = s.Dv;
   a.sa = s.Dv;
   a.sb = 1;
   a.slices = slices(s.Dv);
   hipError_t e = launch_pass(s.type, a, rev, true, st);
-  if (e != hipSuccess) return e;
+  if (e != hipSuccess || !a.scanned) return e;
   const unsigned per = (unsigned)((s.Dk * s.Dv + 255) / 256);
   hipLaunchKernelGGL(ring_linattn_scan_kernel, dim3((unsigned)((size_t)per * s.B * s.H)), dim3(256), 0, st, a, rev);
   return hipGetLastError();
@@ -193,7 +209,7 @@ static hipError_t segment_states(const RingLinShape& s, RingLinArgs a, bool rev,
 
 hipError_t ring_linattn_fwd(const RingLinShape& s, const RingLinTensor& q, const RingLinTensor& k, const RingLinTensor& v,
                             const float* log_decay, const float* s_in, const int* lengths, void* o, float* s_out, void* ws, hipStream_t st) {
-  const int nseg = ring_linattn_segments(s), epv = s.type == RINGATTR_F32 ? 4 : 8;
+  const int nseg = segments(s), epv = s.type == RINGATTR_F32 ? 4 : 8;
   RingLinArgs a = base(s, log_decay, lengths, nseg);
   a.X = q;
   a.Y = k;
@@ -203,10 +219,8 @@ hipError_t ring_linattn_fwd(const RingLinShape& s, const RingLinTensor& q, const
   a.s_in = s_in;
   a.s_out = s_out;
   a.seg = (float*)ws;
-  if (nseg > 1) {
-    hipError_t e = segment_states(s, a, false, st);
-    if (e != hipSuccess) return e;
-  }
+  hipError_t e = segment_states(s, a, false, st);
+  if (e != hipSuccess) return e;
   a.Da = s.Dk;
   a.Db = s.Dv;
   a.sa = s.Dv;
@@ -219,12 +233,13 @@ hipError_t ring_linattn_fwd(const RingLinShape& s, const RingLinTensor& q, const
 }
 
 hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const RingLinTensor& k, const RingLinTensor& v,
-                            const float* log_decay, const float* s_in, const int* lengths, const RingLinTensor& go, const float* gs,
-                            void* gq, void* gk, void* gv, float* gs_in, void* ws, hipStream_t st) {
-  const int nseg = ring_linattn_segments(s), share = s.H / s.G, epv = s.type == RINGATTR_F32 ? 4 : 8;
+                            const float* log_decay, const float* s_in, const int* lengths, const float* states,
+                            const RingLinTensor& go, const float* gs, void* gq, void* gk, void* gv, float* gs_in, void* ws, hipStream_t st) {
+  const int nseg = segments(s), share = s.H / s.G, epv = s.type == RINGATTR_F32 ? 4 : 8;
   unsigned char* w = (unsigned char*)ws;
-  float *seg_f = (float*)w, *seg_r = (float*)(w + states_bytes(s, nseg));
-  w += 2 * states_bytes(s, nseg);
+  const size_t each = states_bytes(s);
+  float *seg_r = (float*)w, *seg_f = states ? const_cast<float*>(states) : (float*)(w + each);
+  w += (states ? 1 : 2) * each;
   float *part_k = (float*)w, *part_v = (float*)(w + round_up((size_t)s.B * s.T * s.H * s.Dk * sizeof(float)));
   hipError_t e;
   RingLinArgs f = base(s, log_decay, lengths, nseg), r = f;
@@ -240,12 +255,12 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
   r.ys = r.zs = 1;
   r.update = s.scale;
   r.s_out = gs_in;
-  if (nseg > 1) {
+  if (!states) {
     e = segment_states(s, f, false, st);
     if (e != hipSuccess) return e;
-    e = segment_states(s, r, true, st);
-    if (e != hipSuccess) return e;
   }
+  e = segment_states(s, r, true, st);
+  if (e != hipSuccess) return e;
   // dq: do against v weighs k, the state transposed
   f.X = go;
   f.xs = 1;

@@ -121,8 +121,15 @@ template <typename T, int ROWS, int COLS> struct Tile16 {
 // What is loaded is there behind a wait for vmcnt and a barrier (nobody else keeps count: the compiler does not see these loads).  It
 // says nothing about memory to the compiler, so that reads of the other buffer pass it by: every use of what it writes, and every
 // use of what was there, is on the other side of wait_and_barrier, which does.
+// base and lds are the same in all lanes.  (The wait states are for a base that a vector instruction has just put into its scalar
+// registers: the compiler does not look into the statement.)
 __device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0");
+  const unsigned long long a = (unsigned long long)(uintptr_t)base;
+  const unsigned low = __builtin_amdgcn_readfirstlane((unsigned)a), high = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+  const unsigned long long s = (unsigned long long)high << 32 | low;
+  unsigned kept;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+               : "=&s"(kept) : "s"(lds), "v"(off), "s"(s));
 }
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
@@ -193,7 +200,9 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
   __shared__ __align__(16) char lds[2 * BUF];
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 15, g = (tid >> 4) & 3;
-  const int seg = blockIdx.x % p.nseg, slice = blockIdx.x / p.nseg % p.slices, head = blockIdx.x / (p.nseg * p.slices);
+  // `order` counts the segments as they follow each other; the pass over states has no use for the last
+  const int per = STATE_ONLY ? p.nseg - 1 : p.nseg, order = blockIdx.x % per, seg = REV ? p.nseg - 1 - order : order;
+  const int slice = blockIdx.x / per % p.slices, head = blockIdx.x / (per * p.slices);
   const int c0 = slice * WC, h = head % p.H, b = head / p.H;
   const int cw = 16 * NC * w;                                  // the wave's columns within the workgroup's
   const int T_ = p.T;
@@ -208,19 +217,44 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
   const T* Z = rows_of<T>(p.Z, b, h, p.zs) + c0;
   const int cols = p.Db - c0;
 
+  // The state in front: a scan has left it, or it is the initial one and what the segments in front have added to it, as they follow
+  // each other.
+  const bool wide = p.Da == DA && cols >= WC;                  // (nothing to leave out)
   f32x4 S[DT][NC];
-  {
-    const float* s = p.nseg > 1 && !STATE_ONLY ? p.seg + (bh * p.nseg + seg) * p.Da * p.Db : (p.s_in ? p.s_in + bh * p.Da * p.Db : nullptr);
-    if (STATE_ONLY) s = nullptr;
+  const size_t D = (size_t)p.Da * p.Db;
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int ct = 0; ct < NC; ++ct)
+    for (int ct = 0; ct < NC; ++ct) S[d][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (!STATE_ONLY) {
+    const float* const segs = p.nseg > 1 ? p.seg + bh * (p.nseg - 1) * D : nullptr;
+    const int sa = (int)p.sa, sb = (int)p.sb, a0 = place<T, true>(0, 4 * g), b0 = cw + place<T, NC == 2>(0, l);
+    for (int u = p.scanned && order > 0 ? order - 1 : (p.s_in ? -1 : 0); u < order; ++u) {
+      const float* s = u < 0 ? p.s_in + bh * D : segs + u * D;
+      const int ts = (REV ? p.nseg - 1 - u : u) * p.seg_tokens, n = min(max(len - ts, 0), p.seg_tokens);
+      const float f = u < 0 ? 0.f : power(g2, n);              // (times zero where u is the first)
+      s += (size_t)c0 * sb;
+      int a1 = a0, b1 = b0;
+      asm volatile("" : "+v"(a1), "+v"(b1));                   // (64 addresses are not to be kept from one turn to the next)
+      const unsigned at = (unsigned)(a1 * sa + b1 * sb);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int a = place<T, true>(d, 4 * g + r), c = cw + place<T, NC == 2>(ct, l);
-          S[d][ct][r] = s && a < p.Da && c < cols ? s[(size_t)a * p.sa + (size_t)(c0 + c) * p.sb] : 0.f;
-        }
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int da = place<T, true>(d, 0) + r, db = place<T, NC == 2>(ct, 0);
+            float x;
+            if (wide) {
+              x = (s + (da * sa + db * sb))[at];
+            } else {
+              x = s[(unsigned)(min(a1 + da, p.Da - 1) * sa + min(b1 + db, cols - 1) * sb)];
+              x = a1 + da < p.Da && b1 + db < cols ? x : 0.f;
+            }
+            S[d][ct][r] = fmaf(f, S[d][ct][r], x);
+            if (r == 3 && ct == NC - 1 && d % 4 == 3) __builtin_amdgcn_sched_barrier(0);       // (not all 64 on their way at once)
+          }
+    }
   }
 
   // powers of the decay: by distance within a pair of tiles, and for the rows of a chunk of n
@@ -285,7 +319,6 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
   if (!STATE_ONLY) fx.init(p.X.st, tid);
   fy.init(p.Y.st, tid);
   fz.init(p.Z.st, tid);
-  const bool wide = p.Da == DA && cols >= WC;                  // (no columns to leave out)
   auto fetch = [&](int c, int buf) {
     const int t = t0 + c * CH, n = min(CH, te - t);
     char* const tile = lds + buf * BUF;
@@ -592,8 +625,7 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
     }
   }
 
-  float* s = STATE_ONLY ? p.seg + (bh * p.nseg + seg) * p.Da * p.Db : (p.s_out ? p.s_out + bh * p.Da * p.Db : nullptr);
-  if (!STATE_ONLY && p.nseg > 1) s = nullptr;                  // (the scan over segments writes it)
+  float* const s = STATE_ONLY ? p.seg + (bh * (p.nseg - 1) + order) * D : (order == p.nseg - 1 && p.s_out ? p.s_out + bh * D : nullptr);
   if (s) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -609,13 +641,13 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
 
 template <typename T, int DA, int NC, bool VEC> hipError_t launch_sized(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
   constexpr int CT = sizeof(T) == 4 ? 1 : 2;
-  const dim3 grid((unsigned)((long)a.nseg * a.slices * a.H * a.B)), block(256);
-  // (only bf16 rows have another way to a state that nobody but this kernel sees)
+  const dim3 grid((unsigned)((long)(state_only ? a.nseg - 1 : a.nseg) * a.slices * a.H * a.B)), block(256);
+  // (EXACT: only bf16 rows have another way to a state that nobody sees)
   constexpr bool SHORT = !Type<T>::BF;
   if (state_only) {
     if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, true, true, true>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, false, true, true>), grid, block, 0, st, a);
-  } else if (!SHORT && a.nseg == 1 && a.s_out) {
+  } else if (!SHORT && a.s_out) {
     if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, true, false, true>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, false, false, true>), grid, block, 0, st, a);
   } else {

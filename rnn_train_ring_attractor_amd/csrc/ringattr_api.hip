@@ -962,10 +962,11 @@ size_t ringattr_linear_attention_fwd_workspace_bytes(int type, int batch_size, i
   return ring_linattn_fwd_bytes(s);
 }
 
-size_t ringattr_linear_attention_bwd_workspace_bytes(int type, int batch_size, int seq_len, int heads, int kv_heads, int dk, int dv) {
+size_t ringattr_linear_attention_bwd_workspace_bytes(int type, int batch_size, int seq_len, int heads, int kv_heads, int dk, int dv,
+                                                     int have_states) {
   RingLinShape s;
   if (!linattn_shape("ringattr_linear_attention", type, batch_size, seq_len, heads, kv_heads, dk, dv, s)) return 0;
-  return ring_linattn_bwd_bytes(s);
+  return ring_linattn_bwd_bytes(s, have_states != 0);
 }
 
 int ringattr_linear_attention_fwd(const void* q, const void* k, const void* v, const long long* strides, const void* log_decay,
@@ -990,8 +991,8 @@ int ringattr_linear_attention_fwd(const void* q, const void* k, const void* v, c
 }
 
 int ringattr_linear_attention_bwd(const void* q, const void* k, const void* v, const void* grad_o, const long long* strides,
-                                  const void* log_decay, const void* initial_state, const void* lengths, const void* grad_final_state,
-                                  void* grad_q, void* grad_k, void* grad_v, void* grad_initial_state, float scale, int type,
+                                  const void* log_decay, const void* initial_state, const void* lengths, const void* states,
+                                  const void* grad_final_state, void* grad_q, void* grad_k, void* grad_v, void* grad_initial_state, float scale, int type,
                                   int batch_size, int seq_len, int heads, int kv_heads, int dk, int dv, void* workspace,
                                   size_t workspace_bytes, void* stream) {
   const char* who = "ringattr_linear_attention_bwd";
@@ -1000,16 +1001,16 @@ int ringattr_linear_attention_bwd(const void* q, const void* k, const void* v, c
   if (!q || !k || !v || !grad_o || !strides || !log_decay || !grad_q || !grad_k || !grad_v)
     return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
   if (!aligned16(grad_q) || !aligned16(grad_k) || !aligned16(grad_v) || !aligned16(initial_state) || !aligned16(grad_final_state) ||
-      !aligned16(grad_initial_state) || !aligned16(workspace))
+      !aligned16(grad_initial_state) || !aligned16(states) || !aligned16(workspace))
     return fail(RINGATTR_ERR_INVALID, "%s: outputs, states and workspace must be 16-byte aligned", who);
-  const size_t need = ring_linattn_bwd_bytes(s);
+  const size_t need = ring_linattn_bwd_bytes(s, states != nullptr);
   if (need && (!workspace || workspace_bytes < need))
     return fail(RINGATTR_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
   s.scale = scale;
   hipError_t e = ring_linattn_bwd(s, rows_tensor(q, strides, dk, type), rows_tensor(k, strides + 3, dk, type),
                                   rows_tensor(v, strides + 6, dv, type), (const float*)log_decay, (const float*)initial_state,
-                                  (const int*)lengths, rows_tensor(grad_o, strides + 9, dv, type), (const float*)grad_final_state, grad_q,
-                                  grad_k, grad_v, (float*)grad_initial_state, workspace, static_cast<hipStream_t>(stream));
+                                  (const int*)lengths, (const float*)states, rows_tensor(grad_o, strides + 9, dv, type),
+                                  (const float*)grad_final_state, grad_q, grad_k, grad_v, (float*)grad_initial_state, workspace, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "linear attention backward launch");
   return RINGATTR_OK;
 }

@@ -113,6 +113,21 @@ def av_to_action_signal_ND(av_signal, action_dim=16, zero_padding=True):
     return torch.relu(av_signal.unsqueeze(-1) * scales)
 
 
+def drop_action_signal(action_signal, p, seed, offset=0):
+    """Sensory dropout: parts of the action signal are missing with probability p (`dropout_func`; seed and offset as there: a step of
+    its own offset, or a device counter that a recorded step advances).  What the signal's builder stated about its channels still
+    holds."""
+    if not p:
+        return action_signal
+    from .dropout import dropout_func
+    from .ring_rnn_cuda import DRIVEN_ATTR
+    out = dropout_func(action_signal, p, seed, offset)
+    driven = getattr(action_signal, DRIVEN_ATTR, None)
+    if driven is not None:
+        setattr(out, DRIVEN_ATTR, driven)
+    return out
+
+
 def generate_av_integration_data_ultra_fast(num_trials, seq_len, zero_padding_start_ratio=0.1, zero_ratios_in_rest=None,
                                             max_av=0.1 * math.pi, device="cpu"):
     """Vectorised AV trials: leading zeros, then exactly len_rest - floor(len_rest*ratio) randomly placed

@@ -14,7 +14,6 @@ import ctypes
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import SEQUENCE_TYPES, check_sequence_tensor
@@ -62,28 +61,30 @@ def _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state):
         if B == 0 or T == 0:
             if want_state:
                 state.zero_() if initial_state is None else state.copy_(initial_state)
-            return o, state
+            return o, state, None
         nbytes = lib.ringattr_linear_attention_fwd_workspace_bytes(kind, B, T, H, G, Dk, Dv)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         strides = _Strides9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
         _lib.check(lib.ringattr_linear_attention_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, log_decay.data_ptr(), _ptr(initial_state), _ptr(lengths), o.data_ptr(),
             _ptr(state), scale, kind, B, T, H, G, Dk, Dv, _ptr(ws), nbytes, _lib.stream_handle(dev)))
-    return o, state
+    return o, state, ws
 
 
 class LinearAttentionFunc(Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale, want_state):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
+        o, state, along = _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state)
+        ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths, along)
         ctx.scale = scale
-        return _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state)
+        return o, state
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_o, grad_state):
-        q, k, v, log_decay, initial_state, lengths = ctx.saved_tensors
+        if torch.is_grad_enabled():              # (create_graph: the result would pass for one that does not depend on q, k and v)
+            raise RuntimeError("linear_attention_func is differentiable once: its backward takes no create_graph=True")
+        q, k, v, log_decay, initial_state, lengths, along = ctx.saved_tensors
         B, T, H, Dk = q.shape
         G, Dv, dev = k.shape[2], v.shape[3], q.device
         lib, kind = _lib.load(), SEQUENCE_TYPES[q.dtype]
@@ -97,12 +98,12 @@ class LinearAttentionFunc(Function):
                     g0.zero_() if gs is None else g0.copy_(gs)
             else:
                 go = torch.zeros(B, T, H, Dv, dtype=q.dtype, device=dev) if grad_o is None else _rows(grad_o.to(q.dtype))
-                nbytes = lib.ringattr_linear_attention_bwd_workspace_bytes(kind, B, T, H, G, Dk, Dv)
+                nbytes = lib.ringattr_linear_attention_bwd_workspace_bytes(kind, B, T, H, G, Dk, Dv, along is not None)
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
                 strides = _Strides12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *go.stride()[:3])
                 _lib.check(lib.ringattr_linear_attention_bwd(
                     q.data_ptr(), k.data_ptr(), v.data_ptr(), go.data_ptr(), strides, log_decay.data_ptr(), _ptr(initial_state),
-                    _ptr(lengths), _ptr(gs), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _ptr(g0), ctx.scale, kind, B, T, H, G, Dk, Dv,
+                    _ptr(lengths), _ptr(along), _ptr(gs), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _ptr(g0), ctx.scale, kind, B, T, H, G, Dk, Dv,
                     _ptr(ws), nbytes, _lib.stream_handle(dev)))
         return gq, gk, gv, None, g0, None, None, None
 
@@ -135,7 +136,7 @@ def linear_attention_func(q, k, v, log_decay, initial_state=None, lengths=None, 
                                     (initial_state is not None and initial_state.requires_grad)):
         o, state = LinearAttentionFunc.apply(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
     else:
-        o, state = _forward(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
+        o, state, _ = _forward(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
     return (o, state) if return_state else o
 
 

@@ -74,19 +74,24 @@ def _turn(xs, positions, frequencies, layout, scale, inverse):
     return ys
 
 
+def _turned(positions, frequencies, layout, scale, inverse, *xs):
+    return tuple(_turn(xs, positions, frequencies, layout, scale, inverse))
+
+
 class RotaryFunc(Function):
     @staticmethod
     def forward(ctx, positions, frequencies, layout, scale, inverse, *xs):
         ctx.save_for_backward(positions, frequencies)
         ctx.how = (layout, scale, inverse)
-        return tuple(_turn(xs, positions, frequencies, layout, scale, inverse))
+        return _turned(positions, frequencies, layout, scale, inverse, *xs)
 
     @staticmethod
     def backward(ctx, *grads):
         positions, frequencies = ctx.saved_tensors
         layout, scale, inverse = ctx.how
         # turned back: the transpose of a turn is the opposite turn, so a gradient of the gradient is this operator again
-        return (None,) * 5 + RotaryFunc.apply(positions, frequencies, layout, scale, 1 - inverse, *grads)
+        back = RotaryFunc.apply if torch.is_grad_enabled() else _turned
+        return (None,) * 5 + back(positions, frequencies, layout, scale, 1 - inverse, *grads)
 
 
 def rotary_func(x, positions, frequencies, layout="half", scale=1.0):
@@ -128,5 +133,5 @@ def rotary_func(x, positions, frequencies, layout="half", scale=1.0):
     if torch.is_grad_enabled() and any(t.requires_grad for t in xs):
         ys = RotaryFunc.apply(positions, frequencies, _LAYOUTS[layout], scale, 0, *xs)
     else:
-        ys = tuple(_turn(xs, positions, frequencies, _LAYOUTS[layout], scale, 0))
+        ys = _turned(positions, frequencies, _LAYOUTS[layout], scale, 0, *xs)
     return ys if pair else ys[0]

@@ -86,7 +86,7 @@ def test_c_abi_refusals():
     st = (ctypes.c_longlong * 12)(*[8] * 12)
     shape = [1, 2, 3, 4, 2, 8, 6]                                        # type, B, T, heads, kv_heads, dk, dv
     fwd = lambda s=shape, q=p, o=p, ws=None, n=0: lib.ringattr_linear_attention_fwd(q, p, p, st, p, None, None, o, None, 1.0, *s, ws, n, None)
-    bwd = lambda s=shape, go=p, gq=p, ws=None, n=0: lib.ringattr_linear_attention_bwd(p, p, p, go, st, p, None, None, None, gq, p, p, None, 1.0, *s,
+    bwd = lambda s=shape, go=p, gq=p, ws=None, n=0: lib.ringattr_linear_attention_bwd(p, p, p, go, st, p, None, None, None, None, gq, p, p, None, 1.0, *s,
                                                                                     ws, n, None)
     step = lambda s, q=p: lib.ringattr_linear_attention_step(q, p, p, st, p, p, None, p, 1.0, *s, None)
     changed = lambda i, x: shape[:i] + [x] + shape[i + 1:]
@@ -104,8 +104,10 @@ def test_c_abi_refusals():
     assert lib.ringattr_linear_attention_fwd_workspace_bytes(*shape) == 0
     need = lib.ringattr_linear_attention_fwd_workspace_bytes(*long)
     assert need > 0 and need % 256 == 0
+    states = [lib.ringattr_linear_attention_bwd_workspace_bytes(*long, have) for have in (0, 1)]
+    assert states == [2 * need, need]                                    # the forward's own states, kept or formed again
     assert fwd(long) == 2 and fwd(long, ws=p, n=need - 1) == 2 and "workspace" in _lib.last_error()
-    assert lib.ringattr_linear_attention_bwd_workspace_bytes(*changed(5, 300)) == 0 and "256" in _lib.last_error()
+    assert lib.ringattr_linear_attention_bwd_workspace_bytes(*changed(5, 300), 0) == 0 and "256" in _lib.last_error()
     one = [1, 2, 4, 2, 8, 6]
     assert step(one, q=None) == 1 and step([1, 2, 4, 3, 8, 6]) == 1 and step([9] + one[1:]) == 1
     rot = lambda kind=0, heads=(2, 0), dim=8, r=8, t=1, x1=None: lib.ringattr_rotary(p, x1, st, p, 0, 1, kind, p, p, None, 1.0, 0, 0, t, 2, 3, *heads, dim,

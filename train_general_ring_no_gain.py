@@ -10,12 +10,15 @@ from train.train_ring_attractor import (
     decode_angle_from_argmax)
 from cpp.ring_rnn_cuda import *  # noqa: F401,F403  (also provides `torch`)
 from rnn_train_ring_attractor_amd.host import (  # noqa: F401
-    GeneralizedRingAttractorNoGain, av_to_action_signal, av_to_action_signal_ND, plot_general_ring_matrices)
+    GeneralizedRingAttractorNoGain, av_to_action_signal, av_to_action_signal_ND, drop_action_signal, plot_general_ring_matrices)
 
 
 def run_training(action_dim=2, num_neurons=256, training_steps=1000, batch_size=128, seq_len=100, lr=1e-3,
-                 activation="gelu", log_every=10, seed=0, fused_loss=False, fused_optimizer=False, hip_graph=False):
-    """hip_graph=True records one training step (action signal, initial bump, time loop, loss head, backward, clipping
+                 activation="gelu", log_every=10, seed=0, fused_loss=False, fused_optimizer=False, hip_graph=False,
+                 input_dropout=0.0):
+    """input_dropout: probability with which a value of the action signal is missing in training, another mask every step (the
+    step's number is kept on the device and advanced by the step itself, recorded or not).
+    hip_graph=True records one training step (action signal, initial bump, time loop, loss head, backward, clipping
     and Adam) into a HIP graph after three eager steps and replays it for the rest of the run: one graph launch per
     step instead of some thirty kernel launches and the Python between them.  It needs both fused options (their
     kernels neither allocate through HIP nor read the device back, and the fused optimizer counts its steps on the
@@ -34,8 +37,10 @@ def run_training(action_dim=2, num_neurons=256, training_steps=1000, batch_size=
     else:
         opt = torch.optim.Adam(model.parameters(), lr=lr)
 
+    steps_done = torch.zeros(1, dtype=torch.int64, device=device)
+
     def train_step(av, target):
-        action = av_to_action_signal_ND(av, action_dim)
+        action = drop_action_signal(av_to_action_signal_ND(av, action_dim), input_dropout, seed % (1 << 64), steps_done)
         r_init = create_initial_bump(target[:, 0], num_neurons, device=device)
         if fused_loss:
             total, loss, _, _ = model.loss_pair(action, target, r_init=r_init, bump_weight=0.2)
@@ -48,6 +53,8 @@ def run_training(action_dim=2, num_neurons=256, training_steps=1000, batch_size=
         if not fused_optimizer:
             torch.nn.utils.clip_grad_norm_(model.parameters(), 1.0)
         opt.step()
+        if input_dropout:
+            steps_done.add_(1)
         return total.detach(), loss.detach()
 
     def report(step, total, loss):
@@ -137,6 +144,8 @@ if __name__ == "__main__":
     ap.add_argument("--fused_optimizer", action="store_true", help="gradient clipping + Adam as one fused HIP step")
     ap.add_argument("--hip_graph", action="store_true",
                     help="record the training step into a HIP graph and replay it (implies both fused options)")
+    ap.add_argument("--input_dropout", type=float, default=0.0, help="probability with which a value of the action signal is missing")
     a = ap.parse_args()
     run_training_and_evaluation(action_dim=a.action_dim, training_steps=a.steps, fused_loss=a.fused_loss or a.hip_graph,
-                                fused_optimizer=a.fused_optimizer or a.hip_graph, hip_graph=a.hip_graph)
+                                fused_optimizer=a.fused_optimizer or a.hip_graph, hip_graph=a.hip_graph,
+                                input_dropout=a.input_dropout)
