@@ -348,7 +348,9 @@ struct RingLinArgs {
   bool scanned;
   const int* lengths;    // tokens of each sequence, null: T
   float intra, inter, update;    // factors of the weights, of what the state gives, of what it takes in
-  int B, T, H, Da, Db, nseg, seg_tokens, slices;
+  int B, T, H, Da, Db, nseg, seg_tokens;
+  bool narrow;           // a workgroup takes 64 columns, not 128
+  int slices;            // workgroups that share the columns
 };
 struct RingLinShape { int B, T, H, G, Dk, Dv, type; float scale; };
 struct RingLinStep {

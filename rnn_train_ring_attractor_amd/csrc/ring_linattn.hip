@@ -21,6 +21,12 @@ hipError_t launch_pass(int type, const RingLinArgs& a, bool rev, bool state_only
 
 int slices(int Db) { return Db <= 64 ? 1 : (Db + 127) / 128; }
 
+void set_columns(RingLinArgs& a, int Db, bool narrow) {
+  a.Db = Db;
+  a.narrow = narrow || Db <= 64;
+  a.slices = a.narrow ? (Db + 63) / 64 : (Db + 127) / 128;
+}
+
 RingLinArgs base(const RingLinShape& s, const float* log_decay, const int* lengths, int nseg) {
   RingLinArgs a = {};
   a.log_decay = log_decay;
@@ -192,14 +198,15 @@ size_t ring_linattn_bwd_bytes(const RingLinShape& s, bool have_states) {
   return n;
 }
 
-// What the segments of Y and Z add to a state (natural states, [Dk][Dv]), or the states behind them, into a.seg
+// What the segments of Y and Z add to a state (natural states, [Dk][Dv]), or the states behind them, into a.seg.  64 columns a
+// workgroup: nothing is formed twice for it, and there are fewer segments here than in the pass behind (us: 8 x 2000 tokens, 8 heads of
+// 256, fp32 220 -> 139; 8 x 4096 tokens, 16 heads of 128, bf16 68 -> 61; one sequence of 32768 71 -> 72).
 static hipError_t segment_states(const RingLinShape& s, RingLinArgs a, bool rev, hipStream_t st) {
   if (a.nseg == 1) return hipSuccess;
   a.Da = s.Dk;
-  a.Db = s.Dv;
   a.sa = s.Dv;
   a.sb = 1;
-  a.slices = slices(s.Dv);
+  set_columns(a, s.Dv, true);
   hipError_t e = launch_pass(s.type, a, rev, true, st);
   if (e != hipSuccess || !a.scanned) return e;
   const unsigned per = (unsigned)((s.Dk * s.Dv + 255) / 256);
@@ -222,10 +229,9 @@ hipError_t ring_linattn_fwd(const RingLinShape& s, const RingLinTensor& q, const
   hipError_t e = segment_states(s, a, false, st);
   if (e != hipSuccess) return e;
   a.Da = s.Dk;
-  a.Db = s.Dv;
   a.sa = s.Dv;
   a.sb = 1;
-  a.slices = slices(a.Db);
+  set_columns(a, s.Dv, false);
   a.out = o;
   a.out_vec = a.Db % epv == 0 && out_fits(a);
   a.intra = a.inter = s.scale;
@@ -267,10 +273,9 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
   f.Y = v;
   f.Z = k;
   f.Da = s.Dv;
-  f.Db = s.Dk;
   f.sa = 1;
   f.sb = s.Dv;
-  f.slices = slices(f.Db);
+  set_columns(f, s.Dk, false);
   f.out = gq;
   f.out_vec = f.Db % epv == 0 && out_fits(f);
   f.intra = f.inter = s.scale;
@@ -280,10 +285,9 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
   r.X = k;
   r.xs = share;
   r.Da = s.Dk;
-  r.Db = s.Dv;
   r.sa = s.Dv;
   r.sb = 1;
-  r.slices = slices(r.Db);
+  set_columns(r, s.Dv, false);
   r.intra = s.scale;
   r.out = share > 1 ? (void*)part_v : gv;
   r.out_f32 = share > 1;
@@ -295,10 +299,9 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
   r.Y = go;
   r.Z = q;
   r.Da = s.Dv;
-  r.Db = s.Dk;
   r.sa = 1;
   r.sb = s.Dv;
-  r.slices = slices(r.Db);
+  set_columns(r, s.Dk, false);
   r.s_out = nullptr;
   r.out = share > 1 ? (void*)part_k : gk;
   r.out_vec = r.Db % epv == 0 && out_fits(r);

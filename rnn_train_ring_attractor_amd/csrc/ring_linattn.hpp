@@ -197,7 +197,12 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
   typedef Filler<T, CH, DA, VEC> FA;
   typedef Filler<T, CH, WC, VEC> FZ;
   constexpr int XB = STATE_ONLY ? 0 : TA::BYTES, BUF = XB + TA::BYTES + TZ::BYTES;
+  // The weights of fp32 products: a wave forms a quarter of the contraction and the four are added up in LDS (with bf16 products there is
+  // nothing to gain: a quarter of the products less is what the exchange takes).
+  constexpr int STEPS = DA / (64 / (int)sizeof(T)), TPS = DT / STEPS;          // steps of 64 bytes a row, tiles of the state in each
+  constexpr bool SHARED = !BF && !STATE_ONLY && STEPS % 4 == 0;
   __shared__ __align__(16) char lds[2 * BUF];
+  __shared__ __align__(16) f32x4 shares[SHARED ? 4 * CT * CT * 64 : 1];
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 15, g = (tid >> 4) & 3;
   // `order` counts the segments as they follow each other; the pass over states has no use for the last
@@ -417,13 +422,36 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
 #pragma unroll
         for (int it = 0; it < CT; ++it) P[jt][it] = f32x4{0.f, 0.f, 0.f, 0.f};
       // O = S X^T, what the state in front gives, and P = Y X^T, the weights; rows are read a step ahead
-      constexpr int STEPS = DA / (64 / (int)sizeof(T)), TPS = DT / STEPS;      // steps of 64 bytes a row, tiles of the state in each
       typename TA::V16 xr[2][CT], yr[2][CT];
+      if constexpr (SHARED) {
+#pragma unroll
+        for (int q = 0; q < STEPS / 4; ++q) {
+          const int s = w * (STEPS / 4) + q;
+          typename TA::V16 x[CT], y[CT];
+#pragma unroll
+          for (int it = 0; it < CT; ++it) {
+            x[it] = TA::rows(lx, rows1, it, s);
+            y[it] = TA::rows(ly, rows1, it, s);
+          }
+#pragma unroll
+          for (int e = 0; e < 16 / (int)sizeof(T); ++e)
+#pragma unroll
+            for (int it = 0; it < CT; ++it)
+#pragma unroll
+              for (int jt = 0; jt < CT; ++jt)
+                if (REV ? jt >= it : jt <= it) P[jt][it] = mfma4((float)y[jt][e], (float)x[it][e], P[jt][it]);
+        }
+#pragma unroll
+        for (int it = 0; it < CT; ++it)
+#pragma unroll
+          for (int jt = 0; jt < CT; ++jt)
+            if (REV ? jt >= it : jt <= it) shares[((w * CT + jt) * CT + it) * 64 + (tid & 63)] = P[jt][it];
+      }
       auto read = [&](int s) {
 #pragma unroll
         for (int it = 0; it < CT; ++it) {
           xr[s & 1][it] = TA::rows(lx, rows1, it, s);
-          yr[s & 1][it] = TA::rows(ly, rows1, it, s);
+          if (!SHARED) yr[s & 1][it] = TA::rows(ly, rows1, it, s);
         }
       };
       read(0);
@@ -453,13 +481,13 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
 #pragma unroll
               for (int it = 0; it < CT; ++it) {
                 x[it] = (float)xr[s & 1][it][4 * q + r];
-                y[it] = (float)yr[s & 1][it][4 * q + r];
+                y[it] = SHARED ? 0.f : (float)yr[s & 1][it][4 * q + r];
               }
 #pragma unroll
               for (int it = 0; it < CT; ++it)
 #pragma unroll
                 for (int jt = 0; jt < CT; ++jt)
-                  if (REV ? jt >= it : jt <= it) P[jt][it] = mfma4(y[jt], x[it], P[jt][it]);
+                  if (!SHARED && (REV ? jt >= it : jt <= it)) P[jt][it] = mfma4(y[jt], x[it], P[jt][it]);
 #pragma unroll
               for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
@@ -475,6 +503,19 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
       for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
         for (int it = 0; it < CT; ++it) O[ct][it] *= inner[it];
+      if constexpr (SHARED) {
+        lds_barrier();
+#pragma unroll
+        for (int it = 0; it < CT; ++it)
+#pragma unroll
+          for (int jt = 0; jt < CT; ++jt)
+            if (REV ? jt >= it : jt <= it) {
+              f32x4 part[4];
+#pragma unroll
+              for (int v = 0; v < 4; ++v) part[v] = shares[((v * CT + jt) * CT + it) * 64 + (tid & 63)];
+              P[jt][it] = (part[0] + part[1]) + (part[2] + part[3]);
+            }
+      }
       // what is not to be seen is left out, not multiplied by zero: it may be anything
 #pragma unroll
       for (int jt = 0; jt < CT; ++jt)
@@ -639,38 +680,39 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
   }
 }
 
-template <typename T, int DA, int NC, bool VEC> hipError_t launch_sized(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
+// EXACT: a state here is a result (only bf16 rows have another way to one that is not)
+template <typename T, int DA, int NC, bool VEC, bool REV> hipError_t launch_sized(const RingLinArgs& a, bool state_only, hipStream_t st) {
   constexpr int CT = sizeof(T) == 4 ? 1 : 2;
+  constexpr bool BF = Type<T>::BF;
   const dim3 grid((unsigned)((long)(state_only ? a.nseg - 1 : a.nseg) * a.slices * a.H * a.B)), block(256);
-  // (EXACT: only bf16 rows have another way to a state that nobody sees)
-  constexpr bool SHORT = !Type<T>::BF;
+  const bool exact = !BF || a.s_out;
   if (state_only) {
-    if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, true, true, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, false, true, true>), grid, block, 0, st, a);
-  } else if (!SHORT && a.s_out) {
-    if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, true, false, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, false, false, true>), grid, block, 0, st, a);
+    if constexpr (NC == 1) {                                   // (see segment_states)
+      if (exact) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, REV, true, true>), grid, block, 0, st, a);
+      else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, REV, true, !BF>), grid, block, 0, st, a);
+    }
   } else {
-    if (rev) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, true, false, SHORT>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, false, false, SHORT>), grid, block, 0, st, a);
+    if (exact) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, REV, false, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, REV, false, !BF>), grid, block, 0, st, a);
   }
   return hipGetLastError();
 }
 
-template <typename T, bool VEC> hipError_t launch_access(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
-  if (a.Db <= 64) {
-    if (a.Da <= 64) return launch_sized<T, 64, 1, VEC>(a, rev, state_only, st);
-    if (a.Da <= 128) return launch_sized<T, 128, 1, VEC>(a, rev, state_only, st);
-    return launch_sized<T, 256, 1, VEC>(a, rev, state_only, st);
+template <typename T, bool VEC, bool REV> hipError_t launch_access(const RingLinArgs& a, bool state_only, hipStream_t st) {
+  if (a.narrow) {
+    if (a.Da <= 64) return launch_sized<T, 64, 1, VEC, REV>(a, state_only, st);
+    if (a.Da <= 128) return launch_sized<T, 128, 1, VEC, REV>(a, state_only, st);
+    return launch_sized<T, 256, 1, VEC, REV>(a, state_only, st);
   }
-  if (a.Da <= 64) return launch_sized<T, 64, 2, VEC>(a, rev, state_only, st);
-  if (a.Da <= 128) return launch_sized<T, 128, 2, VEC>(a, rev, state_only, st);
-  return launch_sized<T, 256, 2, VEC>(a, rev, state_only, st);
+  if (a.Da <= 64) return launch_sized<T, 64, 2, VEC, REV>(a, state_only, st);
+  if (a.Da <= 128) return launch_sized<T, 128, 2, VEC, REV>(a, state_only, st);
+  return launch_sized<T, 256, 2, VEC, REV>(a, state_only, st);
 }
 
 template <typename T> hipError_t launch(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
   const bool vec = a.Y.vec && a.Z.vec && (state_only || (a.X.vec && a.out_vec));
-  return vec ? launch_access<T, true>(a, rev, state_only, st) : launch_access<T, false>(a, rev, state_only, st);
+  if (rev) return vec ? launch_access<T, true, true>(a, state_only, st) : launch_access<T, false, true>(a, state_only, st);
+  return vec ? launch_access<T, true, false>(a, state_only, st) : launch_access<T, false, false>(a, state_only, st);
 }
 
 }  // namespace ring_lin
