@@ -107,6 +107,8 @@ def library_path() -> str:
 def load():
     """Return the loaded library, building it first if no prebuilt file exists."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -196,8 +198,13 @@ _HERE = _Here()
 
 
 def on_device(device):
-    """`torch.cuda.device(device)` for a tensor's device; nothing to enter and leave where it is the current one."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    """`torch.cuda.device(device)` for a tensor's device; nothing to enter and leave where it is the current one.  (The question
+    without the checks around it, where torch still has that private name: there is a tensor on the device.)"""
+    try:
+        here = torch._C._cuda_getDevice()
+    except AttributeError:
+        here = torch.cuda.current_device()
+    return _HERE if here == device.index else torch.cuda.device(device)
 
 
 def stream_handle(device) -> int:

@@ -6,7 +6,7 @@ using namespace ring_lin;
 
 namespace {
 
-constexpr int kChunk = 32;
+constexpr int kChunk = 64;            // segments are whole numbers of these tokens
 // Up to so many segments a workgroup adds up what those in front have added itself; past that a scan does, a launch more but less to read
 // (8 x 4096 tokens, 16 heads of 128 in four segments, us a pass of the chunk kernel: 165 adding up itself, 130 and a scan of 17).
 constexpr int kFold = 2;
@@ -173,11 +173,11 @@ static int segments(const RingLinShape& s) {
     return (double)(work / at_once) * (one ? 1.0 : 1.6) + (rest == 0 ? 0.0 : (one || rest <= 256 ? 1.0 : 1.6));
   };
   int best = 1;
-  double least = rounds(groups) * chunks;
-  for (int n = 2; n <= 64 && 2 * n <= chunks; ++n) {
+  double least = rounds(groups) * 2 * chunks;
+  for (int n = 2; n <= 64 && n <= chunks; ++n) {
     const int per = (chunks + n - 1) / n;
     if ((chunks + per - 1) / per != n) continue;
-    const double t = per * (rounds(groups * n) + 0.45 * rounds(groups * (n - 1))) + 3.0 + (n > kFold ? 3.0 : 0.0);
+    const double t = 2 * per * (rounds(groups * n) + 0.45 * rounds(groups * (n - 1))) + 3.0 + (n > kFold ? 3.0 : 0.0);
     if (t < least) {
       least = t;
       best = n;
@@ -200,7 +200,8 @@ size_t ring_linattn_bwd_bytes(const RingLinShape& s, bool have_states) {
 
 // What the segments of Y and Z add to a state (natural states, [Dk][Dv]), or the states behind them, into a.seg.  64 columns a
 // workgroup: nothing is formed twice for it, and there are fewer segments here than in the pass behind (us: 8 x 2000 tokens, 8 heads of
-// 256, fp32 220 -> 139; 8 x 4096 tokens, 16 heads of 128, bf16 68 -> 61; one sequence of 32768 71 -> 72).
+// 256, fp32 220 -> 139; 8 x 4096 tokens, 16 heads of 128, bf16 68 -> 61; one sequence of 32768 71 -> 72).  fp32 products take chunks of
+// twice the tokens (139 -> 121; bf16 72 -> 77).
 static hipError_t segment_states(const RingLinShape& s, RingLinArgs a, bool rev, hipStream_t st) {
   if (a.nseg == 1) return hipSuccess;
   a.Da = s.Dk;

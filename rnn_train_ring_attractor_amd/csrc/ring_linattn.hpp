@@ -76,8 +76,7 @@ template <typename T, bool PAIR> __device__ __forceinline__ int place(int i, int
 // function of the row, such that what one instruction reads lies in all banks: 16 rows at one place (`rows`), 8 rows at two
 // neighbouring places by the transposing read of 16-bit values, 4 rows at four by single words (`columns`).
 template <typename T, int ROWS, int COLS> struct Tile16 {
-  static constexpr int EPV = 16 / sizeof(T), GPR = COLS / EPV, RB = COLS * sizeof(T), BYTES = ROWS * RB, NU = ROWS * GPR / 256;
-  static_assert(ROWS * GPR % 256 == 0 && 256 % GPR == 0, "");
+  static constexpr int EPV = 16 / sizeof(T), GPR = COLS / EPV, RB = COLS * sizeof(T), BYTES = ROWS * RB;
   typedef typename Type<T>::V4 V4;
 
   static __device__ __forceinline__ int turn(int row) {
@@ -136,9 +135,10 @@ __device__ __forceinline__ unsigned lds_address(const void* p) {
 }
 
 // Fills a tile: rows 0..n-1 of `cols` values from base on, token stride st; what is not loaded is left as it is.
-template <typename T, int ROWS, int COLS, bool VEC> struct Filler {
+template <typename T, int ROWS, int COLS, int NT, bool VEC> struct Filler {
   typedef Tile16<T, ROWS, COLS> Tl;
-  static constexpr int EPV = Tl::EPV, GPR = Tl::GPR, NU = Tl::NU, RS = 256 / GPR;
+  static constexpr int EPV = Tl::EPV, GPR = Tl::GPR, NU = ROWS * GPR / NT, RS = NT / GPR;      // granules of a thread, rows between them
+  static_assert(ROWS * GPR % NT == 0 && NT % GPR == 0, "");
   unsigned off[NU];                                            // byte offsets of the thread's granules in a whole chunk
 
   __device__ __forceinline__ void init(long st, int tid) {
@@ -155,7 +155,7 @@ template <typename T, int ROWS, int COLS, bool VEC> struct Filler {
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         const int row = tid / GPR + u * RS, c = ((tid % GPR) ^ Tl::turn(row)) * EPV;
-        if (WHOLE || (row < n && c < cols)) load_to_lds(base, off[u], lds + u * 4096);
+        if (WHOLE || (row < n && c < cols)) load_to_lds(base, off[u], lds + u * NT * 16);
       }
     } else {
 #pragma unroll
@@ -164,14 +164,14 @@ template <typename T, int ROWS, int COLS, bool VEC> struct Filler {
         T v[EPV];
 #pragma unroll
         for (int e = 0; e < EPV; ++e) v[e] = row < n && c + e < cols ? base[(long)row * st + c + e] : (T)0.f;
-        if (row < n) *reinterpret_cast<u32x4*>(tile + (tid + u * 256) * 16) = *reinterpret_cast<const u32x4*>(v);
+        if (row < n) *reinterpret_cast<u32x4*>(tile + (tid + u * NT) * 16) = *reinterpret_cast<const u32x4*>(v);
       }
     }
   }
   static __device__ __forceinline__ void clear(char* tile, int from, int tid) {
 #pragma unroll
     for (int u = 0; u < NU; ++u)
-      if (tid / GPR + u * RS >= from) *reinterpret_cast<u32x4*>(tile + (tid + u * 256) * 16) = u32x4{0, 0, 0, 0};
+      if (tid / GPR + u * RS >= from) *reinterpret_cast<u32x4*>(tile + (tid + u * NT) * 16) = u32x4{0, 0, 0, 0};
   }
 };
 
@@ -183,26 +183,26 @@ template <int N> __device__ __forceinline__ void wait_and_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// A workgroup: one head of one sequence, WC = 64 NC columns of Z and of the state, one segment of the tokens.  Its waves share the
+// A workgroup: one head of one sequence, WC = 16 NC NW columns of Z and of the state, one segment of the tokens.  Its waves share the
 // chunk's rows in LDS (two buffers: the next chunk's are on their way while one is worked on); each keeps 16 NC columns of the state
 // in registers, where they are an operand as they lie: the matrix units put rows 4g..4g+3 of column l into lane (g, l) and take them
 // as contraction indices from there.  The weights are formed transposed for the same reason, by every wave for itself.
-template <typename T, int DA, int NC, int CT, bool VEC, bool REV, bool STATE_ONLY, bool EXACT>
-__global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(RingLinArgs p) {
-  constexpr int WC = 64 * NC, CH = 16 * CT, DT = DA / 16;
+template <typename T, int DA, int NC, int NW, int CT, bool VEC, bool REV, bool STATE_ONLY, bool EXACT>
+__global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_linattn_kernel(RingLinArgs p) {
+  constexpr int WC = 16 * NC * NW, NT = 64 * NW, CH = 16 * CT, DT = DA / 16;
   constexpr bool BF = Type<T>::BF;
   typedef typename Type<T>::V4 V4;
   typedef Tile16<T, CH, DA> TA;
   typedef Tile16<T, CH, WC> TZ;
-  typedef Filler<T, CH, DA, VEC> FA;
-  typedef Filler<T, CH, WC, VEC> FZ;
+  typedef Filler<T, CH, DA, NT, VEC> FA;
+  typedef Filler<T, CH, WC, NT, VEC> FZ;
   constexpr int XB = STATE_ONLY ? 0 : TA::BYTES, BUF = XB + TA::BYTES + TZ::BYTES;
-  // The weights of fp32 products: a wave forms a quarter of the contraction and the four are added up in LDS (with bf16 products there is
-  // nothing to gain: a quarter of the products less is what the exchange takes).
+  // The weights of fp32 products: each wave forms a part of the contraction and the parts are added up in LDS (with bf16 products there
+  // is nothing to gain: what the products take less is what the exchange takes).
   constexpr int STEPS = DA / (64 / (int)sizeof(T)), TPS = DT / STEPS;          // steps of 64 bytes a row, tiles of the state in each
-  constexpr bool SHARED = !BF && !STATE_ONLY && STEPS % 4 == 0;
+  constexpr bool SHARED = !BF && !STATE_ONLY && STEPS % NW == 0;
   __shared__ __align__(16) char lds[2 * BUF];
-  __shared__ __align__(16) f32x4 shares[SHARED ? 4 * CT * CT * 64 : 1];
+  __shared__ __align__(16) f32x4 shares[SHARED ? NW * CT * CT * 64 : 1];
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 15, g = (tid >> 4) & 3;
   // `order` counts the segments as they follow each other; the pass over states has no use for the last
@@ -425,8 +425,8 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
       typename TA::V16 xr[2][CT], yr[2][CT];
       if constexpr (SHARED) {
 #pragma unroll
-        for (int q = 0; q < STEPS / 4; ++q) {
-          const int s = w * (STEPS / 4) + q;
+        for (int q = 0; q < STEPS / NW; ++q) {
+          const int s = w * (STEPS / NW) + q;
           typename TA::V16 x[CT], y[CT];
 #pragma unroll
           for (int it = 0; it < CT; ++it) {
@@ -510,10 +510,14 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
 #pragma unroll
           for (int jt = 0; jt < CT; ++jt)
             if (REV ? jt >= it : jt <= it) {
-              f32x4 part[4];
+              f32x4 part[NW];
 #pragma unroll
-              for (int v = 0; v < 4; ++v) part[v] = shares[((v * CT + jt) * CT + it) * 64 + (tid & 63)];
-              P[jt][it] = (part[0] + part[1]) + (part[2] + part[3]);
+              for (int v = 0; v < NW; ++v) part[v] = shares[((v * CT + jt) * CT + it) * 64 + (tid & 63)];
+#pragma unroll
+              for (int v = NW / 2; v > 0; v /= 2)
+#pragma unroll
+                for (int x = 0; x < v; ++x) part[x] += part[x + v];
+              P[jt][it] = part[0];
             }
       }
       // what is not to be seen is left out, not multiplied by zero: it may be anything
@@ -681,32 +685,34 @@ __global__ __launch_bounds__(256, (DA <= 128 ? 2 : 1)) void ring_linattn_kernel(
 }
 
 // EXACT: a state here is a result (only bf16 rows have another way to one that is not)
-template <typename T, int DA, int NC, bool VEC, bool REV> hipError_t launch_sized(const RingLinArgs& a, bool state_only, hipStream_t st) {
-  constexpr int CT = sizeof(T) == 4 ? 1 : 2;
+template <typename T, int DA, int NC, int NW, bool VEC, bool REV> hipError_t launch_sized(const RingLinArgs& a, bool state_only, hipStream_t st) {
   constexpr bool BF = Type<T>::BF;
-  const dim3 grid((unsigned)((long)(state_only ? a.nseg - 1 : a.nseg) * a.slices * a.H * a.B)), block(256);
+  constexpr int CT = sizeof(T) == 4 ? 1 : 2, CTS = BF ? CT : 2 * CT;           // tiles of a chunk; for states alone (see segment_states)
+  const dim3 grid((unsigned)((long)(state_only ? a.nseg - 1 : a.nseg) * a.slices * a.H * a.B)), block(64 * NW);
   const bool exact = !BF || a.s_out;
   if (state_only) {
-    if constexpr (NC == 1) {                                   // (see segment_states)
-      if (exact) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, REV, true, true>), grid, block, 0, st, a);
-      else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, REV, true, !BF>), grid, block, 0, st, a);
+    if constexpr (NC == 1 && NW == 4) {                        // (see segment_states)
+      if (exact) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, NW, CTS, VEC, REV, true, true>), grid, block, 0, st, a);
+      else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, NW, CTS, VEC, REV, true, !BF>), grid, block, 0, st, a);
     }
   } else {
-    if (exact) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, REV, false, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, CT, VEC, REV, false, !BF>), grid, block, 0, st, a);
+    if (exact) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, NW, CT, VEC, REV, false, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, NW, CT, VEC, REV, false, !BF>), grid, block, 0, st, a);
   }
   return hipGetLastError();
 }
 
+// Wide heads (a state of 256 rows): four waves of 32 columns fill the registers, one wave a SIMD.  fp32 products take eight waves of 16
+// instead, two a SIMD (WIDE_FIGURES); bf16 products would form the weights twice as often.
 template <typename T, bool VEC, bool REV> hipError_t launch_access(const RingLinArgs& a, bool state_only, hipStream_t st) {
   if (a.narrow) {
-    if (a.Da <= 64) return launch_sized<T, 64, 1, VEC, REV>(a, state_only, st);
-    if (a.Da <= 128) return launch_sized<T, 128, 1, VEC, REV>(a, state_only, st);
-    return launch_sized<T, 256, 1, VEC, REV>(a, state_only, st);
+    if (a.Da <= 64) return launch_sized<T, 64, 1, 4, VEC, REV>(a, state_only, st);
+    if (a.Da <= 128) return launch_sized<T, 128, 1, 4, VEC, REV>(a, state_only, st);
+    return launch_sized<T, 256, 1, 4, VEC, REV>(a, state_only, st);
   }
-  if (a.Da <= 64) return launch_sized<T, 64, 2, VEC, REV>(a, state_only, st);
-  if (a.Da <= 128) return launch_sized<T, 128, 2, VEC, REV>(a, state_only, st);
-  return launch_sized<T, 256, 2, VEC, REV>(a, state_only, st);
+  if (a.Da <= 64) return launch_sized<T, 64, 2, 4, VEC, REV>(a, state_only, st);
+  if (a.Da <= 128) return launch_sized<T, 128, 2, 4, VEC, REV>(a, state_only, st);
+  return launch_sized<T, 256, Type<T>::BF ? 2 : 1, Type<T>::BF ? 4 : 8, VEC, REV>(a, state_only, st);
 }
 
 template <typename T> hipError_t launch(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {

@@ -56,14 +56,14 @@ def _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state):
     G, Dv, dev = k.shape[2], v.shape[3], q.device
     lib, kind = _lib.load(), SEQUENCE_TYPES[q.dtype]
     with _lib.on_device(dev):
-        o = torch.empty(B, T, H, Dv, dtype=q.dtype, device=dev)
-        state = torch.empty(B, H, Dk, Dv, dtype=torch.float32, device=dev) if want_state else None
+        o = q.new_empty((B, T, H, Dv))
+        state = log_decay.new_empty((B, H, Dk, Dv)) if want_state else None
         if B == 0 or T == 0:
             if want_state:
                 state.zero_() if initial_state is None else state.copy_(initial_state)
             return o, state, None
         nbytes = lib.ringattr_linear_attention_fwd_workspace_bytes(kind, B, T, H, G, Dk, Dv)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        ws = log_decay.new_empty((nbytes // 4,)) if nbytes else None
         strides = _Strides9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
         _lib.check(lib.ringattr_linear_attention_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, log_decay.data_ptr(), _ptr(initial_state), _ptr(lengths), o.data_ptr(),
@@ -89,17 +89,17 @@ class LinearAttentionFunc(Function):
         G, Dv, dev = k.shape[2], v.shape[3], q.device
         lib, kind = _lib.load(), SEQUENCE_TYPES[q.dtype]
         with _lib.on_device(dev):
-            gq, gk, gv = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k, v))
+            gq, gk, gv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
             want = initial_state is not None and ctx.needs_input_grad[4]
-            g0 = torch.empty(B, H, Dk, Dv, dtype=torch.float32, device=dev) if want else None
-            gs = None if grad_state is None else grad_state.to(torch.float32).contiguous()
+            g0 = log_decay.new_empty((B, H, Dk, Dv)) if want else None
+            gs = None if grad_state is None else grad_state.contiguous()
             if B == 0 or T == 0:
                 if want:
                     g0.zero_() if gs is None else g0.copy_(gs)
             else:
-                go = torch.zeros(B, T, H, Dv, dtype=q.dtype, device=dev) if grad_o is None else _rows(grad_o.to(q.dtype))
+                go = q.new_zeros((B, T, H, Dv)) if grad_o is None else _rows(grad_o)
                 nbytes = lib.ringattr_linear_attention_bwd_workspace_bytes(kind, B, T, H, G, Dk, Dv, along is not None)
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+                ws = log_decay.new_empty((nbytes // 4,)) if nbytes else None
                 strides = _Strides12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *go.stride()[:3])
                 _lib.check(lib.ringattr_linear_attention_bwd(
                     q.data_ptr(), k.data_ptr(), v.data_ptr(), go.data_ptr(), strides, log_decay.data_ptr(), _ptr(initial_state),
@@ -157,7 +157,7 @@ def linear_attention_step(q, k, v, log_decay, state, active=None, scale=None):
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
     lib = _lib.load()
     with _lib.on_device(dev):
-        o = torch.empty(B, H, Dv, dtype=q.dtype, device=dev)
+        o = q.new_empty((B, H, Dv))
         if B == 0:
             return o
         strides = _Strides6(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])

@@ -60,7 +60,7 @@ def _turn(xs, positions, frequencies, layout, scale, inverse):
     xs = [x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous() for x in xs]
     lib = _lib.load()
     with _lib.on_device(dev):
-        ys = [torch.empty(x.shape, dtype=x.dtype, device=dev) for x in xs]
+        ys = [x.new_empty(x.shape) for x in xs]
         if B == 0 or T == 0:
             return ys
         strides = [s for x in xs for s in x.stride()[:3]]
