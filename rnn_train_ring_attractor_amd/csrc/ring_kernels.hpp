@@ -337,6 +337,9 @@ struct RingLinTensor {
 struct RingLinArgs {
   RingLinTensor X, Y, Z;
   int xs, ys, zs;        // heads that share one of the tensor's
+  RingLinTensor X2;      // two passes at once: rows X2 (Db wide) against rows Z weigh rows Y into out2, the state transposed
+  int x2s;
+  void* out2;
   void* out;             // [B,T,H,Db] in the type of the rows, or in fp32 (out_f32)
   bool out_f32, out_vec; // out_vec: rows are whole numbers of 16 bytes, a token's less than 16 MiB
   const float* log_decay;
@@ -369,8 +372,11 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
                             const RingLinTensor& go, const float* gs, void* gq, void* gk, void* gv, float* gs_in, void* ws, hipStream_t st);
 hipError_t ring_linattn_step(const RingLinShape& s, const RingLinStep& a, hipStream_t st);
 hipError_t ring_launch_linattn_f32(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st);
+hipError_t ring_launch_linattn_pair_f32(const RingLinArgs& a, hipStream_t st);
 hipError_t ring_launch_linattn_bf16(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st);
+hipError_t ring_launch_linattn_pair_bf16(const RingLinArgs& a, hipStream_t st);
 hipError_t ring_launch_linattn_f16(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st);
+hipError_t ring_launch_linattn_pair_f16(const RingLinArgs& a, hipStream_t st);
 
 // Rotary positions (ring_rotary.hip) of one tensor or two ([B,T,heads,D], heads[1] = 0: one)
 struct RingRotaryArgs {

@@ -7,7 +7,7 @@ using namespace ring_lin;
 namespace {
 
 constexpr int kChunk = 64;            // segments are whole numbers of these tokens
-// Up to so many segments a workgroup adds up what those in front have added itself; past that a scan does, a launch more but less to read
+// Of so many segments the second adds what the first has added to the initial state itself; of more a scan does, a launch more but less to read
 // (8 x 4096 tokens, 16 heads of 128 in four segments, us a pass of the chunk kernel: 165 adding up itself, 130 and a scan of 17).
 constexpr int kFold = 2;
 
@@ -198,6 +198,12 @@ size_t ring_linattn_bwd_bytes(const RingLinShape& s, bool have_states) {
   return n;
 }
 
+static hipError_t launch_two(int type, const RingLinArgs& a, hipStream_t st) {
+  if (type == RINGATTR_F32) return ring_launch_linattn_pair_f32(a, st);
+  if (type == RINGATTR_BF16) return ring_launch_linattn_pair_bf16(a, st);
+  return ring_launch_linattn_pair_f16(a, st);
+}
+
 // What the segments of Y and Z add to a state (natural states, [Dk][Dv]), or the states behind them, into a.seg.  64 columns a
 // workgroup: nothing is formed twice for it, and there are fewer segments here than in the pass behind (us: 8 x 2000 tokens, 8 heads of
 // 256, fp32 220 -> 139; 8 x 4096 tokens, 16 heads of 128, bf16 68 -> 61; one sequence of 32768 71 -> 72).  fp32 products take chunks of
@@ -249,6 +255,12 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
   w += (states ? 1 : 2) * each;
   float *part_k = (float*)w, *part_v = (float*)(w + round_up((size_t)s.B * s.T * s.H * s.Dk * sizeof(float)));
   hipError_t e;
+  auto launch_shares = [&]() {
+    hipError_t f = launch_share(s.type, part_k, gk, share, s.Dk, (size_t)s.B * s.T * s.G * s.Dk, st);
+    return f != hipSuccess ? f : launch_share(s.type, part_v, gv, share, s.Dv, (size_t)s.B * s.T * s.G * s.Dv, st);
+  };
+  // dv and dk read the same rows and go backwards together where one kernel does both
+  const bool together = s.Dk <= 128 && s.Dv <= 128 && (s.Dk <= 64) == (s.Dv <= 64);
   RingLinArgs f = base(s, log_decay, lengths, nseg), r = f;
   f.s_in = s_in;
   f.seg = seg_f;
@@ -293,6 +305,15 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
   r.out = share > 1 ? (void*)part_v : gv;
   r.out_f32 = share > 1;
   r.out_vec = r.Db % epv == 0 && out_fits(r);
+  if (together) {
+    r.X2 = v;
+    r.x2s = share;
+    r.out2 = share > 1 ? (void*)part_k : gk;
+    r.out_vec = r.out_vec && r.Da % epv == 0 && (long)s.H * r.Da < (1 << 22);
+    e = launch_two(s.type, r, st);
+    if (e != hipSuccess || share == 1) return e;
+    return launch_shares();
+  }
   e = launch_pass(s.type, r, true, false, st);
   if (e != hipSuccess) return e;
   // dk: v against do weighs q, the state transposed
@@ -308,7 +329,5 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
   r.out_vec = r.Db % epv == 0 && out_fits(r);
   e = launch_pass(s.type, r, true, false, st);
   if (e != hipSuccess || share == 1) return e;
-  e = launch_share(s.type, part_k, gk, share, s.Dk, (size_t)s.B * s.T * s.G * s.Dk, st);
-  if (e != hipSuccess) return e;
-  return launch_share(s.type, part_v, gv, share, s.Dv, (size_t)s.B * s.T * s.G * s.Dv, st);
+  return launch_shares();
 }

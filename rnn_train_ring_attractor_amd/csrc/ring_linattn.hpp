@@ -137,8 +137,9 @@ __device__ __forceinline__ unsigned lds_address(const void* p) {
 // Fills a tile: rows 0..n-1 of `cols` values from base on, token stride st; what is not loaded is left as it is.
 template <typename T, int ROWS, int COLS, int NT, bool VEC> struct Filler {
   typedef Tile16<T, ROWS, COLS> Tl;
-  static constexpr int EPV = Tl::EPV, GPR = Tl::GPR, NU = ROWS * GPR / NT, RS = NT / GPR;      // granules of a thread, rows between them
-  static_assert(ROWS * GPR % NT == 0 && NT % GPR == 0, "");
+  // (the first FT threads fill it: granules of a thread, rows between them)
+  static constexpr int FT = ROWS * Tl::GPR < NT ? ROWS * Tl::GPR : NT, EPV = Tl::EPV, GPR = Tl::GPR, NU = ROWS * GPR / FT, RS = FT / GPR;
+  static_assert(ROWS * GPR % FT == 0 && FT % GPR == 0 && FT % 64 == 0, "");
   unsigned off[NU];                                            // byte offsets of the thread's granules in a whole chunk
 
   __device__ __forceinline__ void init(long st, int tid) {
@@ -150,12 +151,13 @@ template <typename T, int ROWS, int COLS, int NT, bool VEC> struct Filler {
   }
   // WHOLE: all rows and columns are there
   template <bool WHOLE> __device__ __forceinline__ void fill(char* tile, const T* base, long st, int n, int cols, int tid) const {
+    if (FT < NT && tid >= FT) return;
     if constexpr (VEC) {
       const unsigned lds = __builtin_amdgcn_readfirstlane(lds_address(tile) + (tid >> 6) * 1024);
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         const int row = tid / GPR + u * RS, c = ((tid % GPR) ^ Tl::turn(row)) * EPV;
-        if (WHOLE || (row < n && c < cols)) load_to_lds(base, off[u], lds + u * NT * 16);
+        if (WHOLE || (row < n && c < cols)) load_to_lds(base, off[u], lds + u * FT * 16);
       }
     } else {
 #pragma unroll
@@ -164,14 +166,15 @@ template <typename T, int ROWS, int COLS, int NT, bool VEC> struct Filler {
         T v[EPV];
 #pragma unroll
         for (int e = 0; e < EPV; ++e) v[e] = row < n && c + e < cols ? base[(long)row * st + c + e] : (T)0.f;
-        if (row < n) *reinterpret_cast<u32x4*>(tile + (tid + u * NT) * 16) = *reinterpret_cast<const u32x4*>(v);
+        if (row < n) *reinterpret_cast<u32x4*>(tile + (tid + u * FT) * 16) = *reinterpret_cast<const u32x4*>(v);
       }
     }
   }
   static __device__ __forceinline__ void clear(char* tile, int from, int tid) {
+    if (FT < NT && tid >= FT) return;
 #pragma unroll
     for (int u = 0; u < NU; ++u)
-      if (tid / GPR + u * RS >= from) *reinterpret_cast<u32x4*>(tile + (tid + u * NT) * 16) = u32x4{0, 0, 0, 0};
+      if (tid / GPR + u * RS >= from) *reinterpret_cast<u32x4*>(tile + (tid + u * FT) * 16) = u32x4{0, 0, 0, 0};
   }
 };
 
@@ -187,24 +190,28 @@ template <int N> __device__ __forceinline__ void wait_and_barrier() {
 // chunk's rows in LDS (two buffers: the next chunk's are on their way while one is worked on); each keeps 16 NC columns of the state
 // in registers, where they are an operand as they lie: the matrix units put rows 4g..4g+3 of column l into lane (g, l) and take them
 // as contraction indices from there.  The weights are formed transposed for the same reason, by every wave for itself.
-template <typename T, int DA, int NC, int NW, int CT, bool VEC, bool REV, bool STATE_ONLY, bool EXACT>
+template <typename T, int DA, int NC, int NW, int CT, bool VEC, bool REV, bool STATE_ONLY, bool EXACT, bool PAIR = false>
 __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_linattn_kernel(RingLinArgs p) {
-  constexpr int WC = 16 * NC * NW, NT = 64 * NW, CH = 16 * CT, DT = DA / 16;
+  constexpr int GW = PAIR ? NW / 2 : NW, WC = 16 * NC * GW, NT = 64 * NW, CH = 16 * CT, DT = DA / 16;
+  static_assert(!PAIR || (WC == DA && !STATE_ONLY), "");
   constexpr bool BF = Type<T>::BF;
   typedef typename Type<T>::V4 V4;
   typedef Tile16<T, CH, DA> TA;
   typedef Tile16<T, CH, WC> TZ;
   typedef Filler<T, CH, DA, NT, VEC> FA;
   typedef Filler<T, CH, WC, NT, VEC> FZ;
-  constexpr int XB = STATE_ONLY ? 0 : TA::BYTES, BUF = XB + TA::BYTES + TZ::BYTES;
+  constexpr int XB = STATE_ONLY ? 0 : TA::BYTES, BUF = XB + TA::BYTES + TZ::BYTES + (PAIR ? TA::BYTES : 0);
   // The weights of fp32 products: each wave forms a part of the contraction and the parts are added up in LDS (with bf16 products there
   // is nothing to gain: what the products take less is what the exchange takes).
   constexpr int STEPS = DA / (64 / (int)sizeof(T)), TPS = DT / STEPS;          // steps of 64 bytes a row, tiles of the state in each
-  constexpr bool SHARED = !BF && !STATE_ONLY && STEPS % NW == 0;
+  constexpr bool SHARED = !BF && !STATE_ONLY && STEPS % GW == 0;
   __shared__ __align__(16) char lds[2 * BUF];
   __shared__ __align__(16) f32x4 shares[SHARED ? NW * CT * CT * 64 : 1];
 
-  const int tid = threadIdx.x, w = tid >> 6, l = tid & 15, g = (tid >> 4) & 3;
+  const int tid = threadIdx.x, wave = tid >> 6, l = tid & 15, g = (tid >> 4) & 3;
+  // PAIR: the second half of the waves runs the second pass: rows X2 against rows Z weigh rows Y, the state transposed
+  const int second = PAIR ? __builtin_amdgcn_readfirstlane(wave / GW) : 0, w = PAIR ? wave % GW : wave;
+  const int Da = second ? p.Db : p.Da, Db = second ? p.Da : p.Db;
   // `order` counts the segments as they follow each other; the pass over states has no use for the last
   const int per = STATE_ONLY ? p.nseg - 1 : p.nseg, order = blockIdx.x % per, seg = REV ? p.nseg - 1 - order : order;
   const int slice = blockIdx.x / per % p.slices, head = blockIdx.x / (per * p.slices);
@@ -220,45 +227,49 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
   const T* X = STATE_ONLY ? nullptr : rows_of<T>(p.X, b, h, p.xs);
   const T* Y = rows_of<T>(p.Y, b, h, p.ys);
   const T* Z = rows_of<T>(p.Z, b, h, p.zs) + c0;
-  const int cols = p.Db - c0;
+  const T* X2 = PAIR ? rows_of<T>(p.X2, b, h, p.x2s) : nullptr;
+  const int cols = Db - c0;
 
-  // The state in front: a scan has left it, or it is the initial one and what the segments in front have added to it, as they follow
-  // each other.
-  const bool wide = p.Da == DA && cols >= WC;                  // (nothing to leave out)
+  // The state in front: a scan has left it, or it is the initial one and, of two segments, what the first has added to it.
+  const bool wide = p.Da == DA && (PAIR ? p.Db == DA : cols >= WC);            // (nothing to leave out)
   f32x4 S[DT][NC];
   const size_t D = (size_t)p.Da * p.Db;
+  auto add_state = [&](const float* s, float f) {
+    const int sa = (int)(second ? p.sb : p.sa), sb = (int)(second ? p.sa : p.sb);
+    int a0 = place<T, true>(0, 4 * g), b0 = cw + place<T, NC == 2>(0, l);
+    asm volatile("" : "+v"(a0), "+v"(b0));                     // (64 addresses are not to be kept from one call to the next)
+    s += (size_t)c0 * sb;
+    const unsigned at = (unsigned)(a0 * sa + b0 * sb);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int da = place<T, true>(d, 0) + r, db = place<T, NC == 2>(ct, 0);
+          float x;
+          if (wide) {
+            x = (s + (da * sa + db * sb))[at];
+          } else {
+            x = s[(unsigned)(min(a0 + da, Da - 1) * sa + min(b0 + db, cols - 1) * sb)];
+            x = a0 + da < Da && b0 + db < cols ? x : 0.f;
+          }
+          S[d][ct][r] = fmaf(f, S[d][ct][r], x);
+        }
+      if (d % 4 == 3) __builtin_amdgcn_sched_barrier(0);       // (not all on their way at once)
+    }
+  };
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct) S[d][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (!STATE_ONLY) {
+  if constexpr (!STATE_ONLY) {
     const float* const segs = p.nseg > 1 ? p.seg + bh * (p.nseg - 1) * D : nullptr;
-    const int sa = (int)p.sa, sb = (int)p.sb, a0 = place<T, true>(0, 4 * g), b0 = cw + place<T, NC == 2>(0, l);
-    for (int u = p.scanned && order > 0 ? order - 1 : (p.s_in ? -1 : 0); u < order; ++u) {
-      const float* s = u < 0 ? p.s_in + bh * D : segs + u * D;
-      const int ts = (REV ? p.nseg - 1 - u : u) * p.seg_tokens, n = min(max(len - ts, 0), p.seg_tokens);
-      const float f = u < 0 ? 0.f : power(g2, n);              // (times zero where u is the first)
-      s += (size_t)c0 * sb;
-      int a1 = a0, b1 = b0;
-      asm volatile("" : "+v"(a1), "+v"(b1));                   // (64 addresses are not to be kept from one turn to the next)
-      const unsigned at = (unsigned)(a1 * sa + b1 * sb);
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int da = place<T, true>(d, 0) + r, db = place<T, NC == 2>(ct, 0);
-            float x;
-            if (wide) {
-              x = (s + (da * sa + db * sb))[at];
-            } else {
-              x = s[(unsigned)(min(a1 + da, p.Da - 1) * sa + min(b1 + db, cols - 1) * sb)];
-              x = a1 + da < p.Da && b1 + db < cols ? x : 0.f;
-            }
-            S[d][ct][r] = fmaf(f, S[d][ct][r], x);
-            if (r == 3 && ct == NC - 1 && d % 4 == 3) __builtin_amdgcn_sched_barrier(0);       // (not all 64 on their way at once)
-          }
+    const float* const front = p.scanned && order > 0 ? segs + (order - 1) * D : (p.s_in ? p.s_in + bh * D : nullptr);
+    if (front) add_state(front, 0.f);
+    if (!p.scanned && order > 0) {
+      const int n = min(max(len - (REV ? p.seg_tokens : 0), 0), p.seg_tokens);                   // the first segment's tokens
+      add_state(segs, power(g2, n));
     }
   }
 
@@ -275,13 +286,13 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
 
   auto put = [&](const f32x4 (&O)[NC][CT], int t, int rows) {
     const size_t at = ((size_t)b * T_ + t) * p.H + h, size = p.out_f32 || sizeof(T) == 4 ? 4 : sizeof(T);
-    char* const base = (char*)p.out + (at * p.Db + c0) * size;
-    const unsigned step = (unsigned)(p.H * p.Db) * (unsigned)size;                                   // (VEC: within 24 bits)
+    char* const base = (char*)(second ? p.out2 : p.out) + (at * Db + c0) * size;
+    const unsigned step = (unsigned)(p.H * Db) * (unsigned)size;                                   // (VEC: within 24 bits)
 #pragma unroll
     for (int it = 0; it < CT; ++it) {
       const int row = 16 * it + l, c = cw + place<T, NC == 2>(0, 4 * g);
       if (row >= rows || c >= cols) continue;
-      char* const o = (VEC ? base + __umul24((unsigned)row, step) : base + (size_t)row * p.H * p.Db * size) + c * (int)size;
+      char* const o = (VEC ? base + __umul24((unsigned)row, step) : base + (size_t)row * p.H * Db * size) + c * (int)size;
       if (p.out_f32 || sizeof(T) == 4) {
 #pragma unroll
         for (int ct = 0; ct < NC; ++ct) {
@@ -319,23 +330,27 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
     for (int c = full; c < nch; ++c) put(zero, t0 + c * CH, min(CH, t1 - t0 - c * CH));
   }
 
-  FA fx, fy;
+  FA fx, fy, f2;
   FZ fz;
   if (!STATE_ONLY) fx.init(p.X.st, tid);
   fy.init(p.Y.st, tid);
   fz.init(p.Z.st, tid);
+  if (PAIR) f2.init(p.X2.st, tid);
   auto fetch = [&](int c, int buf) {
     const int t = t0 + c * CH, n = min(CH, te - t);
     char* const tile = lds + buf * BUF;
     const T *x = STATE_ONLY ? nullptr : X + (long)t * p.X.st, *y = Y + (long)t * p.Y.st, *zz = Z + (long)t * p.Z.st;
+    const T* x2 = PAIR ? X2 + (long)t * p.X2.st : nullptr;
     if (VEC && wide && n == CH) {
+      if constexpr (PAIR) f2.template fill<true>(tile + XB + TA::BYTES + TZ::BYTES, x2, p.X2.st, n, p.Db, tid);
       if (!STATE_ONLY) fx.template fill<true>(tile, x, p.X.st, n, p.Da, tid);
       fy.template fill<true>(tile + XB, y, p.Y.st, n, p.Da, tid);
-      fz.template fill<true>(tile + XB + TA::BYTES, zz, p.Z.st, n, cols, tid);
+      fz.template fill<true>(tile + XB + TA::BYTES, zz, p.Z.st, n, p.Db - c0, tid);
     } else {
+      if constexpr (PAIR) f2.template fill<false>(tile + XB + TA::BYTES + TZ::BYTES, x2, p.X2.st, n, p.Db, tid);
       if (!STATE_ONLY) fx.template fill<false>(tile, x, p.X.st, n, p.Da, tid);
       fy.template fill<false>(tile + XB, y, p.Y.st, n, p.Da, tid);
-      fz.template fill<false>(tile + XB + TA::BYTES, zz, p.Z.st, n, cols, tid);
+      fz.template fill<false>(tile + XB + TA::BYTES, zz, p.Z.st, n, p.Db - c0, tid);
     }
   };
   int rows1 = TA::rows_first(g, l), cols1[4], cz1[4];
@@ -351,6 +366,7 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
         if (!STATE_ONLY) FA::clear(lds + buf * BUF, 0, tid);
         FA::clear(lds + buf * BUF + XB, 0, tid);
         FZ::clear(lds + buf * BUF + XB + TA::BYTES, 0, tid);
+        if (PAIR) FA::clear(lds + buf * BUF + XB + TA::BYTES + TZ::BYTES, 0, tid);
       }
       lds_barrier();
     }
@@ -359,14 +375,16 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
   bool stored = false;
   for (int i = 0; i < full; ++i) {
     const int c = REV ? full - 1 - i : i, t = t0 + c * CH, n = min(CH, te - t), buf = i & 1;
-    char *const lx = lds + buf * BUF, *const ly = lx + XB, *const lz = ly + TA::BYTES;
+    char *const tile = lds + buf * BUF, *const ty = tile + XB, *const tz = ty + TA::BYTES, *const t2 = tz + TZ::BYTES;
+    char *const lx = second ? t2 : tile, *const ly = second ? tz : ty, *const lz = second ? ty : tz;
     // the chunk's rows are there; the outputs of the one before, stored behind the loads, need not be (a store for each of its tiles)
     if (VEC && !STATE_ONLY && stored) wait_and_barrier<CT>();
     else wait_and_barrier<0>();
     if (n < CH) {                                              // (the last chunk of a sequence)
-      if (!STATE_ONLY) FA::clear(lx, n, tid);
-      FA::clear(ly, n, tid);
-      FZ::clear(lz, n, tid);
+      if (!STATE_ONLY) FA::clear(tile, n, tid);
+      FA::clear(ty, n, tid);
+      FZ::clear(tz, n, tid);
+      if (PAIR) FA::clear(t2, n, tid);
       lds_barrier();
     }
     if (i + 1 < full) fetch(REV ? c - 1 : c + 1, buf ^ 1);
@@ -425,8 +443,8 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
       typename TA::V16 xr[2][CT], yr[2][CT];
       if constexpr (SHARED) {
 #pragma unroll
-        for (int q = 0; q < STEPS / NW; ++q) {
-          const int s = w * (STEPS / NW) + q;
+        for (int q = 0; q < STEPS / GW; ++q) {
+          const int s = w * (STEPS / GW) + q;
           typename TA::V16 x[CT], y[CT];
 #pragma unroll
           for (int it = 0; it < CT; ++it) {
@@ -445,7 +463,7 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
         for (int it = 0; it < CT; ++it)
 #pragma unroll
           for (int jt = 0; jt < CT; ++jt)
-            if (REV ? jt >= it : jt <= it) shares[((w * CT + jt) * CT + it) * 64 + (tid & 63)] = P[jt][it];
+            if (REV ? jt >= it : jt <= it) shares[((wave * CT + jt) * CT + it) * 64 + (tid & 63)] = P[jt][it];
       }
       auto read = [&](int s) {
 #pragma unroll
@@ -510,11 +528,11 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
 #pragma unroll
           for (int jt = 0; jt < CT; ++jt)
             if (REV ? jt >= it : jt <= it) {
-              f32x4 part[NW];
+              f32x4 part[GW];
 #pragma unroll
-              for (int v = 0; v < NW; ++v) part[v] = shares[((v * CT + jt) * CT + it) * 64 + (tid & 63)];
+              for (int v = 0; v < GW; ++v) part[v] = shares[(((second * GW + v) * CT + jt) * CT + it) * 64 + (tid & 63)];
 #pragma unroll
-              for (int v = NW / 2; v > 0; v /= 2)
+              for (int v = GW / 2; v > 0; v /= 2)
 #pragma unroll
                 for (int x = 0; x < v; ++x) part[x] += part[x + v];
               P[jt][it] = part[0];
@@ -559,14 +577,17 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
     }
     if constexpr (!STATE_ONLY) {
       if (bad)
+#pragma clang loop unroll(disable)
         for (int j = 0; j < n; ++j) {
+          int here = 0;                                        // (nothing of this rare turn is to be prepared outside of it)
+          asm volatile("" : "+v"(here));
           float zo[NC][4], zs[NC];                             // row j in the lane's columns of O, of S
           bool any = false;
 #pragma unroll
           for (int ct = 0; ct < NC; ++ct) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) zo[ct][r] = (float)*reinterpret_cast<const T*>(lz + TZ::at(j, cw + place<T, NC == 2>(ct, 4 * g + r)));
-            zs[ct] = (float)*reinterpret_cast<const T*>(lz + TZ::at(j, cw + place<T, NC == 2>(ct, l)));
+            for (int r = 0; r < 4; ++r) zo[ct][r] = (float)*reinterpret_cast<const T*>(lz + here + TZ::at(j, cw + place<T, NC == 2>(ct, 4 * g + r)));
+            zs[ct] = (float)*reinterpret_cast<const T*>(lz + here + TZ::at(j, cw + place<T, NC == 2>(ct, l)));
             any |= nonfinite(zs[ct]);
           }
           if (!__any(any)) continue;
@@ -574,8 +595,10 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
           for (int it = 0; it < CT; ++it) {
             const int row = 16 * it + l, e = REV ? j - row : row - j;
             float dot = 0.f;
+#pragma clang loop unroll(disable) vectorize(disable)
             for (int a = 0; a < DA; ++a)
-              dot = fmaf((float)*reinterpret_cast<const T*>(lx + TA::at(row, a)), (float)*reinterpret_cast<const T*>(ly + TA::at(j, a)), dot);
+              dot = fmaf((float)*reinterpret_cast<const T*>(lx + here + TA::at(row, a)),
+                         (float)*reinterpret_cast<const T*>(ly + here + TA::at(j, a)), dot);
             dot *= e < 0 ? 0.f : p.intra * power(g2, e);
 #pragma unroll
             for (int ct = 0; ct < NC; ++ct)
@@ -588,7 +611,7 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float y = f * (float)*reinterpret_cast<const T*>(ly + TA::at(j, place<T, true>(d, 4 * g + r)));
+              const float y = f * (float)*reinterpret_cast<const T*>(ly + here + TA::at(j, place<T, true>(d, 4 * g + r)));
 #pragma unroll
               for (int ct = 0; ct < NC; ++ct)
                 if (nonfinite(zs[ct])) S[d][ct][r] = fmaf(y, zs[ct], S[d][ct][r]);
@@ -670,7 +693,7 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
     }
   }
 
-  float* const s = STATE_ONLY ? p.seg + (bh * (p.nseg - 1) + order) * D : (order == p.nseg - 1 && p.s_out ? p.s_out + bh * D : nullptr);
+  float* const s = STATE_ONLY ? p.seg + (bh * (p.nseg - 1) + order) * D : (order == p.nseg - 1 && p.s_out && !second ? p.s_out + bh * D : nullptr);
   if (s) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -679,7 +702,7 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int a = place<T, true>(d, 4 * g + r), c = cw + place<T, NC == 2>(ct, l);
-          if (a < p.Da && c < cols) s[(size_t)a * p.sa + (size_t)(c0 + c) * p.sb] = S[d][ct][r];
+          if (a < Da && c < cols) s[(size_t)a * p.sa + (size_t)(c0 + c) * p.sb] = S[d][ct][r];
         }
   }
 }
@@ -713,6 +736,22 @@ template <typename T, bool VEC, bool REV> hipError_t launch_access(const RingLin
   if (a.Da <= 64) return launch_sized<T, 64, 2, 4, VEC, REV>(a, state_only, st);
   if (a.Da <= 128) return launch_sized<T, 128, 2, 4, VEC, REV>(a, state_only, st);
   return launch_sized<T, 256, Type<T>::BF ? 2 : 1, Type<T>::BF ? 4 : 8, VEC, REV>(a, state_only, st);
+}
+
+// Two passes at once, backwards in time: heads whose dk and dv go with the same kernel
+template <typename T, int DA, int NC, bool VEC> hipError_t launch_two(const RingLinArgs& a, hipStream_t st) {
+  constexpr bool BF = Type<T>::BF;
+  constexpr int CT = sizeof(T) == 4 ? 1 : 2;
+  const dim3 grid((unsigned)((long)a.nseg * a.H * a.B)), block(512);
+  if (!BF || a.s_out) hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, 8, CT, VEC, true, false, true, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((ring_linattn_kernel<T, DA, NC, 8, CT, VEC, true, false, !BF, true>), grid, block, 0, st, a);
+  return hipGetLastError();
+}
+
+template <typename T> hipError_t launch_pair(const RingLinArgs& a, hipStream_t st) {
+  const bool vec = a.X.vec && a.Y.vec && a.Z.vec && a.X2.vec && a.out_vec;
+  if (a.Da <= 64) return vec ? launch_two<T, 64, 1, true>(a, st) : launch_two<T, 64, 1, false>(a, st);
+  return vec ? launch_two<T, 128, 2, true>(a, st) : launch_two<T, 128, 2, false>(a, st);
 }
 
 template <typename T> hipError_t launch(const RingLinArgs& a, bool rev, bool state_only, hipStream_t st) {
