@@ -2,6 +2,8 @@
 #include "ring_linattn.hpp"
 #include "ringattr.h"
 
+#include <math.h>
+
 using namespace ring_lin;
 
 namespace {
@@ -160,26 +162,43 @@ hipError_t ring_linattn_step(const RingLinShape& s, const RingLinStep& a, hipStr
   return launch_step<_Float16>(s, a, st);
 }
 
-// Into how many segments the tokens are cut so that there is work for all compute units: the number with the least expected time, in
-// units of what a workgroup alone on its compute unit takes for a chunk of 32 tokens.  Two on one take 1.6 each (heads past 128 wide
-// fill the registers: one at a time).  More than one segment costs a pass over their states, at 0.45 of a chunk, a launch and what the
-// segments behind read of it.
+// Into how many segments the tokens are cut so that there is work for all compute units: the number with the least expected time of a
+// forward.  What it is made of, in us, as measured (P: 64, 128 or 256, what the kernels round a head's widths up to):
+//   a chunk of 32 tokens, a workgroup alone on its compute unit: bf16 1.1, 1.6, 2.7; fp32 products 2.8, 6.2, 12
+//   two workgroups on a compute unit: 1.2 of one's time with P = 64, 1.86 with P = 128 (1.6 where a quarter of them have two); with P = 256
+//   they follow each other
+//   but no less than the rows take from memory, at 5 TB/s
+//   the pass over states: 0.4 of a chunk, and 6 or (P > 64) 10 for its launch and what the pass behind reads of it
+//   the scan (more than kFold segments): 3 or 5, 0.2 a segment, and its states at 5 TB/s
+// us of a forward, and with its backward, by segments, the rule's choice in brackets:
+//   8 x 4096 tokens, 16 heads of 128, bf16    1: 231, 744   [2: 188, 542]    3: 193, 617    4: 179, 572    8: 221, 660
+//   1 x 32768 tokens, 16 heads of 128, bf16   1: 1777, 5772  8: 340, 963   [16: 218, 603]  32: 203, 627   64: 270, 729
+//   8 x 2048 tokens, 16 heads of 64, bf16     1: 70, 220     2: 59, 164     3: 54, 155    [4: 47, 135]    8: 52, 150
+//   8 x 2000 tokens, 8 heads of 256, fp32     1: 678, 2758  [2: 465, 1644]  4: 543, 1879    8: 634, 2124
+//   3 x 4096 tokens, 8 heads of 256, bf16     1: 393, 1487   4: 184, 564   [5: 153, 481]    8: 193, 627   16: 211, 639
+//   20 x 4096 tokens, 16 heads of 128, bf16  [1: 323]        2: 391          4: 444 (the forward alone, as in the next)
+//   2 x 1000 tokens, 4 heads of 64, fp32      1: 86          8: 27         [16: 23]
 static int segments(const RingLinShape& s) {
-  const long groups = (long)s.B * s.H * slices(s.Dv);
-  const int chunks = (s.T + kChunk - 1) / kChunk;
-  const bool one = s.Dk > 128 || s.Dv > 128;
-  auto rounds = [&](long work) {
-    const long at_once = one ? 256 : 512, rest = work % at_once;
-    return (double)(work / at_once) * (one ? 1.0 : 1.6) + (rest == 0 ? 0.0 : (one || rest <= 256 ? 1.0 : 1.6));
+  const int units = (s.T + kChunk - 1) / kChunk;
+  const int widest = s.Dk > s.Dv ? s.Dk : s.Dv, P = widest <= 64 ? 64 : (widest <= 128 ? 128 : 256);
+  const double heads = (double)s.B * s.H, groups = heads * slices(s.Dv);
+  const double chunk = s.type == RINGATTR_BF16 ? 0.6 + 0.0083 * P : 0.047 * P;
+  const double rows = heads * s.T * (s.Dk + s.Dv) * (s.type == RINGATTR_F32 ? 4 : 2) / 5e6;      // Y and Z once
+  auto rounds = [&](double work) {                             // in times of a workgroup alone
+    const double two = P == 64 ? 1.2 : (P == 128 ? 1.86 : 2.0), full = floor(work / 512), rest = work - 512 * full;
+    return full * two + (rest == 0 ? 0.0 : (rest <= 256 ? 1.0 : (rest <= 384 && P == 128 ? 1.6 : two)));
   };
+  auto no_less = [](double a, double b) { return a > b ? a : b; };
   int best = 1;
-  double least = rounds(groups) * 2 * chunks;
-  for (int n = 2; n <= 64 && n <= chunks; ++n) {
-    const int per = (chunks + n - 1) / n;
-    if ((chunks + per - 1) / per != n) continue;
-    const double t = 2 * per * (rounds(groups * n) + 0.45 * rounds(groups * (n - 1))) + 3.0 + (n > kFold ? 3.0 : 0.0);
-    if (t < least) {
-      least = t;
+  double time = 0.0;
+  for (int n = 1; n <= 64 && n <= units; ++n) {
+    const int per = (units + n - 1) / n;
+    if ((units + per - 1) / per != n) continue;
+    double t = no_less(2 * per * chunk * rounds(groups * n), 2 * rows);
+    if (n > 1) t += no_less(0.8 * per * chunk * rounds(groups * (n - 1)), rows * (n - 1) / n) + (P == 64 ? 6 : 10);
+    if (n > kFold) t += (P == 64 ? 3 : 5) + 0.2 * n + heads * n * s.Dk * s.Dv * 8 / 5e6;
+    if (n == 1 || t < time) {
+      time = t;
       best = n;
     }
   }

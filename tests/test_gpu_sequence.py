@@ -114,6 +114,36 @@ def test_padded_batches(kind, gpu_device):
             assert (got[n][b, m:] == 0).all()
 
 
+# (kind, sizes, segments that the tokens are cut into)
+SEGMENTED = [("fp32", (8, 500, 8, 4, 4, 130), 2), ("bf16", (8, 500, 8, 8, 4, 130), 2), ("fp32", (4, 500, 64, 64, 10, 6), 2),
+             ("bf16", (8, 1000, 32, 8, 10, 6), 2), ("fp32", (4, 200, 32, 32, 70, 66), 2), ("bf16", (4, 800, 32, 16, 70, 66), 2),
+             ("fp32", (4, 500, 2, 1, 20, 70), 8), ("bf16", (4, 500, 2, 2, 20, 70), 8), ("fp16", (4, 500, 2, 2, 70, 66), 8),
+             ("bf16", (4, 500, 2, 1, 70, 66), 8), ("fp16", (4, 500, 4, 4, 16, 30), 8), ("bf16", (4, 500, 4, 2, 16, 30), 8),
+             ("fp32", (4, 500, 2, 2, 130, 9), 8), ("bf16", (4, 500, 2, 2, 9, 130), 8)]
+
+
+@pytest.mark.parametrize("kind,sizes,count", SEGMENTED, ids=["-".join([k] + [str(x) for x in s]) for k, s, _ in SEGMENTED])
+def test_lengths_that_end_in_any_segment(kind, sizes, count, gpu_device):
+    """Sequences cut into two segments and into many, heads whose dv and dk go back together and not: lengths that end in front of, at and
+    behind a segment's first token, in the last one, and none."""
+    from rnn_train_ring_attractor_amd import _lib
+    B, T, H, G, Dk, Dv = sizes
+    dtype = TYPES[kind]
+    nbytes = _lib.load().ringattr_linear_attention_fwd_workspace_bytes(_lib.SEQUENCE_TYPES[dtype], *sizes)
+    each = B * H * Dk * Dv * 4
+    assert (count - 1) * each <= nbytes < (count - 1) * each + 256, "the tokens are cut otherwise than this case is for"
+    first = -(-(-(-T // 64)) // count) * 64
+    lengths = [first + 1, T, 0, first, 1, first - 1, T - 1, 65][:B]
+    print(f"[case] segments {kind} {sizes} {lengths}", flush=True)
+    p = _problem(37, *sizes, dtype, start=True)
+    for n in ("q", "k", "v", "do"):
+        for b, m in enumerate(lengths):
+            p[n][b, m:] = math.nan
+    got = _run(p, dtype, gpu_device, lengths)
+    clean = {n: (x.nan_to_num() if n in ("q", "k", "v", "do") else x) for n, x in p.items()}
+    _compare(clean, got, lengths, dtype, H // G)
+
+
 @pytest.mark.parametrize("kind", ["fp32", "bf16"])
 @pytest.mark.parametrize("decays", [[0.0, 0.0], [-math.inf, -1e-7], [-40.0, -3.0]], ids=["none", "all_and_hardly", "strong"])
 def test_decays_at_their_ends(decays, kind, gpu_device):
