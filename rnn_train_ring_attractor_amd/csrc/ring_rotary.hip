@@ -32,7 +32,8 @@ __global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p) {
   typedef T vec __attribute__((ext_vector_type(V)));
   __shared__ f32x2 trig[kAngles];
   const int tid = threadIdx.x, r = p.rot / 2, D = p.D;
-  const long first = (long)blockIdx.x * p.tokens, all = (long)p.B * p.T;
+  const long first = ((long)blockIdx.z * gridDim.x + blockIdx.x) * p.tokens, all = (long)p.B * p.T;
+  if (first >= all) return;
   const int here = (int)(all - first < p.tokens ? all - first : p.tokens);
   for (int i = tid; i < here * r; i += 256) {
     const int tok = i / r, m = i - tok * r;
@@ -112,7 +113,8 @@ template <typename T> static hipError_t launch(RingRotaryArgs p, hipStream_t st)
   int split = blocks < 512 ? (int)(512 / blocks) : 1;
   if (split > heads) split = heads;
   p.heads_per = (heads + split - 1) / split;
-  const dim3 grid((unsigned)blocks, (unsigned)((heads + p.heads_per - 1) / p.heads_per)), block(256);
+  const long row = blocks < (1 << 20) ? blocks : 1 << 20;      // (a launch counts fewer than 2^32 threads along x)
+  const dim3 grid((unsigned)row, (unsigned)((heads + p.heads_per - 1) / p.heads_per), (unsigned)((blocks + row - 1) / row)), block(256);
   if (p.interleaved) {
     if (vec) hipLaunchKernelGGL((ring_rotary_kernel<T, W, false>), grid, block, 0, st, p);
     else hipLaunchKernelGGL((ring_rotary_kernel<T, 1, false>), grid, block, 0, st, p);

@@ -127,6 +127,8 @@ def rotary_func(x, positions, frequencies, layout="half", scale=1.0):
     if positions.requires_grad and torch.is_grad_enabled():
         raise ValueError("positions get no gradient (detach them)")
     check_sequence_tensor("frequencies", frequencies, dtype=torch.float64, device=dev)
+    if frequencies.requires_grad and torch.is_grad_enabled():
+        raise ValueError("frequencies get no gradient (detach them)")
     if frequencies.dim() != 1 or not 1 <= frequencies.numel() <= D // 2:
         raise ValueError(f"frequencies must be one-dimensional, between 1 and {D // 2} of them, got {tuple(frequencies.shape)}")
     frequencies, scale = frequencies.contiguous(), float(scale)

@@ -186,6 +186,44 @@ def test_far_into_large_tensors(gpu_device):
             assert torch.equal(y[first:first + 1000] != 0, keep)
 
 
+def test_results_past_32_bits_and_more_tokens_than_workgroups(gpu_device):
+    from rnn_train_ring_attractor_amd import linear_attention_func, linear_attention_step, rotary_func
+    gen = torch.Generator(device=gpu_device).manual_seed(16)
+    with torch.no_grad():
+        print("[case] attention of 2^32 results: equal heads, equal results", flush=True)
+        T, H, D = 1 << 20, 65, 64
+        q, k, v = (torch.randn(1, T, 1, D, generator=gen, device=gpu_device).bfloat16().expand(1, T, H, D) for _ in range(3))
+        o, s = linear_attention_func(q, k, v, torch.full((H,), -0.05, device=gpu_device), return_state=True)
+        assert o.numel() > 1 << 32
+        for at in (slice(0, 1000), slice(T // 2, T // 2 + 1000), slice(T - 1000, T)):
+            assert all(torch.equal(o[:, at, h], o[:, at, 0]) for h in (1, 31, 63, 64))
+        assert torch.equal(s, s[:, :1].expand_as(s))
+        part = linear_attention_func(*(x[:, T - 1000:, :1] for x in (q, k, v)), torch.full((1,), -0.05, device=gpu_device), return_state=True)
+        # exp(-0.05 * 500) of what came before is left: the two differ by their roundings
+        assert torch.allclose(o[:, -500:, :1].float(), part[0][:, -500:].float(), rtol=2.0 ** -6, atol=2.0 ** -4)
+        del o, s
+        print("[case] step of 2^32 state values", flush=True)
+        B, D = 66000, 256
+        state = torch.zeros(B, 1, D, D, device=gpu_device)
+        row = torch.randn(3, 1, 1, D, generator=gen, device=gpu_device)
+        g, few = torch.full((1,), -0.1, device=gpu_device), torch.zeros(3, 1, D, D, device=gpu_device)
+        for _ in range(2):
+            got = linear_attention_step(*(x.expand(B, 1, D) for x in row), g, state)
+            want = linear_attention_step(*(x.expand(3, 1, D) for x in row), g, few)
+        assert torch.allclose(got[-3:], want, rtol=1e-4, atol=1e-4) and torch.allclose(got[:3], want, rtol=1e-4, atol=1e-4)
+        assert torch.equal(state[-3:], few) and torch.equal(state[B // 2:B // 2 + 3], few)
+        del state
+        print("[case] positions of more tokens than workgroups", flush=True)
+        T, D = (1 << 20) + 1003, 512                                     # a token fills a workgroup
+        x = torch.randn(1, T, 1, D, generator=gen, device=gpu_device).bfloat16()
+        f = torch.rand(D // 2, generator=gen, device=gpu_device, dtype=torch.float64)
+        pos = torch.arange(T, device=gpu_device)
+        for layout in ("half", "interleaved"):
+            y = rotary_func(x, pos, f, layout)
+            for at in (slice(0, 2000), slice((1 << 20) - 1000, (1 << 20) + 1003)):
+                assert torch.equal(y[:, at], rotary_func(x[:, at], pos[at], f, layout))
+
+
 def test_positions_of_every_kind_and_gradients_of_gradients(gpu_device):
     from rnn_train_ring_attractor_amd import dropout_func, linear_attention_func, rotary_func
     print("[case] positions", flush=True)
@@ -241,7 +279,8 @@ def test_refusals_on_the_gpu(gpu_device):
     f, pos = z(4, dtype=torch.float64), torch.arange(3, device=gpu_device)
     for error, args in ((ValueError, (q, pos[:2], f)), (TypeError, (q, pos.double(), f)), (TypeError, (q, pos, f.float())), (ValueError, (q, pos, z(5, dtype=torch.float64))),
                         (ValueError, ((q, z(2, 3, 1, 6)), pos, f)), (ValueError, ((q, q, q), pos, f)), (RuntimeError, (q, pos.cpu(), f)),
-                        (ValueError, (q, pos.float().requires_grad_(True), f)), (ValueError, (q[0], pos, f))):
+                        (ValueError, (q, pos.float().requires_grad_(True), f)), (ValueError, (q[0], pos, f)),
+                        (ValueError, (q, pos, f.clone().requires_grad_(True)))):
         with pytest.raises(error):
             rotary_func(*args)
     for error, kw in ((ValueError, dict(p=1.0)), (ValueError, dict(p=-0.1)), (ValueError, dict(seed=-1)), (ValueError, dict(seed=1 << 64)),
