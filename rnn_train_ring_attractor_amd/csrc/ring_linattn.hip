@@ -21,6 +21,10 @@ hipError_t launch_pass(int type, const RingLinArgs& a, bool rev, bool state_only
   return ring_launch_linattn_f16(a, rev, state_only, st);
 }
 
+// A head's columns go to workgroups of 64 where there are no more, else of 128: in slices of 64 a wide head needs fewer segments, but
+// forms its weights twice as often (us of a forward, and with its backward, each in its best number of segments, 128 and 64: 8 x 4096
+// tokens, 16 heads of 128, bf16 188, 542 and 183, 686; 8 x 2000 tokens, 8 heads of 256, fp32 459, 1647 and 496, 1968; 16 x 1000 tokens, 8
+// heads of 128, fp32 142, 466 and 136, 490).
 int slices(int Db) { return Db <= 64 ? 1 : (Db + 127) / 128; }
 
 void set_columns(RingLinArgs& a, int Db, bool narrow) {
@@ -94,7 +98,8 @@ static hipError_t launch_share(int type, const float* in, void* out, int share, 
 
 // A single token: S = lambda S + k v^T in place, o = scale q S.  A workgroup takes `tc` lanes of V columns each of one state; its other
 // lanes share the rows.  Nothing but the state moves: read once, written once: bound by memory, 93 us for 256 x 16 heads of 128 (537 MB,
-// 5.8 TB/s); few heads are cut into narrower slices (up to 1024 workgroups): 8 heads of 64 take 4.9 us, about a launch.
+// 5.8 TB/s); few heads are cut into narrower slices (us, cut and in whole rows: 8 heads of 64 3.1, 5.2; 16 of 128
+// 3.6, 7.5; 16 x 16 of 128 7.1, 8.9), as long as that makes no more than about 1024 workgroups.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void ring_linattn_step_kernel(RingLinStep p, RingLinShape s, int tc) {
   typedef float vec __attribute__((ext_vector_type(V)));
