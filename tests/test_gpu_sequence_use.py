@@ -251,6 +251,58 @@ def test_positions_of_every_kind_and_gradients_of_gradients(gpu_device):
         torch.autograd.grad([o.sum()], [q], create_graph=True)
 
 
+def test_backward_twice_broadcast_inputs_checkpoints_and_inference(gpu_device):
+    """The same bits from a backward run twice over one forward (which kept its states), from a forward that is formed again, and under
+    inference mode; a broadcast input's gradient is the sum over what it was broadcast to; inputs that ask for no gradient get none."""
+    from torch.utils.checkpoint import checkpoint
+    from rnn_train_ring_attractor_amd import dropout_func, linear_attention_func, linear_attention_step, rotary_func
+    gen = torch.Generator(device=gpu_device).manual_seed(18)
+    B, T, H, D = 2, 700, 4, 32
+    q, k, v, do = (torch.randn(B, T, H, D, generator=gen, device=gpu_device) for _ in range(4))
+    g, f = torch.linspace(-0.3, -0.001, H, device=gpu_device), torch.rand(8, generator=gen, device=gpu_device, dtype=torch.float64)
+    pos = torch.arange(T, device=gpu_device)
+
+    def layer(q, k, v):
+        a, b = rotary_func((q, k), pos, f)
+        return dropout_func(linear_attention_func(a, b, v, g), 0.2, 3, 4, residual=q)
+
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    print("[case] twice", flush=True)
+    o = layer(*leaves)
+    first = torch.autograd.grad(o, leaves, do, retain_graph=True)
+    second = torch.autograd.grad(o, leaves, do)
+    print("[case] checkpoint", flush=True)
+    again = torch.autograd.grad(checkpoint(layer, *leaves, use_reentrant=False), leaves, do)
+    for other in (second, again):
+        assert all(torch.equal(a, b) for a, b in zip(first, other))
+    print("[case] some gradients", flush=True)
+    only, = torch.autograd.grad(layer(q, k, leaves[2]), leaves[2:], do)
+    assert torch.equal(only, first[2])
+    print("[case] broadcast", flush=True)
+    one = torch.randn(1, T, 1, D, generator=gen, device=gpu_device).requires_grad_(True)
+    o1 = linear_attention_func(leaves[0], one.expand(B, T, H, D), leaves[2], g)
+    full = one.detach().expand(B, T, H, D).contiguous().requires_grad_(True)
+    o2 = linear_attention_func(leaves[0], full, leaves[2], g)
+    assert torch.equal(o1, o2)
+    whole, = torch.autograd.grad(o2, full, do)
+    part, = torch.autograd.grad(o1, one, do)
+    # two orders of a sum of B H terms: off by at most B H half steps of the terms' magnitudes each
+    assert ((part - whole.sum((0, 2), keepdim=True)).abs() <= 2 * B * H * 2.0 ** -24 * whole.abs().sum((0, 2), keepdim=True)).all()
+    print("[case] broadcast gradient", flush=True)
+    summed, = torch.autograd.grad(linear_attention_func(q, k, leaves[2], g).sum(), leaves[2:])
+    ones, = torch.autograd.grad(linear_attention_func(q, k, leaves[2], g), leaves[2:], torch.ones_like(do))
+    assert torch.equal(summed, ones)
+    print("[case] inference", flush=True)
+    with torch.inference_mode():
+        assert torch.equal(layer(q, k, v), o)
+        state = torch.zeros(B, H, D, D, device=gpu_device)
+        steps = [linear_attention_step(q[:, t], k[:, t], v[:, t], g, state) for t in range(3)]
+    with torch.no_grad():
+        want = linear_attention_func(q[:, :3], k[:, :3], v[:, :3], g)
+    size = linear_attention_func(q[:, :3].abs(), k[:, :3].abs(), v[:, :3].abs(), g)
+    assert ((torch.stack(steps, dim=1) - want).abs() <= 2 * (3 + 2 * D + 256) * 2.0 ** -24 * size).all()
+
+
 def test_refusals_on_the_gpu(gpu_device):
     from rnn_train_ring_attractor_amd import dropout_func, linear_attention_func, linear_attention_step, rotary_func
     z = lambda *s, **k: torch.zeros(*s, device=gpu_device, **k)
