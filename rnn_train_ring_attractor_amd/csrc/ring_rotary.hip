@@ -17,6 +17,8 @@
 namespace {
 
 constexpr int kAngles = 1024;      // (cos, sin) that a workgroup keeps
+// Bytes that a call reads and writes from which on it leaves nothing in the last cache (256 MB) that a reader behind it would find
+constexpr size_t kPastCache = 320000000;
 
 __device__ __forceinline__ double position_of(const RingRotaryArgs& p, long at) {
   if (p.position_type == RINGATTR_POS_F32) return (double)((const float*)p.positions)[at];
@@ -26,11 +28,19 @@ __device__ __forceinline__ double position_of(const RingRotaryArgs& p, long at) 
 
 }  // namespace
 
-// V values at a time, neighbours in memory (V = 1: any strides and widths)
-template <typename T, int V, bool HALF>
+// V values at a time, neighbours in memory (V = 1: any strides and widths).  PAST: results are stored past the caches, where the call
+// passes them anyway and its inputs would be pushed out (kPastCache), in rows of whole lines (16 + 4 heads of 128, bf16, halves, us with
+// and without: 336 MB with inputs just written 55, 68, inputs from memory 68.4, 69.6, and a call that reads the results 135, 142; smaller,
+// 252 MB: that 106, 97; rows of 128 bytes, 302 MB: 64.4, 63.1 and 130, 125).  Dropout gains nothing by it (403 and 268 MB there and back:
+// 124, 120).
+template <typename T, int V, bool HALF, bool PAST>
 __global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p) {
   constexpr int P = HALF ? V : (V + 1) / 2;                    // pairs of a unit
   typedef T vec __attribute__((ext_vector_type(V)));
+  auto store = [](T* at, vec x) {
+    if constexpr (PAST) __builtin_nontemporal_store(x, (vec*)at);
+    else *(vec*)at = x;
+  };
   __shared__ f32x2 trig[kAngles];
   const int tid = threadIdx.x, r = p.rot / 2, D = p.D;
   const long first = ((long)blockIdx.z * gridDim.x + blockIdx.x) * p.tokens, all = (long)p.B * p.T;
@@ -62,7 +72,7 @@ __global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p) {
     const f32x2* cs = trig + tok * r + u * P;
     if (u >= turned) {
       const int d = p.rot + (u - turned) * V;
-      *(vec*)(y + d) = *(const vec*)(x + d);
+      store(y + d, *(const vec*)(x + d));
     } else if constexpr (HALF) {
       const int d = u * V;
       const vec a = *(const vec*)(x + d), c = *(const vec*)(x + d + r);
@@ -73,8 +83,8 @@ __global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p) {
         ya[e] = (T)((float)a[e] * w[0] - (float)c[e] * w[1]);
         yc[e] = (T)((float)c[e] * w[0] + (float)a[e] * w[1]);
       }
-      *(vec*)(y + d) = ya;
-      *(vec*)(y + d + r) = yc;
+      store(y + d, ya);
+      store(y + d + r, yc);
     } else {
       const int d = u * 2 * P;
       T a[2 * P];
@@ -92,7 +102,7 @@ __global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p) {
         a[2 * e + 1] = (T)(f1 * w[0] + f0 * w[1]);
       }
       if constexpr (V > 1) {
-        *(vec*)(y + d) = *(const vec*)a;
+        store(y + d, *(const vec*)a);
       } else {
         y[d] = a[0];
         y[d + 1] = a[1];
@@ -117,12 +127,16 @@ template <typename T> static hipError_t launch(RingRotaryArgs p, hipStream_t st)
   p.heads_per = (heads + split - 1) / split;
   const long row = blocks < (1 << 20) ? blocks : 1 << 20;      // (a launch counts fewer than 2^32 threads along x)
   const dim3 grid((unsigned)row, (unsigned)((heads + p.heads_per - 1) / p.heads_per), (unsigned)((blocks + row - 1) / row)), block(256);
+  const size_t row_bytes = p.D * sizeof(T);
+  const bool past = row_bytes >= 256 && 2 * row_bytes * heads * (size_t)all >= kPastCache;
   if (p.interleaved) {
-    if (vec) hipLaunchKernelGGL((ring_rotary_kernel<T, W, false>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((ring_rotary_kernel<T, 1, false>), grid, block, 0, st, p);
+    if (vec && past) hipLaunchKernelGGL((ring_rotary_kernel<T, W, false, true>), grid, block, 0, st, p);
+    else if (vec) hipLaunchKernelGGL((ring_rotary_kernel<T, W, false, false>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((ring_rotary_kernel<T, 1, false, false>), grid, block, 0, st, p);
   } else {
-    if (vec) hipLaunchKernelGGL((ring_rotary_kernel<T, W, true>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((ring_rotary_kernel<T, 1, true>), grid, block, 0, st, p);
+    if (vec && past) hipLaunchKernelGGL((ring_rotary_kernel<T, W, true, true>), grid, block, 0, st, p);
+    else if (vec) hipLaunchKernelGGL((ring_rotary_kernel<T, W, true, false>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((ring_rotary_kernel<T, 1, true, false>), grid, block, 0, st, p);
   }
   return hipGetLastError();
 }

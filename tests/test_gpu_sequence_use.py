@@ -187,7 +187,7 @@ def test_far_into_large_tensors(gpu_device):
 
 
 def test_results_past_32_bits_and_more_tokens_than_workgroups(gpu_device):
-    from rnn_train_ring_attractor_amd import linear_attention_func, linear_attention_step, rotary_func
+    from rnn_train_ring_attractor_amd import dropout_func, linear_attention_func, linear_attention_step, rotary_func
     gen = torch.Generator(device=gpu_device).manual_seed(16)
     with torch.no_grad():
         print("[case] attention of 2^32 results: equal heads, equal results", flush=True)
@@ -222,6 +222,23 @@ def test_results_past_32_bits_and_more_tokens_than_workgroups(gpu_device):
             y = rotary_func(x, pos, f, layout)
             for at in (slice(0, 2000), slice((1 << 20) - 1000, (1 << 20) + 1003)):
                 assert torch.equal(y[:, at], rotary_func(x[:, at], pos[at], f, layout))
+        del x, y
+        print("[case] results that pass the caches", flush=True)
+        for dtype in (torch.float32, torch.float16):
+            x = torch.randn(5, 4097, 4100, generator=gen, device=gpu_device).to(dtype)
+            y, both = dropout_func(x, 0.25, SEED, 9), dropout_func(x, 0.25, SEED, 9, residual=x)
+            n = 1000 * 4100
+            assert torch.equal(y.view(-1)[:n], dropout_func(x.view(-1)[:n], 0.25, SEED, 9))      # (a mask by index: the same from the front)
+            keep = torch.from_numpy(O.keep_mask(1000, 0.25, SEED, 9, first=y.numel() - 1000)).to(gpu_device)
+            assert torch.equal(y.view(-1)[-1000:] != 0, keep & (x.view(-1)[-1000:] != 0))
+            kept = y != 0
+            assert torch.equal(both[~kept], x[~kept]) and (both[kept] != x[kept]).float().mean() > 0.99
+            scaled = x[kept].float() * (1 / (1 - 0.25))
+            assert torch.equal(y[kept], scaled.to(dtype))
+            # product and sum in fp32, half a step each (none for the product where both are one instruction), then half a step of the type
+            total = x[kept].double() * (1 + float(torch.tensor(1 / (1 - 0.25))))
+            bound = 2.0 ** -24 * (scaled.abs().double() + 1.001 * total.abs()) + 1.001 * torch.finfo(dtype).eps / 2 * total.abs() + 2.0 ** -25
+            assert ((both[kept].double() - total).abs() <= bound).all()
 
 
 def test_positions_of_every_kind_and_gradients_of_gradients(gpu_device):
