@@ -206,6 +206,9 @@ template <typename T, int DA, int NC, int NW, int CT, bool VEC, bool REV, bool S
 __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_linattn_kernel(RingLinArgs p) {
   constexpr int GW = PAIR ? NW / 2 : NW, WC = 16 * NC * GW, NT = 64 * NW, CH = 16 * CT, DT = DA / 16;
   static_assert(!PAIR || (WC == DA && !STATE_ONLY), "");
+  // States alone are collected against the time, each chunk with its distance: nothing is multiplied from chunk to chunk, and the pass
+  // behind, which goes with the time, finds the rows that were read last in the last cache.
+  constexpr bool DOWN = REV != STATE_ONLY;
   constexpr bool BF = Type<T>::BF;
   typedef typename Type<T>::V4 V4;
   typedef Tile16<T, CH, DA> TA;
@@ -382,11 +385,11 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
       }
       lds_barrier();
     }
-    fetch(REV ? full - 1 : 0, 0);
+    fetch(DOWN ? full - 1 : 0, 0);
   }
   bool stored = false;
   for (int i = 0; i < full; ++i) {
-    const int c = REV ? full - 1 - i : i, t = t0 + c * CH, n = min(CH, te - t), buf = i & 1;
+    const int c = DOWN ? full - 1 - i : i, t = t0 + c * CH, n = min(CH, te - t), buf = i & 1;
     char *const tile = lds + buf * BUF, *const ty = tile + XB, *const tz = ty + TA::BYTES, *const t2 = tz + TZ::BYTES;
     char *const lx = second ? t2 : tile, *const ly = second ? tz : ty, *const lz = second ? ty : tz;
     // the chunk's rows are there; the outputs of the one before, stored behind the loads, need not be (a store for each of its tiles)
@@ -399,7 +402,7 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
       if (PAIR) FA::clear(t2, n, tid);
       lds_barrier();
     }
-    if (i + 1 < full) fetch(REV ? c - 1 : c + 1, buf ^ 1);
+    if (i + 1 < full) fetch(DOWN ? c - 1 : c + 1, buf ^ 1);
     if (n != n_now) {
       n_now = n;
       whole = power(g2, n);
@@ -633,6 +636,7 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
       stored = n == CH && cw + 16 * NC <= cols;
     }
     // the state behind the chunk; Y's columns are read AHEAD tiles ahead
+    const float apart = power(g2, REV ? t - t0 : te - t - n);  // (STATE_ONLY: the tokens between the chunk and the state)
     constexpr int AHEAD = 2;
     V4 yc[AHEAD + 1][CT];
     auto turned = [&](int d) {
@@ -653,7 +657,7 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
           for (int q = 0; q < 2; ++q) {
             f32x4 v = widen(z[ct][jp + q]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] *= outer[jp + q][r];
+            for (int r = 0; r < 4; ++r) v[r] *= STATE_ONLY ? outer[jp + q][r] * apart : outer[jp + q][r];
 #pragma unroll
             for (int m = 0; m < PARTS; ++m) {
               k[q][m] = narrow(v);
@@ -665,9 +669,6 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
         }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-#pragma unroll
-        for (int ct = 0; ct < NC; ++ct)
-          if (STATE_ONLY) S[d][ct] *= whole;
         if (d + AHEAD < DT) turned(d + AHEAD);
 #pragma unroll
         for (int jp = 0; jp < CT; jp += 2)
@@ -685,13 +686,10 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
         for (int jt = 0; jt < CT; ++jt) {
           v[ct][jt] = widen(z[ct][jt]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[ct][jt][r] *= outer[jt][r];
+          for (int r = 0; r < 4; ++r) v[ct][jt][r] *= STATE_ONLY ? outer[jt][r] * apart : outer[jt][r];
         }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-#pragma unroll
-        for (int ct = 0; ct < NC; ++ct)
-          if (STATE_ONLY) S[d][ct] *= whole;
         if (d + AHEAD < DT) turned(d + AHEAD);
 #pragma unroll
         for (int jt = 0; jt < CT; ++jt) {
