@@ -179,13 +179,14 @@ hipError_t ring_linattn_step(const RingLinShape& s, const RingLinStep& a, hipStr
 //   the pass over states: 0.4 of a chunk, and 6 or (P > 64) 10 for its launch and what the pass behind reads of it
 //   the scan (more than kFold segments): 3 or 5, 0.2 a segment, and its states at 5 TB/s
 // us of a forward, and with its backward, by segments, the rule's choice in brackets:
-//   8 x 4096 tokens, 16 heads of 128, bf16    1: 231, 744   [2: 188, 542]    3: 193, 617    4: 179, 572    8: 221, 660
-//   1 x 32768 tokens, 16 heads of 128, bf16   1: 1777, 5772  8: 340, 963   [16: 218, 603]  32: 203, 627   64: 270, 729
-//   8 x 2048 tokens, 16 heads of 64, bf16     1: 70, 220     2: 59, 164     3: 54, 155    [4: 47, 135]    8: 52, 150
-//   8 x 2000 tokens, 8 heads of 256, fp32     1: 678, 2758  [2: 465, 1644]  4: 543, 1879    8: 634, 2124
-//   3 x 4096 tokens, 8 heads of 256, bf16     1: 393, 1487   4: 184, 564   [5: 153, 481]    8: 193, 627   16: 211, 639
-//   20 x 4096 tokens, 16 heads of 128, bf16  [1: 323]        2: 391          4: 444 (the forward alone, as in the next)
-//   2 x 1000 tokens, 4 heads of 64, fp32      1: 86          8: 27         [16: 23]
+//   8 x 4096 tokens, 16 heads of 128, bf16    1: 229, 743   [2: 187, 558]    3: 192, 619    4: 184, 584    8: 218, 672
+//   1 x 32768 tokens, 16 heads of 128, bf16   1: 1777, 5766  8: 333, 978   [16: 200, 585]  32: 208, 637   64: 237, 707
+//   1 x 8192 tokens, 8 heads of 128, bf16     1: 444, 1453   8: 93, 263     16: 60, 166   [32: 51, 134]   64: 60, 167
+//   8 x 2048 tokens, 16 heads of 64, bf16     1: 70, 220     2: 58, 164     3: 54, 155    [4: 47, 140]    8: 53, 149
+//   8 x 2000 tokens, 8 heads of 256, fp32     1: 677, 2760  [2: 455, 1621]  4: 524, 1843    8: 611, 2082
+//   3 x 4096 tokens, 8 heads of 256, bf16     1: 393, 1493   4: 168, 535   [5: 142, 458]    8: 180, 605   16: 203, 632
+//   20 x 4096 tokens, 16 heads of 128, bf16  [1: 345, 1340]  2: 421, 1364   4: 469, 1455
+//   2 x 1000 tokens, 4 heads of 64, fp32      1: 88, 306     8: 27, 135   [16: 24, 135]
 static int segments(const RingLinShape& s) {
   const int units = (s.T + kChunk - 1) / kChunk;
   const int widest = s.Dk > s.Dv ? s.Dk : s.Dv, P = widest <= 64 ? 64 : (widest <= 128 ? 128 : 256);

@@ -198,10 +198,11 @@ template <int N> __device__ __forceinline__ void wait_and_barrier() {
 // many clocks of vector instructions, which hardly overlap them, and a chain from the rows through the weights to the outputs: 1.6 us
 // a chunk in a chip with few workgroups.  With one on every compute unit it is 2.2 us, with two 2.0 for each of their chunks: memory.
 // 8 x 4096 tokens, 16 heads, 537 MB a pass: 130 us with 512 workgroups (4.1 TB/s; a large copy 5.2), 144 with 256; one sequence of 32768
-// tokens 153.  There (us, the latter case) chunks of
+// tokens 150 to 153.  There (us, the latter case) chunks of
 // 64 tokens take 165, eight waves of 16 columns 166, two chunks on their way at once 165.  fp32 and fp16 multiply at 32 clocks for an
 // eighth of the contraction, in chunks of 16 tokens (fp16: 32), and are bound by that: 8 x 2000 tokens, 8 heads of 256, fp32, 33.6 GFLOP
-// a pass without the weights: 390 us, 86 TFLOP/s (154 in a large matrix product).  States alone: 64 columns, 201 MB 58 us (3.5 TB/s).
+// a pass without the weights: 390 us, 86 TFLOP/s (154 in a large matrix product).  States alone, one
+// sequence of 32768 tokens: 252 MB, 70 us (3.6 TB/s).
 template <typename T, int DA, int NC, int NW, int CT, bool VEC, bool REV, bool STATE_ONLY, bool EXACT, bool PAIR = false>
 __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_linattn_kernel(RingLinArgs p) {
   constexpr int GW = PAIR ? NW / 2 : NW, WC = 16 * NC * GW, NT = 64 * NW, CH = 16 * CT, DT = DA / 16;
