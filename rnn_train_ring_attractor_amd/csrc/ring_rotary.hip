@@ -6,7 +6,7 @@
 // Backwards the same with the opposite angle.  A position is a count of tokens or an angle of its own (a heading; the pairs then turn
 // with its harmonics).
 //
-// Bound by memory: everything is read once and written once: 8 x 4096 tokens, 16 + 4 heads of 128, bf16: 336 MB in 69 us, 4.9 TB/s (a
+// Bound by memory: everything is read once and written once: 8 x 4096 tokens, 16 + 4 heads of 128, bf16: 336 MB in 67 us, 5.0 TB/s (a
 // large copy: 5.2).  A workgroup takes a few tokens through all heads of both tensors, so a
 // token's angles are found once: the number of turns as a product in 64 bits, whose whole part is taken off before it is rounded (at
 // position 2^20 a product in 32 bits is off by 0.06 rad), then one sine and cosine in 32.
@@ -20,6 +20,22 @@ constexpr int kAngles = 1024;      // (cos, sin) that a workgroup keeps
 // Bytes that a call reads and writes from which on it leaves nothing in the last cache (256 MB) that a reader behind it would find
 constexpr size_t kPastCache = 320000000;
 
+constexpr int kTokens = 256;       // tokens that a workgroup takes at most
+
+// n / d for n < 2^31 by a product and a shift: with 2^(s - 1) < d <= 2^s, floor(n (2^32 + m) / 2^(32 + s)) for m = floor(2^32 (2^s - d) / d) + 1
+// (the excess of (2^32 + m) / 2^(32 + s) over 1 / d is at most 2^-(32 + s), which n < 2^32 does not carry past a whole number).  Divisions
+// as such were most of the time of odd widths (the case below of 52 turned 308 us, 213 with products, one value at a time each).
+struct Divisor {
+  unsigned m, s;
+  static Divisor of(unsigned d) {
+    unsigned s = 0;
+    while ((1ull << s) < d) ++s;
+    return Divisor{(unsigned)((((1ull << s) - d) << 32) / d + 1), s};
+  }
+  __device__ __forceinline__ unsigned div(unsigned n) const { return (__umulhi(n, m) + n) >> s; }
+};
+struct Divisors { Divisor units, heads, pairs, T, last_heads; };
+
 __device__ __forceinline__ double position_of(const RingRotaryArgs& p, long at) {
   if (p.position_type == RINGATTR_POS_F32) return (double)((const float*)p.positions)[at];
   if (p.position_type == RINGATTR_POS_I32) return (double)((const int*)p.positions)[at];
@@ -28,27 +44,37 @@ __device__ __forceinline__ double position_of(const RingRotaryArgs& p, long at) 
 
 }  // namespace
 
-// V values at a time, neighbours in memory (V = 1: any strides and widths).  PAST: results are stored past the caches, where the call
+// V values at a time, neighbours in memory: 16 bytes, two values, or one (any strides and widths); what is copied C at a time.  PAST: results are stored past the caches, where the call
 // passes them anyway and its inputs would be pushed out (kPastCache), in rows of whole lines (16 + 4 heads of 128, bf16, halves, us with
 // and without: 336 MB with inputs just written 55, 68, inputs from memory 68.4, 69.6, and a call that reads the results 135, 142; smaller,
 // 252 MB: that 106, 97; rows of 128 bytes, 302 MB: 64.4, 63.1 and 130, 125).  Dropout gains nothing by it (403 and 268 MB there and back:
 // 124, 120).
-template <typename T, int V, bool HALF, bool PAST>
-__global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p) {
+template <typename T, int V, int C, bool HALF, bool PAST>
+__global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p, Divisors by) {
   constexpr int P = HALF ? V : (V + 1) / 2;                    // pairs of a unit
   typedef T vec __attribute__((ext_vector_type(V)));
-  auto store = [](T* at, vec x) {
-    if constexpr (PAST) __builtin_nontemporal_store(x, (vec*)at);
-    else *(vec*)at = x;
+  typedef T copied __attribute__((ext_vector_type(C)));
+  auto store = [](T* at, auto x) {
+    if constexpr (PAST) __builtin_nontemporal_store(x, (decltype(x)*)at);
+    else *(decltype(x)*)at = x;
   };
   __shared__ f32x2 trig[kAngles];
+  __shared__ long base[2][kTokens];
   const int tid = threadIdx.x, r = p.rot / 2, D = p.D;
   const long first = ((long)blockIdx.z * gridDim.x + blockIdx.x) * p.tokens, all = (long)p.B * p.T;
   if (first >= all) return;
   const int here = (int)(all - first < p.tokens ? all - first : p.tokens);
+  const unsigned b0 = (unsigned)first / (unsigned)p.T, t0 = (unsigned)first - b0 * (unsigned)p.T;
+  if (tid < here) {
+    const unsigned more = by.T.div(t0 + tid);
+    const long b = b0 + more, t = t0 + tid - more * (unsigned)p.T;
+    base[0][tid] = b * p.in[0].sb + t * p.in[0].st;
+    base[1][tid] = b * p.in[1].sb + t * p.in[1].st;
+  }
   for (int i = tid; i < here * r; i += 256) {
-    const int tok = i / r, m = i - tok * r;
-    const long b = (first + tok) / p.T, t = (first + tok) - b * p.T;
+    const int tok = by.pairs.div(i), m = i - tok * r;
+    const unsigned more = by.T.div(t0 + tok);
+    const long b = b0 + more, t = t0 + tok - more * (unsigned)p.T;
     const double pos = position_of(p, b * p.pos_b + t * p.pos_t), f = p.frequencies[m] * 0.15915494309189535;      // turns
     const double turns = rint(pos * f);
     const float x = 2.f * (float)fma(pos, f, -turns);
@@ -57,22 +83,21 @@ __global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p) {
     trig[i] = f32x2{p.scale * c, p.inverse ? -p.scale * s : p.scale * s};
   }
   __syncthreads();
-  // a row's units: P pairs each, then V values to copy
-  const int turned = r / P, units = turned + (D - p.rot) / V;
+  // a row's units: P pairs each, then C values to copy
+  const int turned = r / P, units = turned + (D - p.rot) / C;
   const int heads = p.heads[0] + p.heads[1], h0 = blockIdx.y * p.heads_per, h1 = min(heads, h0 + p.heads_per), nh = h1 - h0;
   for (int i = tid; i < here * nh * units; i += 256) {
-    const int row = i / units, u = i - row * units, tok = row / nh;
+    const int row = by.units.div(i), u = i - row * units, tok = (blockIdx.y + 1 == gridDim.y ? by.last_heads : by.heads).div(row);
     int h = h0 + row - tok * nh;
     const int which = h >= p.heads[0];
     if (which) h -= p.heads[0];
-    const long b = (first + tok) / p.T, t = (first + tok) - b * p.T;
     const RingLinTensor& in = p.in[which];
-    const T* x = (const T*)in.p + b * in.sb + t * in.st + h * in.sh;
+    const T* x = (const T*)in.p + base[which][tok] + h * in.sh;
     T* y = (T*)p.out[which] + ((first + tok) * p.heads[which] + h) * D;
     const f32x2* cs = trig + tok * r + u * P;
     if (u >= turned) {
-      const int d = p.rot + (u - turned) * V;
-      store(y + d, *(const vec*)(x + d));
+      const int d = p.rot + (u - turned) * C;
+      store(y + d, *(const copied*)(x + d));
     } else if constexpr (HALF) {
       const int d = u * V;
       const vec a = *(const vec*)(x + d), c = *(const vec*)(x + d + r);
@@ -111,10 +136,37 @@ __global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p) {
   }
 }
 
+// The largest of 16 bytes, two values and one that rows, pairs (halves: r, else all that is turned) and addresses are whole numbers of (us,
+// 8 x 4096 tokens, 16 + 4 heads of 128, bf16, halves: 64 turned 68; 52 turned, by two values 127, by one 213; 50 turned, by one and what is copied
+// by two 158; heads of 127 215).
+template <typename T> static int values_at_once(const RingRotaryArgs& p, int pairs) {
+  for (int v = 16 / sizeof(T); v > 1; v = v > 2 ? 2 : 1) {
+    bool fits = p.D % v == 0 && pairs % v == 0;
+    for (int i = 0; i < (p.heads[1] ? 2 : 1); ++i)
+      fits = fits && p.in[i].sb % v == 0 && p.in[i].st % v == 0 && p.in[i].sh % v == 0 &&
+             (reinterpret_cast<uintptr_t>(p.in[i].p) | reinterpret_cast<uintptr_t>(p.out[i])) % (v * sizeof(T)) == 0;
+    if (fits) return v;
+  }
+  return 1;
+}
+
+template <typename T, int V, int C, bool PAST> static void launch_kernel(const RingRotaryArgs& p, dim3 grid, hipStream_t st) {
+  const int r = p.rot / 2, pairs = p.interleaved ? (V + 1) / 2 : V;
+  // (the last heads of a grid row are fewer: their workgroups divide by their own number)
+  const int heads = p.heads[0] + p.heads[1], units = r / pairs + (p.D - p.rot) / C, last = heads - ((int)grid.y - 1) * p.heads_per;
+  const Divisors by = {Divisor::of(units), Divisor::of(p.heads_per), Divisor::of(r), Divisor::of(p.T), Divisor::of(last)};
+  if constexpr (V == C) {                                      // (neighbours: where two values fit, a pair does)
+    if (p.interleaved) {
+      hipLaunchKernelGGL((ring_rotary_kernel<T, V, C, false, PAST>), grid, dim3(256), 0, st, p, by);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((ring_rotary_kernel<T, V, C, true, PAST>), grid, dim3(256), 0, st, p, by);
+}
+
 template <typename T> static hipError_t launch(RingRotaryArgs p, hipStream_t st) {
   constexpr int W = 16 / sizeof(T);
-  const int r = p.rot / 2;
-  const bool vec = p.D % W == 0 && (p.interleaved ? p.rot % W == 0 : r % W == 0) && p.in[0].vec && (p.heads[1] == 0 || p.in[1].vec);
+  const int r = p.rot / 2, v = values_at_once<T>(p, p.interleaved ? p.rot : r), c = v > 1 ? v : values_at_once<T>(p, 2);
   const long all = (long)p.B * p.T;
   // As many tokens as give every lane an angle, fewer where that leaves compute units without work, then fewer heads (us, so and
   // with whole workgroups, bf16, 16 + 4 heads of 128: 64 x 1 tokens 3.0, 4.4; 100 tokens 3.0, 4.4; 1000 tokens 4.2, 5.1; 4 x 1000 8.9, 9.0).
@@ -126,18 +178,14 @@ template <typename T> static hipError_t launch(RingRotaryArgs p, hipStream_t st)
   if (split > heads) split = heads;
   p.heads_per = (heads + split - 1) / split;
   const long row = blocks < (1 << 20) ? blocks : 1 << 20;      // (a launch counts fewer than 2^32 threads along x)
-  const dim3 grid((unsigned)row, (unsigned)((heads + p.heads_per - 1) / p.heads_per), (unsigned)((blocks + row - 1) / row)), block(256);
+  const dim3 grid((unsigned)row, (unsigned)((heads + p.heads_per - 1) / p.heads_per), (unsigned)((blocks + row - 1) / row));
   const size_t row_bytes = p.D * sizeof(T);
   const bool past = row_bytes >= 256 && 2 * row_bytes * heads * (size_t)all >= kPastCache;
-  if (p.interleaved) {
-    if (vec && past) hipLaunchKernelGGL((ring_rotary_kernel<T, W, false, true>), grid, block, 0, st, p);
-    else if (vec) hipLaunchKernelGGL((ring_rotary_kernel<T, W, false, false>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((ring_rotary_kernel<T, 1, false, false>), grid, block, 0, st, p);
-  } else {
-    if (vec && past) hipLaunchKernelGGL((ring_rotary_kernel<T, W, true, true>), grid, block, 0, st, p);
-    else if (vec) hipLaunchKernelGGL((ring_rotary_kernel<T, W, true, false>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((ring_rotary_kernel<T, 1, true, false>), grid, block, 0, st, p);
-  }
+  if (v == W && past) launch_kernel<T, W, W, true>(p, grid, st);
+  else if (v == W) launch_kernel<T, W, W, false>(p, grid, st);
+  else if (v == 2) launch_kernel<T, 2, 2, false>(p, grid, st);
+  else if (c == 2) launch_kernel<T, 1, 2, false>(p, grid, st);
+  else launch_kernel<T, 1, 1, false>(p, grid, st);
   return hipGetLastError();
 }
 

@@ -1055,11 +1055,7 @@ int ringattr_rotary(const void* x0, const void* x1, const long long* strides, co
     return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
   RingRotaryArgs p = {};
   p.in[0] = rows_tensor(x0, strides, dim, type);
-  p.in[0].vec = p.in[0].vec && aligned16(y0);
-  if (heads1) {
-    p.in[1] = rows_tensor(x1, strides + 3, dim, type);
-    p.in[1].vec = p.in[1].vec && aligned16(y1);
-  }
+  if (heads1) p.in[1] = rows_tensor(x1, strides + 3, dim, type);
   p.out[0] = y0;
   p.out[1] = y1;
   p.heads[0] = heads0;

@@ -269,7 +269,9 @@ def test_single_tokens_go_on_from_a_prompt(B, H, G, Dk, Dv, kind, gpu_device):
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 @pytest.mark.parametrize("B,T,H,G,D,r,pos", [(1, 1, 1, 1, 2, 1, "shared"), (2, 7, 3, 1, 33, 16, "each"), (3, 5, 4, 2, 64, 32, "each"),
-                                             (2, 130, 2, 2, 128, 32, "shared"), (2, 3, 5, 5, 96, 24, "angle"), (1, 4, 1, 1, 520, 260, "angle")])
+                                             (2, 130, 2, 2, 128, 32, "shared"), (2, 3, 5, 5, 96, 24, "angle"), (1, 4, 1, 1, 520, 260, "angle"),
+                                             (2, 9, 3, 1, 64, 25, "each"), (1, 600, 2, 2, 62, 10, "shared"), (3, 33, 4, 1, 128, 26, "angle"),
+                                             (500, 1, 2, 1, 16, 3, "each"), (1, 2, 7, 3, 20, 5, "shared"), (1, 1, 900, 7, 6, 2, "each")])
 def test_rotary(B, T, H, G, D, r, pos, layout, kind, gpu_device):
     """Bound: cos and sin are fp32 numbers of an angle known to 2^-24 turns (2 pi 2^-24 rad) and each product and the sum are rounded:
     (2 pi + 4) 2^-24 of |a| + |b|, then the type's half step."""
@@ -308,6 +310,27 @@ def test_rotary(B, T, H, G, D, r, pos, layout, kind, gpu_device):
         size[..., i], size[..., j] = both, both
         err = (y.double().cpu() - want).abs()
         assert (err <= torch.finfo(dtype).eps / 2 * want.abs() * 1.0001 + (2 * math.pi + 4) * 2.0 ** -24 * size + 1e-7 * (dtype == torch.float16)).all()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotary_of_rows_at_any_address(layout, kind, gpu_device):
+    """Rows that start on 16 bytes, on two values and on one, heads stepped over, time-major: the same bits as contiguous ones."""
+    from rnn_train_ring_attractor_amd import rotary_func
+    gen = torch.Generator().manual_seed(41)
+    pos = torch.arange(19, device=gpu_device)
+    for D, r in ((64, 24), (64, 20), (64, 23), (62, 8)):
+        f = torch.rand(r, generator=gen, dtype=torch.float64).to(gpu_device)
+        x = _rand(gen, 3, 19, 5, D).to(TYPES[kind]).to(gpu_device)
+        want = rotary_func(x, pos, f, layout)
+        for lead, row in ((8, 80), (2, 72), (2, 71), (1, 72), (4, 66)):
+            print(f"[case] rotary rows {layout} {kind} {D} {r} {lead} {row}", flush=True)
+            wide = torch.full((19, 3, 10, row), math.nan, dtype=x.dtype, device=gpu_device)
+            placed = wide.transpose(0, 1)[:, :, ::2, lead:lead + D] if lead + D <= row else wide.transpose(0, 1)[:, :, ::2, :D]
+            placed.copy_(x)
+            assert torch.equal(rotary_func(placed, pos, f, layout), want)
+            both = rotary_func((placed, x[:, :, :2]), pos, f, layout)
+            assert torch.equal(both[0], want) and torch.equal(both[1], want[:, :, :2])
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
