@@ -23,7 +23,7 @@ constexpr size_t kPastCache = 320000000;
 constexpr int kTokens = 256;       // tokens that a workgroup takes at most
 
 // n / d for n < 2^31 by a product and a shift: with 2^(s - 1) < d <= 2^s, floor(n (2^32 + m) / 2^(32 + s)) for m = floor(2^32 (2^s - d) / d) + 1
-// (the excess of (2^32 + m) / 2^(32 + s) over 1 / d is at most 2^-(32 + s), which n < 2^32 does not carry past a whole number).  Divisions
+// (the excess of (2^32 + m) / 2^(32 + s) over 1 / d is at most 2^-(32 + s), which n < 2^31 does not carry past a whole number).  Divisions
 // as such were most of the time of odd widths (the case below of 52 turned 308 us, 213 with products, one value at a time each).
 struct Divisor {
   unsigned m, s;
@@ -44,9 +44,9 @@ __device__ __forceinline__ double position_of(const RingRotaryArgs& p, long at) 
 
 }  // namespace
 
-// V values at a time, neighbours in memory: 16 bytes, two values, or one (any strides and widths); what is copied C at a time.  PAST: results are stored past the caches, where the call
-// passes them anyway and its inputs would be pushed out (kPastCache), in rows of whole lines (16 + 4 heads of 128, bf16, halves, us with
-// and without: 336 MB with inputs just written 55, 68, inputs from memory 68.4, 69.6, and a call that reads the results 135, 142; smaller,
+// V values at a time, neighbours in memory: 16 bytes, two values, or one (any strides and widths); what is copied C at a time.
+// PAST: results are stored past the caches, where the call passes them anyway and its inputs would be pushed out (kPastCache), in rows of
+// whole lines (16 + 4 heads of 128, bf16, halves, us with and without: 336 MB with inputs just written 55, 68, inputs from memory 68.4, 69.6, and a call that reads the results 135, 142; smaller,
 // 252 MB: that 106, 97; rows of 128 bytes, 302 MB: 64.4, 63.1 and 130, 125).  Dropout gains nothing by it (403 and 268 MB there and back:
 // 124, 120).
 template <typename T, int V, int C, bool HALF, bool PAST>
