@@ -28,10 +28,11 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 namespace ring_lin {
 
 // bf16 operands go to the matrix units as they are, and what is computed on the way enters them so (half a step of bf16 is 2^-9 to 2^-8):
-//   weights, and the state in a product with a row: rounded to one bf16 number.  Each term of an output passes one of them: an output's
-//     error is 0.0023 of its size, its own rounding alone 0.0017 (with sums of two numbers 0.0017, and 167 us a pass against 130)
+//   weights, and the state in a product with a row: a sum of two bf16 numbers, 2^-15.  Each term of an output passes one of them, so that
+//     an output's error is its own rounding, 0.0017 of its size (with one number 0.0023; a forward of 8 x 4096 tokens, 16 heads of 128,
+//     takes 213 us so and 189 with one)
 //   a decayed row that goes into the state: a sum of two, 2^-16, because a state collects the errors of all that came before
-//   the same where the state is itself a result: a sum of three, 2^-24, as exact as fp32 sums (EXACT; 157 against 144 us a pass)
+//   the same where the state is itself a result: a sum of three, 2^-24, as exact as fp32 sums (EXACT)
 // The state is kept in 32 bits throughout.  fp32 and fp16 go to the fp32 matrix units: fp16 because weights and states can pass its range.
 template <typename T> struct Type;
 template <> struct Type<__bf16> { static constexpr bool BF = true; static constexpr unsigned EXPONENT = 0x7f80u; typedef bf16x4 V4; typedef unsigned short Bits; };
@@ -49,6 +50,14 @@ __device__ __forceinline__ f32x4 widen(bf16x4 x) {
 __device__ __forceinline__ f32x4 widen(f16x4 x) { return __builtin_convertvector(x, f32x4); }
 __device__ __forceinline__ f32x4 widen(f32x4 x) { return x; }
 __device__ __forceinline__ bf16x4 narrow(f32x4 x) { return __builtin_convertvector(x, bf16x4); }
+// x as the sum of two bf16 numbers, 2^-15 of it left out at most: x cut off behind its first 8 bits (cut off, so that the largest finite
+// numbers stay finite), then what is left, rounded
+struct Halves { bf16x4 high, low; };
+__device__ __forceinline__ Halves halves(f32x4 x) {
+  const u32x4 b = __builtin_bit_cast(u32x4, x);
+  const u32x2 high = {__builtin_amdgcn_perm(b[1], b[0], 0x07060302u), __builtin_amdgcn_perm(b[3], b[2], 0x07060302u)};
+  return {__builtin_bit_cast(bf16x4, high), narrow(x - __builtin_bit_cast(f32x4, b & 0xffff0000u))};
+}
 __device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
@@ -500,11 +509,14 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
               if (REV ? jt >= it : jt <= it) P[jt][it] = mfma16(yr[s & 1][jt], xr[s & 1][it], P[jt][it]);
 #pragma unroll
           for (int ct = 0; ct < NC; ++ct) {
-            const bf16x8 state = join(narrow(S[2 * s][ct]), narrow(S[2 * s + 1][ct]));
+            const Halves a0 = halves(S[2 * s][ct]), a1 = halves(S[2 * s + 1][ct]);
+            const bf16x8 high = join(a0.high, a1.high), low = join(a0.low, a1.low);
             S[2 * s][ct] *= whole;
             S[2 * s + 1][ct] *= whole;
 #pragma unroll
-            for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(state, xr[s & 1][it], O[ct][it]);
+            for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(high, xr[s & 1][it], O[ct][it]);
+#pragma unroll
+            for (int it = 0; it < CT; ++it) O[ct][it] = mfma16(low, xr[s & 1][it], O[ct][it]);
           }
         } else {
 #pragma unroll
@@ -571,9 +583,12 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
 #pragma unroll
           for (int it = 0; it < CT; ++it)
             if (REV ? jp + 1 >= it : jp <= it) {
-              const bf16x8 weights = join(narrow(P[jp][it]), narrow(P[jp + 1][it]));
+              const Halves a0 = halves(P[jp][it]), a1 = halves(P[jp + 1][it]);
+              const bf16x8 high = join(a0.high, a1.high), low = join(a0.low, a1.low);
 #pragma unroll
-              for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma16(join(z[ct][jp], z[ct][jp + 1]), weights, O[ct][it]);
+              for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma16(join(z[ct][jp], z[ct][jp + 1]), high, O[ct][it]);
+#pragma unroll
+              for (int ct = 0; ct < NC; ++ct) O[ct][it] = mfma16(join(z[ct][jp], z[ct][jp + 1]), low, O[ct][it]);
             }
       } else {
 #pragma unroll

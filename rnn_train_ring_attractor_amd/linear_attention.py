@@ -6,8 +6,9 @@
 initial state, by the same kernels run over other operands), `linear_attention_step` one token for each sequence of a batch (serving:
 the recurrent form, the state updated in place).  What the one leaves as its state the other goes on from.
 
-The operands are float32, bfloat16 or float16; states are float32.  With bfloat16 each term of a result passes one operand that is
-rounded to bfloat16, its weight or the state in front of its chunk; states that are results are as exact as float32 sums."""
+The operands are float32, bfloat16 or float16; states are float32.  With bfloat16 what is computed on the way, weights and states, enters
+products as sums of two bfloat16 numbers (2^-15), so that a result's error is its own rounding; states that are results are as exact as
+float32 sums."""
 from __future__ import annotations
 
 import ctypes

@@ -1,0 +1,85 @@
+"""What the sequence operators' documentation promises, call by call, where the tests of their formulas do not look: how exact bf16 results are,
+also without a returned state.
+
+A bf16 result is a sum in fp32, rounded once: half a step, 2^-8 of it.  Each term of it passes an operand that is computed on the way and
+enters a product as the sum of two bf16 numbers (a weight or a state: x cut off behind 8 bits, 2^-7 of it left, then that rounded, 2^-8 of
+it: 2^-15), and, in a state that is no result, a decayed row in two rounded ones (2^-16); K additions and products in fp32, 2^-24 each.
+The last three are bounded against the same sum over the terms' magnitudes."""
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_sequence import SEGMENTED, SHAPES, TYPES, _problem, _reference
+
+pytestmark = pytest.mark.gpu
+
+
+def _call(p, dtype, dev, lengths=None, state=True, scale=None):
+    """linear_attention_func and its gradients; state: whether the final one is asked for (and has a gradient)."""
+    from rnn_train_ring_attractor_amd import linear_attention_func
+    leaves = [p[n].to(dtype).to(dev).requires_grad_(True) for n in ("q", "k", "v")]
+    s0 = None if p["s0"] is None else p["s0"].float().to(dev).requires_grad_(True)
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=dev)
+    got = linear_attention_func(*leaves, p["g"].float().to(dev), initial_state=s0, lengths=lens, scale=scale, return_state=state)
+    outs, given = ([*got], [p["do"].to(dtype).to(dev), p["ds"].float().to(dev)]) if state else ([got], [p["do"].to(dtype).to(dev)])
+    grads = torch.autograd.grad(outs, leaves + ([] if s0 is None else [s0]), given)
+    return dict(zip(["o", "state"][:len(outs)] + ["dq", "dk", "dv", "ds0"], [x.detach() for x in (*outs, *grads)]))
+
+
+def _without_state_gradient(p):
+    return {**p, "ds": torch.zeros_like(p["ds"])}
+
+
+def _lengths(T, B, count):
+    first = -(-(-(-T // 64)) // count) * 64
+    return [first + 1, T, 0, first, 1, first - 1, T - 1, 65][:B]
+
+
+def _bf16_bound(want, size, K):
+    return 2.0 ** -8 * want.abs() + (1 + 2.0 ** -8) * (2.0 ** -15 + 2.0 ** -16 + K * 2.0 ** -24) * size + 1e-37
+
+
+BF16 = [(s, 1) for s in SHAPES if s[1] > 1] + [(s, n) for k, s, n in SEGMENTED if k == "bf16"]
+
+
+@pytest.mark.parametrize("state", [True, False], ids=["state", "no_state"])
+@pytest.mark.parametrize("sizes,count", BF16, ids=["x".join(map(str, s)) for s, _ in BF16])
+def test_bf16_results_carry_their_own_rounding(sizes, count, state, gpu_device):
+    print(f"[case] bf16 {sizes} state={state}", flush=True)
+    B, T, H, G, Dk, Dv = sizes
+    p = _problem(43, *sizes, torch.bfloat16, start=T % 2 == 0)
+    p = p if state else _without_state_gradient(p)
+    lengths = _lengths(T, B, count) if count > 1 else None
+    got, want, size = _call(p, torch.bfloat16, gpu_device, lengths, state), _reference(p, lengths), _reference(p, lengths, magnitudes=True)
+    for name in ("o", "dq", "dk", "dv"):
+        err = (got[name].double().cpu() - want[name]).abs()
+        bound = _bf16_bound(want[name], size[name], T + Dk + Dv + H // G + 256)
+        assert (err <= bound).all(), (name, float((err / bound).max()))
+        if want[name].numel() >= 10000:
+            # A rounding error is even within half a step of 2^-9 to 2^-8 of a value: of numbers of even logarithms the root mean square is
+            # 2^-8 (3 / (8 ln 2) / 3) ** 0.5 = 0.00166 of theirs; a tenth more for numbers that are not
+            rms = math.sqrt(float((err ** 2).sum() / (want[name] ** 2).sum()))
+            print(f"[rms] {name} {rms:.5f}", flush=True)
+            assert rms <= 1.1 * 0.00166, (name, rms)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("sizes,count", [((2, 333, 2, 1, 40, 72), 0)] + [(s, n) for _, s, n in SEGMENTED], ids=lambda x: "x".join(map(str, x)) if isinstance(x, tuple) else str(x))
+def test_sums_of_small_whole_numbers_are_exact(sizes, count, kind, gpu_device):
+    """Operands of -1, 0 and 1 without decay: weights, states (below 2^16) and sums (below 2^24) are whole numbers that every step holds, so
+    each result is the sum rounded once, and a token too many or too few shows."""
+    print(f"[case] whole numbers {sizes} {kind}", flush=True)
+    B, T, H, G, Dk, Dv = sizes
+    gen = torch.Generator().manual_seed(47)
+    whole = lambda *s: torch.randint(-1, 2, s, generator=gen).double()
+    p = {"q": whole(B, T, H, Dk), "k": whole(B, T, G, Dk), "v": whole(B, T, G, Dv), "do": whole(B, T, H, Dv), "g": torch.zeros(H, dtype=torch.float64),
+         "s0": whole(B, H, Dk, Dv), "ds": whole(B, H, Dk, Dv)}
+    lengths = _lengths(T, B, max(count, 2))
+    got = _call(p, TYPES[kind], gpu_device, lengths, True, 1.0)
+    want = _reference({**p, "q": p["q"] * Dk ** 0.5}, lengths)           # (the oracle's scale is Dk ** -0.5)
+    want["dq"] = want["dq"] * Dk ** 0.5
+    for name in want:
+        exact = want[name].round()
+        assert (exact - want[name]).abs().max() < 1e-6 and exact.abs().max() < 60000
+        assert torch.equal(got[name].cpu(), exact.to(got[name].dtype)), name
