@@ -648,6 +648,13 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
                 if (nonfinite(zs[ct])) S[d][ct][r] = fmaf(y, zs[ct], S[d][ct][r]);
             }
         }
+      // rows that do not count come from rows of zeros, but zero times what is not finite is not zero
+      if (n < CH)
+#pragma unroll
+        for (int it = 0; it < CT; ++it)
+          if (16 * it + l >= n)
+#pragma unroll
+            for (int ct = 0; ct < NC; ++ct) O[ct][it] = f32x4{0.f, 0.f, 0.f, 0.f};
       put(O, t, min(CH, t1 - t));
       stored = n == CH && cw + 16 * NC <= cols;
     }

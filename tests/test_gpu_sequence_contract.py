@@ -83,3 +83,29 @@ def test_sums_of_small_whole_numbers_are_exact(sizes, count, kind, gpu_device):
         exact = want[name].round()
         assert (exact - want[name]).abs().max() < 1e-6 and exact.abs().max() < 60000
         assert torch.equal(got[name].cpu(), exact.to(got[name].dtype)), name
+
+
+# (sizes, lengths): ends inside chunks, heads whose dv and dk go back together and not, rows of whole 16 bytes and not, segments
+PADDED = [((4, 90, 2, 1, 32, 48), [45, 90, 1, 33]), ((4, 90, 2, 2, 33, 47), [45, 90, 1, 70]), ((3, 70, 2, 1, 40, 72), [37, 70, 0]),
+          ((2, 70, 1, 1, 256, 136), [41, 69]), ((4, 500, 2, 2, 20, 70), [70, 500, 0, 499]), ((4, 500, 2, 1, 70, 66), [129, 65, 3, 450])]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("sizes,lengths", PADDED, ids=["x".join(map(str, s)) for s, _ in PADDED])
+def test_rows_behind_a_length_are_zero_whatever_the_others_hold(sizes, lengths, kind, gpu_device):
+    """An infinity or NaN in a row that counts, in the initial state or in the final one's gradient leaves everything behind the lengths zero,
+    and other sequences as they were."""
+    dtype = TYPES[kind]
+    p = _problem(53, *sizes, dtype, start=True)
+    clean = _call(p, dtype, gpu_device, lengths)
+    for name in ("q", "k", "v", "do", "s0", "ds"):
+        for value in (math.inf, math.nan):
+            for at in ((0,) if name in ("s0", "ds") else (0, lengths[0] - 1)):
+                print(f"[case] {value} in {name} at {at} {sizes} {kind}", flush=True)
+                bad = {n: (None if x is None else x.clone()) for n, x in p.items()}
+                (bad[name][0] if name in ("s0", "ds") else bad[name][0, at])[..., 2] = value
+                got = _call(bad, dtype, gpu_device, lengths)
+                for n in ("o", "dq", "dk", "dv"):
+                    assert all((got[n][b, m:] == 0).all() for b, m in enumerate(lengths)), n
+                assert all(torch.equal(got[n][1:], clean[n][1:]) for n in got)
+                assert not all(torch.isfinite(got[n][0]).all() for n in got)
