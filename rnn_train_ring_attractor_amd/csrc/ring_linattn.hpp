@@ -298,14 +298,15 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
     }
   }
 
-  // powers of the decay: by distance within a pair of tiles, and for the rows of a chunk of n
+  // powers of the decay: by distance within a pair of tiles, and for the rows of a chunk of n.  None that no token has: with a decay above one it
+  // could be infinite, and a row of zeros times it no longer zero.
   float near[CT][4], inner[CT], outer[CT][4], whole = 1.f;
 #pragma unroll
   for (int d = 0; d < CT; ++d)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int e = 16 * d + (REV ? 4 * g + r - l : l - 4 * g - r);
-      near[d][r] = e < 0 ? 0.f : p.intra * power(g2, e);
+      near[d][r] = e < 0 || e >= te - t0 ? 0.f : p.intra * power(g2, e);
     }
   int n_now = -1;
 
@@ -422,7 +423,7 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int j = 16 * it + 4 * g + r;
-          outer[it][r] = p.update * power(g2, REV ? j + 1 : max(n - 1 - j, 0));
+          outer[it][r] = p.update * power(g2, REV ? min(j, n - 1) + 1 : max(n - 1 - j, 0));
         }
       }
     }

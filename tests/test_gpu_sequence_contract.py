@@ -109,3 +109,19 @@ def test_rows_behind_a_length_are_zero_whatever_the_others_hold(sizes, lengths, 
                     assert all((got[n][b, m:] == 0).all() for b, m in enumerate(lengths)), n
                 assert all(torch.equal(got[n][1:], clean[n][1:]) for n in got)
                 assert not all(torch.isfinite(got[n][0]).all() for n in got)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_a_state_that_grows_in_a_short_chunk(kind, gpu_device):
+    """A decay above one: powers of places behind a chunk's last token can pass fp32's range, those of its tokens do not."""
+    dtype = TYPES[kind]
+    for T, lengths in ((1, None), (3, None), (5, [5, 2]), (40, [3, 1])):
+        print(f"[case] growing state {T} {lengths} {kind}", flush=True)
+        p = _problem(59, 2, T, 2, 1, 16, 24, dtype, start=True, decays=[6.0, 0.5])
+        got, want, size = _call(p, dtype, gpu_device, lengths), _reference(p, lengths), _reference(p, lengths, magnitudes=True)
+        for name in want:
+            half = 2.0 ** -24 if name in ("state", "ds0") else torch.finfo(dtype).eps / 2
+            path = (2.0 ** -15 + 2.0 ** -16 if kind == "bf16" else 0.0) + (T + 16 + 24 + 2 + 256) * 2.0 ** -24
+            err = (got[name].double().cpu() - want[name]).abs()
+            fits = want[name].abs() * (1 + half) < torch.finfo(got[name].dtype).max
+            assert (err <= half * want[name].abs() + (1 + half) * path * size[name] + 1e-7)[fits].all(), (name, T)
