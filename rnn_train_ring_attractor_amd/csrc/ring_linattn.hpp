@@ -131,7 +131,7 @@ template <typename T, int ROWS, int COLS> struct Tile16 {
 // Global memory -> LDS without registers: a wave's instruction fills 64 granules one behind the other, each lane from where it likes.
 // What is loaded is there behind a wait for vmcnt and a barrier (nobody else keeps count: the compiler does not see these loads).  It
 // says nothing about memory to the compiler, so that reads of the other buffer pass it by: every use of what it writes, and every
-// use of what was there, is on the other side of wait_and_barrier, which does.
+// use of what was there, is on the other side of such a wait and barrier, which do.
 // base and lds are the same in all lanes.  (The wait states are for a base that a vector instruction has just put into its scalar
 // registers: the compiler does not look into the statement.)
 __device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned lds) {
@@ -194,9 +194,8 @@ template <typename T> __device__ __forceinline__ const T* rows_of(const RingLinT
   return reinterpret_cast<const T*>(t.p) + (long)b * t.sb + (long)(h / share) * t.sh;
 }
 
-template <int N> __device__ __forceinline__ void wait_and_barrier() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
+// Waits until no more than N of the wave's accesses to memory are on their way, the last N that it issued
+template <int N> __device__ __forceinline__ void wait_for_memory() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
 
 // A workgroup: one head of one sequence, WC = 16 NC NW columns of Z and of the state, one segment of the tokens.  Its waves share the
 // chunk's rows in LDS (two buffers: the next chunk's are on their way while one is worked on); each keeps 16 NC columns of the state
@@ -404,8 +403,9 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
     char *const tile = lds + buf * BUF, *const ty = tile + XB, *const tz = ty + TA::BYTES, *const t2 = tz + TZ::BYTES;
     char *const lx = second ? t2 : tile, *const ly = second ? tz : ty, *const lz = second ? ty : tz;
     // the chunk's rows are there; the outputs of the one before, stored behind the loads, need not be (a store for each of its tiles)
-    if (VEC && !STATE_ONLY && stored) wait_and_barrier<CT>();
-    else wait_and_barrier<0>();
+    if (VEC && !STATE_ONLY && stored) wait_for_memory<CT>();
+    else wait_for_memory<0>();
+    lds_barrier();
     if (n < CH) {                                              // (the last chunk of a sequence)
       if (!STATE_ONLY) FA::clear(tile, n, tid);
       FA::clear(ty, n, tid);
@@ -656,8 +656,11 @@ __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_
           if (16 * it + l >= n)
 #pragma unroll
             for (int ct = 0; ct < NC; ++ct) O[ct][it] = f32x4{0.f, 0.f, 0.f, 0.f};
+      // What the wait at the next chunk's front counts on: its loads go out ahead of these stores.  The loads say nothing about memory to the
+      // compiler; statements like them it leaves in order, and the stores in order with this one.
+      asm volatile("" ::: "memory");
       put(O, t, min(CH, t1 - t));
-      stored = n == CH && cw + 16 * NC <= cols;
+      stored = n == CH && __builtin_amdgcn_readfirstlane(cw) + 16 * NC <= cols;      // (the same in all lanes: a barrier depends on it)
     }
     // the state behind the chunk; Y's columns are read AHEAD tiles ahead
     const float apart = power(g2, REV ? t - t0 : te - t - n);  // (STATE_ONLY: the tokens between the chunk and the state)
