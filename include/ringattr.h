@@ -290,7 +290,8 @@ RINGATTR_API int ringattr_clip_adam_counted(int n_tensors, void* const* params, 
  * 256; states fp32 [B,heads,dk,dv].  initial_state NULL: zeros; final_state NULL: not wanted.  lengths (device int32 [B], NULL:
  * seq_len) says how many tokens of each sequence count: outputs and gradients behind them are zero, nothing there is read, the
  * final state is the one behind the last token that counts.  Values that are infinite or NaN do not reach rows that do not see
- * them.  strides: host array, three for each of q, k, v (and grad_o), in that order. */
+ * them.  strides: host array, three for each of q, k, v (and grad_o), in that order.  Outputs and workspaces start at 16 bytes, everything that is
+ * read at its own type's size. */
 #define RINGATTR_ATTENTION_MAX_DIM 256
 RINGATTR_API size_t ringattr_linear_attention_fwd_workspace_bytes(int type, int batch_size, int seq_len, int heads, int kv_heads,
                       int dk, int dv);

@@ -125,3 +125,31 @@ def test_a_state_that_grows_in_a_short_chunk(kind, gpu_device):
             err = (got[name].double().cpu() - want[name]).abs()
             fits = want[name].abs() * (1 + half) < torch.finfo(got[name].dtype).max
             assert (err <= half * want[name].abs() + (1 + half) * path * size[name] + 1e-7)[fits].all(), (name, T)
+
+
+@pytest.mark.parametrize("sizes", [(2, 9, 3, 1, 5, 7), (1, 300, 1, 1, 5, 7)])
+def test_states_at_any_address(sizes, gpu_device):
+    """States and their gradients that are views into a larger tensor, off 16 bytes: the same bits."""
+    from rnn_train_ring_attractor_amd import linear_attention_func
+    print(f"[case] states at any address {sizes}", flush=True)
+    B, T, H, G, Dk, Dv = sizes
+    gen = torch.Generator(device=gpu_device).manual_seed(61)
+    r = lambda *s: torch.randn(*s, generator=gen, device=gpu_device)
+    q, k, v = r(B, T, H, Dk).requires_grad_(True), r(B, T, G, Dk).requires_grad_(True), r(B, T, G, Dv).requires_grad_(True)
+    g, pool = -torch.rand(H, generator=gen, device=gpu_device), r(4, B, H, Dk, Dv)
+    assert any(pool[i].data_ptr() % 16 for i in range(4))
+    for i in range(4):
+        ds = r(4, B, H, Dk, Dv)
+        results = []
+        for s0, d in ((pool[i], ds[i]), (pool[i].clone(), ds[i].clone())):
+            s0 = s0.detach().requires_grad_(True)
+            o, s = linear_attention_func(q, k, v, g, initial_state=s0, return_state=True)
+            results.append([o, s, *torch.autograd.grad([o, s], [q, k, v, s0], [torch.ones_like(o), d])])
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+    # autograd hands the pieces of a stacked gradient on as views
+    s0 = pool[1].detach().requires_grad_(True)
+    ends = [linear_attention_func(q, k, v, g, initial_state=s0, return_state=True)[1] for _ in range(3)]
+    weights = r(3, B, H, Dk, Dv)
+    together, = torch.autograd.grad((torch.stack(ends) * weights).sum(), [s0], retain_graph=True)
+    alone = sum(torch.autograd.grad([e], [s0], [w.clone()], retain_graph=True)[0] for e, w in zip(ends, weights))
+    assert torch.allclose(together, alone, rtol=1e-5, atol=1e-5)
