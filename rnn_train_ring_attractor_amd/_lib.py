@@ -222,9 +222,26 @@ def plain_gpu_tensor(t) -> bool:
     tracing, compilation, a dispatch or function mode) to miss them."""
     if type(t) is not torch.Tensor or not t.is_cuda or t.dtype != torch.float32 or t.layout != torch.strided:
         return False
-    if (t.requires_grad and torch.is_grad_enabled()) or torch.compiler.is_compiling() or torch.jit.is_tracing():
+    if t.requires_grad and torch.is_grad_enabled():
         return False
-    return not _watched() and not t.is_neg() and t.numel() > 0
+    return not watched() and not t.is_neg() and t.numel() > 0
+
+
+def watched() -> bool:
+    """Whether something beside autograd's backward may follow or transform the operations.  An operator is called as an autograd Function
+    then, which is refused where it lacks a rule (forward mode, functorch) and recorded (tracing, compilation)."""
+    return torch.compiler.is_compiling() or torch.jit.is_tracing() or _watched()
+
+
+def refuse_derivatives(who, *tensors) -> None:
+    """For an operator without any derivative, which is no Function: forward mode, function transforms and tracing of these tensors."""
+    if torch.compiler.is_compiling():        # (a compiler leaves the call to Python, where the question comes again)
+        return
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{who} cannot be traced")
+    for t in tensors:
+        if torch._C._functorch.is_functorch_wrapped_tensor(t) or torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{who} has no gradient, in forward mode and function transforms neither")
 
 
 def _watched() -> bool:

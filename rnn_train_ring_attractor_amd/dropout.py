@@ -59,6 +59,6 @@ def dropout_func(x, p, seed, offset=0, residual=None):
     seed, offset = int(seed), int(offset)
     if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
         raise ValueError("seed and offset must be whole numbers from 0 to 2^64 - 1")
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+    if _lib.watched() or (torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))):
         return DropoutFunc.apply(x, residual, p, seed, offset, counter)
     return _drop(x, residual, p, seed, offset, counter)

@@ -133,8 +133,8 @@ def linear_attention_func(q, k, v, log_decay, initial_state=None, lengths=None, 
         lengths = lengths.contiguous()
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
     scale = Dk ** -0.5 if scale is None else float(scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
-                                    (initial_state is not None and initial_state.requires_grad)):
+    if _lib.watched() or (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                                       (initial_state is not None and initial_state.requires_grad))):
         o, state = LinearAttentionFunc.apply(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
     else:
         o, state, _ = _forward(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
@@ -152,6 +152,8 @@ def linear_attention_step(q, k, v, log_decay, state, active=None, scale=None):
         raise RuntimeError("state must be contiguous: it is updated in place")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise RuntimeError("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention_func to train")
+    if _lib.watched():
+        _lib.refuse_derivatives("linear_attention_step", q, k, v, log_decay, state)
     if active is not None:
         check_sequence_tensor("active", active, (B,), torch.uint8 if getattr(active, "dtype", None) == torch.uint8 else torch.bool, dev)
         active = active.contiguous()

@@ -132,7 +132,7 @@ def rotary_func(x, positions, frequencies, layout="half", scale=1.0):
     if frequencies.dim() != 1 or not 1 <= frequencies.numel() <= D // 2:
         raise ValueError(f"frequencies must be one-dimensional, between 1 and {D // 2} of them, got {tuple(frequencies.shape)}")
     frequencies, scale = frequencies.contiguous(), float(scale)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in xs):
+    if _lib.watched() or (torch.is_grad_enabled() and any(t.requires_grad for t in xs)):
         ys = RotaryFunc.apply(positions, frequencies, _LAYOUTS[layout], scale, 0, *xs)
     else:
         ys = _turned(positions, frequencies, _LAYOUTS[layout], scale, 0, *xs)

@@ -153,3 +153,54 @@ def test_states_at_any_address(sizes, gpu_device):
     together, = torch.autograd.grad((torch.stack(ends) * weights).sum(), [s0], retain_graph=True)
     alone = sum(torch.autograd.grad([e], [s0], [w.clone()], retain_graph=True)[0] for e, w in zip(ends, weights))
     assert torch.allclose(together, alone, rtol=1e-5, atol=1e-5)
+
+
+def _entries(dev):
+    from rnn_train_ring_attractor_amd import dropout_func, linear_attention_func, rotary_func
+    gen = torch.Generator(device=dev).manual_seed(67)
+    k, v, g = (torch.randn(2, 5, 2, d, generator=gen, device=dev) for d in (8, 6, 1))
+    g = torch.tensor([-0.1, -0.5], device=dev)
+    pos, f = torch.arange(5, device=dev), torch.rand(4, generator=gen, dtype=torch.float64, device=dev)
+    return {"attention": lambda x: linear_attention_func(x, k, v, g), "rotary": lambda x: rotary_func(x, pos, f), "pair": lambda x: rotary_func((k, x), pos, f)[1],
+            "dropout": lambda x: dropout_func(x, 0.3, 5, 6), "residual": lambda x: dropout_func(k, 0.3, 5, 6, residual=x)}, torch.randn(2, 5, 2, 8, generator=gen, device=dev)
+
+
+@pytest.mark.parametrize("name", ["attention", "rotary", "pair", "dropout", "residual"])
+def test_what_watches_the_operators_sees_them(name, gpu_device):
+    """Forward mode and function transforms, which they have no rules for, are refused instead of losing the derivative; a trace records the call."""
+    import torch.autograd.forward_ad as forward
+    entries, x = _entries(gpu_device)
+    op = entries[name]
+    print(f"[case] watched {name}", flush=True)
+    want = op(x)
+    with forward.dual_level():
+        assert torch.equal(op(x), want)                          # nothing of it is differentiated
+        with pytest.raises(NotImplementedError, match="jvp"):
+            op(forward.make_dual(x, torch.ones_like(x)))
+    for transformed in (lambda: torch.func.jvp(op, (x,), (x,)), lambda: torch.func.vmap(op)(x[None]), lambda: torch.func.grad(lambda t: op(t).sum())(x)):
+        with pytest.raises(RuntimeError):
+            transformed()
+    traced = torch.jit.trace(op, x)
+    other = x.flip(0).contiguous() * 2
+    for _ in range(2):
+        assert torch.equal(traced(other), op(other))
+
+
+def test_what_watches_a_single_token(gpu_device):
+    import torch.autograd.forward_ad as forward
+    from rnn_train_ring_attractor_amd import linear_attention_step
+    q, k, v, s = (torch.randn(2, 2, *d, device=gpu_device) for d in ((8,), (8,), (6,), (8, 6)))
+    g = torch.tensor([-0.1, -0.5], device=gpu_device)
+    step = lambda q, s: linear_attention_step(q, k, v, g, s)
+    want = step(q, s.clone())
+    before = s.clone()
+    with forward.dual_level():
+        assert torch.equal(step(q, s.clone()), want)
+        for a, b in ((forward.make_dual(q, q), s), (q, forward.make_dual(s, s))):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                step(a, b)
+    for transformed in (lambda: torch.func.jvp(lambda t: step(t, s), (q,), (q,)), lambda: torch.func.vmap(lambda t: step(t, s))(q[None]),
+                        lambda: torch.func.grad(lambda t: step(t, s).sum())(q), lambda: torch.jit.trace(step, (q, s))):
+        with pytest.raises(RuntimeError):
+            transformed()
+    assert torch.equal(s, before)
