@@ -171,6 +171,11 @@ def profile_read():
 SEQUENCE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # RINGATTR_F32, _BF16, _F16
 
 
+def as_lies(t):
+    """t, written out if torch keeps it negated lazily (the imaginary part of a conjugate): kernels read memory as it lies."""
+    return t.resolve_neg() if t is not None and t.is_neg() else t
+
+
 def check_sequence_tensor(name, t, shape=None, dtype=None, device=None) -> None:
     """What the sequence operators ask of a tensor: one of their types (or the one given), on the GPU, and the shape."""
     if not isinstance(t, torch.Tensor):

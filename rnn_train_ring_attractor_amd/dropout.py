@@ -5,12 +5,12 @@ import torch
 from torch.autograd import Function
 
 from . import _lib
-from ._lib import SEQUENCE_TYPES, check_sequence_tensor
+from ._lib import SEQUENCE_TYPES, as_lies, check_sequence_tensor
 
 
 def _drop(x, residual, p, seed, offset, counter):
-    x = x.contiguous()
-    residual = None if residual is None else residual.contiguous()
+    x = as_lies(x).contiguous()
+    residual = None if residual is None else as_lies(residual).contiguous()
     y = torch.empty_like(x)
     if x.numel() == 0:
         return y

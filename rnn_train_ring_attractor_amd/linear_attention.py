@@ -17,13 +17,14 @@ import torch
 from torch.autograd import Function
 
 from . import _lib
-from ._lib import SEQUENCE_TYPES, check_sequence_tensor
+from ._lib import SEQUENCE_TYPES, as_lies, check_sequence_tensor
 
 _Strides9, _Strides12, _Strides6 = ctypes.c_longlong * 9, ctypes.c_longlong * 12, ctypes.c_longlong * 6
 
 
 def _rows(t):
     """t with a head's values as neighbours (any other strides are taken as they are)."""
+    t = as_lies(t)
     return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
 
 
@@ -93,7 +94,7 @@ class LinearAttentionFunc(Function):
             gq, gk, gv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
             want = initial_state is not None and ctx.needs_input_grad[4]
             g0 = log_decay.new_empty((B, H, Dk, Dv)) if want else None
-            gs = None if grad_state is None else grad_state.contiguous()
+            gs = None if grad_state is None else as_lies(grad_state).contiguous()
             if B == 0 or T == 0:
                 if want:
                     g0.zero_() if gs is None else g0.copy_(gs)
@@ -125,13 +126,13 @@ def linear_attention_func(q, k, v, log_decay, initial_state=None, lengths=None, 
     B, T = q.shape[:2]
     if initial_state is not None:
         check_sequence_tensor("initial_state", initial_state, (B, H, Dk, Dv), torch.float32, dev)
-        initial_state = initial_state.contiguous()
+        initial_state = as_lies(initial_state).contiguous()
     if lengths is not None:
         if isinstance(lengths, torch.Tensor) and lengths.dtype == torch.int64:
             lengths = lengths.clamp(0, T).to(torch.int32)
         check_sequence_tensor("lengths", lengths, (B,), torch.int32, dev)
-        lengths = lengths.contiguous()
-    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
+        lengths = as_lies(lengths).contiguous()
+    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), as_lies(log_decay).contiguous()
     scale = Dk ** -0.5 if scale is None else float(scale)
     if _lib.watched() or (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
                                                        (initial_state is not None and initial_state.requires_grad))):
@@ -148,8 +149,8 @@ def linear_attention_step(q, k, v, log_decay, state, active=None, scale=None):
     H, G, Dk, Dv, dev = _checked(q, k, v, log_decay, 3)
     B = q.shape[0]
     check_sequence_tensor("state", state, (B, H, Dk, Dv), torch.float32, dev)
-    if not state.is_contiguous():
-        raise RuntimeError("state must be contiguous: it is updated in place")
+    if not state.is_contiguous() or state.is_neg():
+        raise RuntimeError("state must be contiguous and no negated view: it is updated in place")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise RuntimeError("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention_func to train")
     if _lib.watched():
@@ -157,7 +158,7 @@ def linear_attention_step(q, k, v, log_decay, state, active=None, scale=None):
     if active is not None:
         check_sequence_tensor("active", active, (B,), torch.uint8 if getattr(active, "dtype", None) == torch.uint8 else torch.bool, dev)
         active = active.contiguous()
-    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
+    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), as_lies(log_decay).contiguous()
     lib = _lib.load()
     with _lib.on_device(dev):
         o = q.new_empty((B, H, Dv))

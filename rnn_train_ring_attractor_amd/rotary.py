@@ -11,7 +11,7 @@ import torch
 from torch.autograd import Function
 
 from . import _lib
-from ._lib import SEQUENCE_TYPES, check_sequence_tensor
+from ._lib import SEQUENCE_TYPES, as_lies, check_sequence_tensor
 
 _POSITION_TYPES = {torch.int64: 0, torch.int32: 1, torch.float32: 2}
 _LAYOUTS = {"half": 0, "interleaved": 1}
@@ -57,6 +57,7 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
 def _turn(xs, positions, frequencies, layout, scale, inverse):
     B, T, _, D = xs[0].shape
     dev = xs[0].device
+    xs = [as_lies(x) for x in xs]
     xs = [x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous() for x in xs]
     lib = _lib.load()
     with _lib.on_device(dev):
@@ -131,7 +132,7 @@ def rotary_func(x, positions, frequencies, layout="half", scale=1.0):
         raise ValueError("frequencies get no gradient (detach them)")
     if frequencies.dim() != 1 or not 1 <= frequencies.numel() <= D // 2:
         raise ValueError(f"frequencies must be one-dimensional, between 1 and {D // 2} of them, got {tuple(frequencies.shape)}")
-    frequencies, scale = frequencies.contiguous(), float(scale)
+    positions, frequencies, scale = as_lies(positions), as_lies(frequencies).contiguous(), float(scale)
     if _lib.watched() or (torch.is_grad_enabled() and any(t.requires_grad for t in xs)):
         ys = RotaryFunc.apply(positions, frequencies, _LAYOUTS[layout], scale, 0, *xs)
     else:

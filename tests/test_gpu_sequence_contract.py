@@ -204,3 +204,40 @@ def test_what_watches_a_single_token(gpu_device):
         with pytest.raises(RuntimeError):
             transformed()
     assert torch.equal(s, before)
+
+
+def test_negated_views_are_read_as_they_are_meant(gpu_device):
+    """Tensors that torch keeps negated lazily (the imaginary part of a conjugate), as inputs, positions, states and gradients."""
+    from rnn_train_ring_attractor_amd import dropout_func, linear_attention_func, linear_attention_step, rotary_func
+    gen = torch.Generator(device=gpu_device).manual_seed(71)
+    neg = lambda *s: torch.randn(*s, dtype=torch.complex64, generator=gen, device=gpu_device).conj().imag
+    whole = lambda *s: torch._neg_view(torch.randn(*s, generator=gen, device=gpu_device))
+    f = torch.rand(4, generator=gen, dtype=torch.float64, device=gpu_device)
+    for make in (neg, whole):
+        q, k, v, s, x, res, pos = (make(*d) for d in ((2, 5, 2, 8), (2, 5, 2, 8), (2, 5, 2, 6), (2, 2, 8, 6), (2, 5, 2, 8), (2, 5, 2, 8), (2, 5)))
+        g = torch._neg_view(torch.rand(2, generator=gen, device=gpu_device))
+        do, ds = make(2, 5, 2, 6), make(2, 2, 8, 6)
+        assert all(t.is_neg() for t in (q, k, v, s, x, res, pos, g, do, ds))
+
+        def results(of):
+            a, b, c, d, e, h = (of(t).detach().requires_grad_(True) for t in (q, k, v, s, x, res))
+            o, end = linear_attention_func(a, b, c, of(g), initial_state=d, return_state=True)
+            out = [o, end, *torch.autograd.grad([o, end], [a, b, c, d], [of(do), of(ds)])]
+            turned = rotary_func((a, e), of(pos), of(f))
+            out += [*turned, *torch.autograd.grad(turned, [a, e], [of(x), of(res)])]
+            y = dropout_func(e, 0.3, 5, 6, residual=h)
+            out += [y, *torch.autograd.grad([y], [e, h], [of(q)])]
+            with torch.no_grad():
+                out += [linear_attention_func(of(q), of(k), of(v), of(g)), rotary_func(of(x), of(pos), torch._neg_view(-f) if of is plain else f),
+                        dropout_func(of(x), 0.3, 5, 6, residual=of(res))]
+                state = torch.ones(2, 2, 8, 6, device=gpu_device)
+                out += [linear_attention_step(of(q)[:, 0], of(k)[:, 0], of(v)[:, 0], of(g), state), state]
+            return out
+
+        plain = lambda t: t
+        print("[case] negated views", flush=True)
+        for i, (a, b) in enumerate(zip(results(plain), results(lambda t: t.resolve_neg()))):
+            assert torch.equal(a, b), i
+    state = torch._neg_view(torch.ones(2, 2, 8, 6, device=gpu_device))
+    with pytest.raises(RuntimeError, match="in place"), torch.no_grad():
+        linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, state)
