@@ -171,6 +171,12 @@ def profile_read():
 SEQUENCE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # RINGATTR_F32, _BF16, _F16
 
 
+def check_sequence_sizes(*sizes) -> None:
+    """Sizes go to the library in 32 bits with a sign, where larger ones would be others (a dimension that is expanded can be any size)."""
+    if max(sizes) >= 1 << 31:
+        raise ValueError(f"sizes must be below 2^31, got {max(sizes)}")
+
+
 def as_lies(t):
     """t, written out if torch keeps it negated lazily (the imaginary part of a conjugate): kernels read memory as it lies."""
     return t.resolve_neg() if t is not None and t.is_neg() else t

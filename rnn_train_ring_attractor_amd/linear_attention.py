@@ -17,7 +17,7 @@ import torch
 from torch.autograd import Function
 
 from . import _lib
-from ._lib import SEQUENCE_TYPES, as_lies, check_sequence_tensor
+from ._lib import SEQUENCE_TYPES, as_lies, check_sequence_sizes, check_sequence_tensor
 
 _Strides9, _Strides12, _Strides6 = ctypes.c_longlong * 9, ctypes.c_longlong * 12, ctypes.c_longlong * 6
 
@@ -43,6 +43,7 @@ def _checked(q, k, v, log_decay, dims):
     Dv = v.shape[-1]
     if H == 0 or G == 0 or Dk == 0 or Dv == 0 or H % G != 0:
         raise ValueError(f"heads ({H}) must be a positive multiple of kv_heads ({G}), dk and dv positive ({Dk}, {Dv})")
+    check_sequence_sizes(*q.shape, Dv)
     check_sequence_tensor("log_decay", log_decay, (H,), torch.float32, dev)
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError("log_decay is a setting, as the time loop's alpha: it gets no gradient (detach it)")

@@ -11,7 +11,7 @@ import torch
 from torch.autograd import Function
 
 from . import _lib
-from ._lib import SEQUENCE_TYPES, as_lies, check_sequence_tensor
+from ._lib import SEQUENCE_TYPES, as_lies, check_sequence_sizes, check_sequence_tensor
 
 _POSITION_TYPES = {torch.int64: 0, torch.int32: 1, torch.float32: 2}
 _LAYOUTS = {"half": 0, "interleaved": 1}
@@ -119,6 +119,7 @@ def rotary_func(x, positions, frequencies, layout="half", scale=1.0):
             raise ValueError(f"x must be two tensors of [B, T, heads, D], got {tuple(xs[0].shape)} and {tuple(xs[1].shape)}")
     if any(t.shape[2] == 0 for t in xs):
         raise ValueError("x must have at least one head")
+    check_sequence_sizes(*(n for t in xs for n in t.shape))
     if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITION_TYPES:
         raise TypeError("positions must be an int64, int32 or float32 tensor")
     if tuple(positions.shape) not in ((T,), (B, T)):

@@ -241,3 +241,18 @@ def test_negated_views_are_read_as_they_are_meant(gpu_device):
     state = torch._neg_view(torch.ones(2, 2, 8, 6, device=gpu_device))
     with pytest.raises(RuntimeError, match="in place"), torch.no_grad():
         linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g, state)
+
+
+def test_sizes_past_31_bits_are_refused(gpu_device):
+    from rnn_train_ring_attractor_amd import linear_attention_func, linear_attention_step, rotary_func
+    n = (1 << 32) + 2
+    one = lambda *s: torch.zeros(1, device=gpu_device, dtype=torch.bfloat16).expand(*s)
+    g = torch.zeros(1, device=gpu_device)
+    print("[case] sizes past 31 bits", flush=True)
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="2\\^31"):
+            rotary_func(one(1, n, 1, 2), torch.zeros(1, device=gpu_device).expand(n), torch.ones(1, device=gpu_device, dtype=torch.float64))
+        with pytest.raises(ValueError, match="2\\^31"):
+            linear_attention_func(one(1, n, 1, 1), one(1, n, 1, 1), one(1, n, 1, 1), g)
+        with pytest.raises(ValueError, match="2\\^31"):
+            linear_attention_step(one(n, 1, 1), one(n, 1, 1), one(n, 1, 1), g, torch.zeros(1, device=gpu_device).expand(n, 1, 1, 1))
