@@ -299,7 +299,8 @@ RINGATTR_API int ringattr_linear_attention_fwd(const void* q, const void* k, con
                       const void* log_decay, const void* initial_state, const void* lengths, void* o, void* final_state,
                       float scale, int type, int batch_size, int seq_len, int heads, int kv_heads, int dk, int dv,
                       void* workspace, size_t workspace_bytes, void* stream);
-/* Gradients of q, k, v and (NULL: not wanted) of the initial state, from those of o and (NULL: zero) of the final state.
+/* Gradients of q, k, v and the initial state (each NULL: not wanted, and its pass left out; the initial state's takes grad_v along), from
+ * those of o and (NULL: zero) of the final state.
  * The gradients of shared heads are summed in fp32 in a fixed order.  states: the workspace that a forward of the same
  * arguments left (its states along the sequences; a caller that keeps it spares the backward a pass), or NULL: they are
  * formed again. */

@@ -284,11 +284,11 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
   float *part_k = (float*)w, *part_v = (float*)(w + round_up((size_t)s.B * s.T * s.H * s.Dk * sizeof(float)));
   hipError_t e;
   auto launch_shares = [&]() {
-    hipError_t f = launch_share(s.type, part_k, gk, share, s.Dk, (size_t)s.B * s.T * s.G * s.Dk, st);
-    return f != hipSuccess ? f : launch_share(s.type, part_v, gv, share, s.Dv, (size_t)s.B * s.T * s.G * s.Dv, st);
+    hipError_t f = gk ? launch_share(s.type, part_k, gk, share, s.Dk, (size_t)s.B * s.T * s.G * s.Dk, st) : hipSuccess;
+    return f != hipSuccess || !gv ? f : launch_share(s.type, part_v, gv, share, s.Dv, (size_t)s.B * s.T * s.G * s.Dv, st);
   };
   // dv and dk read the same rows and go backwards together where one kernel does both
-  const bool together = s.Dk <= 128 && s.Dv <= 128 && (s.Dk <= 64) == (s.Dv <= 64);
+  const bool together = gk && gv && s.Dk <= 128 && s.Dv <= 128 && (s.Dk <= 64) == (s.Dv <= 64);
   RingLinArgs f = base(s, log_decay, lengths, nseg), r = f;
   f.s_in = s_in;
   f.seg = seg_f;
@@ -302,25 +302,28 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
   r.ys = r.zs = 1;
   r.update = s.scale;
   r.s_out = gs_in;
-  if (!states) {
-    e = segment_states(s, f, false, st);
+  if (gq) {
+    if (!states) {
+      e = segment_states(s, f, false, st);
+      if (e != hipSuccess) return e;
+    }
+    // dq: do against v weighs k, the state transposed
+    f.X = go;
+    f.xs = 1;
+    f.Y = v;
+    f.Z = k;
+    f.Da = s.Dv;
+    f.sa = 1;
+    f.sb = s.Dv;
+    set_columns(f, s.Dk, false);
+    f.out = gq;
+    f.out_vec = f.Db % epv == 0 && out_fits(f);
+    f.intra = f.inter = s.scale;
+    e = launch_pass(s.type, f, false, false, st);
     if (e != hipSuccess) return e;
   }
+  if (!gk && !gv) return hipSuccess;
   e = segment_states(s, r, true, st);
-  if (e != hipSuccess) return e;
-  // dq: do against v weighs k, the state transposed
-  f.X = go;
-  f.xs = 1;
-  f.Y = v;
-  f.Z = k;
-  f.Da = s.Dv;
-  f.sa = 1;
-  f.sb = s.Dv;
-  set_columns(f, s.Dk, false);
-  f.out = gq;
-  f.out_vec = f.Db % epv == 0 && out_fits(f);
-  f.intra = f.inter = s.scale;
-  e = launch_pass(s.type, f, false, false, st);
   if (e != hipSuccess) return e;
   // dv: k against q weighs do
   r.X = k;
@@ -342,9 +345,12 @@ hipError_t ring_linattn_bwd(const RingLinShape& s, const RingLinTensor& q, const
     if (e != hipSuccess || share == 1) return e;
     return launch_shares();
   }
-  e = launch_pass(s.type, r, true, false, st);
-  if (e != hipSuccess) return e;
+  if (gv) {
+    e = launch_pass(s.type, r, true, false, st);
+    if (e != hipSuccess) return e;
+  }
   // dk: v against do weighs q, the state transposed
+  if (!gk) return share > 1 ? launch_shares() : hipSuccess;
   r.X = v;
   r.Y = go;
   r.Z = q;

@@ -998,8 +998,8 @@ int ringattr_linear_attention_bwd(const void* q, const void* k, const void* v, c
   const char* who = "ringattr_linear_attention_bwd";
   RingLinShape s;
   if (!linattn_shape(who, type, batch_size, seq_len, heads, kv_heads, dk, dv, s)) return RINGATTR_ERR_INVALID;
-  if (!q || !k || !v || !grad_o || !strides || !log_decay || !grad_q || !grad_k || !grad_v)
-    return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  if (!q || !k || !v || !grad_o || !strides || !log_decay) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  if (grad_initial_state && !grad_v) return fail(RINGATTR_ERR_INVALID, "%s: grad_initial_state is found together with grad_v (null)", who);
   if (!aligned16(grad_q) || !aligned16(grad_k) || !aligned16(grad_v) || !aligned16(grad_initial_state) || !aligned16(states) || !aligned16(workspace))
     return fail(RINGATTR_ERR_INVALID, "%s: outputs and workspace must be 16-byte aligned", who);
   const size_t need = ring_linattn_bwd_bytes(s, states != nullptr);

@@ -92,8 +92,10 @@ class LinearAttentionFunc(Function):
         G, Dv, dev = k.shape[2], v.shape[3], q.device
         lib, kind = _lib.load(), SEQUENCE_TYPES[q.dtype]
         with _lib.on_device(dev):
-            gq, gk, gv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
             want = initial_state is not None and ctx.needs_input_grad[4]
+            # (what is frozen costs no pass; the initial state's gradient is found along with v's)
+            gq, gk, gv = (x.new_empty(x.shape) if needed else None
+                          for x, needed in zip((q, k, v), (*ctx.needs_input_grad[:2], ctx.needs_input_grad[2] or want)))
             g0 = log_decay.new_empty((B, H, Dk, Dv)) if want else None
             gs = None if grad_state is None else as_lies(grad_state).contiguous()
             if B == 0 or T == 0:
@@ -106,9 +108,9 @@ class LinearAttentionFunc(Function):
                 strides = _Strides12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *go.stride()[:3])
                 _lib.check(lib.ringattr_linear_attention_bwd(
                     q.data_ptr(), k.data_ptr(), v.data_ptr(), go.data_ptr(), strides, log_decay.data_ptr(), _ptr(initial_state),
-                    _ptr(lengths), _ptr(along), _ptr(gs), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _ptr(g0), ctx.scale, kind, B, T, H, G, Dk, Dv,
+                    _ptr(lengths), _ptr(along), _ptr(gs), _ptr(gq), _ptr(gk), _ptr(gv), _ptr(g0), ctx.scale, kind, B, T, H, G, Dk, Dv,
                     _ptr(ws), nbytes, _lib.stream_handle(dev)))
-        return gq, gk, gv, None, g0, None, None, None
+        return gq, gk, gv if ctx.needs_input_grad[2] else None, None, g0, None, None, None
 
 
 def linear_attention_func(q, k, v, log_decay, initial_state=None, lengths=None, scale=None, return_state=False):

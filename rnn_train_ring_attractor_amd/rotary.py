@@ -92,7 +92,9 @@ class RotaryFunc(Function):
         layout, scale, inverse = ctx.how
         # turned back: the transpose of a turn is the opposite turn, so a gradient of the gradient is this operator again
         back = RotaryFunc.apply if torch.is_grad_enabled() else _turned
-        return (None,) * 5 + back(positions, frequencies, layout, scale, 1 - inverse, *grads)
+        needed = ctx.needs_input_grad[5:]
+        turned = iter(back(positions, frequencies, layout, scale, 1 - inverse, *(g for g, n in zip(grads, needed) if n)))
+        return (None,) * 5 + tuple(next(turned) if n else None for n in needed)
 
 
 def rotary_func(x, positions, frequencies, layout="half", scale=1.0):

@@ -256,3 +256,73 @@ def test_sizes_past_31_bits_are_refused(gpu_device):
             linear_attention_func(one(1, n, 1, 1), one(1, n, 1, 1), one(1, n, 1, 1), g)
         with pytest.raises(ValueError, match="2\\^31"):
             linear_attention_step(one(n, 1, 1), one(n, 1, 1), one(n, 1, 1), g, torch.zeros(1, device=gpu_device).expand(n, 1, 1, 1))
+
+
+class _Spy:
+    """The library, with a note of every call of a backward and of rotary positions."""
+
+    def __init__(self, lib, calls):
+        self.lib, self.calls = lib, calls
+
+    def __getattr__(self, name):
+        fn = getattr(self.lib, name)
+
+        def call(*args):
+            if name in ("ringattr_linear_attention_bwd", "ringattr_rotary"):
+                self.calls.append(args)
+            return fn(*args)
+
+        return call
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("sizes", [(2, 90, 4, 2, 32, 48), (2, 70, 2, 2, 40, 72), (4, 500, 2, 1, 70, 66), (4, 500, 2, 2, 20, 70), (3, 70, 2, 1, 136, 140)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_gradients_that_nobody_asks_for(sizes, kind, gpu_device, monkeypatch):
+    """What is frozen gets no gradient and costs no pass; the others are what they are all together."""
+    from rnn_train_ring_attractor_amd import _lib, linear_attention_func
+    print(f"[case] frozen {sizes} {kind}", flush=True)
+    dtype = TYPES[kind]
+    p = _problem(73, *sizes, dtype, start=True)
+    t = {n: p[n].to(torch.float32 if n in ("s0", "ds", "g") else dtype).to(gpu_device) for n in ("q", "k", "v", "s0", "do", "ds", "g")}
+    calls = []
+    spy = _Spy(_lib.load(), calls)
+    monkeypatch.setattr(_lib, "load", lambda: spy)
+    names = ("q", "k", "v", "s0")
+    for with_state in (True, False):
+        full = None
+        for mask in (15, *range(1, 15)):
+            leaves = {n: t[n].detach().requires_grad_(bool(mask >> i & 1)) for i, n in enumerate(names)}
+            o, s = linear_attention_func(leaves["q"], leaves["k"], leaves["v"], t["g"], initial_state=leaves["s0"], return_state=True)
+            wanted = [n for n in names if leaves[n].requires_grad]
+            outs, given = ([o, s], [t["do"], t["ds"]]) if with_state else ([o], [t["do"]])
+            if not any(x.requires_grad for x in outs):
+                continue
+            calls.clear()
+            got = dict(zip(wanted, torch.autograd.grad(outs, [leaves[n] for n in wanted], given, allow_unused=True)))
+            args, = calls
+            asked = [n for n, x in zip(names, args[10:14]) if x is not None]
+            assert asked == [n for n in names if n in wanted or (n == "v" and "s0" in wanted)], mask
+            full = got if mask == 15 else full
+            for n in wanted:
+                # (bf16: a state that is a result as well is exact to 2^-24 in place of 2^-16, which a gradient can show as its last bit)
+                a, b = got[n].double(), full[n].double()
+                assert torch.equal(a, b) if kind != "bf16" or n == "q" else ((a - b).norm() <= 2.0 ** -8 * b.norm()), (mask, n)
+
+
+def test_turned_tensors_that_nobody_asks_a_gradient_of(gpu_device, monkeypatch):
+    from rnn_train_ring_attractor_amd import _lib, rotary_func
+    q, k = torch.randn(2, 5, 3, 8, device=gpu_device), torch.randn(2, 5, 1, 8, device=gpu_device)
+    pos, f = torch.arange(5, device=gpu_device), torch.rand(4, dtype=torch.float64, device=gpu_device)
+    calls = []
+    spy = _Spy(_lib.load(), calls)
+    a, b = q.clone().requires_grad_(True), k.clone().requires_grad_(True)
+    both = torch.autograd.grad(rotary_func((a, b), pos, f), [a, b], [q, k])
+    monkeypatch.setattr(_lib, "load", lambda: spy)
+    for i, pair in enumerate(((a, k), (q, b))):
+        out = rotary_func(pair, pos, f)
+        calls.clear()
+        got, = torch.autograd.grad([out[i]], [pair[i]], [(q, k)[i]])
+        assert torch.equal(got, both[i])
+        args, = calls
+        assert args[1] is None and args[9] is None           # one tensor
