@@ -326,3 +326,43 @@ def test_turned_tensors_that_nobody_asks_a_gradient_of(gpu_device, monkeypatch):
         assert torch.equal(got, both[i])
         args, = calls
         assert args[1] is None and args[9] is None           # one tensor
+
+
+@pytest.mark.parametrize("kind,sizes,count", [(k, s, n) for k, s, n in SEGMENTED if s[0] <= 4 and k != "fp16"],
+                         ids=["-".join([k] + [str(x) for x in s]) for k, s, n in SEGMENTED if s[0] <= 4 and k != "fp16"])
+def test_a_backward_that_forms_the_states_again(kind, sizes, count, gpu_device):
+    """The C ABI's backward without the forward's states against the definition, and next to one that is given them."""
+    import ctypes
+    from rnn_train_ring_attractor_amd import _lib
+    B, T, H, G, Dk, Dv = sizes
+    dtype, lib = TYPES[kind], _lib.load()
+    code = _lib.SEQUENCE_TYPES[dtype]
+    print(f"[case] states again {kind} {sizes}", flush=True)
+    p = _without_state_gradient(_problem(79, *sizes, dtype, start=True))
+    lengths = _lengths(T, B, count)
+    t = {n: p[n].to(torch.float32 if n in ("g", "s0") else dtype).to(gpu_device) for n in ("q", "k", "v", "do", "g", "s0")}
+    lens = torch.tensor(lengths, dtype=torch.int32, device=gpu_device)
+    room = lambda n: torch.full((n // 4,), math.nan, device=gpu_device)
+    need = lib.ringattr_linear_attention_fwd_workspace_bytes(code, *sizes)
+    assert need > 0
+    ws, o = room(need), torch.empty(B, T, H, Dv, dtype=dtype, device=gpu_device)
+    strides = lambda names: (ctypes.c_longlong * (3 * len(names)))(*(s for n in names for s in t[n].stride()[:3]))
+    scale, stream = Dk ** -0.5, _lib.stream_handle(torch.device("cuda", 0))
+    _lib.check(lib.ringattr_linear_attention_fwd(t["q"].data_ptr(), t["k"].data_ptr(), t["v"].data_ptr(), strides("qkv"), t["g"].data_ptr(),
+                                                 t["s0"].data_ptr(), lens.data_ptr(), o.data_ptr(), None, scale, code, *sizes, ws.data_ptr(), need, stream))
+    results = []
+    for states in (None, ws):
+        nbytes = lib.ringattr_linear_attention_bwd_workspace_bytes(code, *sizes, states is not None)
+        own, out = room(nbytes), {n: torch.full_like(t[n], math.nan) for n in "qkv"}
+        _lib.check(lib.ringattr_linear_attention_bwd(
+            t["q"].data_ptr(), t["k"].data_ptr(), t["v"].data_ptr(), t["do"].data_ptr(), strides(["q", "k", "v", "do"]), t["g"].data_ptr(),
+            t["s0"].data_ptr(), lens.data_ptr(), None if states is None else states.data_ptr(), None, *(out[n].data_ptr() for n in "qkv"), None, scale,
+            code, *sizes, own.data_ptr(), nbytes, stream))
+        results.append(out)
+    want, size = _reference(p, lengths), _reference(p, lengths, magnitudes=True)
+    for n in "qkv":
+        assert torch.equal(results[0][n], results[1][n])
+        err = (results[0][n].double().cpu() - want["d" + n]).abs()
+        K = T + Dk + Dv + H // G + 256
+        bound = _bf16_bound(want["d" + n], size["d" + n], K) if kind == "bf16" else 2.0 ** -24 * (want["d" + n].abs() + K * 1.01 * size["d" + n]) + 1e-37
+        assert (err <= bound).all(), n
