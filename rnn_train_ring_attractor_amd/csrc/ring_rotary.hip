@@ -8,8 +8,8 @@
 //
 // Bound by memory: everything is read once and written once: 8 x 4096 tokens, 16 + 4 heads of 128, bf16: 336 MB in 67 us, 5.0 TB/s (a
 // large copy: 5.2).  A workgroup takes a few tokens through all heads of both tensors, so a
-// token's angles are found once: the number of turns as a product in 64 bits, whose whole part is taken off before it is rounded (at
-// position 2^20 a product in 32 bits is off by 0.06 rad), then one sine and cosine in 32.
+// token's angles are found once: the number of turns without its whole part, exact to 2^-40 for every 64-bit position (at position 2^20 a product
+// in 32 bits is off by 0.06 rad, at 2^40 one in 64 bits by 2e-4), then one sine and cosine in 32.
 #include "ring_common.hpp"
 #include "ring_kernels.hpp"
 #include "ringattr.h"
@@ -36,10 +36,22 @@ struct Divisor {
 };
 struct Divisors { Divisor units, heads, pairs, T, last_heads; };
 
-__device__ __forceinline__ double position_of(const RingRotaryArgs& p, long at) {
-  if (p.position_type == RINGATTR_POS_F32) return (double)((const float*)p.positions)[at];
-  if (p.position_type == RINGATTR_POS_I32) return (double)((const int*)p.positions)[at];
-  return (double)((const long long*)p.positions)[at];
+// A position as the sum of two numbers in 64 bits, both exact
+struct Position { double high, low; };
+__device__ __forceinline__ Position position_of(const RingRotaryArgs& p, long at) {
+  if (p.position_type == RINGATTR_POS_F32) return {0.0, (double)((const float*)p.positions)[at]};
+  if (p.position_type == RINGATTR_POS_I32) return {0.0, (double)((const int*)p.positions)[at]};
+  const long long x = ((const long long*)p.positions)[at];
+  return {(double)(int)(x >> 32) * 4294967296.0, (double)(unsigned)x};
+}
+
+// position * frequency / (2 pi) less whole turns.  frequency / (2 pi) = f + g with 106 bits; of the products with f whole turns are taken off
+// inside the fma, ahead of its rounding.
+__device__ __forceinline__ float turns(Position x, double frequency) {
+  constexpr double R = 0.15915494309189535, S = -9.839338337591243e-18;          // 1 / (2 pi) = R + S
+  const double f = frequency * R, g = fma(frequency, R, -f) + frequency * S;
+  const double t = fma(x.high, f, -rint(x.high * f)) + fma(x.low, f, -rint(x.low * f)) + fma(x.high, g, x.low * g);
+  return (float)(t - rint(t));
 }
 
 }  // namespace
@@ -75,11 +87,8 @@ __global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p, Divi
     const int tok = by.pairs.div(i), m = i - tok * r;
     const unsigned more = by.T.div(t0 + tok);
     const long b = b0 + more, t = t0 + tok - more * (unsigned)p.T;
-    const double pos = position_of(p, b * p.pos_b + t * p.pos_t), f = p.frequencies[m] * 0.15915494309189535;      // turns
-    const double turns = rint(pos * f);
-    const float x = 2.f * (float)fma(pos, f, -turns);
     float s, c;
-    sincospif(x, &s, &c);
+    sincospif(2.f * turns(position_of(p, b * p.pos_b + t * p.pos_t), p.frequencies[m]), &s, &c);
     trig[i] = f32x2{p.scale * c, p.inverse ? -p.scale * s : p.scale * s};
   }
   __syncthreads();

@@ -102,8 +102,8 @@ def rotary_func(x, positions, frequencies, layout="half", scale=1.0):
     2 * len(frequencies) values of each head, (m, m + len(frequencies)) in layout "half" or (2m, 2m + 1) in layout "interleaved", by the
     angle position * frequencies[m] and multiplied by `scale`; the rest of a head is copied.
 
-    positions [T] or [B,T], int64, int32 or float32 (an angle); frequencies float64 (`rotary_frequencies`).  The angle is formed in 64
-    bits.  Differentiable with respect to x.  Returns a tensor, or a tuple where x is a pair."""
+    positions [T] or [B,T], int64, int32 or float32 (an angle); frequencies float64 (`rotary_frequencies`).  The angle, less whole turns, is
+    that of the exact product for every int64 position (of frequencies up to 1000: to 2^-24 turns).  Differentiable with respect to x.  Returns a tensor, or a tuple where x is a pair."""
     pair = isinstance(x, (tuple, list))
     xs = tuple(x) if pair else (x,)
     if len(xs) not in (1, 2):

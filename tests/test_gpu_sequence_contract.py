@@ -366,3 +366,34 @@ def test_a_backward_that_forms_the_states_again(kind, sizes, count, gpu_device):
         K = T + Dk + Dv + H // G + 256
         bound = _bf16_bound(want["d" + n], size["d" + n], K) if kind == "bf16" else 2.0 ** -24 * (want["d" + n].abs() + K * 1.01 * size["d" + n]) + 1e-37
         assert (err <= bound).all(), n
+
+
+def _turned_exactly(x, positions, frequencies):
+    """x [B,T,H,D] turned in halves by the exact product of positions and frequencies, 1 / (2 pi) to 60 digits."""
+    from fractions import Fraction
+    pi = Fraction("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899")
+    out, r = x.clone(), len(frequencies)
+    for m, f in enumerate(frequencies.tolist()):
+        turns = [Fraction(p) * Fraction(f) / (2 * pi) for p in positions.tolist()]
+        angle = 2 * math.pi * torch.tensor([float(t - round(t)) for t in turns], dtype=torch.float64)[None, :, None]
+        a, b = x[..., m], x[..., m + r]
+        out[..., m], out[..., m + r] = a * torch.cos(angle) - b * torch.sin(angle), b * torch.cos(angle) + a * torch.sin(angle)
+    return out
+
+
+def test_positions_however_far(gpu_device):
+    """Bound: an angle known to 2^-24 turns, cosine and sine in fp32, two products and a sum: (2 pi + 4) 2^-24 of |a| + |b|, then half a step."""
+    from rnn_train_ring_attractor_amd import rotary_func
+    print("[case] far positions", flush=True)
+    far = torch.tensor([0, 3, -(1 << 31), (1 << 40) + 1, 987654321987654321, (1 << 53) + 1, (1 << 62) + 12345, (1 << 63) - 1, -(1 << 63), -(1 << 40) - 77])
+    angles = torch.tensor([0.0, 1e7, -3.3e6, 16777215.0, 1e-3, 12345.678, -7.5, 1e9, 3e4, -1e-20], dtype=torch.float32)
+    gen = torch.Generator().manual_seed(83)
+    for positions, f in ((far, 10000.0 ** (-torch.arange(8, dtype=torch.float64) / 8)), (far, 1000 * torch.rand(8, generator=gen, dtype=torch.float64)),
+                         (far.clamp(-(1 << 31), (1 << 31) - 1).int(), torch.rand(8, generator=gen, dtype=torch.float64)),
+                         (angles, torch.arange(1, 9, dtype=torch.float64) * 125)):
+        x = torch.randn(1, 10, 2, 16, generator=gen, dtype=torch.float64).float()
+        got = rotary_func(x.to(gpu_device), positions.to(gpu_device), f.to(gpu_device)).double().cpu()
+        want = _turned_exactly(x.double(), positions, f)
+        size = (x[..., :8].abs() + x[..., 8:].abs()).repeat(1, 1, 1, 2).double()
+        err = (got - want).abs()
+        assert (err <= 2.0 ** -24 * 1.0001 * want.abs() + (2 * math.pi + 4) * 2.0 ** -24 * size).all(), (positions.dtype, float((err / size).max()))
