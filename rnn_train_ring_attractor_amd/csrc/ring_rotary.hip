@@ -17,9 +17,6 @@
 namespace {
 
 constexpr int kAngles = 1024;      // (cos, sin) that a workgroup keeps
-// Bytes that a call reads and writes from which on it leaves nothing in the last cache (256 MB) that a reader behind it would find
-constexpr size_t kPastCache = 320000000;
-
 constexpr int kTokens = 256;       // tokens that a workgroup takes at most
 
 // n / d for n < 2^31 by a product and a shift: with 2^(s - 1) < d <= 2^s, floor(n (2^32 + m) / 2^(32 + s)) for m = floor(2^32 (2^s - d) / d) + 1
@@ -57,19 +54,12 @@ __device__ __forceinline__ float turns(Position x, double frequency) {
 }  // namespace
 
 // V values at a time, neighbours in memory: 16 bytes, two values, or one (any strides and widths); what is copied C at a time.
-// PAST: results are stored past the caches, where the call passes them anyway and its inputs would be pushed out (kPastCache), in rows of
-// whole lines (16 + 4 heads of 128, bf16, halves, us with and without: 336 MB with inputs just written 55, 68, inputs from memory 68.4, 69.6, and a call that reads the results 135, 142; smaller,
-// 252 MB: that 106, 97; rows of 128 bytes, 302 MB: 64.4, 63.1 and 130, 125).  Dropout gains nothing by it (403 and 268 MB there and back:
-// 124, 120).
-template <typename T, int V, int C, bool HALF, bool PAST>
+// (Results stored past the caches: 68.4 us in place of 69.6 for 336 MB from memory, 106 in place of 97 for 252 MB with a reader behind it: not done.)
+template <typename T, int V, int C, bool HALF>
 __global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p, Divisors by) {
   constexpr int P = HALF ? V : (V + 1) / 2;                    // pairs of a unit
   typedef T vec __attribute__((ext_vector_type(V)));
   typedef T copied __attribute__((ext_vector_type(C)));
-  auto store = [](T* at, auto x) {
-    if constexpr (PAST) __builtin_nontemporal_store(x, (decltype(x)*)at);
-    else *(decltype(x)*)at = x;
-  };
   __shared__ f32x2 trig[kAngles];
   __shared__ long base[2][kTokens];
   const int tid = threadIdx.x, r = p.rot / 2, D = p.D;
@@ -106,7 +96,7 @@ __global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p, Divi
     const f32x2* cs = trig + tok * r + u * P;
     if (u >= turned) {
       const int d = p.rot + (u - turned) * C;
-      store(y + d, *(const copied*)(x + d));
+      *(copied*)(y + d) = *(const copied*)(x + d);
     } else if constexpr (HALF) {
       const int d = u * V;
       const vec a = *(const vec*)(x + d), c = *(const vec*)(x + d + r);
@@ -117,8 +107,8 @@ __global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p, Divi
         ya[e] = (T)((float)a[e] * w[0] - (float)c[e] * w[1]);
         yc[e] = (T)((float)c[e] * w[0] + (float)a[e] * w[1]);
       }
-      store(y + d, ya);
-      store(y + d + r, yc);
+      *(vec*)(y + d) = ya;
+      *(vec*)(y + d + r) = yc;
     } else {
       const int d = u * 2 * P;
       T a[2 * P];
@@ -136,7 +126,7 @@ __global__ __launch_bounds__(256) void ring_rotary_kernel(RingRotaryArgs p, Divi
         a[2 * e + 1] = (T)(f1 * w[0] + f0 * w[1]);
       }
       if constexpr (V > 1) {
-        store(y + d, *(const vec*)a);
+        *(vec*)(y + d) = *(const vec*)a;
       } else {
         y[d] = a[0];
         y[d + 1] = a[1];
@@ -159,18 +149,18 @@ template <typename T> static int values_at_once(const RingRotaryArgs& p, int pai
   return 1;
 }
 
-template <typename T, int V, int C, bool PAST> static void launch_kernel(const RingRotaryArgs& p, dim3 grid, hipStream_t st) {
+template <typename T, int V, int C> static void launch_kernel(const RingRotaryArgs& p, dim3 grid, hipStream_t st) {
   const int r = p.rot / 2, pairs = p.interleaved ? (V + 1) / 2 : V;
   // (the last heads of a grid row are fewer: their workgroups divide by their own number)
   const int heads = p.heads[0] + p.heads[1], units = r / pairs + (p.D - p.rot) / C, last = heads - ((int)grid.y - 1) * p.heads_per;
   const Divisors by = {Divisor::of(units), Divisor::of(p.heads_per), Divisor::of(r), Divisor::of(p.T), Divisor::of(last)};
   if constexpr (V == C) {                                      // (neighbours: where two values fit, a pair does)
     if (p.interleaved) {
-      hipLaunchKernelGGL((ring_rotary_kernel<T, V, C, false, PAST>), grid, dim3(256), 0, st, p, by);
+      hipLaunchKernelGGL((ring_rotary_kernel<T, V, C, false>), grid, dim3(256), 0, st, p, by);
       return;
     }
   }
-  hipLaunchKernelGGL((ring_rotary_kernel<T, V, C, true, PAST>), grid, dim3(256), 0, st, p, by);
+  hipLaunchKernelGGL((ring_rotary_kernel<T, V, C, true>), grid, dim3(256), 0, st, p, by);
 }
 
 template <typename T> static hipError_t launch(RingRotaryArgs p, hipStream_t st) {
@@ -188,13 +178,10 @@ template <typename T> static hipError_t launch(RingRotaryArgs p, hipStream_t st)
   p.heads_per = (heads + split - 1) / split;
   const long row = blocks < (1 << 20) ? blocks : 1 << 20;      // (a launch counts fewer than 2^32 threads along x)
   const dim3 grid((unsigned)row, (unsigned)((heads + p.heads_per - 1) / p.heads_per), (unsigned)((blocks + row - 1) / row));
-  const size_t row_bytes = p.D * sizeof(T);
-  const bool past = row_bytes >= 256 && 2 * row_bytes * heads * (size_t)all >= kPastCache;
-  if (v == W && past) launch_kernel<T, W, W, true>(p, grid, st);
-  else if (v == W) launch_kernel<T, W, W, false>(p, grid, st);
-  else if (v == 2) launch_kernel<T, 2, 2, false>(p, grid, st);
-  else if (c == 2) launch_kernel<T, 1, 2, false>(p, grid, st);
-  else launch_kernel<T, 1, 1, false>(p, grid, st);
+  if (v == W) launch_kernel<T, W, W>(p, grid, st);
+  else if (v == 2) launch_kernel<T, 2, 2>(p, grid, st);
+  else if (c == 2) launch_kernel<T, 1, 2>(p, grid, st);
+  else launch_kernel<T, 1, 1>(p, grid, st);
   return hipGetLastError();
 }
 
