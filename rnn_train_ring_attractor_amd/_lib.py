@@ -168,16 +168,19 @@ def profile_read():
     return {KERNEL_NAMES[i]: (ms[i], cnt[i]) for i in range(n)}
 
 
+_C, _forward_ad = torch._C, torch.autograd.forward_ad
+_SIZE_LIMIT = 1 << 31
 SEQUENCE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # RINGATTR_F32, _BF16, _F16
 
 
-def check_sequence_sizes(*sizes) -> None:
+def check_sequence_sizes(*tensors) -> None:
     """Sizes go to the library in 32 bits with a sign, where larger ones would be others (a dimension that is expanded can be any size)."""
-    if max(sizes) >= 1 << 31:
-        raise ValueError(f"sizes must be below 2^31, got {max(sizes)}")
+    for t in tensors:
+        if t.numel() >= _SIZE_LIMIT and max(t.shape) >= _SIZE_LIMIT:
+            raise ValueError(f"sizes must be below 2^31, got {tuple(t.shape)}")
 
 
-def as_lies(t):
+def resolved(t):
     """t, written out if torch keeps it negated lazily (the imaginary part of a conjugate): kernels read memory as it lies."""
     return t.resolve_neg() if t is not None and t.is_neg() else t
 
@@ -233,26 +236,9 @@ def plain_gpu_tensor(t) -> bool:
     tracing, compilation, a dispatch or function mode) to miss them."""
     if type(t) is not torch.Tensor or not t.is_cuda or t.dtype != torch.float32 or t.layout != torch.strided:
         return False
-    if t.requires_grad and torch.is_grad_enabled():
+    if (t.requires_grad and torch.is_grad_enabled()) or torch.compiler.is_compiling() or torch.jit.is_tracing():
         return False
-    return not watched() and not t.is_neg() and t.numel() > 0
-
-
-def watched() -> bool:
-    """Whether something beside autograd's backward may follow or transform the operations.  An operator is called as an autograd Function
-    then, which is refused where it lacks a rule (forward mode, functorch) and recorded (tracing, compilation)."""
-    return torch.compiler.is_compiling() or torch.jit.is_tracing() or _watched()
-
-
-def refuse_derivatives(who, *tensors) -> None:
-    """For an operator without any derivative, which is no Function: forward mode, function transforms and tracing of these tensors."""
-    if torch.compiler.is_compiling():        # (a compiler leaves the call to Python, where the question comes again)
-        return
-    if torch.jit.is_tracing():
-        raise RuntimeError(f"{who} cannot be traced")
-    for t in tensors:
-        if torch._C._functorch.is_functorch_wrapped_tensor(t) or torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
-            raise RuntimeError(f"{who} has no gradient, in forward mode and function transforms neither")
+    return not _watched() and not t.is_neg() and t.numel() > 0
 
 
 def _watched() -> bool:
@@ -263,3 +249,23 @@ def _watched() -> bool:
                 or torch._C._len_torch_dispatch_stack() != 0 or torch._C._len_torch_function_stack() != 0)
     except AttributeError:
         return True
+
+
+def followed() -> bool:
+    """Whether something beside autograd's backward follows the operations on tensors (tracing, functorch, forward mode; `_watched`'s private
+    names).  An operator is called as an autograd Function then, which is recorded, or refused where it lacks a rule."""
+    try:
+        return _C._is_tracing() or _C._functorch.maybe_current_level() is not None or _forward_ad._current_level >= 0
+    except AttributeError:
+        return True
+
+
+def refuse_followed(who, *tensors) -> None:
+    """The same for an operator without any derivative, which is no Function: it raises."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{who} cannot be traced")
+    # (a private name: without it a wrapped tensor is refused where its memory is asked for)
+    wrapped = getattr(getattr(torch._C, "_functorch", None), "is_functorch_wrapped_tensor", lambda t: False)
+    for t in tensors:
+        if wrapped(t) or torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{who} has no gradient, in forward mode and function transforms neither")

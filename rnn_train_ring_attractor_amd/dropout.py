@@ -5,12 +5,12 @@ import torch
 from torch.autograd import Function
 
 from . import _lib
-from ._lib import SEQUENCE_TYPES, as_lies, check_sequence_tensor
+from ._lib import SEQUENCE_TYPES, check_sequence_tensor, resolved
 
 
 def _drop(x, residual, p, seed, offset, counter):
-    x = as_lies(x).contiguous()
-    residual = None if residual is None else as_lies(residual).contiguous()
+    x = resolved(x).contiguous()
+    residual = None if residual is None else resolved(residual).contiguous()
     y = torch.empty_like(x)
     if x.numel() == 0:
         return y
@@ -59,6 +59,6 @@ def dropout_func(x, p, seed, offset=0, residual=None):
     seed, offset = int(seed), int(offset)
     if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
         raise ValueError("seed and offset must be whole numbers from 0 to 2^64 - 1")
-    if _lib.watched() or (torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))):
+    if _lib.followed() or (torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))):
         return DropoutFunc.apply(x, residual, p, seed, offset, counter)
     return _drop(x, residual, p, seed, offset, counter)

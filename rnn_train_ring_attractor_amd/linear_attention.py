@@ -17,15 +17,16 @@ import torch
 from torch.autograd import Function
 
 from . import _lib
-from ._lib import SEQUENCE_TYPES, as_lies, check_sequence_sizes, check_sequence_tensor
+from ._lib import SEQUENCE_TYPES, check_sequence_sizes, check_sequence_tensor, resolved
 
 _Strides9, _Strides12, _Strides6 = ctypes.c_longlong * 9, ctypes.c_longlong * 12, ctypes.c_longlong * 6
 
 
 def _rows(t):
     """t with a head's values as neighbours (any other strides are taken as they are)."""
-    t = as_lies(t)
-    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+    if t.is_neg():
+        t = resolved(t)
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _checked(q, k, v, log_decay, dims):
@@ -43,7 +44,7 @@ def _checked(q, k, v, log_decay, dims):
     Dv = v.shape[-1]
     if H == 0 or G == 0 or Dk == 0 or Dv == 0 or H % G != 0:
         raise ValueError(f"heads ({H}) must be a positive multiple of kv_heads ({G}), dk and dv positive ({Dk}, {Dv})")
-    check_sequence_sizes(*q.shape, Dv)
+    check_sequence_sizes(q, v)
     check_sequence_tensor("log_decay", log_decay, (H,), torch.float32, dev)
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError("log_decay is a setting, as the time loop's alpha: it gets no gradient (detach it)")
@@ -97,7 +98,7 @@ class LinearAttentionFunc(Function):
             gq, gk, gv = (x.new_empty(x.shape) if needed else None
                           for x, needed in zip((q, k, v), (*ctx.needs_input_grad[:2], ctx.needs_input_grad[2] or want)))
             g0 = log_decay.new_empty((B, H, Dk, Dv)) if want else None
-            gs = None if grad_state is None else as_lies(grad_state).contiguous()
+            gs = None if grad_state is None else resolved(grad_state).contiguous()
             if B == 0 or T == 0:
                 if want:
                     g0.zero_() if gs is None else g0.copy_(gs)
@@ -129,15 +130,15 @@ def linear_attention_func(q, k, v, log_decay, initial_state=None, lengths=None, 
     B, T = q.shape[:2]
     if initial_state is not None:
         check_sequence_tensor("initial_state", initial_state, (B, H, Dk, Dv), torch.float32, dev)
-        initial_state = as_lies(initial_state).contiguous()
+        initial_state = resolved(initial_state).contiguous()
     if lengths is not None:
         if isinstance(lengths, torch.Tensor) and lengths.dtype == torch.int64:
             lengths = lengths.clamp(0, T).to(torch.int32)
         check_sequence_tensor("lengths", lengths, (B,), torch.int32, dev)
-        lengths = as_lies(lengths).contiguous()
-    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), as_lies(log_decay).contiguous()
+        lengths = resolved(lengths).contiguous()
+    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), resolved(log_decay).contiguous()
     scale = Dk ** -0.5 if scale is None else float(scale)
-    if _lib.watched() or (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+    if _lib.followed() or (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
                                                        (initial_state is not None and initial_state.requires_grad))):
         o, state = LinearAttentionFunc.apply(q, k, v, log_decay, initial_state, lengths, scale, bool(return_state))
     else:
@@ -156,12 +157,12 @@ def linear_attention_step(q, k, v, log_decay, state, active=None, scale=None):
         raise RuntimeError("state must be contiguous and no negated view: it is updated in place")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise RuntimeError("linear_attention_step has no gradient: call it under torch.no_grad(), or linear_attention_func to train")
-    if _lib.watched():
-        _lib.refuse_derivatives("linear_attention_step", q, k, v, log_decay, state)
+    if _lib.followed():
+        _lib.refuse_followed("linear_attention_step", q, k, v, log_decay, state)
     if active is not None:
         check_sequence_tensor("active", active, (B,), torch.uint8 if getattr(active, "dtype", None) == torch.uint8 else torch.bool, dev)
         active = active.contiguous()
-    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), as_lies(log_decay).contiguous()
+    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), resolved(log_decay).contiguous()
     lib = _lib.load()
     with _lib.on_device(dev):
         o = q.new_empty((B, H, Dv))

@@ -11,7 +11,7 @@ import torch
 from torch.autograd import Function
 
 from . import _lib
-from ._lib import SEQUENCE_TYPES, as_lies, check_sequence_sizes, check_sequence_tensor
+from ._lib import SEQUENCE_TYPES, check_sequence_sizes, check_sequence_tensor, resolved
 
 _POSITION_TYPES = {torch.int64: 0, torch.int32: 1, torch.float32: 2}
 _LAYOUTS = {"half": 0, "interleaved": 1}
@@ -57,7 +57,7 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, origi
 def _turn(xs, positions, frequencies, layout, scale, inverse):
     B, T, _, D = xs[0].shape
     dev = xs[0].device
-    xs = [as_lies(x) for x in xs]
+    xs = [resolved(x) for x in xs]
     xs = [x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous() for x in xs]
     lib = _lib.load()
     with _lib.on_device(dev):
@@ -121,7 +121,7 @@ def rotary_func(x, positions, frequencies, layout="half", scale=1.0):
             raise ValueError(f"x must be two tensors of [B, T, heads, D], got {tuple(xs[0].shape)} and {tuple(xs[1].shape)}")
     if any(t.shape[2] == 0 for t in xs):
         raise ValueError("x must have at least one head")
-    check_sequence_sizes(*(n for t in xs for n in t.shape))
+    check_sequence_sizes(*xs)
     if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITION_TYPES:
         raise TypeError("positions must be an int64, int32 or float32 tensor")
     if tuple(positions.shape) not in ((T,), (B, T)):
@@ -135,8 +135,8 @@ def rotary_func(x, positions, frequencies, layout="half", scale=1.0):
         raise ValueError("frequencies get no gradient (detach them)")
     if frequencies.dim() != 1 or not 1 <= frequencies.numel() <= D // 2:
         raise ValueError(f"frequencies must be one-dimensional, between 1 and {D // 2} of them, got {tuple(frequencies.shape)}")
-    positions, frequencies, scale = as_lies(positions), as_lies(frequencies).contiguous(), float(scale)
-    if _lib.watched() or (torch.is_grad_enabled() and any(t.requires_grad for t in xs)):
+    positions, frequencies, scale = resolved(positions), resolved(frequencies).contiguous(), float(scale)
+    if _lib.followed() or (torch.is_grad_enabled() and any(t.requires_grad for t in xs)):
         ys = RotaryFunc.apply(positions, frequencies, _LAYOUTS[layout], scale, 0, *xs)
     else:
         ys = _turned(positions, frequencies, _LAYOUTS[layout], scale, 0, *xs)
