@@ -397,3 +397,28 @@ def test_positions_however_far(gpu_device):
         size = (x[..., :8].abs() + x[..., 8:].abs()).repeat(1, 1, 1, 2).double()
         err = (got - want).abs()
         assert (err <= 2.0 ** -24 * 1.0001 * want.abs() + (2 * math.pi + 4) * 2.0 ** -24 * size).all(), (positions.dtype, float((err / size).max()))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("sizes", [(1, 100, 2, 2, 128, 128), (2, 90, 2, 1, 33, 47), (1, 70, 2, 1, 40, 72), (1, 70, 1, 1, 256, 136), (4, 500, 2, 2, 20, 70),
+                                   (4, 500, 2, 1, 70, 66), (4, 500, 2, 2, 130, 9)], ids=lambda s: "x".join(map(str, s)))
+def test_what_is_not_finite_reaches_rows_that_see_it_only(sizes, kind, gpu_device):
+    """At every width, within a chunk, across chunks and across segments."""
+    dtype, T = TYPES[kind], sizes[1]
+    p = _without_state_gradient(_problem(89, *sizes, dtype, start=True))
+    clean = _call(p, dtype, gpu_device, None, state=False)
+    for at in (0, 45, T - 1):
+        for name in ("q", "k", "v", "do"):
+            for value in (-math.inf, math.nan):
+                print(f"[case] {value} in {name} at {at} {sizes} {kind}", flush=True)
+                bad = {n: (None if x is None else x.clone()) for n, x in p.items()}
+                bad[name][0, at, :, -1] = value
+                got = _call(bad, dtype, gpu_device, None, state=False)
+                front, back, other = slice(0, at), slice(at + 1, T), slice(0, T)
+                same = {"q": {"o": (front, back), "dq": (other,), "dk": (back,), "dv": (back,)}, "k": {"o": (front,), "dq": (front,), "dk": (other,), "dv": (front, back)},
+                        "v": {"o": (front,), "dq": (front,), "dk": (front, back), "dv": (other,)}, "do": {"o": (other,), "dq": (front, back), "dk": (back,), "dv": (back,)}}[name]
+                for n, rows in same.items():
+                    assert torch.equal(got[n][1:], clean[n][1:]), n
+                    assert all(torch.equal(got[n][0, r], clean[n][0, r]) for r in rows), n
+                if name in ("k", "v"):
+                    assert not torch.isfinite(got["o"][0, at:]).all(-1).any(), "rows that see it"
