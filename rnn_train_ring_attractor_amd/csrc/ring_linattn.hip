@@ -10,7 +10,7 @@ namespace {
 
 constexpr int kChunk = 64;            // segments are whole numbers of these tokens
 // Of so many segments the second adds what the first has added to the initial state itself; of more a scan does, a launch more but less to read
-// (8 x 4096 tokens, 16 heads of 128 in four segments, us a pass of the chunk kernel: 165 adding up itself, 130 and a scan of 17).
+// (8 x 4096 tokens, 16 heads of 128, bf16, in four segments, us a pass of the chunk kernel: 129 behind a scan of 14; adding up itself took 35 more).
 constexpr int kFold = 2;
 
 size_t round_up(size_t x) { return (x + 255) / 256 * 256; }
@@ -23,8 +23,8 @@ hipError_t launch_pass(int type, const RingLinArgs& a, bool rev, bool state_only
 
 // A head's columns go to workgroups of 64 where there are no more, else of 128: in slices of 64 a wide head needs fewer segments, but
 // forms its weights twice as often (us of a forward, and with its backward, each in its best number of segments, 128 and 64: 8 x 4096
-// tokens, 16 heads of 128, bf16 188, 542 and 183, 686; 8 x 2000 tokens, 8 heads of 256, fp32 459, 1647 and 496, 1968; 16 x 1000 tokens, 8
-// heads of 128, fp32 142, 466 and 136, 490).
+// tokens, 16 heads of 128, bf16 195, 618 and 204, 708; 8 x 2000 tokens, 8 heads of 256, fp32 441, 1639 and 489, 2013; 16 x 1000 tokens, 8
+// heads of 128, fp32 139, 472 and 136, 499).
 int slices(int Db) { return Db <= 64 ? 1 : (Db + 127) / 128; }
 
 void set_columns(RingLinArgs& a, int Db, bool narrow) {
@@ -172,26 +172,27 @@ hipError_t ring_linattn_step(const RingLinShape& s, const RingLinStep& a, hipStr
 
 // Into how many segments the tokens are cut so that there is work for all compute units: the number with the least expected time of a
 // forward.  What it is made of, in us, as measured (P: 64, 128 or 256, what the kernels round a head's widths up to):
-//   a chunk of 32 tokens, a workgroup alone on its compute unit: bf16 1.1, 1.6, 2.7; fp32 products 2.8, 6.2, 12
+//   a chunk of 32 tokens, a workgroup alone on its compute unit: bf16 1.2, 2.0, 3.5; fp32 products 2.8, 6.2, 12
 //   two workgroups on a compute unit: 1.2 of one's time with P = 64, 1.86 with P = 128 (1.6 where a quarter of them have two); with P = 256
 //   they follow each other
 //   but no less than the rows take from memory, at 5 TB/s
-//   the pass over states: 0.4 of a chunk, and 6 or (P > 64) 10 for its launch and what the pass behind reads of it
+//   the pass over states: 0.34 (bf16) or 0.4 of a chunk, and 6 or (P > 64) 10 for its launch and what the pass behind reads of it
 //   the scan (more than kFold segments): 3 or 5, 0.2 a segment, and its states at 5 TB/s
-// us of a forward, and with its backward, by segments, the rule's choice in brackets:
-//   8 x 4096 tokens, 16 heads of 128, bf16    1: 229, 743   [2: 187, 558]    3: 192, 619    4: 184, 584    8: 218, 672
-//   1 x 32768 tokens, 16 heads of 128, bf16   1: 1777, 5766  8: 333, 978   [16: 200, 585]  32: 208, 637   64: 237, 707
-//   1 x 8192 tokens, 8 heads of 128, bf16     1: 444, 1453   8: 93, 263     16: 60, 166   [32: 51, 134]   64: 60, 167
-//   8 x 2048 tokens, 16 heads of 64, bf16     1: 70, 220     2: 58, 164     3: 54, 155    [4: 47, 140]    8: 53, 149
-//   8 x 2000 tokens, 8 heads of 256, fp32     1: 677, 2760  [2: 455, 1621]  4: 524, 1843    8: 611, 2082
-//   3 x 4096 tokens, 8 heads of 256, bf16     1: 393, 1493   4: 168, 535   [5: 142, 458]    8: 180, 605   16: 203, 632
-//   20 x 4096 tokens, 16 heads of 128, bf16  [1: 345, 1340]  2: 421, 1364   4: 469, 1455
-//   2 x 1000 tokens, 4 heads of 64, fp32      1: 88, 306     8: 27, 135   [16: 24, 135]
+// us of a forward with its final state, and with its backward, by segments, the rule's choice in brackets:
+//   8 x 4096 tokens, 16 heads of 128, bf16    1: 282, 937   [2: 214, 625]    3: 211, 712    4: 196, 628    8: 228, 707
+//   1 x 32768 tokens, 16 heads of 128, bf16   1: 2219, 7301  8: 390, 1178  [16: 227, 677]  32: 220, 680   64: 243, 746
+//   1 x 8192 tokens, 8 heads of 128, bf16     1: 551, 1833   8: 107, 312    16: 68, 191   [32: 55, 147]   64: 63, 178
+//   8 x 2048 tokens, 16 heads of 64, bf16     1: 81, 262     2: 66, 189     3: 61, 180    [4: 51, 149]    8: 52, 159
+//   8 x 2000 tokens, 8 heads of 256, fp32     1: 686, 2792  [2: 455, 1637]  4: 532, 1858    8: 621, 2109
+//   3 x 4096 tokens, 8 heads of 256, bf16     1: 502, 1868   4: 196, 633   [5: 162, 536]    8: 207, 697   16: 221, 698
+//   20 x 4096 tokens, 16 heads of 128, bf16  [1: 430, 1612]  2: 457, 1531   4: 496, 1605
+//   2 x 1000 tokens, 4 heads of 64, fp32      1: 91, 308     8: 28, 146   [16: 26, 145]
 static int segments(const RingLinShape& s) {
   const int units = (s.T + kChunk - 1) / kChunk;
   const int widest = s.Dk > s.Dv ? s.Dk : s.Dv, P = widest <= 64 ? 64 : (widest <= 128 ? 128 : 256);
   const double heads = (double)s.B * s.H, groups = heads * slices(s.Dv);
-  const double chunk = s.type == RINGATTR_BF16 ? 0.6 + 0.0083 * P : 0.047 * P;
+  const bool bf16 = s.type == RINGATTR_BF16;
+  const double chunk = bf16 ? 0.45 + 0.0118 * P : 0.047 * P;
   const double rows = heads * s.T * (s.Dk + s.Dv) * (s.type == RINGATTR_F32 ? 4 : 2) / 5e6;      // Y and Z once
   auto rounds = [&](double work) {                             // in times of a workgroup alone
     const double two = P == 64 ? 1.2 : (P == 128 ? 1.86 : 2.0), full = floor(work / 512), rest = work - 512 * full;
@@ -204,7 +205,7 @@ static int segments(const RingLinShape& s) {
     const int per = (units + n - 1) / n;
     if ((units + per - 1) / per != n) continue;
     double t = no_less(2 * per * chunk * rounds(groups * n), 2 * rows);
-    if (n > 1) t += no_less(0.8 * per * chunk * rounds(groups * (n - 1)), rows * (n - 1) / n) + (P == 64 ? 6 : 10);
+    if (n > 1) t += no_less((bf16 ? 0.68 : 0.8) * per * chunk * rounds(groups * (n - 1)), rows * (n - 1) / n) + (P == 64 ? 6 : 10);
     if (n > kFold) t += (P == 64 ? 3 : 5) + 0.2 * n + heads * n * s.Dk * s.Dv * 8 / 5e6;
     if (n == 1 || t < time) {
       time = t;

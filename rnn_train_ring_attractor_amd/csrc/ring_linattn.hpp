@@ -202,15 +202,14 @@ template <int N> __device__ __forceinline__ void wait_for_memory() { asm volatil
 // in registers, where they are an operand as they lie: the matrix units put rows 4g..4g+3 of column l into lane (g, l) and take them
 // as contraction indices from there.  The weights are formed transposed for the same reason, by every wave for itself.
 //
-// What bounds it.  bf16, a state of 128 x 128: a chunk of 32 tokens is 64 matrix instructions of 16 clocks a wave (EXACT: 80), about as
-// many clocks of vector instructions, which hardly overlap them, and a chain from the rows through the weights to the outputs: 1.6 us
-// a chunk in a chip with few workgroups.  With one on every compute unit it is 2.2 us, with two 2.0 for each of their chunks: memory.
-// 8 x 4096 tokens, 16 heads, 537 MB a pass: 130 us with 512 workgroups (4.1 TB/s; a large copy 5.2), 144 with 256; one sequence of 32768
-// tokens 150 to 153.  There (us, the latter case) chunks of
-// 64 tokens take 165, eight waves of 16 columns 166, two chunks on their way at once 165.  fp32 and fp16 multiply at 32 clocks for an
-// eighth of the contraction, in chunks of 16 tokens (fp16: 32), and are bound by that: 8 x 2000 tokens, 8 heads of 256, fp32, 33.6 GFLOP
-// a pass without the weights: 390 us, 86 TFLOP/s (154 in a large matrix product).  States alone, one
-// sequence of 32768 tokens: 252 MB, 70 us (3.6 TB/s).
+// What bounds it.  bf16, a state of 128 x 128: a chunk of 32 tokens is 84 matrix instructions of 16 clocks a wave (EXACT: 100), more
+// clocks than that of vector instructions (a third of them split the state), which hardly overlap them, and a chain from the rows through the
+// weights to the outputs: 2.0 us a chunk in a chip with few workgroups (EXACT: 2.2).  8 x 4096 tokens, 16 heads, 537 MB a pass: 129 us with
+// 512 workgroups (4.2 TB/s; a large copy 5.2), 156 with 256, EXACT 179 and 197; one sequence of 32768 tokens, EXACT, 180.  Before weights and
+// states were two numbers (153 there) chunks of 64 tokens took 165, eight waves of 16 columns 166, two chunks on their way at once 165.  fp32
+// and fp16 multiply at 32 clocks for an eighth of the contraction, in chunks of 16 tokens (fp16: 32), and are bound by that: 8 x 2000 tokens,
+// 8 heads of 256, fp32, 33.6 GFLOP a pass without the weights: 390 to 416 us, 81 to 86 TFLOP/s (154 in a large matrix product).  States alone,
+// one sequence of 32768 tokens: 252 MB, 68 us (3.7 TB/s).
 template <typename T, int DA, int NC, int NW, int CT, bool VEC, bool REV, bool STATE_ONLY, bool EXACT, bool PAIR = false>
 __global__ __launch_bounds__(64 * NW, (DA <= 128 || NW == 8 ? 2 : 1)) void ring_linattn_kernel(RingLinArgs p) {
   constexpr int GW = PAIR ? NW / 2 : NW, WC = 16 * NC * GW, NT = 64 * NW, CH = 16 * CT, DT = DA / 16;

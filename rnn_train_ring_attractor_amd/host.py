@@ -114,9 +114,9 @@ def av_to_action_signal_ND(av_signal, action_dim=16, zero_padding=True):
 
 
 def drop_action_signal(action_signal, p, seed, offset=0):
-    """Sensory dropout: parts of the action signal are missing with probability p (`dropout_func`; seed and offset as there: a step of
-    its own offset, or a device counter that a recorded step advances).  What the signal's builder stated about its channels still
-    holds."""
+    """Sensory dropout: parts of the action signal, a GPU tensor, are missing with probability p (`dropout_func`; seed and offset as there:
+    a step of its own offset, or a device counter that a recorded step advances).  What the signal's builder stated about its channels
+    still holds."""
     if not p:
         return action_signal
     from .dropout import dropout_func
