@@ -32,7 +32,7 @@ class DropoutFunc(Function):
     def backward(ctx, grad):
         counter, = ctx.saved_tensors
         p, seed, offset = ctx.how
-        again = DropoutFunc.apply if torch.is_grad_enabled() else _drop          # (a gradient of the gradient is this operator again)
+        again = DropoutFunc.apply if torch.is_grad_enabled() or _lib.followed() else _drop          # (a gradient of the gradient is this operator again)
         gx = again(grad, None, p, seed, offset, counter) if ctx.needs_input_grad[0] else None
         return gx, grad if ctx.needs_input_grad[1] else None, None, None, None, None
 

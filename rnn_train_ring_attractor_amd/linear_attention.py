@@ -88,6 +88,8 @@ class LinearAttentionFunc(Function):
     def backward(ctx, grad_o, grad_state):
         if torch.is_grad_enabled():              # (create_graph: the result would pass for one that does not depend on q, k and v)
             raise RuntimeError("linear_attention_func is differentiable once: its backward takes no create_graph=True")
+        if _lib.followed():
+            _lib.refuse_followed("the backward of linear_attention_func", *(g for g in (grad_o, grad_state) if g is not None))
         q, k, v, log_decay, initial_state, lengths, along = ctx.saved_tensors
         B, T, H, Dk = q.shape
         G, Dv, dev = k.shape[2], v.shape[3], q.device

@@ -91,7 +91,7 @@ class RotaryFunc(Function):
         positions, frequencies = ctx.saved_tensors
         layout, scale, inverse = ctx.how
         # turned back: the transpose of a turn is the opposite turn, so a gradient of the gradient is this operator again
-        back = RotaryFunc.apply if torch.is_grad_enabled() else _turned
+        back = RotaryFunc.apply if torch.is_grad_enabled() or _lib.followed() else _turned
         needed = ctx.needs_input_grad[5:]
         turned = iter(back(positions, frequencies, layout, scale, 1 - inverse, *(g for g, n in zip(grads, needed) if n)))
         return (None,) * 5 + tuple(next(turned) if n else None for n in needed)
@@ -103,7 +103,8 @@ def rotary_func(x, positions, frequencies, layout="half", scale=1.0):
     angle position * frequencies[m] and multiplied by `scale`; the rest of a head is copied.
 
     positions [T] or [B,T], int64, int32 or float32 (an angle); frequencies float64 (`rotary_frequencies`).  The angle, less whole turns, is
-    that of the exact product for every int64 position (of frequencies up to 1000: to 2^-24 turns).  Differentiable with respect to x.  Returns a tensor, or a tuple where x is a pair."""
+    that of the exact product for every int64 position (of frequencies up to 1000: to 2^-24 turns).  Differentiable with respect to x.
+    Returns a tensor, or a tuple where x is a pair."""
     pair = isinstance(x, (tuple, list))
     xs = tuple(x) if pair else (x,)
     if len(xs) not in (1, 2):

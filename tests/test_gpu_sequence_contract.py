@@ -422,3 +422,20 @@ def test_what_is_not_finite_reaches_rows_that_see_it_only(sizes, kind, gpu_devic
                     assert all(torch.equal(got[n][0, r], clean[n][0, r]) for r in rows), n
                 if name in ("k", "v"):
                     assert not torch.isfinite(got["o"][0, at:]).all(-1).any(), "rows that see it"
+
+
+def test_forward_mode_over_a_backward_is_refused(gpu_device):
+    """A gradient that carries a tangent goes into no backward without a rule for it; one that carries none does."""
+    import torch.autograd.forward_ad as forward
+    entries, x = _entries(gpu_device)
+    for name, op in entries.items():
+        print(f"[case] forward over backward {name}", flush=True)
+        leaf = x.clone().requires_grad_(True)
+        y = op(leaf)
+        g = torch.ones_like(y)
+        want, = torch.autograd.grad(y, leaf, g, retain_graph=True)
+        with forward.dual_level():
+            assert torch.equal(torch.autograd.grad(y, leaf, g, retain_graph=True)[0], want)
+            if name != "residual":                               # (whose gradient is the one that comes in)
+                with pytest.raises((RuntimeError, NotImplementedError)):
+                    torch.autograd.grad(y, leaf, forward.make_dual(g, g))
