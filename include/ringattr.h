@@ -334,6 +334,82 @@ RINGATTR_API int ringattr_rotary(const void* x0, const void* x1, const long long
 RINGATTR_API int ringattr_dropout(const void* x, const void* residual, void* y, size_t n, unsigned int threshold, float scale,
                       unsigned long long seed, unsigned long long offset, const void* offset_ptr, int type, void* stream);
 
+/* A recurrent layer's operators, for sequences and for single tokens; no counterpart in the reference.  `type` holds for every tensor
+ * that is not said to be fp32; parameters are fp32.  A tensor [B,T,C] is given by its address and its strides (batch, token, in elements; channels
+ * are neighbours), outputs are contiguous.  lengths as above: outputs and gradients behind a length are zero and nothing there is read.
+ * Outputs, kept states and workspaces start at 16 bytes, everything else at its own type's size.  Sums over tokens, sequences and channels are
+ * fp32, in a fixed order. */
+#define RINGATTR_ACT_NONE 0
+#define RINGATTR_ACT_SILU 1
+#define RINGATTR_ACT_SIGMOID 2
+
+/* Short causal convolution of each channel by itself, taps up to 8 (weight [channels,taps], bias [channels] or NULL):
+ *   y_t = act(bias + sum_k weight[k] x_(t - taps + 1 + k)),  act none or silu
+ * initial_state [B,taps - 1,channels]: the inputs in front of the sequences (NULL: zeros), final_state (NULL: not wanted): the last taps - 1
+ * inputs that count.  strides: host array, two for x (and two for grad_y). */
+#define RINGATTR_CONV_MAX_TAPS 8
+RINGATTR_API int ringattr_causal_conv_fwd(const void* x, const long long* strides, const void* weight, const void* bias,
+                      const void* initial_state, const void* lengths, void* y, void* final_state, int activation, int type,
+                      int batch_size, int seq_len, int channels, int taps, void* stream);
+/* Gradients, each NULL where it is not wanted.  weights: whether grad_weight or grad_bias is. */
+RINGATTR_API size_t ringattr_causal_conv_bwd_workspace_bytes(int type, int batch_size, int seq_len, int channels, int taps, int weights);
+RINGATTR_API int ringattr_causal_conv_bwd(const void* x, const void* grad_y, const long long* strides, const void* weight,
+                      const void* bias, const void* initial_state, const void* lengths, const void* grad_final_state, void* grad_x,
+                      void* grad_weight, void* grad_bias, void* grad_initial_state, int activation, int type, int batch_size,
+                      int seq_len, int channels, int taps, void* workspace, size_t workspace_bytes, void* stream);
+/* One token for each sequence: x [B,channels] (stride: batch), the state [B,taps - 1,channels] moved on in place, y [B,channels].
+ * active (device bytes [B], NULL: all): where it is zero the state is left as it is and y is zero. */
+RINGATTR_API int ringattr_causal_conv_step(const void* x, long long stride, const void* weight, const void* bias, void* state,
+                      const void* active, void* y, int activation, int type, int batch_size, int channels, int taps, void* stream);
+
+/* Selective state space scan, up to 64 states a channel, d_t = delta_t + delta_bias or softplus of it:
+ *   h_t[n] = e^(d_t A[n]) h_(t-1)[n] + d_t x_t B_t[n],  y_t = (sum_n C_t[n] h_t[n] + D x_t) silu(z_t)
+ * x, delta, z [B,T,channels] (z NULL: no gate), B, C [B,T,groups,states] (channel c uses group c / (channels / groups); a group's states are
+ * neighbours), A [channels,states], D, delta_bias [channels] or NULL, states of a sequence fp32 [B,channels,states].  strides: host array, two for each
+ * of x, delta, z, three (batch, token, group) for each of B and C, two for grad_y.  states_kept (NULL: not kept): what a backward
+ * of the same arguments needs, ringattr_selective_scan_states_bytes of it. */
+#define RINGATTR_SCAN_MAX_STATES 64
+RINGATTR_API size_t ringattr_selective_scan_states_bytes(int type, int batch_size, int seq_len, int channels, int states, int groups);
+RINGATTR_API size_t ringattr_selective_scan_fwd_workspace_bytes(int type, int batch_size, int seq_len, int channels, int states,
+                      int groups);
+RINGATTR_API int ringattr_selective_scan_fwd(const void* x, const void* delta, const void* z, const void* B, const void* C,
+                      const long long* strides, const void* A, const void* D, const void* delta_bias, const void* initial_state,
+                      const void* lengths, void* y, void* final_state, void* states_kept, int softplus, int type, int batch_size,
+                      int seq_len, int channels, int states, int groups, void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients, each NULL where it is not wanted.  shared: whether grad_B or grad_C is, parameters: whether one of grad_A, grad_D, grad_delta_bias is.
+ * grad_final_state NULL: zeros. */
+RINGATTR_API size_t ringattr_selective_scan_bwd_workspace_bytes(int type, int batch_size, int seq_len, int channels, int states,
+                      int groups, int shared, int parameters);
+RINGATTR_API int ringattr_selective_scan_bwd(const void* x, const void* delta, const void* z, const void* B, const void* C,
+                      const void* grad_y, const long long* strides, const void* A, const void* D, const void* delta_bias,
+                      const void* lengths, const void* states_kept, const void* grad_final_state, void* grad_x, void* grad_delta,
+                      void* grad_z, void* grad_B, void* grad_C, void* grad_A, void* grad_D, void* grad_delta_bias,
+                      void* grad_initial_state, int softplus, int type, int batch_size, int seq_len, int channels, int states,
+                      int groups, void* workspace, size_t workspace_bytes, void* stream);
+/* One token for each sequence: x, delta, z [B,channels], B, C [B,groups,states] (strides: batch of x, delta, z; batch, group of B, of C), the state
+ * [B,channels,states] updated in place, y [B,channels].  active as above. */
+RINGATTR_API int ringattr_selective_scan_step(const void* x, const void* delta, const void* z, const void* B, const void* C,
+                      const long long* strides, const void* A, const void* D, const void* delta_bias, void* state, const void* active,
+                      void* y, int softplus, int type, int batch_size, int channels, int states, int groups, void* stream);
+
+/* Norm, gate and scaled residual around a block, rows of up to 8192 channels:
+ *   unit = (x - mean) / sqrt(mean of squares + eps) over every `group` neighbouring channels (layer 0: without the mean),
+ *   y = residual + scale unit weight act(gate),   n = unit of y over the whole row, times next_weight
+ * residual, scale, gate NULL: left out; next_weight NULL: no n.  act none, silu or sigmoid.  strides: host array, a row's of x, gate, residual (and
+ * grad_y, grad_n). */
+#define RINGATTR_NORM_MAX_CHANNELS 8192
+RINGATTR_API int ringattr_norm_gate_fwd(const void* x, const void* gate, const void* residual, const long long* strides,
+                      const void* weight, const void* scale, const void* next_weight, void* y, void* n, float eps, int layer,
+                      int activation, int type, size_t rows, int channels, int group, void* stream);
+/* Gradients, each NULL where it is not wanted, from those of y and n (one of them may be NULL: zero).  weights: whether grad_weight, grad_scale or
+ * grad_next_weight is. */
+RINGATTR_API size_t ringattr_norm_gate_bwd_workspace_bytes(int type, size_t rows, int channels, int group, int weights);
+RINGATTR_API int ringattr_norm_gate_bwd(const void* x, const void* gate, const void* residual, const void* grad_y,
+                      const void* grad_n, const long long* strides, const void* weight, const void* scale, const void* next_weight,
+                      void* grad_x, void* grad_gate, void* grad_residual, void* grad_weight, void* grad_scale,
+                      void* grad_next_weight, float eps, int layer, int activation, int type, size_t rows, int channels, int group,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 /* Per-kernel timing for benchmarks; no counterpart in the reference.  ringattr_profile_enable(n): n = 0 switches it
  * off; n >= 1 brackets every n-th launch of each kernel (counted per kernel from this call on) by two HIP events
  * recorded on the launch stream.  The two records cost about 4-5 us of stream time per bracketed launch (23 us per

@@ -12,6 +12,9 @@ _EXPORTS = {
     "linear_attention_step": "linear_attention",
     "rotary_func": "rotary", "RotaryFunc": "rotary", "rotary_frequencies": "rotary",
     "dropout_func": "dropout", "DropoutFunc": "dropout",
+    "causal_conv_func": "causal_conv", "CausalConvFunc": "causal_conv", "causal_conv_step": "causal_conv",
+    "selective_scan_func": "selective_scan", "SelectiveScanFunc": "selective_scan", "selective_scan_step": "selective_scan",
+    "norm_gate_func": "norm_gate", "NormGateFunc": "norm_gate",
 }
 
 

@@ -87,6 +87,24 @@ PROTOTYPES = {
                         [c_void_p] * 3 + [c_float] + [c_int] * 9 + [c_void_p]),
     "ringattr_dropout": (c_int, [c_void_p] * 3 + [c_size_t, ctypes.c_uint, c_float, ctypes.c_ulonglong, ctypes.c_ulonglong, c_void_p, c_int,
                                  c_void_p]),
+    "ringattr_causal_conv_fwd": (c_int, [c_void_p, ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 6 + [c_int] * 6 + [c_void_p]),
+    "ringattr_causal_conv_bwd_workspace_bytes": (c_size_t, [c_int] * 6),
+    "ringattr_causal_conv_bwd": (c_int, [c_void_p] * 2 + [ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 9 + [c_int] * 6 +
+                                 [c_void_p, c_size_t, c_void_p]),
+    "ringattr_causal_conv_step": (c_int, [c_void_p, ctypes.c_longlong] + [c_void_p] * 5 + [c_int] * 5 + [c_void_p]),
+    "ringattr_selective_scan_states_bytes": (c_size_t, [c_int] * 6),
+    "ringattr_selective_scan_fwd_workspace_bytes": (c_size_t, [c_int] * 6),
+    "ringattr_selective_scan_fwd": (c_int, [c_void_p] * 5 + [ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 8 + [c_int] * 7 +
+                                    [c_void_p, c_size_t, c_void_p]),
+    "ringattr_selective_scan_bwd_workspace_bytes": (c_size_t, [c_int] * 8),
+    "ringattr_selective_scan_bwd": (c_int, [c_void_p] * 6 + [ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 15 + [c_int] * 7 +
+                                    [c_void_p, c_size_t, c_void_p]),
+    "ringattr_selective_scan_step": (c_int, [c_void_p] * 5 + [ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 6 + [c_int] * 6 + [c_void_p]),
+    "ringattr_norm_gate_fwd": (c_int, [c_void_p] * 3 + [ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 5 + [c_float] + [c_int] * 3 +
+                               [c_size_t, c_int, c_int, c_void_p]),
+    "ringattr_norm_gate_bwd_workspace_bytes": (c_size_t, [c_int, c_size_t] + [c_int] * 3),
+    "ringattr_norm_gate_bwd": (c_int, [c_void_p] * 5 + [ctypes.POINTER(ctypes.c_longlong)] + [c_void_p] * 9 + [c_float] + [c_int] * 3 +
+                               [c_size_t, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "ringattr_profile_enable": (c_int, [c_int]),
     "ringattr_profile_read": (c_int, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_longlong)]),
     "ringattr_last_kernel_name": (c_int, [c_int, ctypes.c_char_p, ctypes.c_size_t]),
@@ -198,6 +216,47 @@ def check_sequence_tensor(name, t, shape=None, dtype=None, device=None) -> None:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_cuda or (device is not None and t.device != device):
         raise RuntimeError(f"{name} must be on {device if device is not None else 'a GPU'} (got {t.device}); there is no CPU path")
+
+
+def rows_of(t):
+    """t, or a copy of it, with its last dimension's values as neighbours and as they are meant (any other strides are taken as they are)."""
+    if t.is_neg():
+        t = resolved(t)
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def pointer(t):
+    return None if t is None else t.data_ptr()
+
+
+def checked_lengths(lengths, B, T, device):
+    """The tokens that count of each sequence of a padded batch, as the library takes them."""
+    if lengths is None:
+        return None
+    if isinstance(lengths, torch.Tensor) and lengths.dtype == torch.int64:
+        lengths = lengths.clamp(0, T).to(torch.int32)
+    check_sequence_tensor("lengths", lengths, (B,), torch.int32, device)
+    return resolved(lengths).contiguous()
+
+
+def checked_active(active, B, device):
+    """Which places of a served batch take part in a step, as the library takes them."""
+    if active is None:
+        return None
+    check_sequence_tensor("active", active, (B,), torch.uint8 if getattr(active, "dtype", None) == torch.uint8 else torch.bool, device)
+    return active.contiguous()
+
+
+def checked_parameter(name, t, shape, device):
+    """A parameter, float32 and contiguous."""
+    if t is None:
+        return None
+    check_sequence_tensor(name, t, shape, torch.float32, device)
+    return resolved(t).contiguous()
+
+
+def wants_gradient(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 class _Here:

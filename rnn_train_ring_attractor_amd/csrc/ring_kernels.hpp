@@ -403,3 +403,104 @@ struct RingDropoutArgs {
   float scale;
 };
 hipError_t ring_launch_dropout(const RingDropoutArgs& p, int type, hipStream_t st);
+
+// Rows [B,T,C] of a recurrent layer's operators: strides in elements of a sequence and a token, channels are neighbours
+struct RingRows {
+  const void* p;
+  long sb, st;
+};
+
+// Selective state space scan (ring_scan*.hip).  A pass of one of its kernels; see ring_scan.hpp
+enum { RING_SCAN_OUTPUTS = 0, RING_SCAN_STATE = 1, RING_SCAN_ADJOINT = 2, RING_SCAN_GRADIENTS = 3 };
+struct RingScanArgs {
+  static constexpr int kSave = 16;       // tokens between two states that are kept for the backward
+  RingRows x, delta, z, dy;              // z.p null: no gate
+  const void *Bm, *Cm;                   // [B,T,G,N], a group's states are neighbours
+  long bsb, bst, bsg, csb, cst, csg;
+  const float *A, *D, *bias;             // [C,N], [C], [C]; the last two may be null
+  const float* s_in;                     // [B,C,N], null: zeros (backwards: the final state's gradient)
+  float* s_out;                          // null: not wanted (backwards: the initial state's gradient)
+  const int* lengths;                    // tokens of each sequence, null: T
+  void* y;                               // [B,T,C]
+  float* states;                         // [B,saved,C,NS] in front of every kSave-th token, null: not kept
+  float *seg, *total;                    // nseg > 1: [nseg - 1,B,C,NS] states or adjoints between the segments; [nseg - 1,B,C] sums of d
+  void *dx, *ddelta, *dz;                // [B,T,C], null: not wanted
+  float* part_bc;                        // [tiles,B,T,G,2,NS] sums of dB and dC over a tile's channels, null: not wanted
+  float* part_a;                         // [nseg,B,C,NS + 2] gradients of A, D and bias of a segment, null: not wanted
+  int B, T, C, N, G, saved, nseg, seg_tokens, softplus;
+  bool wide, wide_out;                   // rows read, and written, are whole numbers of eight channels at 16 bytes
+  int tiles;                             // (the launcher's) of a group's channels
+};
+struct RingScanShape { int B, T, C, N, G, type; };
+struct RingScanStep {
+  const void *x, *delta, *z, *Bm, *Cm;
+  long xs, ds, zs, bsb, bsg, csb, csg;   // strides of a sequence, and of a group
+  const float *A, *D, *bias;
+  float* state;                          // [B,C,N]
+  const unsigned char* active;
+  void* y;                               // [B,C]
+  int softplus;
+};
+size_t ring_scan_states_bytes(const RingScanShape& s);
+size_t ring_scan_fwd_bytes(const RingScanShape& s);
+size_t ring_scan_bwd_bytes(const RingScanShape& s, bool shared, bool params);
+// Outputs of a backward that are not wanted are null
+struct RingScanGrads { void *B, *C; float *A, *D, *bias; };
+hipError_t ring_scan_fwd(const RingScanShape& s, RingScanArgs a, void* ws, hipStream_t st);
+hipError_t ring_scan_bwd(const RingScanShape& s, RingScanArgs a, const RingScanGrads& g, void* ws, hipStream_t st);
+hipError_t ring_scan_step(const RingScanShape& s, const RingScanStep& a, hipStream_t st);
+hipError_t ring_launch_scan_f32(const RingScanArgs& p, int mode, hipStream_t st);
+hipError_t ring_launch_scan_bf16(const RingScanArgs& p, int mode, hipStream_t st);
+hipError_t ring_launch_scan_f16(const RingScanArgs& p, int mode, hipStream_t st);
+
+// Sums of `parts` rows of n values in their order (ring_recur.hip).  A value belongs to column i / per and is number i % per of it: the first N
+// go to out[column][N], number `per - rest` + k to more[k][column] (null: dropped)
+struct RingSumArgs {
+  const float* part;
+  int parts, per, N, rest;
+  size_t n;
+  float *out, *more[2];
+};
+hipError_t ring_launch_sum_parts(const RingSumArgs& p, hipStream_t st);
+
+// Short causal convolution (ring_conv.hip)
+struct RingConvArgs {
+  RingRows x, dy;
+  const float *w, *bias;                 // [C,K], [C] or null
+  const void *start, *dend;              // [B,K-1,C] or null
+  const int* lengths;
+  void *y, *end, *dx, *dstart;           // null: not wanted
+  float *dw, *dbias;
+  float* part;                           // [parts,C,K + 1]
+  int B, T, C, K, act, seg_tokens, nseg, parts;
+  bool wide, wide_out, wide_state;
+};
+struct RingConvStep {
+  const void* x;
+  long xs;
+  const float *w, *bias;
+  void *state, *y;
+  const unsigned char* active;
+  int B, C, K, act;
+};
+size_t ring_conv_bwd_bytes(int type, int B, int T, int C, int K, bool params);
+hipError_t ring_conv_fwd(RingConvArgs p, int type, hipStream_t st);
+hipError_t ring_conv_bwd(RingConvArgs p, int type, hipStream_t st);
+hipError_t ring_conv_step(const RingConvStep& p, int type, hipStream_t st);
+
+// Norm, gate and scaled residual (ring_norm.hip)
+struct RingNormArgs {
+  const void *x, *gate, *residual, *dy, *dn;      // [rows,C]; the strides of a row
+  long xs, gs, rs, dys, dns;
+  const float *w, *scale, *next;         // [C]; scale and next may be null
+  void *y, *n;                           // [rows,C]
+  void *dx, *dgate, *dresidual;
+  float *dw, *dscale, *dnext;            // [C], null: not wanted
+  float* part;                           // [parts,3,C]
+  long rows;
+  int C, group, layer, act, parts;
+  float eps;
+};
+size_t ring_norm_bwd_bytes(int type, long rows, int C, int group, bool params);
+hipError_t ring_norm_fwd(const RingNormArgs& p, int type, hipStream_t st);
+hipError_t ring_norm_bwd(RingNormArgs p, int type, hipStream_t st);

@@ -1,0 +1,450 @@
+// What stands around a block: its output normalised, gated and added to the residual stream, which the next block's norm then reads,
+//
+//   unit = (x - mean) rstd over each group of neighbouring values (kind rms: without the mean),  rstd = (mean of squares + eps)^-1/2,
+//   y = residual + scale unit w act(gate),   n = unit(y) next over the whole row.
+//
+// Backwards, t = dy + what n gives back: dresidual = t, dgate = t scale unit w act'(gate), d unit = t scale act(gate) w, dx = rstd (d unit - mean(d unit)
+// - unit mean(d unit unit)); the weights' gradients are sums over rows.  Units and y are found again from what was read.
+//
+// Bound by memory: every tensor is read once or written once.  A row lies in the registers of one workgroup (several rows, where they are short);
+// backwards a workgroup walks rows and keeps the sums of its columns until it is done.
+#include "ring_recur.hpp"
+#include "ringattr.h"
+
+using namespace ring_recur;
+
+namespace {
+
+enum { kIdentity = 0, kSilu = 1, kSigmoid = 2 };
+
+// How a row lies on threads: groups of `lanes` threads (a power of two), `slots` groups side by side (a power of two), `rows` rows a workgroup.  MANY: a thread
+// holds one unit of V values of each of I groups, else I units of one group.
+struct Lie { int lanes, slots, rows, units, groups; };
+
+// Sums of K values over `n` neighbouring threads, a power of two, the same in each
+template <int K> __device__ __forceinline__ void add_up(float (&v)[K], int n, float* room) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (n > 1) v[k] = plus_dpp<kXor1>(v[k]);
+    if (n > 2) v[k] = plus_dpp<kXor2>(v[k]);
+    if (n > 4) v[k] = plus_dpp<0x141>(v[k]);        // mirrored within 8, 16: whole quads, whole eights
+    if (n > 8) v[k] = plus_dpp<0x140>(v[k]);
+    if (n > 16) v[k] = fold16(v[k], v[k]);
+    if (n > 32) v[k] = fold32(v[k], v[k]);
+  }
+  if (n > 64) {
+    const int w = threadIdx.x >> 6, per = n >> 6, first = w / per * per;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) room[k * 16 + w] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float s = room[k * 16 + first];
+      for (int i = 1; i < per; ++i) s += room[k * 16 + first + i];
+      v[k] = s;
+    }
+  }
+}
+
+__device__ __forceinline__ float act_of(float x, int act) { return act == kSilu ? silu(x) : (act == kSigmoid ? sigmoid(x) : x); }
+__device__ __forceinline__ float slope_of(float x, int act) {
+  if (act == kIdentity) return 1.f;
+  const float s = sigmoid(x);
+  return act == kSilu ? silu_slope(x, s) : s * (1.f - s);
+}
+
+// A thread's place in a row
+template <int V, int I, bool MANY> struct Spot {
+  int lane, slot, row, threads;
+  __device__ __forceinline__ Spot(const Lie& l) {
+    threads = l.lanes * l.slots;
+    lane = threadIdx.x & (l.lanes - 1);
+    slot = threadIdx.x / l.lanes & (l.slots - 1);
+    row = threadIdx.x / threads;
+  }
+  __device__ __forceinline__ int column(const Lie& l, int i, int group) const {
+    const int g = MANY ? i * l.slots + slot : slot, u = MANY ? lane : i * l.lanes + lane;
+    return g * group + u * V;
+  }
+  __device__ __forceinline__ int here(const Lie& l, int i, int group) const {      // values of unit i that are there
+    const int g = MANY ? i * l.slots + slot : slot, u = MANY ? lane : i * l.lanes + lane;
+    return g < l.groups ? min(max(group - u * V, 0), V) : 0;
+  }
+};
+
+// sums[i] += the sum over its group of the thread's values of unit i
+template <int V, int I, bool MANY> __device__ __forceinline__ void group_sums(float (&sums)[I], const Lie& l, float* room) {
+  if constexpr (MANY) {
+    add_up<I>(sums, l.lanes, room);
+  } else {
+    float one[1] = {sums[0]};
+#pragma unroll
+    for (int i = 1; i < I; ++i) one[0] += sums[i];
+    add_up<1>(one, l.lanes, room);
+#pragma unroll
+    for (int i = 0; i < I; ++i) sums[i] = one[0];
+  }
+}
+
+// v becomes (v - mean) over its groups, rstd beside it
+template <int V, int I, bool MANY>
+__device__ __forceinline__ void normalise(float (&v)[I][V], float (&rstd)[I], const int (&here)[I], const Lie& l, float count, bool layer, float eps, float* room) {
+  float s[I];
+  if (layer) {
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      s[i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[i] += v[i][e];
+    }
+    group_sums<V, I, MANY>(s, l, room);
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[i][e] = e < here[i] ? v[i][e] - s[i] / count : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    s[i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[i] = fmaf(v[i][e], v[i][e], s[i]);
+  }
+  group_sums<V, I, MANY>(s, l, room);
+#pragma unroll
+  for (int i = 0; i < I; ++i) rstd[i] = 1.f / sqrtf(s[i] / count + eps);
+}
+
+}  // namespace
+
+template <typename T, int V, int I, bool MANY>
+__global__ __launch_bounds__(1024) void ring_norm_fwd_kernel(RingNormArgs p, Lie l) {
+  __shared__ float room[64];
+  const Spot<V, I, MANY> at(l);
+  const Lie whole = {at.threads, 1, l.rows, 0, 1};
+  const long row = ((long)blockIdx.y * gridDim.x + blockIdx.x) * l.rows + at.row;
+  const bool real = row < p.rows;
+  int here[I], col[I];
+  float v[I][V], rstd[I];
+  Row<T, V> rx[I], rg[I], rr[I];
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    here[i] = real ? at.here(l, i, p.group) : 0;
+    col[i] = at.column(l, i, p.group);
+    rx[i].zero(), rg[i].zero(), rr[i].zero();
+    if (here[i] > 0) {
+      rx[i].load((const T*)p.x + row * p.xs + col[i], V > 1, here[i]);
+      if (p.gate) rg[i].load((const T*)p.gate + row * p.gs + col[i], V > 1, here[i]);
+      if (p.residual) rr[i].load((const T*)p.residual + row * p.rs + col[i], V > 1, here[i]);
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[i][e] = (float)rx[i].v[e];
+  }
+  normalise<V, I, MANY>(v, rstd, here, l, (float)p.group, p.layer, p.eps, room);
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    Row<T, V> out;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float y = 0.f;
+      if (e < here[i]) {
+        y = v[i][e] * rstd[i] * p.w[col[i] + e];
+        if (p.gate) y *= act_of((float)rg[i].v[e], p.act);
+        if (p.scale) y *= p.scale[col[i] + e];
+        if (p.residual) y += (float)rr[i].v[e];
+      }
+      v[i][e] = y;
+      out.v[e] = (T)y;
+    }
+    if (here[i] > 0) out.store((T*)p.y + row * p.C + col[i], V > 1, here[i]);
+  }
+  if (!p.next) return;
+  normalise<V, I, false>(v, rstd, here, whole, (float)p.C, p.layer, p.eps, room);
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+    if (here[i] > 0) {
+      Row<T, V> out;
+#pragma unroll
+      for (int e = 0; e < V; ++e) out.v[e] = (T)(e < here[i] ? v[i][e] * rstd[i] * p.next[col[i] + e] : 0.f);
+      out.store((T*)p.n + row * p.C + col[i], V > 1, here[i]);
+    }
+}
+
+template <typename T, int V, int I, bool MANY>
+__global__ __launch_bounds__(1024) void ring_norm_bwd_kernel(RingNormArgs p, Lie l) {
+  __shared__ float room[64];
+  extern __shared__ float sums[];        // [threads][V]: rows of a workgroup are added up
+  const Spot<V, I, MANY> at(l);
+  const Lie whole = {at.threads, 1, l.rows, 0, 1};
+  int there[I], col[I];
+  float aw[I][V], as[I][V], an[I][V];
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    there[i] = at.here(l, i, p.group);
+    col[i] = at.column(l, i, p.group);
+#pragma unroll
+    for (int e = 0; e < V; ++e) aw[i][e] = as[i][e] = an[i][e] = 0.f;
+  }
+  for (long first = (long)blockIdx.x * l.rows; first < p.rows; first += (long)gridDim.x * l.rows) {
+    const long row = first + at.row;
+    const bool real = row < p.rows;
+    int here[I];
+    float unit[I][V], rstd[I], total[I][V];
+    Row<T, V> rx[I], rg[I], rr[I], rt[I], rn[I];
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      here[i] = real ? there[i] : 0;
+      rx[i].zero(), rg[i].zero(), rr[i].zero(), rt[i].zero(), rn[i].zero();
+      if (here[i] > 0) {
+        rx[i].load((const T*)p.x + row * p.xs + col[i], V > 1, here[i]);
+        if (p.gate) rg[i].load((const T*)p.gate + row * p.gs + col[i], V > 1, here[i]);
+        if (p.dy) rt[i].load((const T*)p.dy + row * p.dys + col[i], V > 1, here[i]);
+        if (p.dn) {
+          rn[i].load((const T*)p.dn + row * p.dns + col[i], V > 1, here[i]);
+          if (p.residual) rr[i].load((const T*)p.residual + row * p.rs + col[i], V > 1, here[i]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        unit[i][e] = (float)rx[i].v[e];
+        total[i][e] = (float)rt[i].v[e];
+      }
+    }
+    normalise<V, I, MANY>(unit, rstd, here, l, (float)p.group, p.layer, p.eps, room);
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) unit[i][e] *= rstd[i];
+    if (p.dn) {
+      float y[I][V], r2[I], s[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          y[i][e] = 0.f;
+          if (e < here[i]) {
+            y[i][e] = unit[i][e] * p.w[col[i] + e];
+            if (p.gate) y[i][e] *= act_of((float)rg[i].v[e], p.act);
+            if (p.scale) y[i][e] *= p.scale[col[i] + e];
+            if (p.residual) y[i][e] += (float)rr[i].v[e];
+          }
+        }
+      normalise<V, I, false>(y, r2, here, whole, (float)p.C, p.layer, p.eps, room);
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          y[i][e] *= r2[i];
+          const float g = e < here[i] ? (float)rn[i].v[e] * p.next[col[i] + e] : 0.f;
+          an[i][e] = fmaf((float)rn[i].v[e], y[i][e], an[i][e]);
+          s[0] = fmaf(g, y[i][e], s[0]);
+          s[1] += g;
+        }
+      add_up<2>(s, at.threads, room);
+      const float m1 = s[0] / (float)p.C, m0 = p.layer ? s[1] / (float)p.C : 0.f;
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (e < here[i]) total[i][e] += r2[i] * ((float)rn[i].v[e] * p.next[col[i] + e] - m0 - y[i][e] * m1);
+    }
+    float s1[I], s0[I];
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      Row<T, V> res, dg;
+      s1[i] = s0[i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        res.v[e] = (T)total[i][e];
+        float g = 0.f, back = 0.f;
+        if (e < here[i]) {
+          const float w = p.w[col[i] + e], a = p.gate ? act_of((float)rg[i].v[e], p.act) : 1.f, normed = unit[i][e] * w;
+          g = total[i][e];
+          as[i][e] = fmaf(g, normed * a, as[i][e]);
+          if (p.scale) g *= p.scale[col[i] + e];
+          back = p.gate ? g * normed * slope_of((float)rg[i].v[e], p.act) : 0.f;
+          g *= a;
+          aw[i][e] = fmaf(g, unit[i][e], aw[i][e]);
+          g *= w;
+        }
+        dg.v[e] = (T)back;
+        total[i][e] = g;
+        s1[i] = fmaf(g, unit[i][e], s1[i]);
+        s0[i] += g;
+      }
+      if (here[i] > 0) {
+        if (p.dresidual) res.store((T*)p.dresidual + row * p.C + col[i], V > 1, here[i]);
+        if (p.dgate) dg.store((T*)p.dgate + row * p.C + col[i], V > 1, here[i]);
+      }
+    }
+    if (!p.dx) continue;
+    group_sums<V, I, MANY>(s1, l, room);
+    if (p.layer) group_sums<V, I, MANY>(s0, l, room);
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+      if (here[i] > 0) {
+        Row<T, V> out;
+        const float m1 = s1[i] / (float)p.group, m0 = p.layer ? s0[i] / (float)p.group : 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) out.v[e] = (T)(rstd[i] * (total[i][e] - m0 - unit[i][e] * m1));
+        out.store((T*)p.dx + row * p.C + col[i], V > 1, here[i]);
+      }
+  }
+  if (!p.part) return;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    if (k == 1 && !p.dscale) continue;
+    if (k == 2 && !p.dnext) continue;
+    if (k == 0 && !p.dw) continue;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      float (&a)[V] = k == 0 ? aw[i] : (k == 1 ? as[i] : an[i]);
+      if (l.rows > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < V; ++e) sums[e * blockDim.x + threadIdx.x] = a[e];
+        __syncthreads();
+        if (at.row == 0)
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            for (int m = 1; m < l.rows; ++m) a[e] += sums[e * blockDim.x + m * at.threads + threadIdx.x];
+      }
+      if (at.row == 0)
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (e < there[i]) p.part[((size_t)blockIdx.x * 3 + k) * p.C + col[i] + e] = a[e];
+    }
+  }
+}
+
+// dw, dscale, dnext [C] from the workgroups' parts, in their order
+__global__ __launch_bounds__(256) void ring_norm_sum_kernel(RingNormArgs p) {
+  constexpr int W = 16, COLS = 256 / W;
+  __shared__ float sums[256];
+  const int k = blockIdx.y, c = blockIdx.x * COLS + threadIdx.x % COLS, w = threadIdx.x / COLS, each = (p.parts + W - 1) / W;
+  float* out = k == 0 ? p.dw : (k == 1 ? p.dscale : p.dnext);
+  if (!out) return;
+  float sum = 0.f;
+  if (c < p.C)
+#pragma unroll 4
+    for (int m = w * each; m < min(p.parts, (w + 1) * each); ++m) sum += p.part[((size_t)m * 3 + k) * p.C + c];
+  sums[threadIdx.x] = sum;
+  __syncthreads();
+  if (w > 0 || c >= p.C) return;
+  for (int m = 1; m < W; ++m) sum += sums[m * COLS + threadIdx.x];
+  out[c] = sum;
+}
+
+namespace {
+
+int pow2(int n) {
+  int p = 1;
+  while (p < n) p *= 2;
+  return p;
+}
+
+struct Plan { Lie lie; int V, I, threads; bool many; };
+
+// One unit a thread as long as 1024 threads are enough for that (units of 16 bytes: at most 2 or 4 each, of one value 16, for rows of 8192 whose groups fill
+// little more than half of their threads)
+Plan plan_of(int C, int group, int V) {
+  Plan a = {};
+  const int groups = C / group, units = (group + V - 1) / V;
+  a.V = V;
+  a.many = groups > 1 && units <= 64;
+  for (a.threads = 64; a.threads <= 1024; a.threads *= 2) {
+    a.lie = {0, 0, 1, units, groups};
+    if (a.many) {
+      a.lie.lanes = pow2(units);
+      a.lie.slots = a.threads / a.lie.lanes;
+      if (a.lie.slots > pow2(groups)) a.lie.slots = pow2(groups);
+      a.I = (groups + a.lie.slots - 1) / a.lie.slots;
+    } else {
+      a.lie.slots = pow2(groups);
+      a.lie.lanes = a.threads / a.lie.slots;
+      if (a.lie.lanes < 1) continue;
+      if (a.lie.lanes > pow2(units)) a.lie.lanes = pow2(units);
+      a.I = (units + a.lie.lanes - 1) / a.lie.lanes;
+    }
+    if (a.I == 1 || a.threads == 1024) break;
+  }
+  // several short rows a workgroup
+  const int row = a.lie.lanes * a.lie.slots;
+  if (row < 256) {
+    a.threads = 256;
+    a.lie.rows = 256 / row;
+  } else {
+    a.threads = row;
+  }
+  return a;
+}
+
+int parts_of(const Plan& a, long rows) {
+  const long wanted = (rows + a.lie.rows - 1) / a.lie.rows, most = 512 * 256 / a.threads;
+  return (int)(wanted < most ? wanted : most);
+}
+
+template <typename T, int V, int I, bool MANY> void launch_one(const RingNormArgs& p, const Plan& a, bool back, hipStream_t st) {
+  if (back) {
+    hipLaunchKernelGGL((ring_norm_bwd_kernel<T, V, I, MANY>), dim3((unsigned)p.parts), dim3(a.threads), a.threads * V * sizeof(float), st, p, a.lie);
+  } else {
+    const long blocks = (p.rows + a.lie.rows - 1) / a.lie.rows, row = blocks < (1 << 20) ? blocks : 1 << 20;      // (a launch counts fewer than 2^32 threads along x)
+    hipLaunchKernelGGL((ring_norm_fwd_kernel<T, V, I, MANY>), dim3((unsigned)row, (unsigned)((blocks + row - 1) / row)), dim3(a.threads), 0, st, p, a.lie);
+  }
+}
+
+template <typename T, int V, bool MANY> void launch_units(const RingNormArgs& p, const Plan& a, bool back, hipStream_t st) {
+  if (a.I == 1) launch_one<T, V, 1, MANY>(p, a, back, st);
+  else if constexpr (V == 8) launch_one<T, V, 2, MANY>(p, a, back, st);
+  else if constexpr (V == 4) {
+    if (a.I == 2) launch_one<T, V, 2, MANY>(p, a, back, st);
+    else launch_one<T, V, 4, MANY>(p, a, back, st);
+  } else {
+    if (a.I <= 4) launch_one<T, V, 4, MANY>(p, a, back, st);
+    else launch_one<T, V, 16, MANY>(p, a, back, st);
+  }
+}
+
+// 16 bytes at a time where rows, groups and addresses are whole numbers of that
+template <typename T> bool wide(const RingNormArgs& p) {
+  constexpr int V = 16 / sizeof(T);
+  const uintptr_t all = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.gate) | reinterpret_cast<uintptr_t>(p.residual) |
+                        reinterpret_cast<uintptr_t>(p.dy) | reinterpret_cast<uintptr_t>(p.dn);
+  return p.group % V == 0 && (all & 15) == 0 && (p.xs | p.gs | p.rs | p.dys | p.dns) % V == 0;
+}
+
+template <typename T> hipError_t launch(RingNormArgs p, bool back, hipStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool w = wide<T>(p);
+  const Plan a = plan_of(p.C, p.group, w ? V : 1);
+  if (back) p.parts = parts_of(a, p.rows);
+  if (w) {
+    if (a.many) launch_units<T, V, true>(p, a, back, st);
+    else launch_units<T, V, false>(p, a, back, st);
+  } else {
+    if (a.many) launch_units<T, 1, true>(p, a, back, st);
+    else launch_units<T, 1, false>(p, a, back, st);
+  }
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !back || !p.part) return e;
+  hipLaunchKernelGGL(ring_norm_sum_kernel, dim3((unsigned)((p.C + 15) / 16), 3), dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+
+hipError_t launch_type(const RingNormArgs& p, int type, bool back, hipStream_t st) {
+  if (type == RINGATTR_F32) return launch<float>(p, back, st);
+  if (type == RINGATTR_BF16) return launch<__bf16>(p, back, st);
+  return launch<_Float16>(p, back, st);
+}
+
+}  // namespace
+
+size_t ring_norm_bwd_bytes(int type, long rows, int C, int group, bool params) {
+  if (!params) return 0;
+  const int V = type == RINGATTR_F32 ? 4 : 8, a = group % V == 0 ? parts_of(plan_of(C, group, V), rows) : 0, b = parts_of(plan_of(C, group, 1), rows);
+  return (size_t)(a > b ? a : b) * 3 * C * sizeof(float);
+}
+
+hipError_t ring_norm_fwd(const RingNormArgs& p, int type, hipStream_t st) { return launch_type(p, type, false, st); }
+hipError_t ring_norm_bwd(RingNormArgs p, int type, hipStream_t st) { return launch_type(p, type, true, st); }

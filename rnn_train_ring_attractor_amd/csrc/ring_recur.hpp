@@ -1,0 +1,104 @@
+// What the kernels of the recurrent layer's operators (short convolution, selective scan, norm and gate) share: functions in fp32 and
+// rows of values read and written some at a time.
+#pragma once
+#include "ring_common.hpp"
+#include "ring_kernels.hpp"
+
+namespace ring_recur {
+
+constexpr float kLog2e = 1.44269504088896341f, kLog2eLow = 1.92596299e-8f, kLn2 = 0.693147180559945309f;
+
+// e^x for -126 <= x log2(e) <= 126: the power's argument as a sum of two numbers, the second to first order (2^x itself is off by a step)
+__device__ __forceinline__ float exp_of(float x) {
+  const float high = x * kLog2e, low = fmaf(x, kLog2eLow, fmaf(x, kLog2e, -high));
+  const float e = __builtin_amdgcn_exp2f(high);
+  return fmaf(e, low * kLn2, e);
+}
+
+// 1 / (1 + e^-x); NaN only through what it is multiplied by
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + exp_of(fminf(fmaxf(-x, -87.f), 87.f))); }
+__device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
+// the derivative of x sigmoid(x), s = sigmoid(x)
+__device__ __forceinline__ float silu_slope(float x, float s) { return s * fmaf(x, 1.f - s, 1.f); }
+
+// ln(1 + e^x) = max(x, 0) + ln(1 + e), e = e^-|x|; ln(1 + e) = 2 artanh(e / (2 + e)) by its series, the square of the argument at most 1/9
+__device__ __forceinline__ float softplus(float x) {
+  const float e = exp_of(fmaxf(-fabsf(x), -87.f)), s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
+  float r = 1.f / 15.f;
+  r = fmaf(r, q, 1.f / 13.f);
+  r = fmaf(r, q, 1.f / 11.f);
+  r = fmaf(r, q, 1.f / 9.f);
+  r = fmaf(r, q, 1.f / 7.f);
+  r = fmaf(r, q, 1.f / 5.f);
+  r = fmaf(r, q, 1.f / 3.f);
+  r = fmaf(r, q, 1.f);
+  const float y = fmaf(2.f * s, r, x > 0.f ? x : 0.f);
+  return x == x ? y : x;
+}
+
+// E values, neighbours in memory.  WIDE: the address is a whole number of min(16, E sizeof(T)) bytes; otherwise one by one, `here` of them.
+template <typename T, int E> struct Row {
+  typedef T vec __attribute__((ext_vector_type(E)));
+  T v[E];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = (T)0.f;
+  }
+  __device__ __forceinline__ void load(const T* p, bool wide, int here) {
+    constexpr int W = E * sizeof(T) > 16 ? 16 / sizeof(T) : E;
+    typedef T part __attribute__((ext_vector_type(W)));
+    if (wide) {
+      if (here >= E) {
+#pragma unroll
+        for (int i = 0; i < E / W; ++i) {
+          const part w = *reinterpret_cast<const part*>(p + i * W);
+#pragma unroll
+          for (int e = 0; e < W; ++e) v[i * W + e] = w[e];
+        }
+      } else {
+        zero();
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = e < here ? p[e] : (T)0.f;
+    }
+  }
+  __device__ __forceinline__ void store(T* p, bool wide, int here) const {
+    constexpr int W = E * sizeof(T) > 16 ? 16 / sizeof(T) : E;
+    typedef T part __attribute__((ext_vector_type(W)));
+    if (wide) {
+      if (here >= E) {
+#pragma unroll
+        for (int i = 0; i < E / W; ++i) {
+          part w;
+#pragma unroll
+          for (int e = 0; e < W; ++e) w[e] = v[i * W + e];
+          *reinterpret_cast<part*>(p + i * W) = w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e < here) p[e] = v[e];
+    }
+  }
+};
+
+// Sums across lanes.  Of a and b, the wave's halves (its odd and even rows of 16) added: a's sum in the lower half (even rows), b's in the other.
+__device__ __forceinline__ float fold32(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float fold16(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// the lane's value plus that of the lane CTRL names within a row of 16
+template <int CTRL> __device__ __forceinline__ float plus_dpp(float x) {
+  return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+constexpr int kRor8 = 0x128, kRor4 = 0x124, kXor1 = 0xB1, kXor2 = 0x4E;
+
+__device__ __forceinline__ int length_of(const int* lengths, int b, int T) { return lengths ? min(max(lengths[b], 0), T) : T; }
+
+}  // namespace ring_recur

@@ -1,0 +1,201 @@
+// Selective state space scan: the passes of a forward and of a backward, sums over parts, and the single token.
+#include "ring_recur.hpp"
+#include "ringattr.h"
+
+using namespace ring_recur;
+
+namespace {
+
+constexpr int kChunk = 32;            // segments are whole numbers of these tokens
+
+size_t round_up(size_t x) { return (x + 255) / 256 * 256; }
+int padded(int N) { return N <= 4 ? 4 : (N <= 8 ? 8 : (N <= 16 ? 16 : (N <= 32 ? 32 : 64))); }
+int tile(int N) { return N <= 16 ? 64 : (N <= 32 ? 32 : 16); }        // channels of a workgroup
+int tiles_of(const RingScanShape& s) { return (s.C / s.G + tile(s.N) - 1) / tile(s.N); }
+int saved_of(const RingScanShape& s) { return (s.T + RingScanArgs::kSave - 1) / RingScanArgs::kSave; }
+
+// Segments that the tokens are cut into, so that every compute unit has work
+int segments(const RingScanShape& s, int wanted) {
+  const long groups = (long)tiles_of(s) * s.G * s.B;
+  const int units = (s.T + kChunk - 1) / kChunk;
+  long n = (wanted + groups - 1) / groups;
+  if (n > units / 2) n = units / 2;
+  if (n < 1) n = 1;
+  const int per = (int)((units + n - 1) / n);
+  return (units + per - 1) / per;
+}
+int fwd_segments(const RingScanShape& s) { return segments(s, 256); }
+int bwd_segments(const RingScanShape& s) { return segments(s, 256); }
+
+size_t seg_bytes(const RingScanShape& s, int nseg) {
+  const size_t rows = (size_t)(nseg - 1) * s.B * s.C;
+  return round_up(rows * padded(s.N) * sizeof(float)) + round_up(rows * sizeof(float));
+}
+size_t shared_bytes(const RingScanShape& s) {
+  return round_up((size_t)tiles_of(s) * s.B * s.T * s.G * 2 * padded(s.N) * sizeof(float));
+}
+
+void set_segments(RingScanArgs& a, const RingScanShape& s, int nseg, void* ws) {
+  const int units = (s.T + kChunk - 1) / kChunk;
+  a.nseg = nseg;
+  a.seg_tokens = (units + nseg - 1) / nseg * kChunk;
+  a.saved = saved_of(s);
+  a.seg = (float*)ws;
+  a.total = (float*)((char*)ws + round_up((size_t)(nseg - 1) * s.B * s.C * padded(s.N) * sizeof(float)));
+}
+
+hipError_t launch_pass(int type, const RingScanArgs& a, int mode, hipStream_t st) {
+  if (type == RINGATTR_F32) return ring_launch_scan_f32(a, mode, st);
+  if (type == RINGATTR_BF16) return ring_launch_scan_bf16(a, mode, st);
+  return ring_launch_scan_f16(a, mode, st);
+}
+
+}  // namespace
+
+// What the segments add to a state of zeros becomes the states behind them, in place; a segment's whole decay is the power of its sum of d.
+// A thread walks one state through them.
+__global__ __launch_bounds__(256) void ring_scan_between_kernel(float* seg, const float* total, const float* A, const float* s_in, int B, int C, int N,
+                                                                int NS, int ns) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, rows = (size_t)B * C;
+  if (i >= rows * NS) return;
+  const size_t row = i / NS;
+  const int n = (int)(i - row * NS), c = (int)(row % C);
+  const float A2 = n < N ? (float)((double)A[(size_t)c * N + n] * 1.4426950408889634) : 0.f;
+  float run = s_in && n < N ? s_in[row * N + n] : 0.f;
+#pragma unroll 4
+  for (int u = 0; u < ns; ++u) {
+    const float local = seg[u * rows * NS + i], d = total[u * rows + row];
+    run = fmaf(__builtin_amdgcn_exp2f(d * A2), run, local);
+    seg[u * rows * NS + i] = run;
+  }
+}
+
+static hipError_t between(const RingScanShape& s, RingScanArgs a, int mode, hipStream_t st) {
+  if (a.nseg == 1) return hipSuccess;
+  hipError_t e = launch_pass(s.type, a, mode, st);
+  if (e != hipSuccess) return e;
+  const size_t n = (size_t)s.B * s.C * padded(s.N);
+  hipLaunchKernelGGL(ring_scan_between_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a.seg, a.total, a.A, a.s_in, s.B, s.C, s.N,
+                     padded(s.N), a.nseg - 1);
+  return hipGetLastError();
+}
+
+size_t ring_scan_states_bytes(const RingScanShape& s) { return round_up((size_t)s.B * saved_of(s) * s.C * padded(s.N) * sizeof(float)); }
+size_t ring_scan_fwd_bytes(const RingScanShape& s) { return seg_bytes(s, fwd_segments(s)); }
+size_t ring_scan_bwd_bytes(const RingScanShape& s, bool shared, bool params) {
+  const int nseg = bwd_segments(s);
+  return seg_bytes(s, nseg) + (shared ? shared_bytes(s) : 0) +
+         (params ? round_up((size_t)nseg * s.B * s.C * (padded(s.N) + 2) * sizeof(float)) : 0);
+}
+
+hipError_t ring_scan_fwd(const RingScanShape& s, RingScanArgs a, void* ws, hipStream_t st) {
+  set_segments(a, s, fwd_segments(s), ws);
+  hipError_t e = between(s, a, RING_SCAN_STATE, st);
+  return e == hipSuccess ? launch_pass(s.type, a, RING_SCAN_OUTPUTS, st) : e;
+}
+
+// dB and dC [B,T,G,N] from the sums over the tiles of a group's channels, in their order; rows that do not count are zero
+template <typename T>
+__global__ __launch_bounds__(256) void ring_scan_share_kernel(const float* __restrict__ part, T* dB, T* dC, const int* lengths, int tiles, int B, int Tn, int G,
+                                                              int N, int NS) {
+  const size_t rows = (size_t)B * Tn * G, all = rows * 2 * NS;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
+    const size_t row = i / (2 * NS);
+    const int k = (int)(i - row * 2 * NS), n = k % NS;
+    T* out = k < NS ? dB : dC;
+    if (n >= N || !out) continue;
+    const int b = (int)(row / ((size_t)Tn * G)), t = (int)(row / G % Tn);
+    float sum = 0.f;
+    if (t < length_of(lengths, b, Tn))
+#pragma unroll 4
+      for (int m = 0; m < tiles; ++m) sum += part[m * all + i];
+    out[row * N + n] = (T)sum;
+  }
+}
+
+template <typename T> static void launch_share(const RingScanShape& s, const RingScanArgs& a, const RingScanGrads& g, hipStream_t st) {
+  const size_t blocks = ((size_t)s.B * s.T * s.G * 2 * padded(s.N) + 255) / 256;
+  hipLaunchKernelGGL(ring_scan_share_kernel<T>, dim3((unsigned)(blocks < (1 << 22) ? blocks : 1 << 22)), dim3(256), 0, st, a.part_bc, (T*)g.B, (T*)g.C, a.lengths,
+                     tiles_of(s), s.B, s.T, s.G, s.N, padded(s.N));
+}
+
+hipError_t ring_scan_bwd(const RingScanShape& s, RingScanArgs a, const RingScanGrads& g, void* ws, hipStream_t st) {
+  const int nseg = bwd_segments(s);
+  set_segments(a, s, nseg, ws);
+  char* at = (char*)ws + seg_bytes(s, nseg);
+  if (g.B || g.C) {
+    a.part_bc = (float*)at;
+    at += shared_bytes(s);
+  }
+  if (g.A || g.D || g.bias) a.part_a = (float*)at;
+  hipError_t e = between(s, a, RING_SCAN_ADJOINT, st);
+  if (e == hipSuccess) e = launch_pass(s.type, a, RING_SCAN_GRADIENTS, st);
+  if (e != hipSuccess) return e;
+  if (a.part_bc) {
+    if (s.type == RINGATTR_F32) launch_share<float>(s, a, g, st);
+    else if (s.type == RINGATTR_BF16) launch_share<__bf16>(s, a, g, st);
+    else launch_share<_Float16>(s, a, g, st);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  if (!a.part_a) return hipSuccess;
+  const int per = padded(s.N) + 2;
+  return ring_launch_sum_parts(RingSumArgs{a.part_a, nseg * s.B, per, s.N, 2, (size_t)s.C * per, g.A, {g.D, g.bias}}, st);
+}
+
+// A single token.  A lane takes V states of a channel, `lanes` of them a channel; bound by the states, read and written once.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void ring_scan_step_kernel(RingScanStep p, RingScanShape s, int lanes) {
+  typedef float vec __attribute__((ext_vector_type(V)));
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, row = i / lanes;
+  const int n = (int)(i - row * lanes) * V;
+  if (row >= (size_t)s.B * s.C) return;          // (whole channels: a channel's lanes go together)
+  const int b = (int)(row / s.C), c = (int)(row - (size_t)b * s.C), g = c / (s.C / s.G);
+  T* out = (T*)p.y + row;
+  if (p.active && !p.active[b]) {
+    if (n == 0) *out = (T)0.f;
+    return;
+  }
+  const float x = (float)((const T*)p.x)[b * p.xs + c];
+  float d = (float)((const T*)p.delta)[b * p.ds + c];
+  if (p.bias) d += p.bias[c];
+  if (p.softplus) d = softplus(d);
+  float y = 0.f;
+  if (n < s.N) {
+    vec* at = reinterpret_cast<vec*>(p.state + row * s.N + n);
+    const vec A = *reinterpret_cast<const vec*>(p.A + (size_t)c * s.N + n);
+    const T* B = (const T*)p.Bm + b * p.bsb + g * p.bsg + n;
+    const T* C = (const T*)p.Cm + b * p.csb + g * p.csg + n;
+    vec h = *at;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      // (the power as the sequences' kernels form it)
+      h[e] = fmaf(__builtin_amdgcn_exp2f(d * (float)((double)A[e] * 1.4426950408889634)), h[e], d * x * (float)B[e]);
+      y = fmaf(h[e], (float)C[e], y);
+    }
+    *at = h;
+  }
+  for (int half = lanes / 2; half > 0; half /= 2) y += __shfl_xor(y, half);
+  if (n == 0) {
+    if (p.D) y = fmaf(p.D[c], x, y);
+    if (p.z) y *= silu((float)((const T*)p.z)[b * p.zs + c]);
+    *out = (T)y;
+  }
+}
+
+template <typename T> static hipError_t launch_step(const RingScanShape& s, const RingScanStep& a, hipStream_t st) {
+  const bool vec = s.N % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.state) | reinterpret_cast<uintptr_t>(a.A)) & 15) == 0;
+  const int width = vec ? s.N / 4 : s.N;
+  int lanes = 1;
+  while (lanes < width) lanes *= 2;
+  const size_t threads = (size_t)s.B * s.C * lanes;
+  const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
+  if (vec) hipLaunchKernelGGL((ring_scan_step_kernel<T, 4>), grid, block, 0, st, a, s, lanes);
+  else hipLaunchKernelGGL((ring_scan_step_kernel<T, 1>), grid, block, 0, st, a, s, lanes);
+  return hipGetLastError();
+}
+
+hipError_t ring_scan_step(const RingScanShape& s, const RingScanStep& a, hipStream_t st) {
+  if (s.type == RINGATTR_F32) return launch_step<float>(s, a, st);
+  if (s.type == RINGATTR_BF16) return launch_step<__bf16>(s, a, st);
+  return launch_step<_Float16>(s, a, st);
+}

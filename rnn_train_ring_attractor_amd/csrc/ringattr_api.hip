@@ -1088,6 +1088,365 @@ int ringattr_dropout(const void* x, const void* residual, void* y, size_t n, uns
   return RINGATTR_OK;
 }
 
+// ---- a recurrent layer's operators ----
+
+static bool known_activation(const char* who, int act, int most) {
+  if (act >= RINGATTR_ACT_NONE && act <= most) return true;
+  fail(RINGATTR_ERR_INVALID, "%s: activation %d is not one of 0 none, 1 silu%s", who, act, most > 1 ? ", 2 sigmoid" : "");
+  return false;
+}
+
+// Workgroups are counted in one launch dimension and rows within a tensor in 64 bits.
+static bool rows_shape(const char* who, int type, int B, int T, int C) {
+  if (!known_type(who, type)) return false;
+  if (B <= 0 || T <= 0 || C <= 0) {
+    fail(RINGATTR_ERR_INVALID, "%s: batch_size, seq_len, channels must be positive (got %d, %d, %d)", who, B, T, C);
+    return false;
+  }
+  if (B > (1 << 20) || C > (1 << 20) || (double)B * C > 1.6e7 || T > (1 << 30)) {
+    fail(RINGATTR_ERR_INVALID, "%s: batch_size and channels up to 2^20, their product up to 16000000, seq_len up to 2^30 (got %d, %d, %d)", who, B, C, T);
+    return false;
+  }
+  return true;
+}
+
+// Whether rows of channels can be read (or written) 16 bytes at a time; `per` channels are what belongs together.
+static bool rows_wide(const void* p, const long long* strides, int per, int unit) {
+  return !p || (per % unit == 0 && aligned16(p) && (!strides || (strides[0] % unit == 0 && strides[1] % unit == 0)));
+}
+
+static RingRows rows_of_channels(const void* p, const long long* strides) { return RingRows{p, (long)strides[0], (long)strides[1]}; }
+
+static bool conv_shape(const char* who, int act, int type, int B, int T, int C, int K) {
+  if (!known_activation(who, act, RINGATTR_ACT_SILU) || !rows_shape(who, type, B, T, C)) return false;
+  if (K < 1 || K > RINGATTR_CONV_MAX_TAPS) {
+    fail(RINGATTR_ERR_INVALID, "%s: taps between 1 and %d (got %d)", who, RINGATTR_CONV_MAX_TAPS, K);
+    return false;
+  }
+  return true;
+}
+
+size_t ringattr_causal_conv_bwd_workspace_bytes(int type, int batch_size, int seq_len, int channels, int taps, int weights) {
+  if (!conv_shape("ringattr_causal_conv", RINGATTR_ACT_NONE, type, batch_size, seq_len, channels, taps)) return 0;
+  return ring_conv_bwd_bytes(type, batch_size, seq_len, channels, taps, weights != 0);
+}
+
+int ringattr_causal_conv_fwd(const void* x, const long long* strides, const void* weight, const void* bias, const void* initial_state,
+                             const void* lengths, void* y, void* final_state, int activation, int type, int batch_size, int seq_len,
+                             int channels, int taps, void* stream) {
+  const char* who = "ringattr_causal_conv_fwd";
+  if (!conv_shape(who, activation, type, batch_size, seq_len, channels, taps)) return RINGATTR_ERR_INVALID;
+  if (!x || !strides || !weight || !y) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  if (!aligned16(y) || !aligned16(final_state)) return fail(RINGATTR_ERR_INVALID, "%s: outputs must be 16-byte aligned", who);
+  const int unit = type == RINGATTR_F32 ? 4 : 8;
+  RingConvArgs p = {};
+  p.x = rows_of_channels(x, strides);
+  p.w = (const float*)weight;
+  p.bias = (const float*)bias;
+  p.start = taps > 1 ? initial_state : nullptr;
+  p.lengths = (const int*)lengths;
+  p.y = y;
+  p.end = taps > 1 ? final_state : nullptr;
+  p.B = batch_size;
+  p.T = seq_len;
+  p.C = channels;
+  p.K = taps;
+  p.act = activation;
+  p.wide = rows_wide(x, strides, channels, unit);
+  p.wide_state = rows_wide(p.start, nullptr, channels, unit);
+  p.wide_out = channels % unit == 0;
+  hipError_t e = ring_conv_fwd(p, type, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "causal convolution forward launch");
+  return RINGATTR_OK;
+}
+
+int ringattr_causal_conv_bwd(const void* x, const void* grad_y, const long long* strides, const void* weight, const void* bias,
+                             const void* initial_state, const void* lengths, const void* grad_final_state, void* grad_x, void* grad_weight,
+                             void* grad_bias, void* grad_initial_state, int activation, int type, int batch_size, int seq_len, int channels,
+                             int taps, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "ringattr_causal_conv_bwd";
+  if (!conv_shape(who, activation, type, batch_size, seq_len, channels, taps)) return RINGATTR_ERR_INVALID;
+  if (!x || !grad_y || !strides || !weight) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  if (!aligned16(grad_x) || !aligned16(grad_initial_state) || !aligned16(workspace))
+    return fail(RINGATTR_ERR_INVALID, "%s: outputs and workspace must be 16-byte aligned", who);
+  const bool weights = grad_weight || grad_bias;
+  const size_t need = ring_conv_bwd_bytes(type, batch_size, seq_len, channels, taps, weights);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(RINGATTR_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
+  const int unit = type == RINGATTR_F32 ? 4 : 8;
+  RingConvArgs p = {};
+  p.x = rows_of_channels(x, strides);
+  p.dy = rows_of_channels(grad_y, strides + 2);
+  p.w = (const float*)weight;
+  p.bias = (const float*)bias;
+  p.start = taps > 1 ? initial_state : nullptr;
+  p.dend = taps > 1 ? grad_final_state : nullptr;
+  p.lengths = (const int*)lengths;
+  p.dx = grad_x;
+  p.dstart = taps > 1 ? grad_initial_state : nullptr;
+  p.dw = (float*)grad_weight;
+  p.dbias = (float*)grad_bias;
+  p.part = weights ? (float*)workspace : nullptr;
+  p.B = batch_size;
+  p.T = seq_len;
+  p.C = channels;
+  p.K = taps;
+  p.act = activation;
+  p.wide = rows_wide(x, strides, channels, unit) && rows_wide(grad_y, strides + 2, channels, unit);
+  p.wide_state = rows_wide(p.start, nullptr, channels, unit) && rows_wide(p.dend, nullptr, channels, unit);
+  p.wide_out = channels % unit == 0;
+  hipError_t e = ring_conv_bwd(p, type, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "causal convolution backward launch");
+  return RINGATTR_OK;
+}
+
+int ringattr_causal_conv_step(const void* x, long long stride, const void* weight, const void* bias, void* state, const void* active, void* y,
+                              int activation, int type, int batch_size, int channels, int taps, void* stream) {
+  const char* who = "ringattr_causal_conv_step";
+  if (!conv_shape(who, activation, type, batch_size, 1, channels, taps)) return RINGATTR_ERR_INVALID;
+  if (!x || !weight || (!state && taps > 1) || !y) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  RingConvStep p = {x, (long)stride, (const float*)weight, (const float*)bias, state, y, (const unsigned char*)active, batch_size, channels, taps,
+                    activation};
+  hipError_t e = ring_conv_step(p, type, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "causal convolution step launch");
+  return RINGATTR_OK;
+}
+
+static bool scan_shape(const char* who, int type, int B, int T, int C, int N, int G, RingScanShape& s) {
+  if (!rows_shape(who, type, B, T, C)) return false;
+  if (N < 1 || N > RINGATTR_SCAN_MAX_STATES) {
+    fail(RINGATTR_ERR_INVALID, "%s: states between 1 and %d (got %d)", who, RINGATTR_SCAN_MAX_STATES, N);
+    return false;
+  }
+  if (G < 1 || C % G != 0) {
+    fail(RINGATTR_ERR_INVALID, "%s: channels (%d) must be a multiple of groups (%d)", who, C, G);
+    return false;
+  }
+  s = RingScanShape{B, T, C, N, G, type};
+  return true;
+}
+
+size_t ringattr_selective_scan_states_bytes(int type, int batch_size, int seq_len, int channels, int states, int groups) {
+  RingScanShape s;
+  return scan_shape("ringattr_selective_scan", type, batch_size, seq_len, channels, states, groups, s) ? ring_scan_states_bytes(s) : 0;
+}
+
+size_t ringattr_selective_scan_fwd_workspace_bytes(int type, int batch_size, int seq_len, int channels, int states, int groups) {
+  RingScanShape s;
+  return scan_shape("ringattr_selective_scan", type, batch_size, seq_len, channels, states, groups, s) ? ring_scan_fwd_bytes(s) : 0;
+}
+
+size_t ringattr_selective_scan_bwd_workspace_bytes(int type, int batch_size, int seq_len, int channels, int states, int groups, int shared,
+                                                   int parameters) {
+  RingScanShape s;
+  if (!scan_shape("ringattr_selective_scan", type, batch_size, seq_len, channels, states, groups, s)) return 0;
+  return ring_scan_bwd_bytes(s, shared != 0, parameters != 0);
+}
+
+// What both directions read: x, delta, z (or null), B, C with their strides in that order.
+static RingScanArgs scan_args(const RingScanShape& s, const void* x, const void* delta, const void* z, const void* B, const void* C,
+                              const long long* st, const void* A, const void* D, const void* bias, const void* lengths, int softplus) {
+  RingScanArgs a = {};
+  a.x = rows_of_channels(x, st);
+  a.delta = rows_of_channels(delta, st + 2);
+  a.z = rows_of_channels(z, st + 4);
+  a.Bm = B;
+  a.Cm = C;
+  a.bsb = (long)st[6];
+  a.bst = (long)st[7];
+  a.bsg = (long)st[8];
+  a.csb = (long)st[9];
+  a.cst = (long)st[10];
+  a.csg = (long)st[11];
+  a.A = (const float*)A;
+  a.D = (const float*)D;
+  a.bias = (const float*)bias;
+  a.lengths = (const int*)lengths;
+  a.B = s.B;
+  a.T = s.T;
+  a.C = s.C;
+  a.N = s.N;
+  a.G = s.G;
+  a.softplus = softplus ? 1 : 0;
+  const int per = s.C / s.G;
+  a.wide = rows_wide(x, st, per, 8) && rows_wide(delta, st + 2, per, 8) && rows_wide(z, st + 4, per, 8);
+  a.wide_out = per % 8 == 0;
+  return a;
+}
+
+int ringattr_selective_scan_fwd(const void* x, const void* delta, const void* z, const void* B, const void* C, const long long* strides,
+                                const void* A, const void* D, const void* delta_bias, const void* initial_state, const void* lengths, void* y,
+                                void* final_state, void* states_kept, int softplus, int type, int batch_size, int seq_len, int channels,
+                                int states, int groups, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "ringattr_selective_scan_fwd";
+  RingScanShape s;
+  if (!scan_shape(who, type, batch_size, seq_len, channels, states, groups, s)) return RINGATTR_ERR_INVALID;
+  if (!x || !delta || !B || !C || !strides || !A || !y) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  if (!aligned16(y) || !aligned16(final_state) || !aligned16(states_kept) || !aligned16(workspace))
+    return fail(RINGATTR_ERR_INVALID, "%s: outputs and workspace must be 16-byte aligned", who);
+  const size_t need = ring_scan_fwd_bytes(s);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(RINGATTR_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
+  RingScanArgs a = scan_args(s, x, delta, z, B, C, strides, A, D, delta_bias, lengths, softplus);
+  a.s_in = (const float*)initial_state;
+  a.s_out = (float*)final_state;
+  a.y = y;
+  a.states = (float*)states_kept;
+  hipError_t e = ring_scan_fwd(s, a, workspace, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "selective scan forward launch");
+  return RINGATTR_OK;
+}
+
+int ringattr_selective_scan_bwd(const void* x, const void* delta, const void* z, const void* B, const void* C, const void* grad_y,
+                                const long long* strides, const void* A, const void* D, const void* delta_bias, const void* lengths,
+                                const void* states_kept, const void* grad_final_state, void* grad_x, void* grad_delta, void* grad_z, void* grad_B,
+                                void* grad_C, void* grad_A, void* grad_D, void* grad_delta_bias, void* grad_initial_state, int softplus,
+                                int type, int batch_size, int seq_len, int channels, int states, int groups, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  const char* who = "ringattr_selective_scan_bwd";
+  RingScanShape s;
+  if (!scan_shape(who, type, batch_size, seq_len, channels, states, groups, s)) return RINGATTR_ERR_INVALID;
+  if (!x || !delta || !B || !C || !grad_y || !strides || !A || !states_kept) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  if (grad_z && !z) return fail(RINGATTR_ERR_INVALID, "%s: grad_z without z", who);
+  if (!aligned16(grad_x) || !aligned16(grad_delta) || !aligned16(grad_z) || !aligned16(grad_initial_state) || !aligned16(states_kept) || !aligned16(workspace))
+    return fail(RINGATTR_ERR_INVALID, "%s: outputs, kept states and workspace must be 16-byte aligned", who);
+  const size_t need = ring_scan_bwd_bytes(s, grad_B || grad_C, grad_A || grad_D || grad_delta_bias);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(RINGATTR_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
+  RingScanArgs a = scan_args(s, x, delta, z, B, C, strides, A, D, delta_bias, lengths, softplus);
+  a.dy = rows_of_channels(grad_y, strides + 12);
+  a.wide = a.wide && rows_wide(grad_y, strides + 12, channels / groups, 8);
+  a.states = (float*)const_cast<void*>(states_kept);
+  a.s_in = (const float*)grad_final_state;
+  a.s_out = (float*)grad_initial_state;
+  a.dx = grad_x;
+  a.ddelta = grad_delta;
+  a.dz = grad_z;
+  hipError_t e = ring_scan_bwd(s, a, RingScanGrads{grad_B, grad_C, (float*)grad_A, (float*)grad_D, (float*)grad_delta_bias}, workspace,
+                               static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "selective scan backward launch");
+  return RINGATTR_OK;
+}
+
+int ringattr_selective_scan_step(const void* x, const void* delta, const void* z, const void* B, const void* C, const long long* strides,
+                                 const void* A, const void* D, const void* delta_bias, void* state, const void* active, void* y, int softplus,
+                                 int type, int batch_size, int channels, int states, int groups, void* stream) {
+  const char* who = "ringattr_selective_scan_step";
+  RingScanShape s;
+  if (!scan_shape(who, type, batch_size, 1, channels, states, groups, s)) return RINGATTR_ERR_INVALID;
+  if (!x || !delta || !B || !C || !strides || !A || !state || !y) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  RingScanStep a = {};
+  a.x = x;
+  a.delta = delta;
+  a.z = z;
+  a.Bm = B;
+  a.Cm = C;
+  a.xs = (long)strides[0];
+  a.ds = (long)strides[1];
+  a.zs = (long)strides[2];
+  a.bsb = (long)strides[3];
+  a.bsg = (long)strides[4];
+  a.csb = (long)strides[5];
+  a.csg = (long)strides[6];
+  a.A = (const float*)A;
+  a.D = (const float*)D;
+  a.bias = (const float*)delta_bias;
+  a.state = (float*)state;
+  a.active = (const unsigned char*)active;
+  a.y = y;
+  a.softplus = softplus ? 1 : 0;
+  hipError_t e = ring_scan_step(s, a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "selective scan step launch");
+  return RINGATTR_OK;
+}
+
+static bool norm_shape(const char* who, int act, int type, size_t rows, int C, int group) {
+  if (!known_type(who, type) || !known_activation(who, act, RINGATTR_ACT_SIGMOID)) return false;
+  if (rows < 1 || rows > ((size_t)1 << 32) || C < 1 || C > RINGATTR_NORM_MAX_CHANNELS) {
+    fail(RINGATTR_ERR_INVALID, "%s: between 1 and 2^32 rows of 1 to %d channels (got %zu of %d)", who, RINGATTR_NORM_MAX_CHANNELS, rows, C);
+    return false;
+  }
+  if (group < 1 || C % group != 0) {
+    fail(RINGATTR_ERR_INVALID, "%s: channels (%d) must be a multiple of group (%d)", who, C, group);
+    return false;
+  }
+  return true;
+}
+
+size_t ringattr_norm_gate_bwd_workspace_bytes(int type, size_t rows, int channels, int group, int weights) {
+  if (!norm_shape("ringattr_norm_gate", RINGATTR_ACT_NONE, type, rows, channels, group)) return 0;
+  return ring_norm_bwd_bytes(type, (long)rows, channels, group, weights != 0);
+}
+
+static RingNormArgs norm_args(const void* x, const void* gate, const void* residual, const long long* st, const void* weight, const void* scale,
+                              const void* next_weight, float eps, int layer, int act, size_t rows, int C, int group) {
+  RingNormArgs p = {};
+  p.x = x;
+  p.gate = gate;
+  p.residual = residual;
+  p.xs = (long)st[0];
+  p.gs = gate ? (long)st[1] : 0;
+  p.rs = residual ? (long)st[2] : 0;
+  p.w = (const float*)weight;
+  p.scale = (const float*)scale;
+  p.next = (const float*)next_weight;
+  p.rows = (long)rows;
+  p.C = C;
+  p.group = group;
+  p.layer = layer ? 1 : 0;
+  p.act = act;
+  p.eps = eps;
+  return p;
+}
+
+int ringattr_norm_gate_fwd(const void* x, const void* gate, const void* residual, const long long* strides, const void* weight,
+                           const void* scale, const void* next_weight, void* y, void* n, float eps, int layer, int activation, int type,
+                           size_t rows, int channels, int group, void* stream) {
+  const char* who = "ringattr_norm_gate_fwd";
+  if (!norm_shape(who, activation, type, rows, channels, group)) return RINGATTR_ERR_INVALID;
+  if (!x || !strides || !weight || !y || (next_weight && !n)) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  if (!aligned16(y) || !aligned16(n)) return fail(RINGATTR_ERR_INVALID, "%s: outputs must be 16-byte aligned", who);
+  RingNormArgs p = norm_args(x, gate, residual, strides, weight, scale, next_weight, eps, layer, activation, rows, channels, group);
+  p.y = y;
+  p.n = n;
+  hipError_t e = ring_norm_fwd(p, type, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "norm and gate forward launch");
+  return RINGATTR_OK;
+}
+
+int ringattr_norm_gate_bwd(const void* x, const void* gate, const void* residual, const void* grad_y, const void* grad_n,
+                           const long long* strides, const void* weight, const void* scale, const void* next_weight, void* grad_x,
+                           void* grad_gate, void* grad_residual, void* grad_weight, void* grad_scale, void* grad_next_weight, float eps,
+                           int layer, int activation, int type, size_t rows, int channels, int group, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  const char* who = "ringattr_norm_gate_bwd";
+  if (!norm_shape(who, activation, type, rows, channels, group)) return RINGATTR_ERR_INVALID;
+  if (!x || !strides || !weight || (!grad_y && !grad_n)) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
+  if ((grad_n && !next_weight) || (grad_gate && !gate) || (grad_scale && !scale) || (grad_next_weight && !grad_n))
+    return fail(RINGATTR_ERR_INVALID, "%s: the gradient of a tensor that is null", who);
+  if (!aligned16(grad_x) || !aligned16(grad_gate) || !aligned16(grad_residual) || !aligned16(workspace))
+    return fail(RINGATTR_ERR_INVALID, "%s: outputs and workspace must be 16-byte aligned", who);
+  const bool weights = grad_weight || grad_scale || grad_next_weight;
+  const size_t need = ring_norm_bwd_bytes(type, (long)rows, channels, group, weights);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(RINGATTR_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
+  RingNormArgs p = norm_args(x, gate, residual, strides, weight, scale, next_weight, eps, layer, activation, rows, channels, group);
+  p.dy = grad_y;
+  p.dn = grad_n;
+  p.dys = grad_y ? (long)strides[3] : 0;
+  p.dns = grad_n ? (long)strides[4] : 0;
+  p.dx = grad_x;
+  p.dgate = grad_gate;
+  p.dresidual = grad_residual;
+  p.dw = (float*)grad_weight;
+  p.dscale = (float*)grad_scale;
+  p.dnext = (float*)grad_next_weight;
+  p.part = weights ? (float*)workspace : nullptr;
+  hipError_t e = ring_norm_bwd(p, type, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "norm and gate backward launch");
+  return RINGATTR_OK;
+}
+
 int ringattr_profile_enable(int on) {
   ring_profile_set(on);
   return RINGATTR_OK;
