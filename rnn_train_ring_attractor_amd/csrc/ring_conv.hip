@@ -10,12 +10,13 @@
 #include "ring_recur.hpp"
 #include "ringattr.h"
 
+#include <type_traits>
+
 using namespace ring_recur;
 
 namespace {
 
 enum { kIdentity = 0, kSilu = 1 };
-constexpr int U = 4;                  // tokens at a time
 
 struct Piece { int b, seg, c, first, last, sub; bool mine; };
 
@@ -32,18 +33,21 @@ template <int E> __device__ __forceinline__ Piece piece(const RingConvArgs& p, i
 
 }  // namespace
 
+// (E > 1: rows are whole numbers of E channels, which are all there)
+template <int E> constexpr bool kWide = E > 1;
+
 // KT taps are built for; K < KT (only where KT = 8): the first KT - K are left out
-template <typename T, int E, int KT>
+template <typename T, int E, int KT, int U>      // U tokens at a time
 __global__ __launch_bounds__(256) void ring_conv_fwd_kernel(RingConvArgs p, int tx, int blocks) {
   const Piece a = piece<E>(p, tx, blocks);
   if (!a.mine) return;
-  const int K = KT == 8 ? p.K : KT, skip = KT - K, here = p.C - a.c, len = length_of(p.lengths, a.b, p.T), end = min(a.last, len);
+  const int K = KT == 8 ? p.K : KT, skip = KT - K, len = length_of(p.lengths, a.b, p.T), end = min(a.last, len);
   float w[KT][E], bias[E], win[KT - 1 + U][E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    bias[e] = p.bias && e < here ? p.bias[a.c + e] : 0.f;
+    bias[e] = p.bias && a.mine ? p.bias[a.c + e] : 0.f;
 #pragma unroll
-    for (int k = 0; k < KT; ++k) w[k][e] = k >= skip && e < here ? p.w[(size_t)(a.c + e) * K + k - skip] : 0.f;
+    for (int k = 0; k < KT; ++k) w[k][e] = k >= skip && a.mine ? p.w[(size_t)(a.c + e) * K + k - skip] : 0.f;
   }
   const T* const x = (const T*)p.x.p + a.b * p.x.sb + a.c;
   const T* const start = p.start ? (const T*)p.start + (size_t)a.b * (K - 1) * p.C + a.c : nullptr;
@@ -51,12 +55,12 @@ __global__ __launch_bounds__(256) void ring_conv_fwd_kernel(RingConvArgs p, int 
   auto input = [&](int t) {              // x at t, or the state's where that is in front of the sequence
     Row<T, E> r;
     r.zero();
-    if (t >= 0) r.load(x + t * p.x.st, p.wide, here);
-    else if (start && t >= -(K - 1)) r.load(start + (size_t)(t + K - 1) * p.C, p.wide_state, here);
+    if (t >= 0) r.load(x + t * p.x.st, kWide<E>, E);
+    else if (start && t >= -(K - 1)) r.load(start + (size_t)(t + K - 1) * p.C, kWide<E>, E);
     return r;
   };
   if (a.seg == 0 && a.sub == 0 && p.end)
-    for (int j = 0; j < K - 1; ++j) input(len - (K - 1) + j).store((T*)p.end + ((size_t)a.b * (K - 1) + j) * p.C + a.c, p.wide_out, here);
+    for (int j = 0; j < K - 1; ++j) input(len - (K - 1) + j).store((T*)p.end + ((size_t)a.b * (K - 1) + j) * p.C + a.c, kWide<E>, E);
   if (a.first < end) {
 #pragma unroll
     for (int j = 0; j < KT - 1; ++j) {
@@ -68,53 +72,71 @@ __global__ __launch_bounds__(256) void ring_conv_fwd_kernel(RingConvArgs p, int 
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       next[i].zero();
-      if (a.first + i < end) next[i].load(x + (a.first + i) * p.x.st, p.wide, here);
+      if (a.first + i < end) next[i].load(x + (a.first + i) * p.x.st, kWide<E>, E);
     }
-    for (int t = a.first; t < end; t += U) {
+    const T* xp = x + (a.first + U) * p.x.st;
+    T* yp = y + (size_t)a.first * p.C;
+    auto tokens = [&](int t, auto inner) {       // inner: these tokens and the next ones are all there
 #pragma unroll
       for (int i = 0; i < U; ++i)
 #pragma unroll
         for (int e = 0; e < E; ++e) win[KT - 1 + i][e] = (float)next[i].v[e];
 #pragma unroll
       for (int i = 0; i < U; ++i)
-        if (t + U + i < end) next[i].load(x + (t + U + i) * p.x.st, p.wide, here);
+        if (decltype(inner)::value || t + U + i < end) next[i].load(xp + i * p.x.st, kWide<E>, E);
+      xp += U * p.x.st;
+      float s[U][E];
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[i][e] = bias[e];
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+        if (KT < 8 || k >= skip)
+#pragma unroll
+          for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) s[i][e] = fmaf(w[k][e], win[i + k][e], s[i][e]);
+      if (p.act == kSilu)
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+          for (int e = 0; e < E; ++e) s[i][e] = silu<sizeof(T) == 4>(s[i][e]);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         Row<T, E> out;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          float s = bias[e];
-#pragma unroll
-          for (int k = 0; k < KT; ++k)
-            if (KT < 8 || k >= skip) s = fmaf(w[k][e], win[i + k][e], s);
-          out.v[e] = (T)(p.act == kSilu ? silu(s) : s);
-        }
-        if (t + i < end) out.store(y + (size_t)(t + i) * p.C, p.wide_out, here);
+        for (int e = 0; e < E; ++e) out.v[e] = (T)s[i][e];
+        if (decltype(inner)::value || t + i < end) out.store(yp + (size_t)i * p.C, kWide<E>, E);
       }
+      yp += (size_t)U * p.C;
 #pragma unroll
       for (int j = 0; j < KT - 1; ++j)
 #pragma unroll
         for (int e = 0; e < E; ++e) win[j][e] = win[j + U][e];
-    }
+    };
+    int t = a.first;
+    for (; t + 2 * U <= end; t += U) tokens(t, std::true_type{});
+    for (; t < end; t += U) tokens(t, std::false_type{});
   }
   Row<T, E> none;                        // tokens that do not count
   none.zero();
-  for (int t = max(a.first, end); t < a.last; ++t) none.store(y + (size_t)t * p.C, p.wide_out, here);
+  for (int t = max(a.first, end); t < a.last; ++t) none.store(y + (size_t)t * p.C, kWide<E>, E);
 }
 
-template <typename T, int E, int KT>
+template <typename T, int E, int KT, int U>      // U tokens at a time
 __global__ __launch_bounds__(256) void ring_conv_bwd_kernel(RingConvArgs p, int tx, int blocks) {
   __shared__ float sums[256 * E];
   const Piece a = piece<E>(p, tx, blocks);
-  const int K = KT == 8 ? p.K : KT, skip = KT - K, here = p.C - a.c, len = length_of(p.lengths, a.b, p.T);
+  const int K = KT == 8 ? p.K : KT, skip = KT - K, len = length_of(p.lengths, a.b, p.T);
   float w[KT][E], bias[E], dw[KT][E], db[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    bias[e] = p.bias && e < here ? p.bias[a.c + e] : 0.f;
+    bias[e] = p.bias && a.mine ? p.bias[a.c + e] : 0.f;
     db[e] = 0.f;
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
-      w[k][e] = k >= skip && e < here ? p.w[(size_t)(a.c + e) * K + k - skip] : 0.f;
+      w[k][e] = k >= skip && a.mine ? p.w[(size_t)(a.c + e) * K + k - skip] : 0.f;
       dw[k][e] = 0.f;
     }
   }
@@ -133,8 +155,8 @@ __global__ __launch_bounds__(256) void ring_conv_bwd_kernel(RingConvArgs p, int 
       Row<T, E> r;
       r.zero();
       if (j >= skip && a.first < len) {
-        if (t >= 0) r.load(x + t * p.x.st, p.wide, here);
-        else if (start) r.load(start + (size_t)(t + K - 1) * p.C, p.wide_state, here);
+        if (t >= 0) r.load(x + t * p.x.st, kWide<E>, E);
+        else if (start) r.load(start + (size_t)(t + K - 1) * p.C, kWide<E>, E);
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -150,11 +172,14 @@ __global__ __launch_bounds__(256) void ring_conv_bwd_kernel(RingConvArgs p, int 
       nx[i].zero(), ny[i].zero();
       const int t = a.first + i;
       if (t < min(to, len)) {
-        nx[i].load(x + t * p.x.st, p.wide, here);
-        ny[i].load(dy + t * p.dy.st, p.wide, here);
+        nx[i].load(x + t * p.x.st, kWide<E>, E);
+        ny[i].load(dy + t * p.dy.st, kWide<E>, E);
       }
     }
-    for (int t = a.first; t < to; t += U) {
+    const T *xp = x + (a.first + U) * p.x.st, *yp = dy + (a.first + U) * p.dy.st;
+    T* dxp = dx + (long)(a.first - K + 1) * p.C;       // (of token t - K + 1; used where that is one)
+    auto tokens = [&](int t, auto inner) {       // inner: these tokens count in the sums, the next ones are there, gradients are complete and of the piece
+      constexpr bool IN = decltype(inner)::value;
       Row<T, E> ky[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
@@ -163,30 +188,35 @@ __global__ __launch_bounds__(256) void ring_conv_bwd_kernel(RingConvArgs p, int 
         for (int e = 0; e < E; ++e) win[KT - 1 + i][e] = (float)nx[i].v[e];
       }
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int s = t + U + i;
-        if (s < min(to, len)) {
-          nx[i].load(x + s * p.x.st, p.wide, here);
-          ny[i].load(dy + s * p.dy.st, p.wide, here);
+      for (int i = 0; i < U; ++i)
+        if (IN || t + U + i < min(to, len)) {
+          nx[i].load(xp + i * p.x.st, kWide<E>, E);
+          ny[i].load(yp + i * p.dy.st, kWide<E>, E);
         }
-      }
+      xp += U * p.x.st;
+      yp += U * p.dy.st;
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int s = t + i, back = s - K + 1;
-        const bool counts = s < len;
+        const bool counts = IN || s < len;
+        float q[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          float v = (float)ky[i].v[e];
-          if (p.act == kSilu) {
-            float q = bias[e];
+          g[KT - 1 + i][e] = (float)ky[i].v[e];
+          q[e] = bias[e];
+        }
+        if (p.act == kSilu)
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
 #pragma unroll
             for (int k = 0; k < KT; ++k)
-              if (KT < 8 || k >= skip) q = fmaf(w[k][e], win[i + k][e], q);
-            v *= silu_slope(q, sigmoid(q));
+              if (KT < 8 || k >= skip) q[e] = fmaf(w[k][e], win[i + k][e], q[e]);
+            g[KT - 1 + i][e] *= silu_slope(q[e], sigmoid<sizeof(T) == 4>(q[e]));
           }
-          g[KT - 1 + i][e] = counts ? v : 0.f;
-        }
-        if (s < a.last && counts) {
+        if (!IN)
+#pragma unroll
+          for (int e = 0; e < E; ++e) g[KT - 1 + i][e] = counts ? g[KT - 1 + i][e] : 0.f;
+        if (IN || (s < a.last && counts)) {
 #pragma unroll
           for (int e = 0; e < E; ++e) {
             db[e] += g[KT - 1 + i][e];
@@ -195,23 +225,25 @@ __global__ __launch_bounds__(256) void ring_conv_bwd_kernel(RingConvArgs p, int 
               if (KT < 8 || k >= skip) dw[k][e] = fmaf(g[KT - 1 + i][e], win[i + k][e], dw[k][e]);
           }
         }
-        T* const to_row = back >= a.first ? (dx && back < a.last ? dx + (size_t)back * p.C : nullptr)
-                                          : (dstart && back < 0 && back >= -(K - 1) && s < to ? dstart + (size_t)(back + K - 1) * p.C : nullptr);
+        T* to_row = nullptr;
+        if (IN || (back >= a.first && back < a.last)) to_row = dx ? dxp + (long)i * p.C : nullptr;
+        else if (!IN && back < 0 && back >= -(K - 1) && s < to && dstart) to_row = dstart + (size_t)(back + K - 1) * p.C;
         if (to_row) {
           Row<T, E> out, more;
           more.zero();
-          if (dend && back < len && back >= len - (K - 1)) more.load(dend + (size_t)(back - len + K - 1) * p.C, p.wide_state, here);
+          if (!IN && dend && back < len && back >= len - (K - 1)) more.load(dend + (size_t)(back - len + K - 1) * p.C, kWide<E>, E);
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            float v = (float)more.v[e];
+            float v = IN ? 0.f : (float)more.v[e];
 #pragma unroll
             for (int k = 0; k < KT; ++k)
               if (KT < 8 || k >= skip) v = fmaf(w[k][e], g[KT - 1 + i - (k - skip)][e], v);
-            out.v[e] = (T)(back < len ? v : 0.f);
+            out.v[e] = (T)(IN || back < len ? v : 0.f);
           }
-          out.store(to_row, p.wide_out, here);
+          out.store(to_row, kWide<E>, E);
         }
       }
+      dxp += (long)U * p.C;
 #pragma unroll
       for (int j = 0; j < KT - 1; ++j)
 #pragma unroll
@@ -219,7 +251,12 @@ __global__ __launch_bounds__(256) void ring_conv_bwd_kernel(RingConvArgs p, int 
           win[j][e] = win[j + U][e];
           g[j][e] = g[j + U][e];
         }
-    }
+    };
+    int t = a.first;
+    const int full = min(a.last, len);
+    for (; t < min(to, a.first + KT - 1); t += U) tokens(t, std::false_type{});
+    for (; t + 2 * U <= full; t += U) tokens(t, std::true_type{});
+    for (; t < to; t += U) tokens(t, std::false_type{});
   }
   if (!p.part) return;
   // the workgroup's pieces, in order
@@ -237,7 +274,7 @@ __global__ __launch_bounds__(256) void ring_conv_bwd_kernel(RingConvArgs p, int 
       for (int e = 0; e < E; ++e) {
         float s = 0.f;
         for (int i = 0; i < subs; ++i) s += sums[e * 256 + i * tx + threadIdx.x];
-        if (e < here) part[(size_t)e * (K + 1) + k - skip] = s;
+        part[(size_t)e * (K + 1) + k - skip] = s;
       }
   }
 }
@@ -275,7 +312,7 @@ __global__ __launch_bounds__(64) void ring_conv_step_kernel(RingConvStep p, int 
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     s[e] = fmaf(e < here ? p.w[(size_t)(c + e) * p.K + p.K - 1] : 0.f, (float)x.v[e], s[e]);
-    out.v[e] = (T)(p.act == kSilu ? silu(s[e]) : s[e]);
+    out.v[e] = (T)(p.act == kSilu ? silu<sizeof(T) == 4>(s[e]) : s[e]);
   }
   out.store(y, wide, here);
 }
@@ -300,20 +337,21 @@ template <typename T, int E> static hipError_t launch(RingConvArgs p, bool back,
   cut(p, tx, blocks);
   const dim3 grid((unsigned)((size_t)blocks * p.nseg * p.B)), block(256);
 #define RING_CONV(KT)                                                                             \
-  if (back) hipLaunchKernelGGL((ring_conv_bwd_kernel<T, E, KT>), grid, block, 0, st, p, tx, blocks); \
-  else hipLaunchKernelGGL((ring_conv_fwd_kernel<T, E, KT>), grid, block, 0, st, p, tx, blocks)
+  if (back) hipLaunchKernelGGL((ring_conv_bwd_kernel<T, E, KT, 1>), grid, block, 0, st, p, tx, blocks); \
+  else hipLaunchKernelGGL((ring_conv_fwd_kernel<T, E, KT, 4>), grid, block, 0, st, p, tx, blocks)
   if (p.K == 2) { RING_CONV(2); }
   else if (p.K == 3) { RING_CONV(3); }
   else if (p.K == 4) { RING_CONV(4); }
-  else { RING_CONV(8); }
+  else if constexpr (E < 8) { RING_CONV(8); }
 #undef RING_CONV
   return hipGetLastError();
 }
 
 template <typename T> static hipError_t launch_wide(const RingConvArgs& p, bool back, hipStream_t st) {
-  constexpr int V = 16 / sizeof(T);
-  if (p.wide && p.wide_out && p.wide_state) return launch<T, V>(p, back, st);
-  return launch<T, 1>(p, back, st);
+  if (!(p.wide && p.wide_out && p.wide_state)) return launch<T, 1>(p, back, st);
+  if constexpr (sizeof(T) == 2)
+    if (p.K <= 4) return launch<T, 8>(p, back, st);
+  return launch<T, 4>(p, back, st);
 }
 
 static hipError_t launch_type(const RingConvArgs& p, int type, bool back, hipStream_t st) {
@@ -323,8 +361,8 @@ static hipError_t launch_type(const RingConvArgs& p, int type, bool back, hipStr
 }
 
 // (rows that allow 16 bytes make fewer parts or as many)
-static int parts_of(int type, int B, int T, int C, bool wide) {
-  const int E = wide ? (type == RINGATTR_F32 ? 4 : 8) : 1, tx = along(C, E), blocks = (C + tx * E - 1) / (tx * E);
+static int parts_of(int type, int B, int T, int C, int K, bool wide) {
+  const int E = wide ? (type == RINGATTR_F32 || K > 4 ? 4 : 8) : 1, tx = along(C, E), blocks = (C + tx * E - 1) / (tx * E);
   RingConvArgs p = {};
   p.B = B;
   p.T = T;
@@ -335,7 +373,7 @@ static int parts_of(int type, int B, int T, int C, bool wide) {
 
 size_t ring_conv_bwd_bytes(int type, int B, int T, int C, int K, bool params) {
   if (!params) return 0;
-  const int a = parts_of(type, B, T, C, true), b = parts_of(type, B, T, C, false);
+  const int a = parts_of(type, B, T, C, K, true), b = parts_of(type, B, T, C, K, false);
   return (size_t)(a > b ? a : b) * C * (K + 1) * sizeof(float);
 }
 
@@ -344,7 +382,7 @@ hipError_t ring_conv_fwd(RingConvArgs p, int type, hipStream_t st) { return laun
 hipError_t ring_conv_bwd(RingConvArgs p, int type, hipStream_t st) {
   hipError_t e = launch_type(p, type, true, st);
   if (e != hipSuccess || !p.part) return e;
-  return ring_launch_sum_parts(RingSumArgs{p.part, parts_of(type, p.B, p.T, p.C, p.wide && p.wide_out && p.wide_state), p.K + 1, p.K, 1,
+  return ring_launch_sum_parts(RingSumArgs{p.part, parts_of(type, p.B, p.T, p.C, p.K, p.wide && p.wide_out && p.wide_state), p.K + 1, p.K, 1,
                                            (size_t)p.C * (p.K + 1), p.dw, {p.dbias, nullptr}}, st);
 }
 

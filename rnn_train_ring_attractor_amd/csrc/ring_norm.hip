@@ -21,8 +21,14 @@ enum { kIdentity = 0, kSilu = 1, kSigmoid = 2 };
 // holds one unit of V values of each of I groups, else I units of one group.
 struct Lie { int lanes, slots, rows, units, groups; };
 
-// Sums of K values over `n` neighbouring threads, a power of two, the same in each
-template <int K> __device__ __forceinline__ void add_up(float (&v)[K], int n, float* room) {
+// Sums of K values over `n` neighbouring threads, a power of two, the same in each.  Across waves through one of two rooms by turns: who writes into a room
+// for the next but one sum has passed the barrier of the next one, which nobody reaches before this one is read.
+struct Room {
+  float* at;
+  int turn;
+};
+constexpr int kRoom = 2 * 32;
+template <int K> __device__ __forceinline__ void add_up(float (&v)[K], int n, Room& room) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     if (n > 1) v[k] = plus_dpp<kXor1>(v[k]);
@@ -32,27 +38,28 @@ template <int K> __device__ __forceinline__ void add_up(float (&v)[K], int n, fl
     if (n > 16) v[k] = fold16(v[k], v[k]);
     if (n > 32) v[k] = fold32(v[k], v[k]);
   }
-  if (n > 64) {
-    const int w = threadIdx.x >> 6, per = n >> 6, first = w / per * per;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0)
+  if constexpr (K <= 2) {
+    if (n > 64) {
+      float* const at = room.at + room.turn * 32;
+      const int w = threadIdx.x >> 6, per = n >> 6, first = w / per * per;
+      room.turn ^= 1;
+      if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int k = 0; k < K; ++k) room[k * 16 + w] = v[k];
-    __syncthreads();
+        for (int k = 0; k < K; ++k) at[k * 16 + w] = v[k];
+      __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      float s = room[k * 16 + first];
-      for (int i = 1; i < per; ++i) s += room[k * 16 + first + i];
-      v[k] = s;
+      for (int k = 0; k < K; ++k) {
+        float s = at[k * 16 + first];
+        for (int i = 1; i < per; ++i) s += at[k * 16 + first + i];
+        v[k] = s;
+      }
     }
   }
 }
 
-__device__ __forceinline__ float act_of(float x, int act) { return act == kSilu ? silu(x) : (act == kSigmoid ? sigmoid(x) : x); }
-__device__ __forceinline__ float slope_of(float x, int act) {
-  if (act == kIdentity) return 1.f;
-  const float s = sigmoid(x);
-  return act == kSilu ? silu_slope(x, s) : s * (1.f - s);
+template <typename T> __device__ __forceinline__ float act_of(T y, int act) {
+  const float x = (float)y;
+  return act == kSilu ? silu<sizeof(T) == 4>(x) : (act == kSigmoid ? sigmoid<sizeof(T) == 4>(x) : x);
 }
 
 // A thread's place in a row
@@ -75,9 +82,9 @@ template <int V, int I, bool MANY> struct Spot {
 };
 
 // sums[i] += the sum over its group of the thread's values of unit i
-template <int V, int I, bool MANY> __device__ __forceinline__ void group_sums(float (&sums)[I], const Lie& l, float* room) {
+template <int V, int I, bool MANY> __device__ __forceinline__ void group_sums(float (&sums)[I], const Lie& l, Room& room) {
   if constexpr (MANY) {
-    add_up<I>(sums, l.lanes, room);
+    add_up<I>(sums, l.lanes, room);      // (at most 64 lanes)
   } else {
     float one[1] = {sums[0]};
 #pragma unroll
@@ -90,7 +97,7 @@ template <int V, int I, bool MANY> __device__ __forceinline__ void group_sums(fl
 
 // v becomes (v - mean) over its groups, rstd beside it
 template <int V, int I, bool MANY>
-__device__ __forceinline__ void normalise(float (&v)[I][V], float (&rstd)[I], const int (&here)[I], const Lie& l, float count, bool layer, float eps, float* room) {
+__device__ __forceinline__ void normalise(float (&v)[I][V], float (&rstd)[I], const int (&here)[I], const Lie& l, float count, bool layer, float eps, Room& room) {
   float s[I];
   if (layer) {
 #pragma unroll
@@ -120,7 +127,8 @@ __device__ __forceinline__ void normalise(float (&v)[I][V], float (&rstd)[I], co
 
 template <typename T, int V, int I, bool MANY>
 __global__ __launch_bounds__(1024) void ring_norm_fwd_kernel(RingNormArgs p, Lie l) {
-  __shared__ float room[64];
+  __shared__ float rooms[kRoom];
+  Room room = {rooms, 0};
   const Spot<V, I, MANY> at(l);
   const Lie whole = {at.threads, 1, l.rows, 0, 1};
   const long row = ((long)blockIdx.y * gridDim.x + blockIdx.x) * l.rows + at.row;
@@ -145,13 +153,18 @@ __global__ __launch_bounds__(1024) void ring_norm_fwd_kernel(RingNormArgs p, Lie
 #pragma unroll
   for (int i = 0; i < I; ++i) {
     Row<T, V> out;
+    Row<float, V> w, s;
+    if (here[i] > 0) {
+      w.load(p.w + col[i], V > 1, here[i]);
+      if (p.scale) s.load(p.scale + col[i], V > 1, here[i]);
+    }
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       float y = 0.f;
       if (e < here[i]) {
-        y = v[i][e] * rstd[i] * p.w[col[i] + e];
-        if (p.gate) y *= act_of((float)rg[i].v[e], p.act);
-        if (p.scale) y *= p.scale[col[i] + e];
+        y = v[i][e] * rstd[i] * w.v[e];
+        if (p.gate) y *= act_of(rg[i].v[e], p.act);
+        if (p.scale) y *= s.v[e];
         if (p.residual) y += (float)rr[i].v[e];
       }
       v[i][e] = y;
@@ -165,110 +178,162 @@ __global__ __launch_bounds__(1024) void ring_norm_fwd_kernel(RingNormArgs p, Lie
   for (int i = 0; i < I; ++i)
     if (here[i] > 0) {
       Row<T, V> out;
+      Row<float, V> w;
+      w.load(p.next + col[i], V > 1, here[i]);
 #pragma unroll
-      for (int e = 0; e < V; ++e) out.v[e] = (T)(e < here[i] ? v[i][e] * rstd[i] * p.next[col[i] + e] : 0.f);
+      for (int e = 0; e < V; ++e) out.v[e] = (T)(v[i][e] * rstd[i] * w.v[e]);
       out.store((T*)p.n + row * p.C + col[i], V > 1, here[i]);
     }
 }
 
-template <typename T, int V, int I, bool MANY>
-__global__ __launch_bounds__(1024) void ring_norm_bwd_kernel(RingNormArgs p, Lie l) {
-  __shared__ float room[64];
+// MOST threads a workgroup.  Up to 512 of one unit each keep the weights and read the next row ahead; more have no registers left for that.
+template <typename T, int V, int I, bool MANY, int MOST>
+__global__ __launch_bounds__(MOST) void ring_norm_bwd_kernel(RingNormArgs p, Lie l) {
+  constexpr bool KEEP = MOST <= 512, FINE = sizeof(T) == 4;
+  __shared__ float rooms[kRoom];
+  Room room = {rooms, 0};
   extern __shared__ float sums[];        // [threads][V]: rows of a workgroup are added up
   const Spot<V, I, MANY> at(l);
   const Lie whole = {at.threads, 1, l.rows, 0, 1};
+  struct Unit { Row<T, V> x, g, r, t, n; };          // of the row: x, gate, residual, gradients of y and n
+  struct Weights { Row<float, V> w, s, n; } kept;
+  Unit next[I];
   int there[I], col[I];
   float aw[I][V], as[I][V], an[I][V];
+  auto weights = [&](int i) {
+    Weights k;
+    k.w.zero(), k.s.zero(), k.n.zero();
+    if (there[i] > 0) {
+      k.w.load(p.w + col[i], V > 1, there[i]);
+      if (p.scale) k.s.load(p.scale + col[i], V > 1, there[i]);
+      if (p.dn) k.n.load(p.next + col[i], V > 1, there[i]);
+    }
+    if (!p.scale)
+#pragma unroll
+      for (int e = 0; e < V; ++e) k.s.v[e] = 1.f;
+    return k;
+  };
+  auto load = [&](long row) {
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      if (row >= p.rows || there[i] <= 0) continue;
+      next[i].x.load((const T*)p.x + row * p.xs + col[i], V > 1, there[i]);
+      if (p.gate) next[i].g.load((const T*)p.gate + row * p.gs + col[i], V > 1, there[i]);
+      if (p.dy) next[i].t.load((const T*)p.dy + row * p.dys + col[i], V > 1, there[i]);
+      if (p.dn) {
+        next[i].n.load((const T*)p.dn + row * p.dns + col[i], V > 1, there[i]);
+        if (p.residual) next[i].r.load((const T*)p.residual + row * p.rs + col[i], V > 1, there[i]);
+      }
+    }
+  };
 #pragma unroll
   for (int i = 0; i < I; ++i) {
     there[i] = at.here(l, i, p.group);
     col[i] = at.column(l, i, p.group);
+    next[i].x.zero(), next[i].g.zero(), next[i].r.zero(), next[i].t.zero(), next[i].n.zero();
 #pragma unroll
     for (int e = 0; e < V; ++e) aw[i][e] = as[i][e] = an[i][e] = 0.f;
   }
-  for (long first = (long)blockIdx.x * l.rows; first < p.rows; first += (long)gridDim.x * l.rows) {
+  if constexpr (KEEP) kept = weights(0);
+  const bool gated = p.gate && p.act != kSigmoid;
+  const long step = (long)gridDim.x * l.rows;
+  load((long)blockIdx.x * l.rows + at.row);
+  for (long first = (long)blockIdx.x * l.rows; first < p.rows; first += step) {
     const long row = first + at.row;
     const bool real = row < p.rows;
     int here[I];
-    float unit[I][V], rstd[I], total[I][V];
-    Row<T, V> rx[I], rg[I], rr[I], rt[I], rn[I];
+    float unit[I][V], rstd[I], total[I][V], sig[I][V];      // sig: the gate's sigmoid, which its activation and slope follow from
+    Unit now[I];
+    if constexpr (!KEEP) {
+      if (first > (long)blockIdx.x * l.rows) load(row);
+    }
 #pragma unroll
     for (int i = 0; i < I; ++i) {
+      now[i] = next[i];
       here[i] = real ? there[i] : 0;
-      rx[i].zero(), rg[i].zero(), rr[i].zero(), rt[i].zero(), rn[i].zero();
-      if (here[i] > 0) {
-        rx[i].load((const T*)p.x + row * p.xs + col[i], V > 1, here[i]);
-        if (p.gate) rg[i].load((const T*)p.gate + row * p.gs + col[i], V > 1, here[i]);
-        if (p.dy) rt[i].load((const T*)p.dy + row * p.dys + col[i], V > 1, here[i]);
-        if (p.dn) {
-          rn[i].load((const T*)p.dn + row * p.dns + col[i], V > 1, here[i]);
-          if (p.residual) rr[i].load((const T*)p.residual + row * p.rs + col[i], V > 1, here[i]);
-        }
-      }
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        unit[i][e] = (float)rx[i].v[e];
-        total[i][e] = (float)rt[i].v[e];
+        unit[i][e] = e < here[i] ? (float)now[i].x.v[e] : 0.f;
+        total[i][e] = (float)now[i].t.v[e];
+        sig[i][e] = 1.f;
       }
     }
+    if constexpr (KEEP) load(row + step);
+    if (p.gate && p.act != kIdentity)
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sig[i][e] = sigmoid<FINE>((float)now[i].g.v[e]);
+    auto act = [&](int i, int e) { return gated ? (float)now[i].g.v[e] * sig[i][e] : sig[i][e]; };      // silu, none: z s; sigmoid, no gate: s
+    auto slope = [&](int i, int e) {
+      const float s = sig[i][e];
+      return p.act == kSilu ? silu_slope((float)now[i].g.v[e], s) : (p.act == kSigmoid ? s * (1.f - s) : 1.f);
+    };
     normalise<V, I, MANY>(unit, rstd, here, l, (float)p.group, p.layer, p.eps, room);
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
       for (int e = 0; e < V; ++e) unit[i][e] *= rstd[i];
     if (p.dn) {
-      float y[I][V], r2[I], s[2] = {0.f, 0.f};
+      // n = (y - mean) r next: sums of y and of the gradient, then of their squares and products, both at once
+      float y[I][V], s[2] = {0.f, 0.f}, mean = 0.f, m0 = 0.f;
 #pragma unroll
-      for (int i = 0; i < I; ++i)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          y[i][e] = 0.f;
-          if (e < here[i]) {
-            y[i][e] = unit[i][e] * p.w[col[i] + e];
-            if (p.gate) y[i][e] *= act_of((float)rg[i].v[e], p.act);
-            if (p.scale) y[i][e] *= p.scale[col[i] + e];
-            if (p.residual) y[i][e] += (float)rr[i].v[e];
-          }
-        }
-      normalise<V, I, false>(y, r2, here, whole, (float)p.C, p.layer, p.eps, room);
-#pragma unroll
-      for (int i = 0; i < I; ++i)
+      for (int i = 0; i < I; ++i) {
+        const Weights k = KEEP ? kept : weights(i);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          y[i][e] *= r2[i];
-          const float g = e < here[i] ? (float)rn[i].v[e] * p.next[col[i] + e] : 0.f;
-          an[i][e] = fmaf((float)rn[i].v[e], y[i][e], an[i][e]);
-          s[0] = fmaf(g, y[i][e], s[0]);
-          s[1] += g;
+          const float v = fmaf(unit[i][e] * k.w.v[e] * act(i, e), k.s.v[e], p.residual ? (float)now[i].r.v[e] : 0.f);
+          y[i][e] = e < here[i] ? v : 0.f;
+          s[0] += y[i][e];
+          s[1] += e < here[i] ? (float)now[i].n.v[e] * k.n.v[e] : 0.f;
         }
+      }
+      if (p.layer) {
+        add_up<2>(s, at.threads, room);
+        mean = s[0] / (float)p.C;
+        m0 = s[1] / (float)p.C;
+      }
+      s[0] = s[1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        const Weights k = KEEP ? kept : weights(i);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          y[i][e] = e < here[i] ? y[i][e] - mean : 0.f;
+          s[0] = fmaf(y[i][e], y[i][e], s[0]);
+          s[1] += e < here[i] ? (float)now[i].n.v[e] * k.n.v[e] * y[i][e] : 0.f;
+        }
+      }
       add_up<2>(s, at.threads, room);
-      const float m1 = s[0] / (float)p.C, m0 = p.layer ? s[1] / (float)p.C : 0.f;
+      const float r = 1.f / sqrtf(s[0] / (float)p.C + p.eps), m1 = s[1] * r / (float)p.C;
 #pragma unroll
-      for (int i = 0; i < I; ++i)
+      for (int i = 0; i < I; ++i) {
+        const Weights k = KEEP ? kept : weights(i);
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (e < here[i]) total[i][e] += r2[i] * ((float)rn[i].v[e] * p.next[col[i] + e] - m0 - y[i][e] * m1);
+        for (int e = 0; e < V; ++e) {
+          const float u = y[i][e] * r;
+          if (real) an[i][e] = fmaf((float)now[i].n.v[e], u, an[i][e]);
+          total[i][e] = fmaf(r, (float)now[i].n.v[e] * k.n.v[e] - m0 - u * m1, total[i][e]);
+        }
+      }
     }
     float s1[I], s0[I];
 #pragma unroll
     for (int i = 0; i < I; ++i) {
+      const Weights k = KEEP ? kept : weights(i);
       Row<T, V> res, dg;
       s1[i] = s0[i] = 0.f;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         res.v[e] = (T)total[i][e];
-        float g = 0.f, back = 0.f;
-        if (e < here[i]) {
-          const float w = p.w[col[i] + e], a = p.gate ? act_of((float)rg[i].v[e], p.act) : 1.f, normed = unit[i][e] * w;
-          g = total[i][e];
-          as[i][e] = fmaf(g, normed * a, as[i][e]);
-          if (p.scale) g *= p.scale[col[i] + e];
-          back = p.gate ? g * normed * slope_of((float)rg[i].v[e], p.act) : 0.f;
-          g *= a;
-          aw[i][e] = fmaf(g, unit[i][e], aw[i][e]);
-          g *= w;
-        }
-        dg.v[e] = (T)back;
+        const float normed = unit[i][e] * k.w.v[e];
+        float g = total[i][e];
+        if (real) as[i][e] = fmaf(g, normed * act(i, e), as[i][e]);
+        g *= k.s.v[e];
+        dg.v[e] = (T)(g * normed * slope(i, e));
+        g *= act(i, e);
+        if (real) aw[i][e] = fmaf(g, unit[i][e], aw[i][e]);
+        g = e < here[i] ? g * k.w.v[e] : 0.f;
         total[i][e] = g;
         s1[i] = fmaf(g, unit[i][e], s1[i]);
         s0[i] += g;
@@ -387,7 +452,14 @@ int parts_of(const Plan& a, long rows) {
 
 template <typename T, int V, int I, bool MANY> void launch_one(const RingNormArgs& p, const Plan& a, bool back, hipStream_t st) {
   if (back) {
-    hipLaunchKernelGGL((ring_norm_bwd_kernel<T, V, I, MANY>), dim3((unsigned)p.parts), dim3(a.threads), a.threads * V * sizeof(float), st, p, a.lie);
+    const size_t room = a.threads * V * sizeof(float);
+    if constexpr (I == 1) {
+      if (a.threads <= 512) {
+        hipLaunchKernelGGL((ring_norm_bwd_kernel<T, V, 1, MANY, 512>), dim3((unsigned)p.parts), dim3(a.threads), room, st, p, a.lie);
+        return;
+      }
+    }
+    hipLaunchKernelGGL((ring_norm_bwd_kernel<T, V, I, MANY, 1024>), dim3((unsigned)p.parts), dim3(a.threads), room, st, p, a.lie);
   } else {
     const long blocks = (p.rows + a.lie.rows - 1) / a.lie.rows, row = blocks < (1 << 20) ? blocks : 1 << 20;      // (a launch counts fewer than 2^32 threads along x)
     hipLaunchKernelGGL((ring_norm_fwd_kernel<T, V, I, MANY>), dim3((unsigned)row, (unsigned)((blocks + row - 1) / row)), dim3(a.threads), 0, st, p, a.lie);
@@ -410,7 +482,8 @@ template <typename T, int V, bool MANY> void launch_units(const RingNormArgs& p,
 template <typename T> bool wide(const RingNormArgs& p) {
   constexpr int V = 16 / sizeof(T);
   const uintptr_t all = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.gate) | reinterpret_cast<uintptr_t>(p.residual) |
-                        reinterpret_cast<uintptr_t>(p.dy) | reinterpret_cast<uintptr_t>(p.dn);
+                        reinterpret_cast<uintptr_t>(p.dy) | reinterpret_cast<uintptr_t>(p.dn) | reinterpret_cast<uintptr_t>(p.w) |
+                        reinterpret_cast<uintptr_t>(p.scale) | reinterpret_cast<uintptr_t>(p.next);
   return p.group % V == 0 && (all & 15) == 0 && (p.xs | p.gs | p.rs | p.dys | p.dns) % V == 0;
 }
 

@@ -8,32 +8,36 @@ namespace ring_recur {
 
 constexpr float kLog2e = 1.44269504088896341f, kLog2eLow = 1.92596299e-8f, kLn2 = 0.693147180559945309f;
 
-// e^x for -126 <= x log2(e) <= 126: the power's argument as a sum of two numbers, the second to first order (2^x itself is off by a step)
-__device__ __forceinline__ float exp_of(float x) {
-  const float high = x * kLog2e, low = fmaf(x, kLog2eLow, fmaf(x, kLog2e, -high));
-  const float e = __builtin_amdgcn_exp2f(high);
+// Functions for rows of fp32 (FINE) and of 16 bits.  FINE: a power's argument as a sum of two numbers, the second to first order, otherwise one
+// (off by |x| 2^-24 then, which is less than the rounding of a 16-bit argument by far).
+
+// e^x, FINE: for |x| <= 87
+template <bool FINE> __device__ __forceinline__ float exp_of(float x) {
+  const float high = x * kLog2e, e = __builtin_amdgcn_exp2f(high);
+  if constexpr (!FINE) return e;
+  const float low = fmaf(x, kLog2eLow, fmaf(x, kLog2e, -high));
   return fmaf(e, low * kLn2, e);
 }
 
-// 1 / (1 + e^-x); NaN only through what it is multiplied by
-__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + exp_of(fminf(fmaxf(-x, -87.f), 87.f))); }
-__device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
+// 1 / (1 + e^-x)
+template <bool FINE> __device__ __forceinline__ float sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.f + exp_of<FINE>(FINE ? __builtin_amdgcn_fmed3f(-x, -87.f, 87.f) : -x));
+}
+template <bool FINE> __device__ __forceinline__ float silu(float x) { return x * sigmoid<FINE>(x); }
 // the derivative of x sigmoid(x), s = sigmoid(x)
 __device__ __forceinline__ float silu_slope(float x, float s) { return s * fmaf(x, 1.f - s, 1.f); }
 
-// ln(1 + e^x) = max(x, 0) + ln(1 + e), e = e^-|x|; ln(1 + e) = 2 artanh(e / (2 + e)) by its series, the square of the argument at most 1/9
-__device__ __forceinline__ float softplus(float x) {
-  const float e = exp_of(fmaxf(-fabsf(x), -87.f)), s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
-  float r = 1.f / 15.f;
-  r = fmaf(r, q, 1.f / 13.f);
-  r = fmaf(r, q, 1.f / 11.f);
-  r = fmaf(r, q, 1.f / 9.f);
-  r = fmaf(r, q, 1.f / 7.f);
-  r = fmaf(r, q, 1.f / 5.f);
-  r = fmaf(r, q, 1.f / 3.f);
-  r = fmaf(r, q, 1.f);
-  const float y = fmaf(2.f * s, r, x > 0.f ? x : 0.f);
-  return x == x ? y : x;
+// ln(1 + e^x) = max(x, 0) + ln(1 + e), e = e^-|x|, and its derivative.  What 1 + e loses of e is added to the logarithm of the sum, whose slope there is one
+// to first order (together within 3.5 2^-24 of ln(1 + e), measured from e = 2^-24 to 1).
+template <bool FINE> __device__ __forceinline__ float softplus(float x, float& slope) {
+  const float e = exp_of<FINE>(FINE ? __builtin_amdgcn_fmed3f(-fabsf(x), -87.f, 0.f) : -fabsf(x)), w = 1.f + e;
+  const float y = fmaf(__builtin_amdgcn_logf(w), kLn2, e - (w - 1.f)) + __builtin_amdgcn_fmed3f(x, 0.f, INFINITY), r = __builtin_amdgcn_rcpf(w);
+  slope = x > 0.f ? r : e * r;
+  return FINE ? (x == x ? y : x) : y;        // (NaN: otherwise through e)
+}
+template <bool FINE> __device__ __forceinline__ float softplus(float x) {
+  float slope;
+  return softplus<FINE>(x, slope);
 }
 
 // E values, neighbours in memory.  WIDE: the address is a whole number of min(16, E sizeof(T)) bytes; otherwise one by one, `here` of them.
@@ -97,7 +101,7 @@ __device__ __forceinline__ float fold16(float a, float b) {
 template <int CTRL> __device__ __forceinline__ float plus_dpp(float x) {
   return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true));
 }
-constexpr int kRor8 = 0x128, kRor4 = 0x124, kXor1 = 0xB1, kXor2 = 0x4E;
+constexpr int kRor8 = 0x128, kUp4 = 0x104, kDown4 = 0x114, kXor1 = 0xB1, kXor2 = 0x4E;      // (up 4: the lane four further on)
 
 __device__ __forceinline__ int length_of(const int* lengths, int b, int T) { return lengths ? min(max(lengths[b], 0), T) : T; }
 

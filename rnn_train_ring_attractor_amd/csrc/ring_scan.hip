@@ -14,18 +14,18 @@ int tile(int N) { return N <= 16 ? 64 : (N <= 32 ? 32 : 16); }        // channel
 int tiles_of(const RingScanShape& s) { return (s.C / s.G + tile(s.N) - 1) / tile(s.N); }
 int saved_of(const RingScanShape& s) { return (s.T + RingScanArgs::kSave - 1) / RingScanArgs::kSave; }
 
-// Segments that the tokens are cut into, so that every compute unit has work
-int segments(const RingScanShape& s, int wanted) {
+// Segments that the tokens are cut into: none where every compute unit has a workgroup without, otherwise so many that each has two (us, bf16, 16 states: one
+// sequence of 32768 tokens, 2048 channels, one a unit 825, two 542; two of 2048, with gradients, 320 and 311; eight of 2048, none 243 and 817 with
+// gradients, two 255 and 955).
+int segments(const RingScanShape& s) {
   const long groups = (long)tiles_of(s) * s.G * s.B;
   const int units = (s.T + kChunk - 1) / kChunk;
-  long n = (wanted + groups - 1) / groups;
+  long n = groups >= 256 ? 1 : (512 + groups - 1) / groups;
   if (n > units / 2) n = units / 2;
   if (n < 1) n = 1;
   const int per = (int)((units + n - 1) / n);
   return (units + per - 1) / per;
 }
-int fwd_segments(const RingScanShape& s) { return segments(s, 256); }
-int bwd_segments(const RingScanShape& s) { return segments(s, 256); }
 
 size_t seg_bytes(const RingScanShape& s, int nseg) {
   const size_t rows = (size_t)(nseg - 1) * s.B * s.C;
@@ -81,15 +81,15 @@ static hipError_t between(const RingScanShape& s, RingScanArgs a, int mode, hipS
 }
 
 size_t ring_scan_states_bytes(const RingScanShape& s) { return round_up((size_t)s.B * saved_of(s) * s.C * padded(s.N) * sizeof(float)); }
-size_t ring_scan_fwd_bytes(const RingScanShape& s) { return seg_bytes(s, fwd_segments(s)); }
+size_t ring_scan_fwd_bytes(const RingScanShape& s) { return seg_bytes(s, segments(s)); }
 size_t ring_scan_bwd_bytes(const RingScanShape& s, bool shared, bool params) {
-  const int nseg = bwd_segments(s);
+  const int nseg = segments(s);
   return seg_bytes(s, nseg) + (shared ? shared_bytes(s) : 0) +
          (params ? round_up((size_t)nseg * s.B * s.C * (padded(s.N) + 2) * sizeof(float)) : 0);
 }
 
 hipError_t ring_scan_fwd(const RingScanShape& s, RingScanArgs a, void* ws, hipStream_t st) {
-  set_segments(a, s, fwd_segments(s), ws);
+  set_segments(a, s, segments(s), ws);
   hipError_t e = between(s, a, RING_SCAN_STATE, st);
   return e == hipSuccess ? launch_pass(s.type, a, RING_SCAN_OUTPUTS, st) : e;
 }
@@ -120,7 +120,7 @@ template <typename T> static void launch_share(const RingScanShape& s, const Rin
 }
 
 hipError_t ring_scan_bwd(const RingScanShape& s, RingScanArgs a, const RingScanGrads& g, void* ws, hipStream_t st) {
-  const int nseg = bwd_segments(s);
+  const int nseg = segments(s);
   set_segments(a, s, nseg, ws);
   char* at = (char*)ws + seg_bytes(s, nseg);
   if (g.B || g.C) {
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(256) void ring_scan_step_kernel(RingScanStep p, Rin
   const float x = (float)((const T*)p.x)[b * p.xs + c];
   float d = (float)((const T*)p.delta)[b * p.ds + c];
   if (p.bias) d += p.bias[c];
-  if (p.softplus) d = softplus(d);
+  if (p.softplus) d = softplus<sizeof(T) == 4>(d);
   float y = 0.f;
   if (n < s.N) {
     vec* at = reinterpret_cast<vec*>(p.state + row * s.N + n);
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256) void ring_scan_step_kernel(RingScanStep p, Rin
   for (int half = lanes / 2; half > 0; half /= 2) y += __shfl_xor(y, half);
   if (n == 0) {
     if (p.D) y = fmaf(p.D[c], x, y);
-    if (p.z) y *= silu((float)((const T*)p.z)[b * p.zs + c]);
+    if (p.z) y *= silu<sizeof(T) == 4>((float)((const T*)p.z)[b * p.zs + c]);
     *out = (T)y;
   }
 }

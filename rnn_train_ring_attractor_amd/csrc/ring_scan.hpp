@@ -18,6 +18,8 @@
 #include "ring_recur.hpp"
 #include "ringattr.h"
 
+#include <type_traits>
+
 namespace ring_scan {
 
 using namespace ring_recur;
@@ -41,42 +43,136 @@ template <int CH> __device__ __forceinline__ Place place(const RingScanArgs& p) 
   return {(int)(i / p.B), (int)(i % p.B), g, g * Cg + first, min(CH, Cg - first)};
 }
 
+// Four sums over the lanes of a quad, of which lane `sub` keeps number sub
+__device__ __forceinline__ float quad_sums(const float* v, int sub) {
+  // (sums first, by all lanes, then the choice)
+  const float a0 = plus_dpp<kXor1>(v[0]), a1 = plus_dpp<kXor1>(v[1]), b0 = plus_dpp<kXor1>(v[2]), b1 = plus_dpp<kXor1>(v[3]);
+  const float a = plus_dpp<kXor2>(sub & 1 ? a1 : a0), b = plus_dpp<kXor2>(sub & 1 ? b1 : b0);
+  return sub & 2 ? b : a;
+}
+// Four sums over a row's quads, of which quad (0, 2, 1, 3)[i] keeps number i
+__device__ __forceinline__ float row_sums(const float* v, int quad) {
+  const float a0 = plus_dpp<kRor8>(v[0]), a1 = plus_dpp<kRor8>(v[1]), b0 = plus_dpp<kRor8>(v[2]), b1 = plus_dpp<kRor8>(v[3]);
+  const float a = plus_dpp<kUp4>(quad & 2 ? a1 : a0), b = plus_dpp<kDown4>(quad & 2 ? b1 : b0);
+  return quad & 1 ? b : a;
+}
+
 enum Mode { kOutputs, kState, kAdjoint };
 
-// Outputs (and the states kept for a backward), or what a segment adds to a state of zeros, or, backwards in time, to an adjoint of zeros
+template <int NL> __device__ __forceinline__ void take(float (&v)[NL], const float* p) {      // NL floats at a whole number of NL of them
+  typedef float vec __attribute__((ext_vector_type(NL)));
+  const vec x = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+  for (int n = 0; n < NL; ++n) v[n] = x[n];
+}
+template <> __device__ __forceinline__ void take<1>(float (&v)[1], const float* p) { v[0] = *p; }
+
+// B or C of a chunk, read by 256 threads and laid down in fp32
+template <typename T, int L, int NS> struct Shared {
+  static constexpr int NV = (L * NS + 255) / 256;
+  T v[NV];
+  __device__ __forceinline__ void load(const T* p, long st, int t0, int end, int N, int tid) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = tid + 256 * i, t = t0 + k / NS, n = k % NS;
+      const T x = p[(long)min(t, end - 1) * st + min(n, N - 1)];       // (t0 < end: there is a row)
+      v[i] = t < end && n < N ? x : (T)0.f;
+    }
+  }
+  __device__ __forceinline__ void lay(float* to, int tid) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (tid + 256 * i < L * NS) to[tid + 256 * i] = (float)v[i];
+  }
+};
+
+// Outputs (and the states kept for a backward), or what a segment adds to a state of zeros, or, backwards in time, to an adjoint of zeros.
+// The first four waves go through the tokens; the other four read and work out the next chunk's rows and finish the last one's outputs meanwhile.
 template <typename T, int NL, int NB, int MODE>
-__global__ __launch_bounds__(256) void ring_scan_kernel(RingScanArgs p) {
+__global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
   constexpr int CH = 64 / NB, L = kL, E = CH / 8, NS = 4 * NL * NB, PL = plane<CH, L>();
-  constexpr int NV = (L * NS + 255) / 256;          // values of B or C that a thread lays down
   constexpr bool REV = MODE == kAdjoint, OUT = MODE == kOutputs;
-  __shared__ __attribute__((aligned(16))) float sd[PL], su[PL], sB[L * NS], sC[OUT ? L * NS : 4], sy[OUT ? NB * PL : 4];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  __shared__ __attribute__((aligned(16))) float sd[2][PL], su[2][PL], sB[2][L * NS], sC[2][OUT ? L * NS : 4], sy[2][OUT ? NB * PL : 4];
+  const int tid = threadIdx.x & 255, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Place at_ = place<CH>(p);
   const int seg = REV ? p.nseg - 1 - at_.seg : at_.seg, b = at_.b;
   const int len = length_of(p.lengths, b, p.T), first = seg * p.seg_tokens, last = min(first + p.seg_tokens, p.T), end = min(last, len);
-  // a lane's channel and states
-  const int nb = w % NB, ch = w / NB * 16 + (lane & 15), sub = lane >> 4, n0 = nb * 4 * NL + sub * NL, c = at_.c0 + ch;
-  const bool mine = ch < at_.here;
+  const int chunks = end > first ? (end - first + L - 1) / L : 0;
+  auto begin = [&](int k) { return first + (REV ? chunks - 1 - k : k) * L; };
+  if (w < 4) {
+    const int nb = w % NB, ch = w / NB * 16 + (lane & 15), sub = lane >> 4, n0 = nb * 4 * NL + sub * NL, c = at_.c0 + ch;
+    const bool mine = ch < at_.here;
+    float A2[NL], h[NL], total = 0.f;      // total: of d, for the segment's whole decay
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      A2[n] = mine && n0 + n < p.N ? (float)((double)p.A[(size_t)c * p.N + n0 + n] * 1.4426950408889634) : 0.f;
+      h[n] = 0.f;
+      if (OUT && mine) {
+        if (seg > 0) h[n] = p.seg[(((size_t)(seg - 1) * p.B + b) * p.C + c) * NS + n0 + n];
+        else if (p.s_in && n0 + n < p.N) h[n] = p.s_in[((size_t)b * p.C + c) * p.N + n0 + n];
+      }
+    }
+    __syncthreads();
+    for (int k = 0; k < chunks; ++k) {
+      const int t0 = begin(k);
+      const float *d_ = sd[k & 1] + at<L>(ch, 0), *u_ = su[k & 1] + at<L>(ch, 0), *B_ = sB[k & 1] + n0, *C_ = sC[k & 1] + n0;
+      float* const y_ = sy[k & 1] + (OUT ? nb * PL + at<L>(ch, (sub & 1) << 1 | sub >> 1) : 0);
+#pragma unroll 4
+      for (int jj = 0; jj < L; jj += 4) {
+        const int j = REV ? L - 4 - jj : jj;
+        if (OUT && p.states && j % kSave == 0 && mine && t0 + j < end) {
+          float* s = p.states + (((size_t)b * p.saved + (t0 + j) / kSave) * p.C + c) * NS + n0;
+#pragma unroll
+          for (int n = 0; n < NL; ++n) s[n] = h[n];
+        }
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(d_ + j), u4 = *reinterpret_cast<const f32x4*>(u_ + j);
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int o = REV ? 3 - i : i;
+          float Bn[NL], Cn[NL];
+          take<NL>(Bn, B_ + (j + o) * NS);
+          if (OUT) take<NL>(Cn, C_ + (j + o) * NS);
+          if (!OUT) total += d4[o];
+#pragma unroll
+          for (int n = 0; n < NL; ++n) {
+            const float a = __builtin_amdgcn_exp2f(d4[o] * A2[n]);
+            if (REV) h[n] = a * fmaf(u4[o], Bn[n], h[n]);
+            else h[n] = fmaf(a, h[n], u4[o] * Bn[n]);
+            if (OUT) y[o] = n == 0 ? h[n] * Cn[n] : fmaf(h[n], Cn[n], y[o]);
+          }
+        }
+        // row r of 16 lanes is left with token (0, 2, 1, 3)[r]
+        if (OUT) y_[j] = fold16(fold32(y[0], y[1]), fold32(y[2], y[3]));
+      }
+      __syncthreads();
+    }
+    if (!mine) return;
+    if (OUT) {
+      if (p.s_out && seg == p.nseg - 1) {
+#pragma unroll
+        for (int n = 0; n < NL; ++n)
+          if (n0 + n < p.N) p.s_out[((size_t)b * p.C + c) * p.N + n0 + n] = h[n];
+      }
+    } else {
+      const size_t row = ((size_t)at_.seg * p.B + b) * p.C + c;
+#pragma unroll
+      for (int n = 0; n < NL; ++n) p.seg[row * NS + n0 + n] = h[n];
+      if (n0 == 0) p.total[row] = total;
+    }
+    return;
+  }
   // a thread's token and channels where rows are read and written
   const int tl = tid >> 3, cl = (tid & 7) * E, cr = at_.c0 + cl, here = at_.here - cl;
-  float A2[NL], h[NL], D[E], bias[E];
-#pragma unroll
-  for (int n = 0; n < NL; ++n) {
-    A2[n] = mine && n0 + n < p.N ? (float)((double)p.A[(size_t)c * p.N + n0 + n] * 1.4426950408889634) : 0.f;
-    h[n] = 0.f;
-    if (OUT && mine) {
-      if (seg > 0) h[n] = p.seg[(((size_t)(seg - 1) * p.B + b) * p.C + c) * NS + n0 + n];
-      else if (p.s_in && n0 + n < p.N) h[n] = p.s_in[((size_t)b * p.C + c) * p.N + n0 + n];
-    }
-  }
+  float D[E], bias[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     D[e] = OUT && p.D && e < here ? p.D[cr + e] : 0.f;
     bias[e] = p.bias && e < here ? p.bias[cr + e] : 0.f;
   }
-  float total = 0.f;                     // of d, for the segment's whole decay
-  Row<T, E> rx, rd, rz, ry, kx, kz;
-  T rB[NV], rC[NV];
+  const bool skip = p.D != nullptr;
+  Row<T, E> rx, rd, rz, ry, kx, kz, px, pz;      // of the next chunk, of the one under way, of the one before
+  Shared<T, L, NS> rB, rC;
   rx.zero(), rd.zero(), rz.zero(), ry.zero();
   const T* const Bp = (const T*)(REV ? p.Cm : p.Bm) + (size_t)b * (REV ? p.csb : p.bsb) + (size_t)at_.g * (REV ? p.csg : p.bsg);
   const T* const Cp = (const T*)p.Cm + (size_t)b * p.csb + (size_t)at_.g * p.csg;
@@ -88,317 +184,331 @@ __global__ __launch_bounds__(256) void ring_scan_kernel(RingScanArgs p) {
       if ((OUT || REV) && p.z.p) rz.load((const T*)p.z.p + b * p.z.sb + t * p.z.st + cr, p.wide, here);
       if (REV) ry.load((const T*)p.dy.p + b * p.dy.sb + t * p.dy.st + cr, p.wide, here);
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int k = tid + 256 * i, tk = t0 + k / NS, n = k % NS;
-      const bool there = k < L * NS && tk < end && n < p.N;
-      rB[i] = there ? Bp[(long)tk * (REV ? p.cst : p.bst) + n] : (T)0.f;
-      if (OUT) rC[i] = there ? Cp[(long)tk * p.cst + n] : (T)0.f;
-    }
+    rB.load(Bp, REV ? p.cst : p.bst, t0, end, p.N, tid);
+    if (OUT) rC.load(Cp, p.cst, t0, end, p.N, tid);
   };
-  auto lay = [&](int t0) {
-    const bool there = t0 + tl < end;
+  auto lay = [&](int k) {
+    const bool there = begin(k) + tl < end;
+    float d[E], u[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) d[e] = (float)rd.v[e] + bias[e];
+    if (p.softplus)
+#pragma unroll
+      for (int e = 0; e < E; ++e) d[e] = softplus<sizeof(T) == 4>(d[e]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) u[e] = REV ? (float)ry.v[e] : d[e] * (float)rx.v[e];
+    if (REV && p.z.p)
+#pragma unroll
+      for (int e = 0; e < E; ++e) u[e] *= silu<sizeof(T) == 4>((float)rz.v[e]);
+    float *const d_ = sd[k & 1] + at<L>(cl, tl), *const u_ = su[k & 1] + at<L>(cl, tl);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      float d = 0.f, u = 0.f;
-      if (there && e < here) {
-        d = (float)rd.v[e] + bias[e];
-        if (p.softplus) d = softplus(d);
-        if (REV) u = p.z.p ? (float)ry.v[e] * silu((float)rz.v[e]) : (float)ry.v[e];
-        else u = d * (float)rx.v[e];
-      }
-      sd[at<L>(cl + e, tl)] = d;
-      su[at<L>(cl + e, tl)] = u;
+      const bool counts = there && e < here;
+      d_[e * (L + 4)] = counts ? d[e] : 0.f;
+      u_[e * (L + 4)] = counts ? u[e] : 0.f;
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int k = tid + 256 * i;
-      if (k < L * NS) {
-        sB[k] = (float)rB[i];
-        if (OUT) sC[k] = (float)rC[i];
-      }
-    }
+    rB.lay(sB[k & 1], tid);
+    if (OUT) rC.lay(sC[k & 1], tid);
   };
-  const int chunks = end > first ? (end - first + L - 1) / L : 0;
-  if (chunks > 0) load(first + (REV ? chunks - 1 : 0) * L);
+  auto finish = [&](int k) {
+    const int t = begin(k) + tl;
+    const float* const y_ = sy[k & 1] + (OUT ? at<L>(cl, tl) : 0);
+    Row<T, E> out;
+    float y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      y[e] = y_[e * (L + 4)];
+#pragma unroll
+      for (int i = 1; i < NB; ++i) y[e] += y_[i * PL + e * (L + 4)];
+      y[e] = skip ? fmaf(D[e], (float)px.v[e], y[e]) : y[e];
+    }
+    if (p.z.p)
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] *= silu<sizeof(T) == 4>((float)pz.v[e]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) out.v[e] = (T)(t < end ? y[e] : 0.f);
+    if (t < last && here > 0) out.store((T*)p.y + ((size_t)b * p.T + t) * p.C + cr, p.wide_out, here);
+  };
+  if (chunks > 0) {
+    load(begin(0));
+    lay(0);
+    kx = rx, kz = rz;
+    if (chunks > 1) load(begin(1));
+  }
+  __syncthreads();
   for (int k = 0; k < chunks; ++k) {
-    const int t0 = first + (REV ? chunks - 1 - k : k) * L;
-    __syncthreads();
-    lay(t0);
-    if (OUT) kx = rx, kz = rz;
-    if (k + 1 < chunks) load(REV ? t0 - L : t0 + L);
-    __syncthreads();
-#pragma unroll 2
-    for (int jj = 0; jj < L; jj += 4) {
-      const int j = REV ? L - 4 - jj : jj;
-      if (OUT && p.states && j % kSave == 0 && mine && t0 + j < end) {
-        float* s = p.states + (((size_t)b * p.saved + (t0 + j) / kSave) * p.C + c) * NS + n0;
-#pragma unroll
-        for (int n = 0; n < NL; ++n) s[n] = h[n];
-      }
-      const f32x4 d4 = *reinterpret_cast<const f32x4*>(sd + at<L>(ch, j)), u4 = *reinterpret_cast<const f32x4*>(su + at<L>(ch, j));
-      float y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int o = REV ? 3 - i : i;
-        float Bn[NL], Cn[NL];
-#pragma unroll
-        for (int n = 0; n < NL; ++n) {
-          Bn[n] = sB[(j + o) * NS + n0 + n];
-          if (OUT) Cn[n] = sC[(j + o) * NS + n0 + n];
-        }
-        y[o] = 0.f;
-        if (!OUT) total += d4[o];
-#pragma unroll
-        for (int n = 0; n < NL; ++n) {
-          const float a = __builtin_amdgcn_exp2f(d4[o] * A2[n]);
-          if (REV) h[n] = a * fmaf(u4[o], Bn[n], h[n]);
-          else h[n] = fmaf(a, h[n], u4[o] * Bn[n]);
-          if (OUT) y[o] = fmaf(h[n], Cn[n], y[o]);
-        }
-      }
-      if (OUT) {
-        // row r of 16 lanes is left with token (0, 2, 1, 3)[r]
-        const float sum = fold16(fold32(y[0], y[1]), fold32(y[2], y[3]));
-        sy[nb * PL + at<L>(ch, j + ((sub & 1) << 1 | sub >> 1))] = sum;
-      }
+    Row<T, E> nx, nz;
+    if (k + 1 < chunks) {
+      lay(k + 1);
+      nx = rx, nz = rz;
+      if (k + 2 < chunks) load(begin(k + 2));
     }
     if (OUT) {
-      __syncthreads();
-      const int t = t0 + tl;
-      if (t < last && here > 0) {
-        Row<T, E> out;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          float y = sy[at<L>(cl + e, tl)];
-#pragma unroll
-          for (int i = 1; i < NB; ++i) y += sy[i * PL + at<L>(cl + e, tl)];
-          if (p.D) y = fmaf(D[e], (float)kx.v[e], y);
-          if (p.z.p) y *= silu((float)kz.v[e]);
-          out.v[e] = (T)(t < end ? y : 0.f);
-        }
-        out.store((T*)p.y + ((size_t)b * p.T + t) * p.C + cr, p.wide_out, here);
-      }
+      if (k > 0) finish(k - 1);
+      px = kx, pz = kz;
+      kx = nx, kz = nz;
     }
+    __syncthreads();
   }
-  if (OUT) {                             // tokens that do not count
-    Row<T, E> none;
-    none.zero();
-    for (int t = first + chunks * L + tl; t < last; t += L)
-      if (here > 0) none.store((T*)p.y + ((size_t)b * p.T + t) * p.C + cr, p.wide_out, here);
-    if (p.s_out && seg == p.nseg - 1 && mine) {
-#pragma unroll
-      for (int n = 0; n < NL; ++n)
-        if (n0 + n < p.N) p.s_out[((size_t)b * p.C + c) * p.N + n0 + n] = h[n];
-    }
-  } else if (mine) {
-    const size_t row = ((size_t)at_.seg * p.B + b) * p.C + c;
-#pragma unroll
-    for (int n = 0; n < NL; ++n) p.seg[row * NS + n0 + n] = h[n];
-    if (n0 == 0) p.total[row] = total;
-  }
+  if (!OUT) return;
+  if (chunks > 0) finish(chunks - 1);
+  Row<T, E> none;                        // tokens that do not count
+  none.zero();
+  for (int t = first + chunks * L + tl; t < last; t += L)
+    if (here > 0) none.store((T*)p.y + ((size_t)b * p.T + t) * p.C + cr, p.wide_out, here);
 }
 
 // The gradients.  Chunks of kSave tokens against the time: forwards through a chunk from the state kept in front of it, powers and states in
 // registers, then back.  A quad of lanes shares a channel: sums over its states cross the quad, sums over channels (of dB and dC) the 16 quads.
 template <typename T, int NL, int NB>
-__global__ __launch_bounds__(256, 2) void ring_scan_bwd_kernel(RingScanArgs p) {
+__global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
   constexpr int CH = 64 / NB, L = kSave, E = CH / 16, NS = 4 * NL * NB, PL = plane<CH, L>(), CW = 4 / NB, R = 8 * NL;
-  constexpr int NV = (L * NS + 255) / 256;
-  __shared__ __attribute__((aligned(16))) float sd[PL], su[PL], sq[PL], sB[L * NS], sC[L * NS], so[3 * NB * PL], red[4][L * 32];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  __shared__ __attribute__((aligned(16))) float sd[2][PL], su[2][PL], sq[2][PL], sB[2][L * NS], sC[2][L * NS], so[2][3 * NB * PL], red[2][4 * L * R],
+      sums[32 * CH];
+  const int tid = threadIdx.x & 255, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Place at_ = place<CH>(p);
   const int seg = at_.seg, b = at_.b;
   const int len = length_of(p.lengths, b, p.T), first = seg * p.seg_tokens, last = min(first + p.seg_tokens, p.T), end = min(last, len);
-  const int nb = w % NB, ch = w / NB * 16 + (lane >> 2), sub = lane & 3, n0 = nb * 4 * NL + sub * NL, c = at_.c0 + ch;
-  const bool mine = ch < at_.here;
-  const int tl = tid >> 4, cl = (tid & 15) * E, cr = at_.c0 + cl, here = at_.here - cl;
-  float A2[NL], G[NL], dA[NL], D[E], bias[E], dD[E], dbias[E];
+  const int chunks = end > first ? (end - first + L - 1) / L : 0;
+  const bool shared = p.part_bc != nullptr;
+  auto begin = [&](int k) { return first + (chunks - 1 - k) * L; };
+  float* const part = p.part_a ? p.part_a + ((size_t)seg * p.B + b) * p.C * (NS + 2) : nullptr;
+  if (w < 4) {
+    const int nb = w % NB, ch = w / NB * 16 + (lane >> 2), sub = lane & 3, n0 = nb * 4 * NL + sub * NL, c = at_.c0 + ch;
+    const bool mine = ch < at_.here;
+    float A2[NL], G[NL], dA[NL], hk[NL];   // hk: the state kept in front of the next chunk
 #pragma unroll
-  for (int n = 0; n < NL; ++n) {
-    A2[n] = mine && n0 + n < p.N ? (float)((double)p.A[(size_t)c * p.N + n0 + n] * 1.4426950408889634) : 0.f;
-    G[n] = dA[n] = 0.f;
-    if (mine) {
-      if (seg < p.nseg - 1) G[n] = p.seg[(((size_t)(p.nseg - 2 - seg) * p.B + b) * p.C + c) * NS + n0 + n];
-      else if (p.s_in && n0 + n < p.N) G[n] = p.s_in[((size_t)b * p.C + c) * p.N + n0 + n];
+    for (int n = 0; n < NL; ++n) {
+      A2[n] = mine && n0 + n < p.N ? (float)((double)p.A[(size_t)c * p.N + n0 + n] * 1.4426950408889634) : 0.f;
+      G[n] = dA[n] = hk[n] = 0.f;
+      if (mine) {
+        if (seg < p.nseg - 1) G[n] = p.seg[(((size_t)(p.nseg - 2 - seg) * p.B + b) * p.C + c) * NS + n0 + n];
+        else if (p.s_in && n0 + n < p.N) G[n] = p.s_in[((size_t)b * p.C + c) * p.N + n0 + n];
+      }
     }
+    auto kept = [&](int k) {
+      if (mine) take<NL>(hk, p.states + (((size_t)b * p.saved + begin(k) / kSave) * p.C + c) * NS + n0);
+    };
+    if (chunks > 0) kept(0);
+    __syncthreads();
+    const int r = lane >> 4, quad = lane >> 2 & 3;
+    auto chunk = [&](int k, auto whole) {
+      const int t0 = begin(k), f = k & 1;
+      float h[NL], hs[L][NL], as[L][NL], dAc[NL];
+#pragma unroll
+      for (int n = 0; n < NL; ++n) {
+        h[n] = hk[n];
+        dAc[n] = 0.f;
+      }
+      if (k + 1 < chunks) kept(k + 1);
+      const float *d_ = sd[f] + at<L>(ch, 0), *u_ = su[f] + at<L>(ch, 0), *q_ = sq[f] + at<L>(ch, 0), *B_ = sB[f] + n0, *C_ = sC[f] + n0;
+      float* const o_ = so[f] + nb * PL + at<L>(ch, sub);
+      // where a lane's sums of dB and dC lie: row r has type r >> 1 and, of four states, half r & 1; quads have values (0, 2, 1, 3) of four
+      constexpr int LEFT = NL > 1 ? NL / 2 : 1, VAL = 4 * LEFT;
+      const int mine4 = quad >> 1 | (quad & 1) << 1;
+      float* const r_ = red[f] + w * L * R + (r >> 1) * 4 * NL + sub * NL + (NL > 1 ? (r & 1) * LEFT : 0) + mine4 / LEFT * R + mine4 % LEFT;
+#pragma unroll
+      for (int j = 0; j < L; j += 4) {
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(d_ + j), u4 = *reinterpret_cast<const f32x4*>(u_ + j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float Bn[NL];
+          take<NL>(Bn, B_ + (j + i) * NS);
+#pragma unroll
+          for (int n = 0; n < NL; ++n) {
+            hs[j + i][n] = h[n];
+            as[j + i][n] = __builtin_amdgcn_exp2f(d4[i] * A2[n]);
+            h[n] = fmaf(as[j + i][n], h[n], u4[i] * Bn[n]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int j = L - 4; j >= 0; j -= 4) {
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(d_ + j), u4 = *reinterpret_cast<const f32x4*>(u_ + j), q4 = *reinterpret_cast<const f32x4*>(q_ + j);
+        float s1[4], s2[4], y[4], val[VAL];
+#pragma unroll
+        for (int i = 3; i >= 0; --i) {
+          float v[2 * NL], Bn[NL], Cn[NL];
+          take<NL>(Bn, B_ + (j + i) * NS);
+          take<NL>(Cn, C_ + (j + i) * NS);
+          // (behind the last token that counts no state takes part in dA, however large)
+          if constexpr (!decltype(whole)::value)
+            if (t0 + j + i + 1 == end)
+#pragma unroll
+              for (int n = 0; n < NL; ++n) dAc[n] = 0.f;
+#pragma unroll
+          for (int n = 0; n < NL; ++n) {
+            y[i] = n == 0 ? Cn[n] * h[n] : fmaf(Cn[n], h[n], y[i]);
+            v[NL + n] = q4[i] * h[n];
+            const float g = fmaf(q4[i], Cn[n], G[n]);
+            v[n] = g * u4[i];
+            s1[i] = n == 0 ? g * Bn[n] : fmaf(g, Bn[n], s1[i]);
+            G[n] = as[j + i][n] * g;
+            h[n] = hs[j + i][n];
+            const float turn = G[n] * h[n];
+            s2[i] = n == 0 ? turn * A2[n] : fmaf(turn, A2[n], s2[i]);
+            dAc[n] = fmaf(d4[i], turn, dAc[n]);
+          }
+          // over the 16 quads: halves, rows
+#pragma unroll
+          for (int m = 0; m < NL; ++m) v[m] = fold32(v[m], v[NL + m]);
+#pragma unroll
+          for (int m = 0; m < LEFT; ++m) val[i * LEFT + m] = fold16(v[m], NL > 1 ? v[NL / 2 + m] : v[m]);
+        }
+        // over a quad, whose lane sub is left with token j + sub
+        o_[j] = quad_sums(s1, sub);
+        o_[NB * PL + j] = quad_sums(s2, sub);
+        o_[2 * NB * PL + j] = quad_sums(y, sub);
+        // over a row's quads
+#pragma unroll
+        for (int m = 0; m < LEFT; ++m) r_[(j + m * 4 / LEFT) * R] = row_sums(val + 4 * m, quad);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int n = 0; n < NL; ++n) dA[n] += dAc[n];
+      __syncthreads();
+    };
+    int k = 0;
+    if (chunks > 0 && begin(0) + L > end) chunk(k++, std::false_type{});
+    for (; k < chunks; ++k) chunk(k, std::true_type{});
+    if (mine) {
+      if (part) {
+#pragma unroll
+        for (int n = 0; n < NL; ++n) part[(size_t)c * (NS + 2) + n0 + n] = dA[n];
+      }
+      if (seg == 0 && p.s_out) {
+#pragma unroll
+        for (int n = 0; n < NL; ++n)
+          if (n0 + n < p.N) p.s_out[((size_t)b * p.C + c) * p.N + n0 + n] = G[n];
+      }
+    }
+    __syncthreads();
+    return;
   }
+  const int tl = tid >> 4, cl = (tid & 15) * E, cr = at_.c0 + cl, here = at_.here - cl;
+  float D[E], bias[E], dD[E], dbias[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     D[e] = p.D && e < here ? p.D[cr + e] : 0.f;
     bias[e] = p.bias && e < here ? p.bias[cr + e] : 0.f;
     dD[e] = dbias[e] = 0.f;
   }
-  Row<T, E> rx, rd, rz, ry, kx, kz, ky, kd;
-  rx.zero(), rd.zero(), rz.zero(), ry.zero();
-  T rB[NV], rC[NV];
+  struct Rows { Row<T, E> x, d, z, y; } r;       // of the chunk that is read next
+  struct Known { Rows r; float d[E], q[E], slope[E], gate[E]; } next, now, before;      // of the one just laid down, of the one under way, of the one before
+  r.x.zero(), r.d.zero(), r.z.zero(), r.y.zero();
+  Shared<T, L, NS> rB, rC;
   const T* const Bp = (const T*)p.Bm + (size_t)b * p.bsb + (size_t)at_.g * p.bsg;
   const T* const Cp = (const T*)p.Cm + (size_t)b * p.csb + (size_t)at_.g * p.csg;
-  float hk[NL];                          // the state kept in front of a chunk
   auto load = [&](int t0) {
     const int t = t0 + tl;
     if (t < end && here > 0) {
-      rd.load((const T*)p.delta.p + b * p.delta.sb + t * p.delta.st + cr, p.wide, here);
-      rx.load((const T*)p.x.p + b * p.x.sb + t * p.x.st + cr, p.wide, here);
-      if (p.z.p) rz.load((const T*)p.z.p + b * p.z.sb + t * p.z.st + cr, p.wide, here);
-      ry.load((const T*)p.dy.p + b * p.dy.sb + t * p.dy.st + cr, p.wide, here);
+      r.d.load((const T*)p.delta.p + b * p.delta.sb + t * p.delta.st + cr, p.wide, here);
+      r.x.load((const T*)p.x.p + b * p.x.sb + t * p.x.st + cr, p.wide, here);
+      if (p.z.p) r.z.load((const T*)p.z.p + b * p.z.sb + t * p.z.st + cr, p.wide, here);
+      r.y.load((const T*)p.dy.p + b * p.dy.sb + t * p.dy.st + cr, p.wide, here);
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int k = tid + 256 * i, tk = t0 + k / NS, n = k % NS;
-      const bool there = k < L * NS && tk < end && n < p.N;
-      rB[i] = there ? Bp[(long)tk * p.bst + n] : (T)0.f;
-      rC[i] = there ? Cp[(long)tk * p.cst + n] : (T)0.f;
-    }
-#pragma unroll
-    for (int n = 0; n < NL; ++n) hk[n] = mine ? p.states[(((size_t)b * p.saved + t0 / kSave) * p.C + c) * NS + n0 + n] : 0.f;
+    rB.load(Bp, p.bst, t0, end, p.N, tid);
+    rC.load(Cp, p.cst, t0, end, p.N, tid);
   };
-  auto lay = [&](int t0) {
-    const bool there = t0 + tl < end;
+  auto lay = [&](int k) {
+    const bool there = begin(k) + tl < end;
+    float d[E], q[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      float d = 0.f, u = 0.f, q = 0.f;
-      if (there && e < here) {
-        d = (float)rd.v[e] + bias[e];
-        if (p.softplus) d = softplus(d);
-        u = d * (float)rx.v[e];
-        q = p.z.p ? (float)ry.v[e] * silu((float)rz.v[e]) : (float)ry.v[e];
-      }
-      sd[at<L>(cl + e, tl)] = d;
-      su[at<L>(cl + e, tl)] = u;
-      sq[at<L>(cl + e, tl)] = q;
+      d[e] = (float)r.d.v[e] + bias[e];
+      q[e] = (float)r.y.v[e];
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int k = tid + 256 * i;
-      if (k < L * NS) {
-        sB[k] = (float)rB[i];
-        sC[k] = (float)rC[i];
-      }
-    }
-  };
-  const int chunks = end > first ? (end - first + L - 1) / L : 0;
-  const bool shared = p.part_bc != nullptr;
-  if (chunks > 0) load(first + (chunks - 1) * L);
-  for (int k = chunks - 1; k >= 0; --k) {
-    const int t0 = first + k * L;
-    __syncthreads();
-    lay(t0);
-    kx = rx, kz = rz, ky = ry, kd = rd;
-    float h[NL];
+    for (int e = 0; e < E; ++e) next.slope[e] = next.gate[e] = 1.f;
+    if (p.softplus)
 #pragma unroll
-    for (int n = 0; n < NL; ++n) h[n] = hk[n];
-    if (k > 0) load(t0 - L);
-    __syncthreads();
-    float hs[L][NL], as[L][NL], dAc[NL];
-#pragma unroll
-    for (int j = 0; j < L; j += 4) {
-      const f32x4 d4 = *reinterpret_cast<const f32x4*>(sd + at<L>(ch, j)), u4 = *reinterpret_cast<const f32x4*>(su + at<L>(ch, j));
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int n = 0; n < NL; ++n) {
-          hs[j + i][n] = h[n];
-          as[j + i][n] = __builtin_amdgcn_exp2f(d4[i] * A2[n]);
-          h[n] = fmaf(as[j + i][n], h[n], u4[i] * sB[(j + i) * NS + n0 + n]);
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < NL; ++n) dAc[n] = 0.f;
-#pragma unroll
-    for (int j = L - 4; j >= 0; j -= 4) {
-      const f32x4 d4 = *reinterpret_cast<const f32x4*>(sd + at<L>(ch, j)), u4 = *reinterpret_cast<const f32x4*>(su + at<L>(ch, j)),
-                  q4 = *reinterpret_cast<const f32x4*>(sq + at<L>(ch, j));
-#pragma unroll
-      for (int i = 3; i >= 0; --i) {
-        float s1 = 0.f, s2 = 0.f, y = 0.f, v[2 * NL];
-        if (t0 + j + i + 1 == end)         // (behind the last token that counts no state takes part in dA, however large)
-#pragma unroll
-          for (int n = 0; n < NL; ++n) dAc[n] = 0.f;
-#pragma unroll
-        for (int n = 0; n < NL; ++n) {
-          const float Bn = sB[(j + i) * NS + n0 + n], Cn = sC[(j + i) * NS + n0 + n];
-          y = fmaf(Cn, h[n], y);
-          v[NL + n] = q4[i] * h[n];
-          const float g = fmaf(q4[i], Cn, G[n]);
-          v[n] = g * u4[i];
-          s1 = fmaf(g, Bn, s1);
-          G[n] = as[j + i][n] * g;
-          h[n] = hs[j + i][n];
-          const float turn = G[n] * h[n];
-          s2 = fmaf(turn, A2[n], s2);
-          dAc[n] = fmaf(d4[i], turn, dAc[n]);
-        }
-        s1 = plus_dpp<kXor2>(plus_dpp<kXor1>(s1));
-        s2 = plus_dpp<kXor2>(plus_dpp<kXor1>(s2));
-        y = plus_dpp<kXor2>(plus_dpp<kXor1>(y));
-        if (sub < 3) so[(sub * NB + nb) * PL + at<L>(ch, j + i)] = sub == 0 ? s1 : (sub == 1 ? s2 : y);
-        if (shared) {
-          // over the 16 quads: halves, rows, then within a row; a lane of row r keeps the values r >> 1 and r & 1 name
-#pragma unroll
-          for (int m = 0; m < NL; ++m) v[m] = fold32(v[m], v[NL + m]);
-          if constexpr (NL > 1) {
-#pragma unroll
-            for (int m = 0; m < NL / 2; ++m) v[m] = fold16(v[m], v[NL / 2 + m]);
-          } else {
-            v[0] = fold16(v[0], v[0]);
-          }
-          constexpr int LEFT = NL > 1 ? NL / 2 : 1;
-          const int r = lane >> 4, type = r >> 1, half = NL > 1 ? (r & 1) * LEFT : 0;
-#pragma unroll
-          for (int m = 0; m < LEFT; ++m) {
-            const float sum = plus_dpp<kRor4>(plus_dpp<kRor8>(v[m]));
-            if ((lane & 12) == 0) red[w][(j + i) * R + type * 4 * NL + sub * NL + half + m] = sum;
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < NL; ++n) dA[n] += dAc[n];
-    __syncthreads();
-    const int t = t0 + tl;
-    if (t < last && here > 0) {
-      Row<T, E> ox, od, oz;
+      for (int e = 0; e < E; ++e) d[e] = softplus<sizeof(T) == 4>(d[e], next.slope[e]);
+    if (p.z.p)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        float s1 = 0.f, s2 = 0.f, y = 0.f;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          s1 += so[i * PL + at<L>(cl + e, tl)];
-          s2 += so[(NB + i) * PL + at<L>(cl + e, tl)];
-          y += so[(2 * NB + i) * PL + at<L>(cl + e, tl)];
-        }
-        const float d = sd[at<L>(cl + e, tl)], q = sq[at<L>(cl + e, tl)], x = (float)kx.v[e];
-        float dd = fmaf(s1, x, s2 * kLn2);
-        if (p.softplus) dd *= sigmoid((float)kd.v[e] + bias[e]);
-        const bool counts = t < end && e < here;
-        ox.v[e] = (T)(counts ? fmaf(D[e], q, d * s1) : 0.f);
-        od.v[e] = (T)(counts ? dd : 0.f);
-        if (counts) {
-          dD[e] = fmaf(q, x, dD[e]);
-          dbias[e] += dd;
-        }
-        if (p.z.p) {
-          const float z = (float)kz.v[e], s = sigmoid(z);
-          oz.v[e] = (T)(counts ? (float)ky.v[e] * fmaf(D[e], x, y) * silu_slope(z, s) : 0.f);
-        }
+        next.gate[e] = sigmoid<sizeof(T) == 4>((float)r.z.v[e]);
+        q[e] *= (float)r.z.v[e] * next.gate[e];
       }
+    float *const d_ = sd[k & 1] + at<L>(cl, tl), *const u_ = su[k & 1] + at<L>(cl, tl), *const q_ = sq[k & 1] + at<L>(cl, tl);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const bool counts = there && e < here;
+      d_[e * (L + 4)] = counts ? d[e] : 0.f;
+      u_[e * (L + 4)] = counts ? d[e] * (float)r.x.v[e] : 0.f;
+      q_[e * (L + 4)] = counts ? q[e] : 0.f;
+      next.d[e] = d[e];
+      next.q[e] = q[e];
+    }
+    next.r = r;
+    rB.lay(sB[k & 1], tid);
+    rC.lay(sC[k & 1], tid);
+  };
+  const int tile = (at_.c0 - at_.g * (p.C / p.G)) / CH;
+  auto finish = [&](int k) {
+    const int t0 = begin(k), t = t0 + tl, f = k & 1;
+    const float* const o_ = so[f] + at<L>(cl, tl);
+    Row<T, E> ox, od, oz;
+    float s1[E], s2[E], y[E], dd[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      s1[e] = s2[e] = y[e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        s1[e] += o_[i * PL + e * (L + 4)];
+        s2[e] += o_[(NB + i) * PL + e * (L + 4)];
+        y[e] += o_[(2 * NB + i) * PL + e * (L + 4)];
+      }
+      dd[e] = fmaf(s1[e], (float)before.r.x.v[e], s2[e] * kLn2) * before.slope[e];
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const bool counts = t < end && e < here;
+      const float x = (float)before.r.x.v[e];
+      ox.v[e] = (T)(counts ? fmaf(D[e], before.q[e], before.d[e] * s1[e]) : 0.f);
+      od.v[e] = (T)(counts ? dd[e] : 0.f);
+      dD[e] = counts ? fmaf(before.q[e], x, dD[e]) : dD[e];
+      dbias[e] = counts ? dbias[e] + dd[e] : dbias[e];
+    }
+    if (p.z.p)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float g = (float)before.r.y.v[e] * fmaf(D[e], (float)before.r.x.v[e], y[e]) * silu_slope((float)before.r.z.v[e], before.gate[e]);
+        oz.v[e] = (T)(t < end && e < here ? g : 0.f);
+      }
+    if (t < last && here > 0) {
       const size_t row = ((size_t)b * p.T + t) * p.C + cr;
       if (p.dx) ox.store((T*)p.dx + row, p.wide_out, here);
       if (p.ddelta) od.store((T*)p.ddelta + row, p.wide_out, here);
       if (p.dz) oz.store((T*)p.dz + row, p.wide_out, here);
     }
-    if (shared) {
-      const int tile = (at_.c0 - at_.g * (p.C / p.G)) / CH;
+    if (shared)
       for (int i = tid; i < L * 2 * NS; i += 256) {
         const int tk = i / (2 * NS), type = i / NS % 2, n = i % NS, block = n / (4 * NL);
         float sum = 0.f;
 #pragma unroll
-        for (int m = 0; m < CW; ++m) sum += red[m * NB + block][tk * R + type * 4 * NL + n % (4 * NL)];
+        for (int m = 0; m < CW; ++m) sum += red[f][((m * NB + block) * L + tk) * R + type * 4 * NL + n % (4 * NL)];
         if (t0 + tk < end) p.part_bc[((((size_t)tile * p.B + b) * p.T + t0 + tk) * p.G + at_.g) * 2 * NS + type * NS + n] = sum;
       }
-    }
+  };
+  if (chunks > 0) {
+    load(begin(0));
+    lay(0);
+    now = next;
+    if (chunks > 1) load(begin(1));
   }
+  __syncthreads();
+  for (int k = 0; k < chunks; ++k) {
+    if (k + 1 < chunks) {
+      lay(k + 1);
+      if (k + 2 < chunks) load(begin(k + 2));
+    }
+    if (k > 0) finish(k - 1);
+    before = now;
+    now = next;
+    __syncthreads();
+  }
+  if (chunks > 0) finish(chunks - 1);
   Row<T, E> none;                        // tokens that do not count
   none.zero();
   for (int t = first + chunks * L + tl; t < last; t += L)
@@ -408,32 +518,17 @@ __global__ __launch_bounds__(256, 2) void ring_scan_bwd_kernel(RingScanArgs p) {
       if (p.ddelta) none.store((T*)p.ddelta + row, p.wide_out, here);
       if (p.dz) none.store((T*)p.dz + row, p.wide_out, here);
     }
-  if (mine && seg == 0 && p.s_out) {
+  // the 16 threads of a channel, in order
 #pragma unroll
-    for (int n = 0; n < NL; ++n)
-      if (n0 + n < p.N) p.s_out[((size_t)b * p.C + c) * p.N + n0 + n] = G[n];
+  for (int e = 0; e < E; ++e) {
+    sums[tl * CH + cl + e] = dD[e];
+    sums[16 * CH + tl * CH + cl + e] = dbias[e];
   }
-  if (p.part_a) {
-    float* part = p.part_a + ((size_t)seg * p.B + b) * p.C * (NS + 2);
-    if (mine) {
-#pragma unroll
-      for (int n = 0; n < NL; ++n) part[(size_t)c * (NS + 2) + n0 + n] = dA[n];
-    }
-    // the 16 threads of a channel, in order
-    static_assert(sizeof(red) >= 16 * CH * 2 * sizeof(float), "room for the sums");
-    float* sums = &red[0][0];
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      sums[tl * CH + cl + e] = dD[e];
-      sums[16 * CH + tl * CH + cl + e] = dbias[e];
-    }
-    __syncthreads();
-    if (tid < 2 * CH && tid % CH < at_.here) {
-      float sum = 0.f;
-      for (int i = 0; i < 16; ++i) sum += sums[tid / CH * 16 * CH + i * CH + tid % CH];
-      part[(size_t)(at_.c0 + tid % CH) * (NS + 2) + NS + tid / CH] = sum;
-    }
+  __syncthreads();
+  if (part && tid < 2 * CH && tid % CH < at_.here) {
+    float sum = 0.f;
+    for (int i = 0; i < 16; ++i) sum += sums[tid / CH * 16 * CH + i * CH + tid % CH];
+    part[(size_t)(at_.c0 + tid % CH) * (NS + 2) + NS + tid / CH] = sum;
   }
 }
 
@@ -442,7 +537,7 @@ template <typename T, int NL, int NB> hipError_t launch_sized(const RingScanArgs
   RingScanArgs a = p;
   a.tiles = (p.C / p.G + CH - 1) / CH;
   const int segs = mode == RING_SCAN_STATE || mode == RING_SCAN_ADJOINT ? p.nseg - 1 : p.nseg;
-  const dim3 grid((unsigned)((size_t)a.tiles * p.G * p.B * segs)), block(256);
+  const dim3 grid((unsigned)((size_t)a.tiles * p.G * p.B * segs)), block(512);
   if (mode == RING_SCAN_OUTPUTS) hipLaunchKernelGGL((ring_scan_kernel<T, NL, NB, kOutputs>), grid, block, 0, st, a);
   else if (mode == RING_SCAN_STATE) hipLaunchKernelGGL((ring_scan_kernel<T, NL, NB, kState>), grid, block, 0, st, a);
   else if (mode == RING_SCAN_ADJOINT) hipLaunchKernelGGL((ring_scan_kernel<T, NL, NB, kAdjoint>), grid, block, 0, st, a);
