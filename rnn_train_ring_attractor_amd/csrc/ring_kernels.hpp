@@ -428,7 +428,7 @@ struct RingScanArgs {
   float* part_bc;                        // [tiles,B,T,G,2,NS] sums of dB and dC over a tile's channels, null: not wanted
   float* part_a;                         // [nseg,B,C,NS + 2] gradients of A, D and bias of a segment, null: not wanted
   int B, T, C, N, G, saved, nseg, seg_tokens, softplus;
-  bool wide, wide_out;                   // rows read, and written, are whole numbers of eight channels at 16 bytes
+  bool wide;                             // rows are whole numbers of eight channels at 16 bytes
   int tiles;                             // (the launcher's) of a group's channels
 };
 struct RingScanShape { int B, T, C, N, G, type; };

@@ -67,6 +67,15 @@ template <typename T, int E> struct Row {
       for (int e = 0; e < E; ++e) v[e] = e < here ? p[e] : (T)0.f;
     }
   }
+  // The same without conditions: `here` of them (at least one) and copies of the last
+  template <bool WIDE> __device__ __forceinline__ void read(const T* p, int here) {
+    if constexpr (WIDE) {
+      load(p, true, E);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = p[min(e, here - 1)];
+    }
+  }
   __device__ __forceinline__ void store(T* p, bool wide, int here) const {
     constexpr int W = E * sizeof(T) > 16 ? 16 / sizeof(T) : E;
     typedef T part __attribute__((ext_vector_type(W)));

@@ -37,6 +37,7 @@ struct Place { int seg, b, g, c0, here; };      // segment, sequence, group, fir
 template <int CH> __device__ __forceinline__ Place place(const RingScanArgs& p) {
   const unsigned all = (unsigned)p.tiles * p.G;
   unsigned i = blockIdx.x;
+  if (gridDim.x % 8 == 0) i = i % 8 * (gridDim.x / 8) + i / 8;       // neighbours, which share rows, lines and pages, on one XCD
   const int tile = (int)(i % all);
   i /= all;
   const int g = tile / p.tiles, first = (tile - g * p.tiles) * CH, Cg = p.C / p.G;
@@ -88,7 +89,7 @@ template <typename T, int L, int NS> struct Shared {
 
 // Outputs (and the states kept for a backward), or what a segment adds to a state of zeros, or, backwards in time, to an adjoint of zeros.
 // The first four waves go through the tokens; the other four read and work out the next chunk's rows and finish the last one's outputs meanwhile.
-template <typename T, int NL, int NB, int MODE>
+template <typename T, int NL, int NB, int MODE, bool WIDE>
 __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
   constexpr int CH = 64 / NB, L = kL, E = CH / 8, NS = 4 * NL * NB, PL = plane<CH, L>();
   constexpr bool REV = MODE == kAdjoint, OUT = MODE == kOutputs;
@@ -117,29 +118,53 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
       const int t0 = begin(k);
       const float *d_ = sd[k & 1] + at<L>(ch, 0), *u_ = su[k & 1] + at<L>(ch, 0), *B_ = sB[k & 1] + n0, *C_ = sC[k & 1] + n0;
       float* const y_ = sy[k & 1] + (OUT ? nb * PL + at<L>(ch, (sub & 1) << 1 | sub >> 1) : 0);
-#pragma unroll 4
+      // Four tokens at a time, what the next four need on its way from LDS; powers and inputs of the four first, then the states one after another (without
+      // the order, which the compiler does not find by itself, the wave waits for LDS and for every power)
+      struct Four { f32x4 d, u; float B[4][NL], C[4][NL]; } g[2];
+      auto fetch = [&](int j, Four& f) {
+        f.d = *reinterpret_cast<const f32x4*>(d_ + j);
+        f.u = *reinterpret_cast<const f32x4*>(u_ + j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          take<NL>(f.B[i], B_ + (j + i) * NS);
+          if (OUT) take<NL>(f.C[i], C_ + (j + i) * NS);
+        }
+      };
+      fetch(REV ? L - 4 : 0, g[0]);
+#pragma unroll
       for (int jj = 0; jj < L; jj += 4) {
         const int j = REV ? L - 4 - jj : jj;
+        const Four& f = g[jj / 4 & 1];
         if (OUT && p.states && j % kSave == 0 && mine && t0 + j < end) {
           float* s = p.states + (((size_t)b * p.saved + (t0 + j) / kSave) * p.C + c) * NS + n0;
 #pragma unroll
           for (int n = 0; n < NL; ++n) s[n] = h[n];
         }
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(d_ + j), u4 = *reinterpret_cast<const f32x4*>(u_ + j);
-        float y[4];
+        if (jj + 4 < L) fetch(REV ? j - 4 : j + 4, g[jj / 4 + 1 & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+        float a[4][NL], v[4][NL], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (!OUT) total += f.d[i];
+#pragma unroll
+          for (int n = 0; n < NL; ++n) a[i][n] = f.d[i] * A2[n];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int n = 0; n < NL; ++n) {
+            a[i][n] = __builtin_amdgcn_exp2f(a[i][n]);
+            if (!REV) v[i][n] = f.u[i] * f.B[i][n];
+          }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int o = REV ? 3 - i : i;
-          float Bn[NL], Cn[NL];
-          take<NL>(Bn, B_ + (j + o) * NS);
-          if (OUT) take<NL>(Cn, C_ + (j + o) * NS);
-          if (!OUT) total += d4[o];
 #pragma unroll
           for (int n = 0; n < NL; ++n) {
-            const float a = __builtin_amdgcn_exp2f(d4[o] * A2[n]);
-            if (REV) h[n] = a * fmaf(u4[o], Bn[n], h[n]);
-            else h[n] = fmaf(a, h[n], u4[o] * Bn[n]);
-            if (OUT) y[o] = n == 0 ? h[n] * Cn[n] : fmaf(h[n], Cn[n], y[o]);
+            if (REV) h[n] = a[o][n] * fmaf(f.u[o], f.B[o][n], h[n]);
+            else h[n] = fmaf(a[o][n], h[n], v[o][n]);
+            if (OUT) y[o] = n == 0 ? h[n] * f.C[o][n] : fmaf(h[n], f.C[o][n], y[o]);
           }
         }
         // row r of 16 lanes is left with token (0, 2, 1, 3)[r]
@@ -170,36 +195,39 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
     D[e] = OUT && p.D && e < here ? p.D[cr + e] : 0.f;
     bias[e] = p.bias && e < here ? p.bias[cr + e] : 0.f;
   }
+  // Rows two chunks ahead: a chunk takes less time than a row from memory (one chunk ahead: 255 us in place of FWD2 for eight sequences of 2048 tokens, 2048
+  // channels).  Reads have no conditions, which the compiler could not count them by: what is not there is read from a place that is, and left out.
   const bool skip = p.D != nullptr;
-  Row<T, E> rx, rd, rz, ry, kx, kz, px, pz;      // of the next chunk, of the one under way, of the one before
-  Shared<T, L, NS> rB, rC;
-  rx.zero(), rd.zero(), rz.zero(), ry.zero();
+  struct In { Row<T, E> x, d, z, y; Shared<T, L, NS> B, C; } in[2];
+  struct { Row<T, E> x, z; } now, before;
+  const int tr = here > 0 ? here : at_.here, cw = here > 0 ? cr : at_.c0;
+  const T *const dp = (const T*)p.delta.p + b * p.delta.sb + cw, *const xp = (const T*)(REV ? p.dy.p : p.x.p) + b * (REV ? p.dy.sb : p.x.sb) + cw,
+          *const zp = p.z.p ? (const T*)p.z.p + b * p.z.sb + cw : xp;
+  const long xt = REV ? p.dy.st : p.x.st, zt = p.z.p ? p.z.st : xt;
   const T* const Bp = (const T*)(REV ? p.Cm : p.Bm) + (size_t)b * (REV ? p.csb : p.bsb) + (size_t)at_.g * (REV ? p.csg : p.bsg);
   const T* const Cp = (const T*)p.Cm + (size_t)b * p.csb + (size_t)at_.g * p.csg;
-  auto load = [&](int t0) {
-    const int t = t0 + tl;
-    if (t < end && here > 0) {
-      rd.load((const T*)p.delta.p + b * p.delta.sb + t * p.delta.st + cr, p.wide, here);
-      if (!REV) rx.load((const T*)p.x.p + b * p.x.sb + t * p.x.st + cr, p.wide, here);
-      if ((OUT || REV) && p.z.p) rz.load((const T*)p.z.p + b * p.z.sb + t * p.z.st + cr, p.wide, here);
-      if (REV) ry.load((const T*)p.dy.p + b * p.dy.sb + t * p.dy.st + cr, p.wide, here);
-    }
-    rB.load(Bp, REV ? p.cst : p.bst, t0, end, p.N, tid);
-    if (OUT) rC.load(Cp, p.cst, t0, end, p.N, tid);
+  auto load = [&](int k, In& r) {
+    const int t0 = begin(min(k, chunks - 1));
+    const long t = min(t0 + tl, end - 1);
+    r.d.template read<WIDE>(dp + t * p.delta.st, tr);
+    r.x.template read<WIDE>(xp + t * xt, tr);
+    if (OUT || REV) r.z.template read<WIDE>(zp + t * zt, tr);
+    r.B.load(Bp, REV ? p.cst : p.bst, t0, end, p.N, tid);
+    if (OUT) r.C.load(Cp, p.cst, t0, end, p.N, tid);
   };
-  auto lay = [&](int k) {
+  auto lay = [&](int k, const In& r) {
     const bool there = begin(k) + tl < end;
     float d[E], u[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) d[e] = (float)rd.v[e] + bias[e];
+    for (int e = 0; e < E; ++e) d[e] = (float)r.d.v[e] + bias[e];
     if (p.softplus)
 #pragma unroll
       for (int e = 0; e < E; ++e) d[e] = softplus<sizeof(T) == 4>(d[e]);
 #pragma unroll
-    for (int e = 0; e < E; ++e) u[e] = REV ? (float)ry.v[e] : d[e] * (float)rx.v[e];
+    for (int e = 0; e < E; ++e) u[e] = REV ? (float)r.x.v[e] : d[e] * (float)r.x.v[e];
     if (REV && p.z.p)
 #pragma unroll
-      for (int e = 0; e < E; ++e) u[e] *= silu<sizeof(T) == 4>((float)rz.v[e]);
+      for (int e = 0; e < E; ++e) u[e] *= silu<sizeof(T) == 4>((float)r.z.v[e]);
     float *const d_ = sd[k & 1] + at<L>(cl, tl), *const u_ = su[k & 1] + at<L>(cl, tl);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -207,8 +235,8 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
       d_[e * (L + 4)] = counts ? d[e] : 0.f;
       u_[e * (L + 4)] = counts ? u[e] : 0.f;
     }
-    rB.lay(sB[k & 1], tid);
-    if (OUT) rC.lay(sC[k & 1], tid);
+    r.B.lay(sB[k & 1], tid);
+    if (OUT) r.C.lay(sC[k & 1], tid);
   };
   auto finish = [&](int k) {
     const int t = begin(k) + tl;
@@ -220,47 +248,50 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
       y[e] = y_[e * (L + 4)];
 #pragma unroll
       for (int i = 1; i < NB; ++i) y[e] += y_[i * PL + e * (L + 4)];
-      y[e] = skip ? fmaf(D[e], (float)px.v[e], y[e]) : y[e];
+      y[e] = skip ? fmaf(D[e], (float)before.x.v[e], y[e]) : y[e];
     }
     if (p.z.p)
 #pragma unroll
-      for (int e = 0; e < E; ++e) y[e] *= silu<sizeof(T) == 4>((float)pz.v[e]);
+      for (int e = 0; e < E; ++e) y[e] *= silu<sizeof(T) == 4>((float)before.z.v[e]);
 #pragma unroll
     for (int e = 0; e < E; ++e) out.v[e] = (T)(t < end ? y[e] : 0.f);
-    if (t < last && here > 0) out.store((T*)p.y + ((size_t)b * p.T + t) * p.C + cr, p.wide_out, here);
+    if (t < last && here > 0) out.store((T*)p.y + ((size_t)b * p.T + t) * p.C + cr, WIDE, here);
   };
-  if (chunks > 0) {
-    load(begin(0));
-    lay(0);
-    kx = rx, kz = rz;
-    if (chunks > 1) load(begin(1));
-  }
-  __syncthreads();
-  for (int k = 0; k < chunks; ++k) {
+  auto turn = [&](int k, In& r) {                // r: of chunk k + 1
     Row<T, E> nx, nz;
-    if (k + 1 < chunks) {
-      lay(k + 1);
-      nx = rx, nz = rz;
-      if (k + 2 < chunks) load(begin(k + 2));
-    }
+    if (k + 1 < chunks) lay(k + 1, r);
+    if (OUT) nx = r.x, nz = r.z;
+    load(k + 3, r);
     if (OUT) {
       if (k > 0) finish(k - 1);
-      px = kx, pz = kz;
-      kx = nx, kz = nz;
+      before = now;
+      now.x = nx, now.z = nz;
     }
     __syncthreads();
+  };
+  if (chunks > 0) {
+    load(0, in[0]);
+    load(1, in[1]);
+    lay(0, in[0]);
+    now.x = in[0].x, now.z = in[0].z;
+    load(2, in[0]);
+  }
+  __syncthreads();
+  for (int k = 0; k < chunks; k += 2) {
+    turn(k, in[1]);
+    if (k + 1 < chunks) turn(k + 1, in[0]);
   }
   if (!OUT) return;
   if (chunks > 0) finish(chunks - 1);
   Row<T, E> none;                        // tokens that do not count
   none.zero();
   for (int t = first + chunks * L + tl; t < last; t += L)
-    if (here > 0) none.store((T*)p.y + ((size_t)b * p.T + t) * p.C + cr, p.wide_out, here);
+    if (here > 0) none.store((T*)p.y + ((size_t)b * p.T + t) * p.C + cr, WIDE, here);
 }
 
 // The gradients.  Chunks of kSave tokens against the time: forwards through a chunk from the state kept in front of it, powers and states in
 // registers, then back.  A quad of lanes shares a channel: sums over its states cross the quad, sums over channels (of dB and dC) the 16 quads.
-template <typename T, int NL, int NB>
+template <typename T, int NL, int NB, bool WIDE>
 __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
   constexpr int CH = 64 / NB, L = kSave, E = CH / 16, NS = 4 * NL * NB, PL = plane<CH, L>(), CW = 4 / NB, R = 8 * NL;
   __shared__ __attribute__((aligned(16))) float sd[2][PL], su[2][PL], sq[2][PL], sB[2][L * NS], sC[2][L * NS], so[2][3 * NB * PL], red[2][4 * L * R],
@@ -287,7 +318,7 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
       }
     }
     auto kept = [&](int k) {
-      if (mine) take<NL>(hk, p.states + (((size_t)b * p.saved + begin(k) / kSave) * p.C + c) * NS + n0);
+      take<NL>(hk, p.states + (((size_t)b * p.saved + begin(min(k, chunks - 1)) / kSave) * p.C + (mine ? c : at_.c0)) * NS + n0);
     };
     if (chunks > 0) kept(0);
     __syncthreads();
@@ -297,64 +328,105 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
       float h[NL], hs[L][NL], as[L][NL], dAc[NL];
 #pragma unroll
       for (int n = 0; n < NL; ++n) {
-        h[n] = hk[n];
+        h[n] = mine ? hk[n] : 0.f;
         dAc[n] = 0.f;
       }
-      if (k + 1 < chunks) kept(k + 1);
+      kept(k + 1);
       const float *d_ = sd[f] + at<L>(ch, 0), *u_ = su[f] + at<L>(ch, 0), *q_ = sq[f] + at<L>(ch, 0), *B_ = sB[f] + n0, *C_ = sC[f] + n0;
       float* const o_ = so[f] + nb * PL + at<L>(ch, sub);
       // where a lane's sums of dB and dC lie: row r has type r >> 1 and, of four states, half r & 1; quads have values (0, 2, 1, 3) of four
       constexpr int LEFT = NL > 1 ? NL / 2 : 1, VAL = 4 * LEFT;
       const int mine4 = quad >> 1 | (quad & 1) << 1;
       float* const r_ = red[f] + w * L * R + (r >> 1) * 4 * NL + sub * NL + (NL > 1 ? (r & 1) * LEFT : 0) + mine4 / LEFT * R + mine4 % LEFT;
+      // (what the next tokens need is on its way from LDS, as forwards: four tokens on the way there, two back, where the registers are full)
+      struct Four { f32x4 d, u; float B[4][NL]; } g[2];
+      auto fetch = [&](int j, Four& x) {
+        x.d = *reinterpret_cast<const f32x4*>(d_ + j);
+        x.u = *reinterpret_cast<const f32x4*>(u_ + j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) take<NL>(x.B[i], B_ + (j + i) * NS);
+      };
+      struct Two { float B[2][NL], C[2][NL]; } two[2];
+      auto fetch_two = [&](int j, Two& x) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          take<NL>(x.B[i], B_ + (j + i) * NS);
+          take<NL>(x.C[i], C_ + (j + i) * NS);
+        }
+      };
+      fetch(0, g[0]);
 #pragma unroll
       for (int j = 0; j < L; j += 4) {
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(d_ + j), u4 = *reinterpret_cast<const f32x4*>(u_ + j);
+        const Four& x = g[j / 4 & 1];
+        if (j + 4 < L) fetch(j + 4, g[j / 4 + 1 & 1]);
+        else fetch_two(L - 2, two[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        float v[4][NL];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float Bn[NL];
-          take<NL>(Bn, B_ + (j + i) * NS);
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int n = 0; n < NL; ++n) as[j + i][n] = x.d[i] * A2[n];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int n = 0; n < NL; ++n) {
+            as[j + i][n] = __builtin_amdgcn_exp2f(as[j + i][n]);
+            v[i][n] = x.u[i] * x.B[i][n];
+          }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int n = 0; n < NL; ++n) {
             hs[j + i][n] = h[n];
-            as[j + i][n] = __builtin_amdgcn_exp2f(d4[i] * A2[n]);
-            h[n] = fmaf(as[j + i][n], h[n], u4[i] * Bn[n]);
+            h[n] = fmaf(as[j + i][n], h[n], v[i][n]);
           }
-        }
         __builtin_amdgcn_sched_barrier(0);
       }
+      f32x4 d4, u4, q4;
+      auto fetch_rows = [&](int j) {
+        d4 = *reinterpret_cast<const f32x4*>(d_ + j);
+        u4 = *reinterpret_cast<const f32x4*>(u_ + j);
+        q4 = *reinterpret_cast<const f32x4*>(q_ + j);
+      };
+      fetch_rows(L - 4);
 #pragma unroll
       for (int j = L - 4; j >= 0; j -= 4) {
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(d_ + j), u4 = *reinterpret_cast<const f32x4*>(u_ + j), q4 = *reinterpret_cast<const f32x4*>(q_ + j);
         float s1[4], s2[4], y[4], val[VAL];
 #pragma unroll
-        for (int i = 3; i >= 0; --i) {
-          float v[2 * NL], Bn[NL], Cn[NL];
-          take<NL>(Bn, B_ + (j + i) * NS);
-          take<NL>(Cn, C_ + (j + i) * NS);
-          // (behind the last token that counts no state takes part in dA, however large)
-          if constexpr (!decltype(whole)::value)
-            if (t0 + j + i + 1 == end)
+        for (int half = 1; half >= 0; --half) {
+          const Two& x = two[half];
+          if (j + 2 * half > 0) fetch_two(j + 2 * half - 2, two[1 - half]);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-              for (int n = 0; n < NL; ++n) dAc[n] = 0.f;
+          for (int i = 2 * half + 1; i >= 2 * half; --i) {
+            float v[2 * NL];
+            const float(&Bn)[NL] = x.B[i & 1], (&Cn)[NL] = x.C[i & 1];
+            // (behind the last token that counts no state takes part in dA, however large)
+            if constexpr (!decltype(whole)::value)
+              if (t0 + j + i + 1 == end)
 #pragma unroll
-          for (int n = 0; n < NL; ++n) {
-            y[i] = n == 0 ? Cn[n] * h[n] : fmaf(Cn[n], h[n], y[i]);
-            v[NL + n] = q4[i] * h[n];
-            const float g = fmaf(q4[i], Cn[n], G[n]);
-            v[n] = g * u4[i];
-            s1[i] = n == 0 ? g * Bn[n] : fmaf(g, Bn[n], s1[i]);
-            G[n] = as[j + i][n] * g;
-            h[n] = hs[j + i][n];
-            const float turn = G[n] * h[n];
-            s2[i] = n == 0 ? turn * A2[n] : fmaf(turn, A2[n], s2[i]);
-            dAc[n] = fmaf(d4[i], turn, dAc[n]);
+                for (int n = 0; n < NL; ++n) dAc[n] = 0.f;
+#pragma unroll
+            for (int n = 0; n < NL; ++n) {
+              y[i] = n == 0 ? Cn[n] * h[n] : fmaf(Cn[n], h[n], y[i]);
+              v[NL + n] = q4[i] * h[n];
+              const float gn = fmaf(q4[i], Cn[n], G[n]);
+              v[n] = gn * u4[i];
+              s1[i] = n == 0 ? gn * Bn[n] : fmaf(gn, Bn[n], s1[i]);
+              G[n] = as[j + i][n] * gn;
+              h[n] = hs[j + i][n];
+              const float turn = G[n] * h[n];
+              s2[i] = n == 0 ? turn * A2[n] : fmaf(turn, A2[n], s2[i]);
+              dAc[n] = fmaf(d4[i], turn, dAc[n]);
+            }
+            // over the 16 quads: halves, rows
+#pragma unroll
+            for (int n = 0; n < NL; ++n) v[n] = fold32(v[n], v[NL + n]);
+#pragma unroll
+            for (int n = 0; n < LEFT; ++n) val[i * LEFT + n] = fold16(v[n], NL > 1 ? v[NL / 2 + n] : v[n]);
           }
-          // over the 16 quads: halves, rows
-#pragma unroll
-          for (int m = 0; m < NL; ++m) v[m] = fold32(v[m], v[NL + m]);
-#pragma unroll
-          for (int m = 0; m < LEFT; ++m) val[i * LEFT + m] = fold16(v[m], NL > 1 ? v[NL / 2 + m] : v[m]);
+          if (half == 0 && j > 0) fetch_rows(j - 4);
         }
         // over a quad, whose lane sub is left with token j + sub
         o_[j] = quad_sums(s1, sub);
@@ -394,24 +466,25 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
     bias[e] = p.bias && e < here ? p.bias[cr + e] : 0.f;
     dD[e] = dbias[e] = 0.f;
   }
-  struct Rows { Row<T, E> x, d, z, y; } r;       // of the chunk that is read next
-  struct Known { Rows r; float d[E], q[E], slope[E], gate[E]; } next, now, before;      // of the one just laid down, of the one under way, of the one before
-  r.x.zero(), r.d.zero(), r.z.zero(), r.y.zero();
-  Shared<T, L, NS> rB, rC;
+  struct In { Row<T, E> x, d, z, y; Shared<T, L, NS> B, C; } in[2];      // of the next two chunks, as forwards
+  struct Known { Row<T, E> x, z, y; float d[E], q[E], slope[E], gate[E]; } next, now, before;      // of the one just laid down, of the one under way, of the one before
+  const int tr = here > 0 ? here : at_.here, cw = here > 0 ? cr : at_.c0;
+  const T *const dp = (const T*)p.delta.p + b * p.delta.sb + cw, *const xp = (const T*)p.x.p + b * p.x.sb + cw,
+          *const yp = (const T*)p.dy.p + b * p.dy.sb + cw, *const zp = p.z.p ? (const T*)p.z.p + b * p.z.sb + cw : xp;
+  const long zt = p.z.p ? p.z.st : p.x.st;
   const T* const Bp = (const T*)p.Bm + (size_t)b * p.bsb + (size_t)at_.g * p.bsg;
   const T* const Cp = (const T*)p.Cm + (size_t)b * p.csb + (size_t)at_.g * p.csg;
-  auto load = [&](int t0) {
-    const int t = t0 + tl;
-    if (t < end && here > 0) {
-      r.d.load((const T*)p.delta.p + b * p.delta.sb + t * p.delta.st + cr, p.wide, here);
-      r.x.load((const T*)p.x.p + b * p.x.sb + t * p.x.st + cr, p.wide, here);
-      if (p.z.p) r.z.load((const T*)p.z.p + b * p.z.sb + t * p.z.st + cr, p.wide, here);
-      r.y.load((const T*)p.dy.p + b * p.dy.sb + t * p.dy.st + cr, p.wide, here);
-    }
-    rB.load(Bp, p.bst, t0, end, p.N, tid);
-    rC.load(Cp, p.cst, t0, end, p.N, tid);
+  auto load = [&](int k, In& r) {
+    const int t0 = begin(min(k, chunks - 1));
+    const long t = min(t0 + tl, end - 1);
+    r.d.template read<WIDE>(dp + t * p.delta.st, tr);
+    r.x.template read<WIDE>(xp + t * p.x.st, tr);
+    r.z.template read<WIDE>(zp + t * zt, tr);
+    r.y.template read<WIDE>(yp + t * p.dy.st, tr);
+    r.B.load(Bp, p.bst, t0, end, p.N, tid);
+    r.C.load(Cp, p.cst, t0, end, p.N, tid);
   };
-  auto lay = [&](int k) {
+  auto lay = [&](int k, const In& r) {
     const bool there = begin(k) + tl < end;
     float d[E], q[E];
 #pragma unroll
@@ -440,9 +513,9 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
       next.d[e] = d[e];
       next.q[e] = q[e];
     }
-    next.r = r;
-    rB.lay(sB[k & 1], tid);
-    rC.lay(sC[k & 1], tid);
+    next.x = r.x, next.z = r.z, next.y = r.y;
+    r.B.lay(sB[k & 1], tid);
+    r.C.lay(sC[k & 1], tid);
   };
   const int tile = (at_.c0 - at_.g * (p.C / p.G)) / CH;
   auto finish = [&](int k) {
@@ -459,12 +532,12 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
         s2[e] += o_[(NB + i) * PL + e * (L + 4)];
         y[e] += o_[(2 * NB + i) * PL + e * (L + 4)];
       }
-      dd[e] = fmaf(s1[e], (float)before.r.x.v[e], s2[e] * kLn2) * before.slope[e];
+      dd[e] = fmaf(s1[e], (float)before.x.v[e], s2[e] * kLn2) * before.slope[e];
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const bool counts = t < end && e < here;
-      const float x = (float)before.r.x.v[e];
+      const float x = (float)before.x.v[e];
       ox.v[e] = (T)(counts ? fmaf(D[e], before.q[e], before.d[e] * s1[e]) : 0.f);
       od.v[e] = (T)(counts ? dd[e] : 0.f);
       dD[e] = counts ? fmaf(before.q[e], x, dD[e]) : dD[e];
@@ -473,14 +546,14 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
     if (p.z.p)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float g = (float)before.r.y.v[e] * fmaf(D[e], (float)before.r.x.v[e], y[e]) * silu_slope((float)before.r.z.v[e], before.gate[e]);
+        const float g = (float)before.y.v[e] * fmaf(D[e], (float)before.x.v[e], y[e]) * silu_slope((float)before.z.v[e], before.gate[e]);
         oz.v[e] = (T)(t < end && e < here ? g : 0.f);
       }
     if (t < last && here > 0) {
       const size_t row = ((size_t)b * p.T + t) * p.C + cr;
-      if (p.dx) ox.store((T*)p.dx + row, p.wide_out, here);
-      if (p.ddelta) od.store((T*)p.ddelta + row, p.wide_out, here);
-      if (p.dz) oz.store((T*)p.dz + row, p.wide_out, here);
+      if (p.dx) ox.store((T*)p.dx + row, WIDE, here);
+      if (p.ddelta) od.store((T*)p.ddelta + row, WIDE, here);
+      if (p.dz) oz.store((T*)p.dz + row, WIDE, here);
     }
     if (shared)
       for (int i = tid; i < L * 2 * NS; i += 256) {
@@ -491,22 +564,25 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
         if (t0 + tk < end) p.part_bc[((((size_t)tile * p.B + b) * p.T + t0 + tk) * p.G + at_.g) * 2 * NS + type * NS + n] = sum;
       }
   };
-  if (chunks > 0) {
-    load(begin(0));
-    lay(0);
-    now = next;
-    if (chunks > 1) load(begin(1));
-  }
-  __syncthreads();
-  for (int k = 0; k < chunks; ++k) {
-    if (k + 1 < chunks) {
-      lay(k + 1);
-      if (k + 2 < chunks) load(begin(k + 2));
-    }
+  auto turn = [&](int k, In& r) {                // r: of chunk k + 1
+    if (k + 1 < chunks) lay(k + 1, r);
+    load(k + 3, r);
     if (k > 0) finish(k - 1);
     before = now;
     now = next;
     __syncthreads();
+  };
+  if (chunks > 0) {
+    load(0, in[0]);
+    load(1, in[1]);
+    lay(0, in[0]);
+    now = next;
+    load(2, in[0]);
+  }
+  __syncthreads();
+  for (int k = 0; k < chunks; k += 2) {
+    turn(k, in[1]);
+    if (k + 1 < chunks) turn(k + 1, in[0]);
   }
   if (chunks > 0) finish(chunks - 1);
   Row<T, E> none;                        // tokens that do not count
@@ -514,9 +590,9 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
   for (int t = first + chunks * L + tl; t < last; t += L)
     if (here > 0) {
       const size_t row = ((size_t)b * p.T + t) * p.C + cr;
-      if (p.dx) none.store((T*)p.dx + row, p.wide_out, here);
-      if (p.ddelta) none.store((T*)p.ddelta + row, p.wide_out, here);
-      if (p.dz) none.store((T*)p.dz + row, p.wide_out, here);
+      if (p.dx) none.store((T*)p.dx + row, WIDE, here);
+      if (p.ddelta) none.store((T*)p.ddelta + row, WIDE, here);
+      if (p.dz) none.store((T*)p.dz + row, WIDE, here);
     }
   // the 16 threads of a channel, in order
 #pragma unroll
@@ -532,25 +608,29 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
   }
 }
 
-template <typename T, int NL, int NB> hipError_t launch_sized(const RingScanArgs& p, int mode, hipStream_t st) {
+template <typename T, int NL, int NB, bool WIDE> hipError_t launch_sized(const RingScanArgs& p, int mode, hipStream_t st) {
   const int CH = 64 / NB;
   RingScanArgs a = p;
   a.tiles = (p.C / p.G + CH - 1) / CH;
   const int segs = mode == RING_SCAN_STATE || mode == RING_SCAN_ADJOINT ? p.nseg - 1 : p.nseg;
   const dim3 grid((unsigned)((size_t)a.tiles * p.G * p.B * segs)), block(512);
-  if (mode == RING_SCAN_OUTPUTS) hipLaunchKernelGGL((ring_scan_kernel<T, NL, NB, kOutputs>), grid, block, 0, st, a);
-  else if (mode == RING_SCAN_STATE) hipLaunchKernelGGL((ring_scan_kernel<T, NL, NB, kState>), grid, block, 0, st, a);
-  else if (mode == RING_SCAN_ADJOINT) hipLaunchKernelGGL((ring_scan_kernel<T, NL, NB, kAdjoint>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((ring_scan_bwd_kernel<T, NL, NB>), grid, block, 0, st, a);
+  if (mode == RING_SCAN_OUTPUTS) hipLaunchKernelGGL((ring_scan_kernel<T, NL, NB, kOutputs, WIDE>), grid, block, 0, st, a);
+  else if (mode == RING_SCAN_STATE) hipLaunchKernelGGL((ring_scan_kernel<T, NL, NB, kState, WIDE>), grid, block, 0, st, a);
+  else if (mode == RING_SCAN_ADJOINT) hipLaunchKernelGGL((ring_scan_kernel<T, NL, NB, kAdjoint, WIDE>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((ring_scan_bwd_kernel<T, NL, NB, WIDE>), grid, block, 0, st, a);
   return hipGetLastError();
 }
 
+template <typename T, bool WIDE> hipError_t launch_rows(const RingScanArgs& p, int mode, hipStream_t st) {
+  if (p.N <= 4) return launch_sized<T, 1, 1, WIDE>(p, mode, st);
+  if (p.N <= 8) return launch_sized<T, 2, 1, WIDE>(p, mode, st);
+  if (p.N <= 16) return launch_sized<T, 4, 1, WIDE>(p, mode, st);
+  if (p.N <= 32) return launch_sized<T, 4, 2, WIDE>(p, mode, st);
+  return launch_sized<T, 4, 4, WIDE>(p, mode, st);
+}
+
 template <typename T> hipError_t launch(const RingScanArgs& p, int mode, hipStream_t st) {
-  if (p.N <= 4) return launch_sized<T, 1, 1>(p, mode, st);
-  if (p.N <= 8) return launch_sized<T, 2, 1>(p, mode, st);
-  if (p.N <= 16) return launch_sized<T, 4, 1>(p, mode, st);
-  if (p.N <= 32) return launch_sized<T, 4, 2>(p, mode, st);
-  return launch_sized<T, 4, 4>(p, mode, st);
+  return p.wide ? launch_rows<T, true>(p, mode, st) : launch_rows<T, false>(p, mode, st);
 }
 
 }  // namespace ring_scan

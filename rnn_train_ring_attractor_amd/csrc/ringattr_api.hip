@@ -1270,7 +1270,6 @@ static RingScanArgs scan_args(const RingScanShape& s, const void* x, const void*
   a.softplus = softplus ? 1 : 0;
   const int per = s.C / s.G;
   a.wide = rows_wide(x, st, per, 8) && rows_wide(delta, st + 2, per, 8) && rows_wide(z, st + 4, per, 8);
-  a.wide_out = per % 8 == 0;
   return a;
 }
 
