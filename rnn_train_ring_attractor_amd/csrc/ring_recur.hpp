@@ -40,6 +40,13 @@ template <bool FINE> __device__ __forceinline__ float softplus(float x) {
   return softplus<FINE>(x, slope);
 }
 
+// `rows` rows of `st` values as a buffer: what is read behind them is zero, what is written there is left out.  (Their places within it are 32-bit numbers that
+// stay the same from chunk to chunk, the buffer's own address is scalar: no vector instruction for either.)
+template <typename T> __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const T* p, long st, int rows) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, (int)(rows * st * (long)sizeof(T)), 0x00027000);
+}
+constexpr int kOutside = 0x7ffffff0;   // a place behind every buffer
+
 // E values, neighbours in memory.  WIDE: the address is a whole number of min(16, E sizeof(T)) bytes; otherwise one by one, `here` of them.
 template <typename T, int E> struct Row {
   typedef T vec __attribute__((ext_vector_type(E)));
@@ -74,6 +81,51 @@ template <typename T, int E> struct Row {
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e) v[e] = p[min(e, here - 1)];
+    }
+  }
+  // From and to a buffer, at a number of bytes
+  __device__ __forceinline__ void fetch(__amdgpu_buffer_rsrc_t b, int at) {
+    constexpr int BYTES = E * sizeof(T);
+    if constexpr (BYTES >= 16) {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i) {
+        const auto x = __builtin_amdgcn_raw_buffer_load_b128(b, at + 16 * i, 0, 0);
+        __builtin_memcpy(v + i * (16 / sizeof(T)), &x, 16);
+      }
+    } else if constexpr (BYTES == 8) {
+      const auto x = __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, 0);
+      __builtin_memcpy(v, &x, 8);
+    } else if constexpr (BYTES == 4) {
+      const auto x = __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0);
+      __builtin_memcpy(v, &x, 4);
+    } else {
+      const auto x = __builtin_amdgcn_raw_buffer_load_b16(b, at, 0, 0);
+      __builtin_memcpy(v, &x, 2);
+    }
+  }
+  __device__ __forceinline__ void give(__amdgpu_buffer_rsrc_t b, int at) const {
+    constexpr int BYTES = E * sizeof(T);
+    typedef unsigned four __attribute__((ext_vector_type(4)));
+    typedef unsigned two __attribute__((ext_vector_type(2)));
+    if constexpr (BYTES >= 16) {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i) {
+        four x;
+        __builtin_memcpy(&x, v + i * (16 / sizeof(T)), 16);
+        __builtin_amdgcn_raw_buffer_store_b128(x, b, at + 16 * i, 0, 0);
+      }
+    } else if constexpr (BYTES == 8) {
+      two x;
+      __builtin_memcpy(&x, v, 8);
+      __builtin_amdgcn_raw_buffer_store_b64(x, b, at, 0, 0);
+    } else if constexpr (BYTES == 4) {
+      unsigned x;
+      __builtin_memcpy(&x, v, 4);
+      __builtin_amdgcn_raw_buffer_store_b32(x, b, at, 0, 0);
+    } else {
+      unsigned short x;
+      __builtin_memcpy(&x, v, 2);
+      __builtin_amdgcn_raw_buffer_store_b16(x, b, at, 0, 0);
     }
   }
   __device__ __forceinline__ void store(T* p, bool wide, int here) const {

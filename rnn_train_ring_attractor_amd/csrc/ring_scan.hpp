@@ -72,6 +72,18 @@ template <> __device__ __forceinline__ void take<1>(float (&v)[1], const float* 
 template <typename T, int L, int NS> struct Shared {
   static constexpr int NV = (L * NS + 255) / 256;
   T v[NV];
+  static __device__ __forceinline__ int place(int i, long st, int N, int tid) {      // of value i in a chunk's buffer
+    const int k = tid + 256 * i;
+    return k < L * NS && k % NS < N ? (int)((k / NS * st + k % NS) * (long)sizeof(T)) : kOutside;
+  }
+  __device__ __forceinline__ void fetch(__amdgpu_buffer_rsrc_t b, const int (&at)[NV]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      Row<T, 1> x;
+      x.fetch(b, at[i]);
+      v[i] = x.v[0];
+    }
+  }
   __device__ __forceinline__ void load(const T* p, long st, int t0, int end, int N, int tid) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -201,19 +213,37 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
   struct In { Row<T, E> x, d, z, y; Shared<T, L, NS> B, C; } in[2];
   struct { Row<T, E> x, z; } now, before;
   const int tr = here > 0 ? here : at_.here, cw = here > 0 ? cr : at_.c0;
-  const T *const dp = (const T*)p.delta.p + b * p.delta.sb + cw, *const xp = (const T*)(REV ? p.dy.p : p.x.p) + b * (REV ? p.dy.sb : p.x.sb) + cw,
-          *const zp = p.z.p ? (const T*)p.z.p + b * p.z.sb + cw : xp;
+  const T *const dp = (const T*)p.delta.p + b * p.delta.sb, *const xp = (const T*)(REV ? p.dy.p : p.x.p) + b * (REV ? p.dy.sb : p.x.sb),
+          *const zp = p.z.p ? (const T*)p.z.p + b * p.z.sb : xp;
   const long xt = REV ? p.dy.st : p.x.st, zt = p.z.p ? p.z.st : xt;
   const T* const Bp = (const T*)(REV ? p.Cm : p.Bm) + (size_t)b * (REV ? p.csb : p.bsb) + (size_t)at_.g * (REV ? p.csg : p.bsg);
   const T* const Cp = (const T*)p.Cm + (size_t)b * p.csb + (size_t)at_.g * p.csg;
+  const long Bt = REV ? p.cst : p.bst;
+  typedef Shared<T, L, NS> Sh;
+  const int dw = (int)((tl * p.delta.st + cw) * (long)sizeof(T)), xw = (int)((tl * xt + cw) * (long)sizeof(T)), zw = (int)((tl * zt + cw) * (long)sizeof(T)),
+            yw = here > 0 ? (int)((tl * (long)p.C + cr) * (long)sizeof(T)) : kOutside;
+  int Bw[Sh::NV], Cw[Sh::NV];
+#pragma unroll
+  for (int i = 0; i < Sh::NV; ++i) {
+    Bw[i] = Sh::place(i, Bt, p.N, tid);
+    Cw[i] = Sh::place(i, p.cst, p.N, tid);
+  }
   auto load = [&](int k, In& r) {
-    const int t0 = begin(min(k, chunks - 1));
-    const long t = min(t0 + tl, end - 1);
-    r.d.template read<WIDE>(dp + t * p.delta.st, tr);
-    r.x.template read<WIDE>(xp + t * xt, tr);
-    if (OUT || REV) r.z.template read<WIDE>(zp + t * zt, tr);
-    r.B.load(Bp, REV ? p.cst : p.bst, t0, end, p.N, tid);
-    if (OUT) r.C.load(Cp, p.cst, t0, end, p.N, tid);
+    const int t0 = begin(min(k, chunks - 1)), rows = min(end - t0, L);
+    if constexpr (WIDE) {
+      r.d.fetch(buffer_of(dp + t0 * p.delta.st, p.delta.st, rows), dw);
+      r.x.fetch(buffer_of(xp + t0 * xt, xt, rows), xw);
+      if (OUT || REV) r.z.fetch(buffer_of(zp + t0 * zt, zt, rows), zw);
+      r.B.fetch(buffer_of(Bp + t0 * Bt, Bt, rows), Bw);
+      if (OUT) r.C.fetch(buffer_of(Cp + t0 * p.cst, p.cst, rows), Cw);
+    } else {
+      const long t = min(t0 + tl, end - 1);
+      r.d.template read<false>(dp + cw + t * p.delta.st, tr);
+      r.x.template read<false>(xp + cw + t * xt, tr);
+      if (OUT || REV) r.z.template read<false>(zp + cw + t * zt, tr);
+      r.B.load(Bp, Bt, t0, end, p.N, tid);
+      if (OUT) r.C.load(Cp, p.cst, t0, end, p.N, tid);
+    }
   };
   auto lay = [&](int k, const In& r) {
     const bool there = begin(k) + tl < end;
@@ -255,7 +285,8 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
       for (int e = 0; e < E; ++e) y[e] *= silu<sizeof(T) == 4>((float)before.z.v[e]);
 #pragma unroll
     for (int e = 0; e < E; ++e) out.v[e] = (T)(t < end ? y[e] : 0.f);
-    if (t < last && here > 0) out.store((T*)p.y + ((size_t)b * p.T + t) * p.C + cr, WIDE, here);
+    if constexpr (WIDE) out.give(buffer_of((T*)p.y + ((size_t)b * p.T + begin(k)) * p.C, p.C, min(last - begin(k), L)), yw);
+    else if (t < last && here > 0) out.store((T*)p.y + ((size_t)b * p.T + t) * p.C + cr, false, here);
   };
   auto turn = [&](int k, In& r) {                // r: of chunk k + 1
     Row<T, E> nx, nz;
@@ -469,20 +500,38 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
   struct In { Row<T, E> x, d, z, y; Shared<T, L, NS> B, C; } in[2];      // of the next two chunks, as forwards
   struct Known { Row<T, E> x, z, y; float d[E], q[E], slope[E], gate[E]; } next, now, before;      // of the one just laid down, of the one under way, of the one before
   const int tr = here > 0 ? here : at_.here, cw = here > 0 ? cr : at_.c0;
-  const T *const dp = (const T*)p.delta.p + b * p.delta.sb + cw, *const xp = (const T*)p.x.p + b * p.x.sb + cw,
-          *const yp = (const T*)p.dy.p + b * p.dy.sb + cw, *const zp = p.z.p ? (const T*)p.z.p + b * p.z.sb + cw : xp;
+  const T *const dp = (const T*)p.delta.p + b * p.delta.sb, *const xp = (const T*)p.x.p + b * p.x.sb,
+          *const yp = (const T*)p.dy.p + b * p.dy.sb, *const zp = p.z.p ? (const T*)p.z.p + b * p.z.sb : xp;
   const long zt = p.z.p ? p.z.st : p.x.st;
   const T* const Bp = (const T*)p.Bm + (size_t)b * p.bsb + (size_t)at_.g * p.bsg;
   const T* const Cp = (const T*)p.Cm + (size_t)b * p.csb + (size_t)at_.g * p.csg;
+  typedef Shared<T, L, NS> Sh;
+  const int dw = (int)((tl * p.delta.st + cw) * (long)sizeof(T)), xw = (int)((tl * p.x.st + cw) * (long)sizeof(T)), zw = (int)((tl * zt + cw) * (long)sizeof(T)),
+            yw = (int)((tl * p.dy.st + cw) * (long)sizeof(T)), ow = here > 0 ? (int)((tl * (long)p.C + cr) * (long)sizeof(T)) : kOutside;
+  int Bw[Sh::NV], Cw[Sh::NV];
+#pragma unroll
+  for (int i = 0; i < Sh::NV; ++i) {
+    Bw[i] = Sh::place(i, p.bst, p.N, tid);
+    Cw[i] = Sh::place(i, p.cst, p.N, tid);
+  }
   auto load = [&](int k, In& r) {
-    const int t0 = begin(min(k, chunks - 1));
-    const long t = min(t0 + tl, end - 1);
-    r.d.template read<WIDE>(dp + t * p.delta.st, tr);
-    r.x.template read<WIDE>(xp + t * p.x.st, tr);
-    r.z.template read<WIDE>(zp + t * zt, tr);
-    r.y.template read<WIDE>(yp + t * p.dy.st, tr);
-    r.B.load(Bp, p.bst, t0, end, p.N, tid);
-    r.C.load(Cp, p.cst, t0, end, p.N, tid);
+    const int t0 = begin(min(k, chunks - 1)), rows = min(end - t0, L);
+    if constexpr (WIDE) {
+      r.d.fetch(buffer_of(dp + t0 * p.delta.st, p.delta.st, rows), dw);
+      r.x.fetch(buffer_of(xp + t0 * p.x.st, p.x.st, rows), xw);
+      r.z.fetch(buffer_of(zp + t0 * zt, zt, rows), zw);
+      r.y.fetch(buffer_of(yp + t0 * p.dy.st, p.dy.st, rows), yw);
+      r.B.fetch(buffer_of(Bp + t0 * p.bst, p.bst, rows), Bw);
+      r.C.fetch(buffer_of(Cp + t0 * p.cst, p.cst, rows), Cw);
+    } else {
+      const long t = min(t0 + tl, end - 1);
+      r.d.template read<false>(dp + cw + t * p.delta.st, tr);
+      r.x.template read<false>(xp + cw + t * p.x.st, tr);
+      r.z.template read<false>(zp + cw + t * zt, tr);
+      r.y.template read<false>(yp + cw + t * p.dy.st, tr);
+      r.B.load(Bp, p.bst, t0, end, p.N, tid);
+      r.C.load(Cp, p.cst, t0, end, p.N, tid);
+    }
   };
   auto lay = [&](int k, const In& r) {
     const bool there = begin(k) + tl < end;
@@ -549,11 +598,17 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
         const float g = (float)before.y.v[e] * fmaf(D[e], (float)before.x.v[e], y[e]) * silu_slope((float)before.z.v[e], before.gate[e]);
         oz.v[e] = (T)(t < end && e < here ? g : 0.f);
       }
-    if (t < last && here > 0) {
+    if constexpr (WIDE) {
+      const size_t row = ((size_t)b * p.T + t0) * p.C;
+      const int rows = min(last - t0, L);
+      if (p.dx) ox.give(buffer_of((T*)p.dx + row, p.C, rows), ow);
+      if (p.ddelta) od.give(buffer_of((T*)p.ddelta + row, p.C, rows), ow);
+      if (p.dz) oz.give(buffer_of((T*)p.dz + row, p.C, rows), ow);
+    } else if (t < last && here > 0) {
       const size_t row = ((size_t)b * p.T + t) * p.C + cr;
-      if (p.dx) ox.store((T*)p.dx + row, WIDE, here);
-      if (p.ddelta) od.store((T*)p.ddelta + row, WIDE, here);
-      if (p.dz) oz.store((T*)p.dz + row, WIDE, here);
+      if (p.dx) ox.store((T*)p.dx + row, false, here);
+      if (p.ddelta) od.store((T*)p.ddelta + row, false, here);
+      if (p.dz) oz.store((T*)p.dz + row, false, here);
     }
     if (shared)
       for (int i = tid; i < L * 2 * NS; i += 256) {

@@ -1115,6 +1115,9 @@ static bool rows_wide(const void* p, const long long* strides, int per, int unit
   return !p || (per % unit == 0 && aligned16(p) && (!strides || (strides[0] % unit == 0 && strides[1] % unit == 0)));
 }
 
+// Whether a chunk's rows lie behind one another, each as long as it is, within 32 bits of an address.
+static bool rows_apart(long long stride, int n) { return stride >= n && stride <= (1 << 22); }
+
 static RingRows rows_of_channels(const void* p, const long long* strides) { return RingRows{p, (long)strides[0], (long)strides[1]}; }
 
 static bool conv_shape(const char* who, int act, int type, int B, int T, int C, int K) {
@@ -1269,7 +1272,8 @@ static RingScanArgs scan_args(const RingScanShape& s, const void* x, const void*
   a.G = s.G;
   a.softplus = softplus ? 1 : 0;
   const int per = s.C / s.G;
-  a.wide = rows_wide(x, st, per, 8) && rows_wide(delta, st + 2, per, 8) && rows_wide(z, st + 4, per, 8);
+  a.wide = rows_wide(x, st, per, 8) && rows_wide(delta, st + 2, per, 8) && rows_wide(z, st + 4, per, 8) && rows_apart(st[1], s.C) &&
+           rows_apart(st[3], s.C) && (!z || rows_apart(st[5], s.C)) && rows_apart(st[7], s.N) && rows_apart(st[10], s.N);
   return a;
 }
 
@@ -1314,7 +1318,7 @@ int ringattr_selective_scan_bwd(const void* x, const void* delta, const void* z,
     return fail(RINGATTR_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
   RingScanArgs a = scan_args(s, x, delta, z, B, C, strides, A, D, delta_bias, lengths, softplus);
   a.dy = rows_of_channels(grad_y, strides + 12);
-  a.wide = a.wide && rows_wide(grad_y, strides + 12, channels / groups, 8);
+  a.wide = a.wide && rows_wide(grad_y, strides + 12, channels / groups, 8) && rows_apart(strides[13], channels);
   a.states = (float*)const_cast<void*>(states_kept);
   a.s_in = (const float*)grad_final_state;
   a.s_out = (float*)grad_initial_state;
