@@ -499,7 +499,7 @@ struct RingNormArgs {
   float* part;                           // [parts,3,C]
   long rows;
   int C, group, layer, act, parts;
-  float eps;
+  float eps, each, each_row;             // (the last two the launcher's: one over group, over C)
 };
 size_t ring_norm_bwd_bytes(int type, long rows, int C, int group, bool params);
 hipError_t ring_norm_fwd(const RingNormArgs& p, int type, hipStream_t st);

@@ -57,9 +57,18 @@ template <int K> __device__ __forceinline__ void add_up(float (&v)[K], int n, Ro
   }
 }
 
-template <typename T> __device__ __forceinline__ float act_of(T y, int act) {
-  const float x = (float)y;
-  return act == kSilu ? silu<sizeof(T) == 4>(x) : (act == kSigmoid ? sigmoid<sizeof(T) == 4>(x) : x);
+// v times act(gate)
+template <typename T, int V> __device__ __forceinline__ void gate_of(float (&v)[V], const Row<T, V>& g, int act) {
+  if (act == kSilu) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] *= silu<sizeof(T) == 4>((float)g.v[e]);
+  } else if (act == kSigmoid) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] *= sigmoid<sizeof(T) == 4>((float)g.v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] *= (float)g.v[e];
+  }
 }
 
 // A thread's place in a row
@@ -75,9 +84,9 @@ template <int V, int I, bool MANY> struct Spot {
     const int g = MANY ? i * l.slots + slot : slot, u = MANY ? lane : i * l.lanes + lane;
     return g * group + u * V;
   }
-  __device__ __forceinline__ int here(const Lie& l, int i, int group) const {      // values of unit i that are there
+  __device__ __forceinline__ bool there(const Lie& l, int i, int group) const {      // whether unit i is (groups are whole numbers of units)
     const int g = MANY ? i * l.slots + slot : slot, u = MANY ? lane : i * l.lanes + lane;
-    return g < l.groups ? min(max(group - u * V, 0), V) : 0;
+    return g < l.groups && u * V < group;
   }
 };
 
@@ -95,9 +104,10 @@ template <int V, int I, bool MANY> __device__ __forceinline__ void group_sums(fl
   }
 }
 
-// v becomes (v - mean) over its groups, rstd beside it
+// v becomes (v - mean) over its groups, rstd beside it (zero where a unit is not there: what follows from it is zero then, whatever eps is); `each` is one
+// over the values of a group
 template <int V, int I, bool MANY>
-__device__ __forceinline__ void normalise(float (&v)[I][V], float (&rstd)[I], const int (&here)[I], const Lie& l, float count, bool layer, float eps, Room& room) {
+__device__ __forceinline__ void normalise(float (&v)[I][V], float (&rstd)[I], const bool (&there)[I], const Lie& l, float each, bool layer, float eps, Room& room) {
   float s[I];
   if (layer) {
 #pragma unroll
@@ -110,7 +120,7 @@ __device__ __forceinline__ void normalise(float (&v)[I][V], float (&rstd)[I], co
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[i][e] = e < here[i] ? v[i][e] - s[i] / count : 0.f;
+      for (int e = 0; e < V; ++e) v[i][e] = there[i] ? v[i][e] - s[i] * each : 0.f;
   }
 #pragma unroll
   for (int i = 0; i < I; ++i) {
@@ -120,7 +130,7 @@ __device__ __forceinline__ void normalise(float (&v)[I][V], float (&rstd)[I], co
   }
   group_sums<V, I, MANY>(s, l, room);
 #pragma unroll
-  for (int i = 0; i < I; ++i) rstd[i] = 1.f / sqrtf(s[i] / count + eps);
+  for (int i = 0; i < I; ++i) rstd[i] = there[i] ? __builtin_amdgcn_rsqf(fmaf(s[i], each, eps)) : 0.f;
 }
 
 }  // namespace
@@ -133,56 +143,56 @@ __global__ __launch_bounds__(1024) void ring_norm_fwd_kernel(RingNormArgs p, Lie
   const Lie whole = {at.threads, 1, l.rows, 0, 1};
   const long row = ((long)blockIdx.y * gridDim.x + blockIdx.x) * l.rows + at.row;
   const bool real = row < p.rows;
-  int here[I], col[I];
+  bool there[I];
+  int col[I];
   float v[I][V], rstd[I];
   Row<T, V> rx[I], rg[I], rr[I];
 #pragma unroll
   for (int i = 0; i < I; ++i) {
-    here[i] = real ? at.here(l, i, p.group) : 0;
+    there[i] = real && at.there(l, i, p.group);
     col[i] = at.column(l, i, p.group);
     rx[i].zero(), rg[i].zero(), rr[i].zero();
-    if (here[i] > 0) {
-      rx[i].load((const T*)p.x + row * p.xs + col[i], V > 1, here[i]);
-      if (p.gate) rg[i].load((const T*)p.gate + row * p.gs + col[i], V > 1, here[i]);
-      if (p.residual) rr[i].load((const T*)p.residual + row * p.rs + col[i], V > 1, here[i]);
+    if (there[i]) {
+      rx[i].load((const T*)p.x + row * p.xs + col[i], V > 1, V);
+      if (p.gate) rg[i].load((const T*)p.gate + row * p.gs + col[i], V > 1, V);
+      if (p.residual) rr[i].load((const T*)p.residual + row * p.rs + col[i], V > 1, V);
     }
 #pragma unroll
     for (int e = 0; e < V; ++e) v[i][e] = (float)rx[i].v[e];
   }
-  normalise<V, I, MANY>(v, rstd, here, l, (float)p.group, p.layer, p.eps, room);
-#pragma unroll
-  for (int i = 0; i < I; ++i) {
-    Row<T, V> out;
-    Row<float, V> w, s;
-    if (here[i] > 0) {
-      w.load(p.w + col[i], V > 1, here[i]);
-      if (p.scale) s.load(p.scale + col[i], V > 1, here[i]);
-    }
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float y = 0.f;
-      if (e < here[i]) {
-        y = v[i][e] * rstd[i] * w.v[e];
-        if (p.gate) y *= act_of(rg[i].v[e], p.act);
-        if (p.scale) y *= s.v[e];
-        if (p.residual) y += (float)rr[i].v[e];
-      }
-      v[i][e] = y;
-      out.v[e] = (T)y;
-    }
-    if (here[i] > 0) out.store((T*)p.y + row * p.C + col[i], V > 1, here[i]);
-  }
-  if (!p.next) return;
-  normalise<V, I, false>(v, rstd, here, whole, (float)p.C, p.layer, p.eps, room);
+  normalise<V, I, MANY>(v, rstd, there, l, p.each, p.layer, p.eps, room);
 #pragma unroll
   for (int i = 0; i < I; ++i)
-    if (here[i] > 0) {
+    if (there[i]) {
       Row<T, V> out;
       Row<float, V> w;
-      w.load(p.next + col[i], V > 1, here[i]);
+      w.load(p.w + col[i], V > 1, V);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[i][e] *= rstd[i] * w.v[e];
+      if (p.gate) gate_of<T, V>(v[i], rg[i], p.act);
+      if (p.scale) {
+        w.load(p.scale + col[i], V > 1, V);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[i][e] *= w.v[e];
+      }
+      if (p.residual)
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[i][e] += (float)rr[i].v[e];
+#pragma unroll
+      for (int e = 0; e < V; ++e) out.v[e] = (T)v[i][e];
+      out.store((T*)p.y + row * p.C + col[i], V > 1, V);
+    }
+  if (!p.next) return;
+  normalise<V, I, false>(v, rstd, there, whole, p.each_row, p.layer, p.eps, room);
+#pragma unroll
+  for (int i = 0; i < I; ++i)
+    if (there[i]) {
+      Row<T, V> out;
+      Row<float, V> w;
+      w.load(p.next + col[i], V > 1, V);
 #pragma unroll
       for (int e = 0; e < V; ++e) out.v[e] = (T)(v[i][e] * rstd[i] * w.v[e]);
-      out.store((T*)p.n + row * p.C + col[i], V > 1, here[i]);
+      out.store((T*)p.n + row * p.C + col[i], V > 1, V);
     }
 }
 
@@ -198,15 +208,16 @@ __global__ __launch_bounds__(MOST) void ring_norm_bwd_kernel(RingNormArgs p, Lie
   struct Unit { Row<T, V> x, g, r, t, n; };          // of the row: x, gate, residual, gradients of y and n
   struct Weights { Row<float, V> w, s, n; } kept;
   Unit next[I];
-  int there[I], col[I];
+  bool there[I];
+  int col[I];
   float aw[I][V], as[I][V], an[I][V];
   auto weights = [&](int i) {
     Weights k;
     k.w.zero(), k.s.zero(), k.n.zero();
-    if (there[i] > 0) {
-      k.w.load(p.w + col[i], V > 1, there[i]);
-      if (p.scale) k.s.load(p.scale + col[i], V > 1, there[i]);
-      if (p.dn) k.n.load(p.next + col[i], V > 1, there[i]);
+    if (there[i]) {
+      k.w.load(p.w + col[i], V > 1, V);
+      if (p.scale) k.s.load(p.scale + col[i], V > 1, V);
+      if (p.dn) k.n.load(p.next + col[i], V > 1, V);
     }
     if (!p.scale)
 #pragma unroll
@@ -216,33 +227,32 @@ __global__ __launch_bounds__(MOST) void ring_norm_bwd_kernel(RingNormArgs p, Lie
   auto load = [&](long row) {
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      if (row >= p.rows || there[i] <= 0) continue;
-      next[i].x.load((const T*)p.x + row * p.xs + col[i], V > 1, there[i]);
-      if (p.gate) next[i].g.load((const T*)p.gate + row * p.gs + col[i], V > 1, there[i]);
-      if (p.dy) next[i].t.load((const T*)p.dy + row * p.dys + col[i], V > 1, there[i]);
+      if (row >= p.rows || !there[i]) continue;
+      next[i].x.load((const T*)p.x + row * p.xs + col[i], V > 1, V);
+      if (p.gate) next[i].g.load((const T*)p.gate + row * p.gs + col[i], V > 1, V);
+      if (p.dy) next[i].t.load((const T*)p.dy + row * p.dys + col[i], V > 1, V);
       if (p.dn) {
-        next[i].n.load((const T*)p.dn + row * p.dns + col[i], V > 1, there[i]);
-        if (p.residual) next[i].r.load((const T*)p.residual + row * p.rs + col[i], V > 1, there[i]);
+        next[i].n.load((const T*)p.dn + row * p.dns + col[i], V > 1, V);
+        if (p.residual) next[i].r.load((const T*)p.residual + row * p.rs + col[i], V > 1, V);
       }
     }
   };
 #pragma unroll
   for (int i = 0; i < I; ++i) {
-    there[i] = at.here(l, i, p.group);
+    there[i] = at.there(l, i, p.group);
     col[i] = at.column(l, i, p.group);
     next[i].x.zero(), next[i].g.zero(), next[i].r.zero(), next[i].t.zero(), next[i].n.zero();
 #pragma unroll
     for (int e = 0; e < V; ++e) aw[i][e] = as[i][e] = an[i][e] = 0.f;
   }
   if constexpr (KEEP) kept = weights(0);
-  const bool gated = p.gate && p.act != kSigmoid;
   const long step = (long)gridDim.x * l.rows;
   load((long)blockIdx.x * l.rows + at.row);
   for (long first = (long)blockIdx.x * l.rows; first < p.rows; first += step) {
     const long row = first + at.row;
     const bool real = row < p.rows;
-    int here[I];
-    float unit[I][V], rstd[I], total[I][V], sig[I][V];      // sig: the gate's sigmoid, which its activation and slope follow from
+    bool here[I];
+    float unit[I][V], rstd[I], total[I][V], act[I][V], sig[I][V];      // sig: the gate's sigmoid, which its slope follows from
     Unit now[I];
     if constexpr (!KEEP) {
       if (first > (long)blockIdx.x * l.rows) load(row);
@@ -250,97 +260,113 @@ __global__ __launch_bounds__(MOST) void ring_norm_bwd_kernel(RingNormArgs p, Lie
 #pragma unroll
     for (int i = 0; i < I; ++i) {
       now[i] = next[i];
-      here[i] = real ? there[i] : 0;
+      here[i] = real && there[i];
+      if (!real) now[i].x.zero(), now[i].g.zero(), now[i].r.zero(), now[i].t.zero(), now[i].n.zero();
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        unit[i][e] = e < here[i] ? (float)now[i].x.v[e] : 0.f;
+        unit[i][e] = (float)now[i].x.v[e];
         total[i][e] = (float)now[i].t.v[e];
-        sig[i][e] = 1.f;
+        act[i][e] = sig[i][e] = 1.f;
       }
     }
     if constexpr (KEEP) load(row + step);
-    if (p.gate && p.act != kIdentity)
+    if (p.gate)
 #pragma unroll
-      for (int i = 0; i < I; ++i)
+      for (int i = 0; i < I; ++i) {
+        if (p.act != kIdentity)
 #pragma unroll
-        for (int e = 0; e < V; ++e) sig[i][e] = sigmoid<FINE>((float)now[i].g.v[e]);
-    auto act = [&](int i, int e) { return gated ? (float)now[i].g.v[e] * sig[i][e] : sig[i][e]; };      // silu, none: z s; sigmoid, no gate: s
-    auto slope = [&](int i, int e) {
-      const float s = sig[i][e];
-      return p.act == kSilu ? silu_slope((float)now[i].g.v[e], s) : (p.act == kSigmoid ? s * (1.f - s) : 1.f);
-    };
-    normalise<V, I, MANY>(unit, rstd, here, l, (float)p.group, p.layer, p.eps, room);
+          for (int e = 0; e < V; ++e) sig[i][e] = sigmoid<FINE>((float)now[i].g.v[e]);
+        if (p.act == kSigmoid)
+#pragma unroll
+          for (int e = 0; e < V; ++e) act[i][e] = sig[i][e];
+        else
+#pragma unroll
+          for (int e = 0; e < V; ++e) act[i][e] = (float)now[i].g.v[e] * sig[i][e];
+      }
+    normalise<V, I, MANY>(unit, rstd, here, l, p.each, p.layer, p.eps, room);
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
       for (int e = 0; e < V; ++e) unit[i][e] *= rstd[i];
     if (p.dn) {
       // n = (y - mean) r next: sums of y and of the gradient, then of their squares and products, both at once
-      float y[I][V], s[2] = {0.f, 0.f}, mean = 0.f, m0 = 0.f;
+      float y[I][V], gn[I][V], s[2] = {0.f, 0.f}, m0 = 0.f;
 #pragma unroll
       for (int i = 0; i < I; ++i) {
         const Weights k = KEEP ? kept : weights(i);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float v = fmaf(unit[i][e] * k.w.v[e] * act(i, e), k.s.v[e], p.residual ? (float)now[i].r.v[e] : 0.f);
-          y[i][e] = e < here[i] ? v : 0.f;
-          s[0] += y[i][e];
-          s[1] += e < here[i] ? (float)now[i].n.v[e] * k.n.v[e] : 0.f;
+          y[i][e] = fmaf(unit[i][e] * k.w.v[e] * act[i][e], k.s.v[e], (float)now[i].r.v[e]);      // (zero where there is no residual)
+          gn[i][e] = (float)now[i].n.v[e] * k.n.v[e];
         }
       }
       if (p.layer) {
-        add_up<2>(s, at.threads, room);
-        mean = s[0] / (float)p.C;
-        m0 = s[1] / (float)p.C;
-      }
-      s[0] = s[1] = 0.f;
 #pragma unroll
-      for (int i = 0; i < I; ++i) {
-        const Weights k = KEEP ? kept : weights(i);
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            s[0] += y[i][e];
+            s[1] += gn[i][e];
+          }
+        add_up<2>(s, at.threads, room);
+        const float mean = s[0] * p.each_row;
+        m0 = s[1] * p.each_row;
+        s[0] = s[1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+          for (int e = 0; e < V; ++e) y[i][e] = here[i] ? y[i][e] - mean : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < I; ++i)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          y[i][e] = e < here[i] ? y[i][e] - mean : 0.f;
           s[0] = fmaf(y[i][e], y[i][e], s[0]);
-          s[1] += e < here[i] ? (float)now[i].n.v[e] * k.n.v[e] * y[i][e] : 0.f;
+          s[1] = fmaf(gn[i][e], y[i][e], s[1]);
         }
-      }
       add_up<2>(s, at.threads, room);
-      const float r = 1.f / sqrtf(s[0] / (float)p.C + p.eps), m1 = s[1] * r / (float)p.C;
+      const float r = real ? __builtin_amdgcn_rsqf(fmaf(s[0], p.each_row, p.eps)) : 0.f, m1 = s[1] * r * p.each_row;
 #pragma unroll
-      for (int i = 0; i < I; ++i) {
-        const Weights k = KEEP ? kept : weights(i);
+      for (int i = 0; i < I; ++i)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float u = y[i][e] * r;
-          if (real) an[i][e] = fmaf((float)now[i].n.v[e], u, an[i][e]);
-          total[i][e] = fmaf(r, (float)now[i].n.v[e] * k.n.v[e] - m0 - u * m1, total[i][e]);
+          an[i][e] = fmaf((float)now[i].n.v[e], u, an[i][e]);
+          total[i][e] = fmaf(r, fmaf(-u, m1, gn[i][e] - m0), total[i][e]);
         }
-      }
     }
     float s1[I], s0[I];
 #pragma unroll
     for (int i = 0; i < I; ++i) {
       const Weights k = KEEP ? kept : weights(i);
-      Row<T, V> res, dg;
+      Row<T, V> out;
       s1[i] = s0[i] = 0.f;
+      if (here[i] && p.dresidual) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) out.v[e] = (T)total[i][e];
+        out.store((T*)p.dresidual + row * p.C + col[i], V > 1, V);
+      }
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        res.v[e] = (T)total[i][e];
-        const float normed = unit[i][e] * k.w.v[e];
-        float g = total[i][e];
-        if (real) as[i][e] = fmaf(g, normed * act(i, e), as[i][e]);
-        g *= k.s.v[e];
-        dg.v[e] = (T)(g * normed * slope(i, e));
-        g *= act(i, e);
-        if (real) aw[i][e] = fmaf(g, unit[i][e], aw[i][e]);
-        g = e < here[i] ? g * k.w.v[e] : 0.f;
-        total[i][e] = g;
-        s1[i] = fmaf(g, unit[i][e], s1[i]);
-        s0[i] += g;
+        as[i][e] = fmaf(total[i][e], unit[i][e] * k.w.v[e] * act[i][e], as[i][e]);
+        total[i][e] *= k.s.v[e];
       }
-      if (here[i] > 0) {
-        if (p.dresidual) res.store((T*)p.dresidual + row * p.C + col[i], V > 1, here[i]);
-        if (p.dgate) dg.store((T*)p.dgate + row * p.C + col[i], V > 1, here[i]);
+      if (here[i] && p.dgate) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float q = sig[i][e];
+          const float slope = p.act == kSilu ? fmaf(act[i][e], 1.f - q, q) : (p.act == kSigmoid ? q * (1.f - q) : 1.f);
+          out.v[e] = (T)(total[i][e] * unit[i][e] * k.w.v[e] * slope);
+        }
+        out.store((T*)p.dgate + row * p.C + col[i], V > 1, V);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float g = total[i][e] * act[i][e];
+        aw[i][e] = fmaf(g, unit[i][e], aw[i][e]);
+        total[i][e] = g * k.w.v[e];
+        s1[i] = fmaf(total[i][e], unit[i][e], s1[i]);
+        s0[i] += total[i][e];
       }
     }
     if (!p.dx) continue;
@@ -348,12 +374,12 @@ __global__ __launch_bounds__(MOST) void ring_norm_bwd_kernel(RingNormArgs p, Lie
     if (p.layer) group_sums<V, I, MANY>(s0, l, room);
 #pragma unroll
     for (int i = 0; i < I; ++i)
-      if (here[i] > 0) {
+      if (here[i]) {
         Row<T, V> out;
-        const float m1 = s1[i] / (float)p.group, m0 = p.layer ? s0[i] / (float)p.group : 0.f;
+        const float m1 = s1[i] * p.each, m0 = p.layer ? s0[i] * p.each : 0.f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) out.v[e] = (T)(rstd[i] * (total[i][e] - m0 - unit[i][e] * m1));
-        out.store((T*)p.dx + row * p.C + col[i], V > 1, here[i]);
+        for (int e = 0; e < V; ++e) out.v[e] = (T)(rstd[i] * fmaf(-unit[i][e], m1, total[i][e] - m0));
+        out.store((T*)p.dx + row * p.C + col[i], V > 1, V);
       }
   }
   if (!p.part) return;
@@ -378,7 +404,7 @@ __global__ __launch_bounds__(MOST) void ring_norm_bwd_kernel(RingNormArgs p, Lie
       if (at.row == 0)
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          if (e < there[i]) p.part[((size_t)blockIdx.x * 3 + k) * p.C + col[i] + e] = a[e];
+          if (there[i]) p.part[((size_t)blockIdx.x * 3 + k) * p.C + col[i] + e] = a[e];
     }
   }
 }
@@ -474,6 +500,7 @@ template <typename T, int V, bool MANY> void launch_units(const RingNormArgs& p,
     else launch_one<T, V, 4, MANY>(p, a, back, st);
   } else {
     if (a.I <= 4) launch_one<T, V, 4, MANY>(p, a, back, st);
+    else if (a.I <= 8) launch_one<T, V, 8, MANY>(p, a, back, st);
     else launch_one<T, V, 16, MANY>(p, a, back, st);
   }
 }
@@ -490,6 +517,8 @@ template <typename T> bool wide(const RingNormArgs& p) {
 template <typename T> hipError_t launch(RingNormArgs p, bool back, hipStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool w = wide<T>(p);
+  p.each = 1.f / (float)p.group;
+  p.each_row = 1.f / (float)p.C;
   const Plan a = plan_of(p.C, p.group, w ? V : 1);
   if (back) p.parts = parts_of(a, p.rows);
   if (w) {
