@@ -205,6 +205,9 @@ def resolved(t):
 
 def check_sequence_tensor(name, t, shape=None, dtype=None, device=None) -> None:
     """What the sequence operators ask of a tensor: one of their types (or the one given), on the GPU, and the shape."""
+    # (in most cases these three; `device` is that of a tensor that has been looked at)
+    if type(t) is torch.Tensor and t.dtype is dtype and device is not None and t.device == device and (shape is None or t.shape == shape):
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if dtype is None:

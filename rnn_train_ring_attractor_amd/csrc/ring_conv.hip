@@ -124,8 +124,11 @@ __global__ __launch_bounds__(256) void ring_conv_fwd_kernel(RingConvArgs p, int 
   for (int t = max(a.first, end); t < a.last; ++t) none.store(y + (size_t)t * p.C, kWide<E>, E);
 }
 
-template <typename T, int E, int KT, int U>      // U tokens at a time
+// A token at a time, its input and gradient read KT tokens (or more) ahead.  Inputs and gradients of the last KT tokens go round in registers: a piece's token t is in
+// place t % KT, and so many tokens follow each other without a loop between them that places are known.
+template <typename T, int E, int KT, bool SILU>
 __global__ __launch_bounds__(256) void ring_conv_bwd_kernel(RingConvArgs p, int tx, int blocks) {
+  constexpr int N = KT == 2 ? 4 : KT;    // tokens that follow each other
   __shared__ float sums[256 * E];
   const Piece a = piece<E>(p, tx, blocks);
   const int K = KT == 8 ? p.K : KT, skip = KT - K, len = length_of(p.lengths, a.b, p.T);
@@ -141,7 +144,7 @@ __global__ __launch_bounds__(256) void ring_conv_bwd_kernel(RingConvArgs p, int 
     }
   }
   if (a.mine) {
-    float win[KT - 1 + U][E], g[KT - 1 + U][E];      // inputs and gradients of the tokens up to t + U - 1
+    float win[KT][E], g[KT][E];
     const T* const x = (const T*)p.x.p + a.b * p.x.sb + a.c;
     const T* const dy = (const T*)p.dy.p + a.b * p.dy.sb + a.c;
     const size_t state = (size_t)a.b * (K - 1) * p.C + a.c;
@@ -150,13 +153,13 @@ __global__ __launch_bounds__(256) void ring_conv_bwd_kernel(RingConvArgs p, int 
     T* const dx = p.dx ? (T*)p.dx + (size_t)a.b * p.T * p.C + a.c : nullptr;
     T* const dstart = p.dstart ? (T*)p.dstart + state : nullptr;
 #pragma unroll
-    for (int j = 0; j < KT - 1; ++j) {
-      const int t = a.first - (KT - 1) + j;
+    for (int j = 0; j < KT; ++j) {       // (place j has token j - KT of the piece)
+      const int t = a.first - KT + j;
       Row<T, E> r;
       r.zero();
-      if (j >= skip && a.first < len) {
+      if (j > 0 && a.first < len) {
         if (t >= 0) r.load(x + t * p.x.st, kWide<E>, E);
-        else if (start) r.load(start + (size_t)(t + K - 1) * p.C, kWide<E>, E);
+        else if (start && t >= -(K - 1)) r.load(start + (size_t)(t + K - 1) * p.C, kWide<E>, E);
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -164,11 +167,11 @@ __global__ __launch_bounds__(256) void ring_conv_bwd_kernel(RingConvArgs p, int 
         g[j][e] = 0.f;
       }
     }
-    Row<T, E> nx[U], ny[U];
+    Row<T, E> nx[N], ny[N];
     // gradients of the piece's tokens, then those behind it that its last inputs take part in
-    const int to = a.first < a.last || (a.first == 0 && a.sub == 0 && a.seg == 0) ? a.last + K - 1 : a.first;
+    const int to = a.first < a.last || (a.first == 0 && a.sub == 0 && a.seg == 0) ? a.last + KT - 1 : a.first, full = min(a.last, len);
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
+    for (int i = 0; i < N; ++i) {
       nx[i].zero(), ny[i].zero();
       const int t = a.first + i;
       if (t < min(to, len)) {
@@ -176,87 +179,75 @@ __global__ __launch_bounds__(256) void ring_conv_bwd_kernel(RingConvArgs p, int 
         ny[i].load(dy + t * p.dy.st, kWide<E>, E);
       }
     }
-    const T *xp = x + (a.first + U) * p.x.st, *yp = dy + (a.first + U) * p.dy.st;
-    T* dxp = dx + (long)(a.first - K + 1) * p.C;       // (of token t - K + 1; used where that is one)
+    const T *xp = x + (a.first + N) * p.x.st, *yp = dy + (a.first + N) * p.dy.st;
+    T* dxp = dx + (long)(a.first - KT + 1) * p.C;       // (of token t - KT + 1; used where that is one)
     auto tokens = [&](int t, auto inner) {       // inner: these tokens count in the sums, the next ones are there, gradients are complete and of the piece
       constexpr bool IN = decltype(inner)::value;
-      Row<T, E> ky[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        ky[i] = ny[i];
-#pragma unroll
-        for (int e = 0; e < E; ++e) win[KT - 1 + i][e] = (float)nx[i].v[e];
-      }
-#pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (IN || t + U + i < min(to, len)) {
-          nx[i].load(xp + i * p.x.st, kWide<E>, E);
-          ny[i].load(yp + i * p.dy.st, kWide<E>, E);
-        }
-      xp += U * p.x.st;
-      yp += U * p.dy.st;
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int s = t + i, back = s - K + 1;
+      for (int i = 0; i < N; ++i) {
+        constexpr int M = KT;
+        const int s = t + i, back = s - KT + 1, at = i % M;
         const bool counts = IN || s < len;
         float q[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          g[KT - 1 + i][e] = (float)ky[i].v[e];
+          win[at][e] = (float)nx[i].v[e];
+          g[at][e] = (float)ny[i].v[e];
           q[e] = bias[e];
         }
-        if (p.act == kSilu)
+        if (IN || s + N < min(to, len)) {
+          nx[i].load(xp, kWide<E>, E);
+          ny[i].load(yp, kWide<E>, E);
+        }
+        xp += p.x.st;
+        yp += p.dy.st;
+        if (SILU) {
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
+          for (int k = 0; k < KT; ++k)
+            if (KT < 8 || k >= skip)
 #pragma unroll
-            for (int k = 0; k < KT; ++k)
-              if (KT < 8 || k >= skip) q[e] = fmaf(w[k][e], win[i + k][e], q[e]);
-            g[KT - 1 + i][e] *= silu_slope(q[e], sigmoid<sizeof(T) == 4>(q[e]));
-          }
+              for (int e = 0; e < E; ++e) q[e] = fmaf(w[k][e], win[(at + 1 + k) % M][e], q[e]);
+#pragma unroll
+          for (int e = 0; e < E; ++e) g[at][e] *= silu_slope(q[e], sigmoid<sizeof(T) == 4>(q[e]));
+        }
         if (!IN)
 #pragma unroll
-          for (int e = 0; e < E; ++e) g[KT - 1 + i][e] = counts ? g[KT - 1 + i][e] : 0.f;
+          for (int e = 0; e < E; ++e) g[at][e] = counts ? g[at][e] : 0.f;
         if (IN || (s < a.last && counts)) {
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            db[e] += g[KT - 1 + i][e];
+          for (int e = 0; e < E; ++e) db[e] += g[at][e];
 #pragma unroll
-            for (int k = 0; k < KT; ++k)
-              if (KT < 8 || k >= skip) dw[k][e] = fmaf(g[KT - 1 + i][e], win[i + k][e], dw[k][e]);
-          }
+          for (int k = 0; k < KT; ++k)
+            if (KT < 8 || k >= skip)
+#pragma unroll
+              for (int e = 0; e < E; ++e) dw[k][e] = fmaf(g[at][e], win[(at + 1 + k) % M][e], dw[k][e]);
         }
-        T* to_row = nullptr;
-        if (IN || (back >= a.first && back < a.last)) to_row = dx ? dxp + (long)i * p.C : nullptr;
-        else if (!IN && back < 0 && back >= -(K - 1) && s < to && dstart) to_row = dstart + (size_t)(back + K - 1) * p.C;
-        if (to_row) {
+        T* row = nullptr;
+        if (IN || (back >= a.first && back < a.last)) row = dx ? dxp : nullptr;
+        else if (back < 0 && back >= -(K - 1) && s < to && dstart) row = dstart + (size_t)(back + K - 1) * p.C;
+        dxp += p.C;
+        if (row) {
           Row<T, E> out, more;
           more.zero();
           if (!IN && dend && back < len && back >= len - (K - 1)) more.load(dend + (size_t)(back - len + K - 1) * p.C, kWide<E>, E);
+          float v[E];
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            float v = IN ? 0.f : (float)more.v[e];
+          for (int e = 0; e < E; ++e) v[e] = IN ? 0.f : (float)more.v[e];
 #pragma unroll
-            for (int k = 0; k < KT; ++k)
-              if (KT < 8 || k >= skip) v = fmaf(w[k][e], g[KT - 1 + i - (k - skip)][e], v);
-            out.v[e] = (T)(IN || back < len ? v : 0.f);
-          }
-          out.store(to_row, kWide<E>, E);
+          for (int k = 0; k < KT; ++k)
+            if (KT < 8 || k >= skip)
+#pragma unroll
+              for (int e = 0; e < E; ++e) v[e] = fmaf(w[k][e], g[(at + M - k) % M][e], v[e]);
+#pragma unroll
+          for (int e = 0; e < E; ++e) out.v[e] = (T)(IN || back < len ? v[e] : 0.f);
+          out.store(row, kWide<E>, E);
         }
       }
-      dxp += (long)U * p.C;
-#pragma unroll
-      for (int j = 0; j < KT - 1; ++j)
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          win[j][e] = win[j + U][e];
-          g[j][e] = g[j + U][e];
-        }
     };
     int t = a.first;
-    const int full = min(a.last, len);
-    for (; t < min(to, a.first + KT - 1); t += U) tokens(t, std::false_type{});
-    for (; t + 2 * U <= full; t += U) tokens(t, std::true_type{});
-    for (; t < to; t += U) tokens(t, std::false_type{});
+    for (; t < min(to, a.first + KT - 1); t += N) tokens(t, std::false_type{});
+    for (; t + 2 * N <= full; t += N) tokens(t, std::true_type{});
+    for (; t < to; t += N) tokens(t, std::false_type{});
   }
   if (!p.part) return;
   // the workgroup's pieces, in order
@@ -323,11 +314,13 @@ static int along(int C, int E) {         // threads along the channels
   return tx;
 }
 
-// Pieces are short enough that there is work for all compute units, and long beside the K - 1 tokens that they share
+// Pieces are long beside the K - 1 tokens that they share, and short enough that every compute unit has two workgroups, which is what there are registers for
+// backwards (8 x 4096 tokens, 4096 channels, 4 taps, bf16, us forwards and with gradients by a piece's tokens: 32 111, 338; 64 108, 307; 128 105, 289; 192
+// 124, 333; 256 99, 289; 512 155, 438).
 static void cut(RingConvArgs& p, int tx, int blocks) {
   const int subs = 256 / tx;
-  p.seg_tokens = 64;
-  while (p.seg_tokens > 8 && (long)p.B * blocks * ((p.T + (long)subs * p.seg_tokens - 1) / ((long)subs * p.seg_tokens)) < 1024) p.seg_tokens /= 2;
+  p.seg_tokens = 256;
+  while (p.seg_tokens > 8 && (long)p.B * blocks * ((p.T + (long)subs * p.seg_tokens - 1) / ((long)subs * p.seg_tokens)) < 512) p.seg_tokens /= 2;
   p.nseg = (int)((p.T + (long)subs * p.seg_tokens - 1) / ((long)subs * p.seg_tokens));
   if (p.nseg < 1) p.nseg = 1;
 }
@@ -337,7 +330,8 @@ template <typename T, int E> static hipError_t launch(RingConvArgs p, bool back,
   cut(p, tx, blocks);
   const dim3 grid((unsigned)((size_t)blocks * p.nseg * p.B)), block(256);
 #define RING_CONV(KT)                                                                             \
-  if (back) hipLaunchKernelGGL((ring_conv_bwd_kernel<T, E, KT, 1>), grid, block, 0, st, p, tx, blocks); \
+  if (back && p.act == kSilu) hipLaunchKernelGGL((ring_conv_bwd_kernel<T, E, KT, true>), grid, block, 0, st, p, tx, blocks); \
+  else if (back) hipLaunchKernelGGL((ring_conv_bwd_kernel<T, E, KT, false>), grid, block, 0, st, p, tx, blocks); \
   else hipLaunchKernelGGL((ring_conv_fwd_kernel<T, E, KT, 4>), grid, block, 0, st, p, tx, blocks)
   if (p.K == 2) { RING_CONV(2); }
   else if (p.K == 3) { RING_CONV(3); }

@@ -15,12 +15,13 @@ _ACTIVATIONS = {None: 0, "silu": 1, "sigmoid": 2}
 
 
 def _flat(t):
-    """t as rows at one stride, a row's values next to each other (copied where it is not)."""
-    return None if t is None else _lib.rows_of(_lib.resolved(t).reshape(-1, t.shape[-1]))
-
-
-def _stride(t):
-    return 0 if t is None else t.stride(0)
+    """(t as rows at one stride, a row's values next to each other, copied where it is not; the stride)"""
+    if t is None:
+        return None, 0
+    if not t.is_contiguous() or t.is_neg():
+        t = _lib.rows_of(_lib.resolved(t).reshape(-1, t.shape[-1]))
+        return t, t.stride(0)
+    return t, t.shape[-1]
 
 
 def _forward(x, weight, gate, residual, scale, next_weight, group, eps, kind, act):
@@ -30,11 +31,10 @@ def _forward(x, weight, gate, residual, scale, next_weight, group, eps, kind, ac
         n = x.new_empty(x.shape) if next_weight is not None else None
         if x.numel() == 0:
             return y, n
-        fx, fg, fr = _flat(x), _flat(gate), _flat(residual)
+        (fx, sx), (fg, sg), (fr, sr) = _flat(x), _flat(gate), _flat(residual)
         _lib.check(_lib.load().ringattr_norm_gate_fwd(
-            fx.data_ptr(), pointer(fg), pointer(fr), _Strides3(_stride(fx), _stride(fg), _stride(fr)), weight.data_ptr(), pointer(scale),
-            pointer(next_weight), y.data_ptr(), pointer(n), eps, kind, act, SEQUENCE_TYPES[x.dtype], fx.shape[0], C, group,
-            _lib.stream_handle(dev)))
+            fx.data_ptr(), pointer(fg), pointer(fr), _Strides3(sx, sg, sr), weight.data_ptr(), pointer(scale), pointer(next_weight), y.data_ptr(),
+            pointer(n), eps, kind, act, SEQUENCE_TYPES[x.dtype], x.numel() // C, C, group, _lib.stream_handle(dev)))
     return y, n
 
 
@@ -68,15 +68,14 @@ class NormGateFunc(Function):
                     if g is not None:
                         g.zero_()
             elif any(need):
-                fx, fg, fr, fy, fn = _flat(x), _flat(gate), _flat(residual), _flat(grad_y), _flat(grad_n)
+                rows, (fx, sx), (fg, sg), (fr, sr), (fy, sy), (fn, sn) = x.numel() // C, *(_flat(t) for t in (x, gate, residual, grad_y, grad_n))
                 asked = gn if grad_n is not None else None
-                nbytes = lib.ringattr_norm_gate_bwd_workspace_bytes(code, fx.shape[0], C, group, any(g is not None for g in (gw, gs, asked)))
+                nbytes = lib.ringattr_norm_gate_bwd_workspace_bytes(code, rows, C, group, any(g is not None for g in (gw, gs, asked)))
                 ws = weight.new_empty((nbytes // 4,)) if nbytes else None
                 _lib.check(lib.ringattr_norm_gate_bwd(
                     fx.data_ptr(), pointer(fg), pointer(fr), pointer(fy), pointer(fn),
-                    _Strides5(_stride(fx), _stride(fg), _stride(fr), _stride(fy), _stride(fn)), weight.data_ptr(), pointer(scale),
-                    pointer(next_weight), pointer(gx), pointer(gg), pointer(gr), pointer(gw), pointer(gs), pointer(asked), eps, kind, act, code,
-                    fx.shape[0], C, group, pointer(ws), nbytes, _lib.stream_handle(dev)))
+                    _Strides5(sx, sg, sr, sy, sn), weight.data_ptr(), pointer(scale), pointer(next_weight), pointer(gx), pointer(gg), pointer(gr),
+                    pointer(gw), pointer(gs), pointer(asked), eps, kind, act, code, rows, C, group, pointer(ws), nbytes, _lib.stream_handle(dev)))
         return gx, gw, gg, gr, gs, gn, None, None, None, None
 
 
