@@ -18,7 +18,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libringattr.so")
 SOURCES = ["ring_kernels.hip", "ring_res256.hip", "ring_cluster.hip", "ring_team.hip", "ring_team_fwd.hip", "ring_team_fwd_lds1.hip", "ring_team_fwd_lds4.hip",
            "ring_team_bptt.hip", "ring_team_bptt_ga.hip", "ring_team_solo.hip", "ring_team_rows.hip", "ring_team_one.hip", "ring_dw.hip", "ring_loss.hip", "ring_gain.hip", "ring_bign.hip", "ring_block.hip", "ring_panel.hip", "ring_chip.hip", "ring_aux.hip",
            "ring_linattn.hip", "ring_linattn_f32.hip", "ring_linattn_bf16.hip", "ring_linattn_f16.hip", "ring_rotary.hip", "ring_dropout.hip",
-           "ring_norm.hip", "ring_conv.hip", "ring_scan.hip", "ring_scan_f32.hip", "ring_scan_bf16.hip", "ring_scan_f16.hip", "ring_recur.hip",
+           "ring_norm.hip", "ring_norm_f32.hip", "ring_norm_bf16.hip", "ring_norm_f16.hip", "ring_conv.hip", "ring_scan.hip", "ring_scan_f32.hip", "ring_scan_bf16.hip", "ring_scan_f16.hip", "ring_recur.hip",
            "ringattr_api.hip"]
 ARCH = os.environ.get("RINGATTR_ARCH", "gfx950")
 

@@ -504,3 +504,6 @@ struct RingNormArgs {
 size_t ring_norm_bwd_bytes(int type, long rows, int C, int group, bool params);
 hipError_t ring_norm_fwd(const RingNormArgs& p, int type, hipStream_t st);
 hipError_t ring_norm_bwd(RingNormArgs p, int type, hipStream_t st);
+hipError_t ring_launch_norm_f32(const RingNormArgs& p, bool wide, bool back, hipStream_t st);
+hipError_t ring_launch_norm_bf16(const RingNormArgs& p, bool wide, bool back, hipStream_t st);
+hipError_t ring_launch_norm_f16(const RingNormArgs& p, bool wide, bool back, hipStream_t st);
