@@ -334,3 +334,16 @@ def test_norm_of_any_strides(kind, place, gpu_device):
     for C, group in ((64, 32), (33, 11)):
         p = norm_problem(29, (3, 7), C, TYPES[kind])
         check_norm(p, run_norm(p, TYPES[kind], gpu_device, place, group=group), group, "rms", "silu")
+
+
+# rows whose groups ask for each number of units a thread, with and without whole units of 16 bytes
+LIES = [(4096, 512), (4096, 256), (4096, 64), (8192, 512), (8184, 2728), (8184, 264), (8192, 256), (8188, 356), (8188, 92), (8192, 64), (8190, 2730), (8190, 63), (2047, None),
+        (1023, 341), (255, None), (127, None)]
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("C,group", LIES, ids=[f"{a}-{b}" for a, b in LIES])
+def test_norm_at_every_lie_of_its_rows(C, group, kind, gpu_device):
+    print(f"[case] norm lies {C} {group} {kind}", flush=True)
+    p = norm_problem(31, (3,), C, TYPES[kind])
+    check_norm(p, run_norm(p, TYPES[kind], gpu_device, group=group, kind="layer", activation="silu"), group, "layer", "silu")
