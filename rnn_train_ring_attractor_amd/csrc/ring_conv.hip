@@ -45,9 +45,9 @@ __global__ __launch_bounds__(256) void ring_conv_fwd_kernel(RingConvArgs p, int 
   float w[KT][E], bias[E], win[KT - 1 + U][E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    bias[e] = p.bias && a.mine ? p.bias[a.c + e] : 0.f;
+    bias[e] = p.bias ? p.bias[a.c + e] : 0.f;
 #pragma unroll
-    for (int k = 0; k < KT; ++k) w[k][e] = k >= skip && a.mine ? p.w[(size_t)(a.c + e) * K + k - skip] : 0.f;
+    for (int k = 0; k < KT; ++k) w[k][e] = k >= skip ? p.w[(size_t)(a.c + e) * K + k - skip] : 0.f;
   }
   const T* const x = (const T*)p.x.p + a.b * p.x.sb + a.c;
   const T* const start = p.start ? (const T*)p.start + (size_t)a.b * (K - 1) * p.C + a.c : nullptr;
@@ -341,10 +341,13 @@ template <typename T, int E> static hipError_t launch(RingConvArgs p, bool back,
   return hipGetLastError();
 }
 
+// (of 16 bits: eight channels a thread as long as their inputs, weights and sums have registers; one tap goes through the kernel for up to eight)
+static bool units_of_eight(int K) { return K >= 2 && K <= 4; }
+
 template <typename T> static hipError_t launch_wide(const RingConvArgs& p, bool back, hipStream_t st) {
   if (!(p.wide && p.wide_out && p.wide_state)) return launch<T, 1>(p, back, st);
   if constexpr (sizeof(T) == 2)
-    if (p.K <= 4) return launch<T, 8>(p, back, st);
+    if (units_of_eight(p.K)) return launch<T, 8>(p, back, st);
   return launch<T, 4>(p, back, st);
 }
 
@@ -356,7 +359,7 @@ static hipError_t launch_type(const RingConvArgs& p, int type, bool back, hipStr
 
 // (rows that allow 16 bytes make fewer parts or as many)
 static int parts_of(int type, int B, int T, int C, int K, bool wide) {
-  const int E = wide ? (type == RINGATTR_F32 || K > 4 ? 4 : 8) : 1, tx = along(C, E), blocks = (C + tx * E - 1) / (tx * E);
+  const int E = wide ? (type == RINGATTR_F32 || !units_of_eight(K) ? 4 : 8) : 1, tx = along(C, E), blocks = (C + tx * E - 1) / (tx * E);
   RingConvArgs p = {};
   p.B = B;
   p.T = T;

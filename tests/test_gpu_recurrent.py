@@ -109,6 +109,16 @@ def test_conv_and_its_gradients(sizes, kind, gpu_device):
         check_conv(p, run_conv(p, TYPES[kind], gpu_device, act=act), None, act)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("K", range(1, 9))
+def test_conv_with_every_number_of_taps(K, kind, gpu_device):
+    for C in (16, 5):                            # rows of whole units of 16 bytes, and not
+        for act in (None, "silu"):
+            print(f"[case] conv taps {C} {K} {kind} {act}", flush=True)
+            p = conv_problem(7, 2, 19, C, K, TYPES[kind])
+            check_conv(p, run_conv(p, TYPES[kind], gpu_device, act=act), None, act)
+
+
 @pytest.mark.parametrize("place", ["time", "slice"])
 @pytest.mark.parametrize("kind", list(TYPES))
 def test_conv_of_padded_batches(kind, place, gpu_device):
@@ -202,6 +212,16 @@ def test_scan_and_its_gradients(sizes, kind, gpu_device):
         print(f"[case] scan {sizes} {kind} {k}", flush=True)
         p = scan_problem(11 + k, *sizes, TYPES[kind], gate, skip, bias, start)
         check_scan(p, run_scan(p, TYPES[kind], gpu_device, plus=plus), None, plus)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("N", [1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 31, 32, 33, 48, 63, 64])
+def test_scan_with_every_number_of_states(N, kind, gpu_device):
+    """Every number of states a lane and waves a channel, in rows of whole units of 16 bytes and not, over one segment and several."""
+    for channels, G, T in ((40, 1, 133), (24, 3, 45), (10, 2, 133)):
+        print(f"[case] scan states {channels} {N} {G} {T} {kind}", flush=True)
+        p = scan_problem(21, 2, T, channels, N, G, TYPES[kind])
+        check_scan(p, run_scan(p, TYPES[kind], gpu_device), None, True)
 
 
 @pytest.mark.parametrize("place", ["time", "slice"])
