@@ -1225,6 +1225,11 @@ static bool scan_shape(const char* who, int type, int B, int T, int C, int N, in
     fail(RINGATTR_ERR_INVALID, "%s: channels (%d) must be a multiple of groups (%d)", who, C, G);
     return false;
   }
+  // (a workgroup of 512 threads for each group of a sequence and each 16 of its channels or more: a launch counts fewer than 2^32 threads)
+  if ((double)B * G > (double)(1 << 22)) {
+    fail(RINGATTR_ERR_INVALID, "%s: batch_size times groups up to 2^22 (got %d, %d)", who, B, G);
+    return false;
+  }
   s = RingScanShape{B, T, C, N, G, type};
   return true;
 }

@@ -93,6 +93,7 @@ def test_c_abi_refusals():
         assert call(changed(shape, 5, 65)) == 1 and "states" in _lib.last_error()
         assert call(changed(shape, 6, 5)) == 1 and "multiple" in _lib.last_error()
         assert call(changed(shape, 3, (1 << 30) + 1)) == 1
+        assert call([1, 1, 1 << 12, 3, 3000, 16, 3000]) == 1 and "groups" in _lib.last_error()
     sizes = shape[1:]
     assert fwd(x=None) == 1 and fwd(y=p + 4) == 1
     assert lib.ringattr_selective_scan_states_bytes(*sizes) == 2 * 19 * 64 * 16 * 4
