@@ -14,9 +14,9 @@ int tile(int N) { return N <= 16 ? 64 : (N <= 32 ? 32 : 16); }        // channel
 int tiles_of(const RingScanShape& s) { return (s.C / s.G + tile(s.N) - 1) / tile(s.N); }
 int saved_of(const RingScanShape& s) { return (s.T + RingScanArgs::kSave - 1) / RingScanArgs::kSave; }
 
-// Segments that the tokens are cut into: none where every compute unit has a workgroup without, otherwise so many that each has two (us, bf16, 16 states: one
-// sequence of 32768 tokens, 2048 channels, one a unit 825, two 542; two of 2048, with gradients, 320 and 311; eight of 2048, none 243 and 817 with
-// gradients, two 255 and 955).
+// Segments that the tokens are cut into: none where every compute unit has a workgroup without, otherwise so many that each has two (us, bf16, 16 states, 2048
+// channels: one sequence of 32768 tokens by workgroups 256 472, 384 557, 512 424, 768 433; with gradients four of 2048 tokens, none 540, four
+// segments 396; eight, none 549, two 661).
 int segments(const RingScanShape& s) {
   const long groups = (long)tiles_of(s) * s.G * s.B;
   const int units = (s.T + kChunk - 1) / kChunk;
@@ -53,14 +53,14 @@ hipError_t launch_pass(int type, const RingScanArgs& a, int mode, hipStream_t st
 }  // namespace
 
 // What the segments add to a state of zeros becomes the states behind them, in place; a segment's whole decay is the power of its sum of d.
-// A thread walks one state through them.
+// A thread walks one state through them, four reads ahead: bound by latency (16 segments of 2048 channels of 16 states: 7 us; of 630 of 11, 5).
 __global__ __launch_bounds__(256) void ring_scan_between_kernel(float* seg, const float* total, const float* A, const float* s_in, int B, int C, int N,
                                                                 int NS, int ns) {
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, rows = (size_t)B * C;
   if (i >= rows * NS) return;
   const size_t row = i / NS;
   const int n = (int)(i - row * NS), c = (int)(row % C);
-  const float A2 = n < N ? (float)((double)A[(size_t)c * N + n] * 1.4426950408889634) : 0.f;
+  const float A2 = n < N ? times_log2e(A[(size_t)c * N + n]) : 0.f;
   float run = s_in && n < N ? s_in[row * N + n] : 0.f;
 #pragma unroll 4
   for (int u = 0; u < ns; ++u) {
@@ -94,7 +94,8 @@ hipError_t ring_scan_fwd(const RingScanShape& s, RingScanArgs a, void* ws, hipSt
   return e == hipSuccess ? launch_pass(s.type, a, RING_SCAN_OUTPUTS, st) : e;
 }
 
-// dB and dC [B,T,G,N] from the sums over the tiles of a group's channels, in their order; rows that do not count are zero
+// dB and dC [B,T,G,N] from the sums over the tiles of a group's channels, in their order; rows that do not count are zero.  Bound by memory (32 tiles of 16384
+// tokens, 16 states: 67 MB in 13 us, just written and in the last cache in part).
 template <typename T>
 __global__ __launch_bounds__(256) void ring_scan_share_kernel(const float* __restrict__ part, T* dB, T* dC, const int* lengths, int tiles, int B, int Tn, int G,
                                                               int N, int NS) {
@@ -142,34 +143,39 @@ hipError_t ring_scan_bwd(const RingScanShape& s, RingScanArgs a, const RingScanG
   return ring_launch_sum_parts(RingSumArgs{a.part_a, nseg * s.B, per, s.N, 2, (size_t)s.C * per, g.A, {g.D, g.bias}}, st);
 }
 
-// A single token.  A lane takes V states of a channel, `lanes` of them a channel; bound by the states, read and written once.
-template <typename T, int V>
-__global__ __launch_bounds__(256) void ring_scan_step_kernel(RingScanStep p, RingScanShape s, int lanes) {
+// A single token.  A lane takes V states of a channel, 2^log_lanes of them a channel; bound by the states, read and written once (bf16, 16 states, gate: 256
+// sequences of 4096 channels, 143 MB in 28 us, 5.1 TB/s; 34 with places found by divisions of 64 bits, which kept the vector pipes busy; one sequence of 1024
+// channels 4 us, a launch).
+// ONE: a workgroup takes channels of one sequence, whose rows scalar addresses find; otherwise (channels with fewer lanes than that) 2^log_row lanes are a sequence.
+template <typename T, int V, bool ONE>
+__global__ __launch_bounds__(256) void ring_scan_step_kernel(RingScanStep p, RingScanShape s, int log_lanes, int log_row, int blocks) {
   typedef float vec __attribute__((ext_vector_type(V)));
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, row = i / lanes;
-  const int n = (int)(i - row * lanes) * V;
-  if (row >= (size_t)s.B * s.C) return;          // (whole channels: a channel's lanes go together)
-  const int b = (int)(row / s.C), c = (int)(row - (size_t)b * s.C), g = c / (s.C / s.G);
-  T* out = (T*)p.y + row;
+  const int b = ONE ? (int)(blockIdx.x / blocks) : (int)(blockIdx.x * (256 >> log_row) + (threadIdx.x >> log_row));
+  const int i = ONE ? (int)(blockIdx.x - b * blocks) * 256 + (int)threadIdx.x : (int)threadIdx.x & ((1 << log_row) - 1), lanes = 1 << log_lanes;
+  const int c = i >> log_lanes, n = (i & (lanes - 1)) * V;
+  if (b >= s.B || c >= s.C) return;              // (whole channels: a channel's lanes go together)
+  const int g = s.G == 1 ? 0 : c / (s.C / s.G);
+  T* const out = (T*)p.y + (size_t)b * s.C + c;
   if (p.active && !p.active[b]) {
     if (n == 0) *out = (T)0.f;
     return;
   }
-  const float x = (float)((const T*)p.x)[b * p.xs + c];
-  float d = (float)((const T*)p.delta)[b * p.ds + c];
+  const float x = (float)((const T*)p.x + b * p.xs)[c];
+  float d = (float)((const T*)p.delta + b * p.ds)[c], z = 0.f;
+  if (p.z) z = (float)((const T*)p.z + b * p.zs)[c];
   if (p.bias) d += p.bias[c];
   if (p.softplus) d = softplus<sizeof(T) == 4>(d);
   float y = 0.f;
   if (n < s.N) {
-    vec* at = reinterpret_cast<vec*>(p.state + row * s.N + n);
-    const vec A = *reinterpret_cast<const vec*>(p.A + (size_t)c * s.N + n);
-    const T* B = (const T*)p.Bm + b * p.bsb + g * p.bsg + n;
-    const T* C = (const T*)p.Cm + b * p.csb + g * p.csg + n;
+    const int k = c * s.N + n;
+    vec* const at = reinterpret_cast<vec*>(p.state + (size_t)b * s.C * s.N + k);
+    const vec A = *reinterpret_cast<const vec*>(p.A + k);
+    const T* const B = (const T*)p.Bm + b * p.bsb + g * p.bsg + n;
+    const T* const C = (const T*)p.Cm + b * p.csb + g * p.csg + n;
     vec h = *at;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      // (the power as the sequences' kernels form it)
-      h[e] = fmaf(__builtin_amdgcn_exp2f(d * (float)((double)A[e] * 1.4426950408889634)), h[e], d * x * (float)B[e]);
+      h[e] = fmaf(__builtin_amdgcn_exp2f(d * times_log2e(A[e])), h[e], d * x * (float)B[e]);
       y = fmaf(h[e], (float)C[e], y);
     }
     *at = h;
@@ -177,20 +183,23 @@ __global__ __launch_bounds__(256) void ring_scan_step_kernel(RingScanStep p, Rin
   for (int half = lanes / 2; half > 0; half /= 2) y += __shfl_xor(y, half);
   if (n == 0) {
     if (p.D) y = fmaf(p.D[c], x, y);
-    if (p.z) y *= silu<sizeof(T) == 4>((float)((const T*)p.z)[b * p.zs + c]);
+    if (p.z) y *= silu<sizeof(T) == 4>(z);
     *out = (T)y;
   }
 }
 
+template <typename T, int V> static void launch_step_of(const RingScanShape& s, const RingScanStep& a, hipStream_t st) {
+  int log_lanes = 0, log_row = 0;
+  while (V << log_lanes < s.N) ++log_lanes;
+  while (1 << log_row < s.C << log_lanes) ++log_row;
+  const int blocks = ((s.C << log_lanes) + 255) / 256, per = log_row < 8 ? 256 >> log_row : 1;
+  if (log_row >= 8) hipLaunchKernelGGL((ring_scan_step_kernel<T, V, true>), dim3((unsigned)((size_t)blocks * s.B)), dim3(256), 0, st, a, s, log_lanes, log_row, blocks);
+  else hipLaunchKernelGGL((ring_scan_step_kernel<T, V, false>), dim3((unsigned)((s.B + per - 1) / per)), dim3(256), 0, st, a, s, log_lanes, log_row, blocks);
+}
+
 template <typename T> static hipError_t launch_step(const RingScanShape& s, const RingScanStep& a, hipStream_t st) {
-  const bool vec = s.N % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.state) | reinterpret_cast<uintptr_t>(a.A)) & 15) == 0;
-  const int width = vec ? s.N / 4 : s.N;
-  int lanes = 1;
-  while (lanes < width) lanes *= 2;
-  const size_t threads = (size_t)s.B * s.C * lanes;
-  const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
-  if (vec) hipLaunchKernelGGL((ring_scan_step_kernel<T, 4>), grid, block, 0, st, a, s, lanes);
-  else hipLaunchKernelGGL((ring_scan_step_kernel<T, 1>), grid, block, 0, st, a, s, lanes);
+  if (s.N % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.state) | reinterpret_cast<uintptr_t>(a.A)) & 15) == 0) launch_step_of<T, 4>(s, a, st);
+  else launch_step_of<T, 1>(s, a, st);
   return hipGetLastError();
 }
 

@@ -101,6 +101,11 @@ template <typename T, int L, int NS> struct Shared {
 
 // Outputs (and the states kept for a backward), or what a segment adds to a state of zeros, or, backwards in time, to an adjoint of zeros.
 // The first four waves go through the tokens; the other four read and work out the next chunk's rows and finish the last one's outputs meanwhile.
+//
+// Bound by vector instructions: 6 slots of four cycles for a state of a token (a power takes two) and 2.9 for its share of the rows', which keep a unit's four
+// vector pipes busy to 97 percent by their counters; what decides is the one wave of a pipe that goes through the tokens (taking 6 percent of all
+// instructions off the other changed nothing).  Bf16, 16 states, gate: eight sequences of 2048 tokens of 2048 channels 142 us (270 MB: 51 at the
+// rate of a copy; 3.8 T states/s), one of 32768 tokens in 16 segments 190 for what they add, 7 between them and 270 for the outputs.
 template <typename T, int NL, int NB, int MODE, bool WIDE>
 __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
   constexpr int CH = 64 / NB, L = kL, E = CH / 8, NS = 4 * NL * NB, PL = plane<CH, L>();
@@ -118,7 +123,7 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
     float A2[NL], h[NL], total = 0.f;      // total: of d, for the segment's whole decay
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
-      A2[n] = mine && n0 + n < p.N ? (float)((double)p.A[(size_t)c * p.N + n0 + n] * 1.4426950408889634) : 0.f;
+      A2[n] = mine && n0 + n < p.N ? times_log2e(p.A[(size_t)c * p.N + n0 + n]) : 0.f;
       h[n] = 0.f;
       if (OUT && mine) {
         if (seg > 0) h[n] = p.seg[(((size_t)(seg - 1) * p.B + b) * p.C + c) * NS + n0 + n];
@@ -207,8 +212,8 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
     D[e] = OUT && p.D && e < here ? p.D[cr + e] : 0.f;
     bias[e] = p.bias && e < here ? p.bias[cr + e] : 0.f;
   }
-  // Rows two chunks ahead: a chunk takes less time than a row from memory (one chunk ahead: 255 us in place of FWD2 for eight sequences of 2048 tokens, 2048
-  // channels).  Reads have no conditions, which the compiler could not count them by: what is not there is read from a place that is, and left out.
+  // Rows two chunks ahead: a chunk takes less time than a row from memory (one chunk ahead: 255 us in place of 168 for eight sequences of 2048 tokens, 2048
+  // channels, before the rows were buffers).  Reads have no conditions, which the compiler could not count them by: what is not there is read from a place that is, and left out.
   const bool skip = p.D != nullptr;
   struct In { Row<T, E> x, d, z, y; Shared<T, L, NS> B, C; } in[2];
   struct { Row<T, E> x, z; } now, before;
@@ -322,6 +327,10 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
 
 // The gradients.  Chunks of kSave tokens against the time: forwards through a chunk from the state kept in front of it, powers and states in
 // registers, then back.  A quad of lanes shares a channel: sums over its states cross the quad, sums over channels (of dB and dC) the 16 quads.
+//
+// Bound by the vector instructions of the wave that goes through the tokens, 19 for a state of a token: four on the way there, nine on the way back, six for
+// the sums across lanes; it starts one in 69 percent of the cycles that it could.  93 KB of LDS and 250 registers: one workgroup a unit.  Eight sequences of 2048
+// tokens of 2048 channels, 16 states, gate, bf16: 412 us (540 MB with the sums of dB and dC: 102 at the rate of a copy).
 template <typename T, int NL, int NB, bool WIDE>
 __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
   constexpr int CH = 64 / NB, L = kSave, E = CH / 16, NS = 4 * NL * NB, PL = plane<CH, L>(), CW = 4 / NB, R = 8 * NL;
@@ -341,7 +350,7 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
     float A2[NL], G[NL], dA[NL], hk[NL];   // hk: the state kept in front of the next chunk
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
-      A2[n] = mine && n0 + n < p.N ? (float)((double)p.A[(size_t)c * p.N + n0 + n] * 1.4426950408889634) : 0.f;
+      A2[n] = mine && n0 + n < p.N ? times_log2e(p.A[(size_t)c * p.N + n0 + n]) : 0.f;
       G[n] = dA[n] = hk[n] = 0.f;
       if (mine) {
         if (seg < p.nseg - 1) G[n] = p.seg[(((size_t)(p.nseg - 2 - seg) * p.B + b) * p.C + c) * NS + n0 + n];
