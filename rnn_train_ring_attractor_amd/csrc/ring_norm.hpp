@@ -7,7 +7,7 @@
 // - unit mean(d unit unit)); the weights' gradients are sums over rows.  Units and y are found again from what was read.
 //
 // Bound by memory: every tensor is read once or written once.  A row lies in the registers of one workgroup (several rows, where they are short);
-// backwards a workgroup walks rows and keeps the sums of its columns until it is done.
+// backwards a workgroup walks rows and keeps the sums of its columns until it is done.  Rounded are what is written, once each; sums, units and statistics are fp32.
 #pragma once
 #include "ring_recur.hpp"
 #include "ringattr.h"
@@ -136,6 +136,7 @@ __device__ __forceinline__ void normalise(float (&v)[I][V], float (&rstd)[I], co
   for (int i = 0; i < I; ++i) rstd[i] = there[i] ? __builtin_amdgcn_rsqf(fmaf(s[i], each, eps)) : 0.f;
 }
 
+// 32768 rows of 2048, bf16, gate, residual, scale and next norm: 131 us, 671 MB at 5.1 TB/s, which is a copy's; 64 rows 4 us, a launch.
 template <typename T, int V, int I, bool MANY>
 __global__ __launch_bounds__(1024) void ring_norm_fwd_kernel(RingNormArgs p, Lie l) {
   __shared__ float rooms[kRoom];
@@ -197,7 +198,8 @@ __global__ __launch_bounds__(1024) void ring_norm_fwd_kernel(RingNormArgs p, Lie
     }
 }
 
-// MOST threads a workgroup.  Up to 512 of eight values each keep the weights and read the next row ahead; others have no registers left for that.
+// MOST threads a workgroup.  Up to 512 of eight values each keep the weights and read the next row ahead; others have no registers left for that.  32768 rows of
+// 2048, bf16, all of it: 202 us, 1074 MB at 5.3 TB/s, a copy's (240 with sums across waves by a loop over them, which also made the code three times as long).
 template <typename T, int V, int I, bool MANY, int MOST>
 __global__ __launch_bounds__(MOST) void ring_norm_bwd_kernel(RingNormArgs p, Lie l) {
   constexpr bool KEEP = MOST <= 512 && I * V <= 8, FINE = sizeof(T) == 4;
@@ -421,10 +423,10 @@ inline int pow2(int n) {
 struct Plan { Lie lie; int V, I, threads; bool many; };
 
 // Eight values a thread (four of 32 bits) up to 512 threads, whose weights stay in registers; then twice that with 512 threads; then 1024 threads, for rows of 8192
-// whose groups fill little more than half of their threads.  Us of a training step's norms, bf16, 16.8 million values: rows of 8192 as 512 threads of two
+// whose groups fill little more than half of their threads.  Us of a training step's norms, bf16, 67 million values: rows of 8192 as 512 threads of two
 // units 506, as 1024 of one 877; rows of 2047, value by value, as 256 threads of eight 600, as 1024 of two 1279; of 8191 as 512 of sixteen 3588, as 1024 of
-// eight 4115 (both spill registers); fp32, half as many, rows of 2048 as 512 threads of one unit 323, as 256 of two 353; a quarter, of 8192 as 512 threads of
-// four 630, as 1024 of two 949.
+// eight 4115 (both spill registers); fp32, half as many, rows of 2048 as 512 threads of one unit 323, as 256 of two 353, of 8192 as 512 of four 630, as
+// 1024 of two 949.
 inline Plan plan_of(int C, int group, int V) {
   Plan a = {};
   const int groups = C / group, units = (group + V - 1) / V;
