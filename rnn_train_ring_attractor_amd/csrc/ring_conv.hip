@@ -5,8 +5,9 @@
 // Backwards, g_t = dy_t act'(p_t): dx_t = sum_k w[k] g_(t + K - 1 - k), dw[k] = sum_t g_t x_(t - K + 1 + k), dbias = sum_t g_t; p is found again from x.
 //
 // Bound by memory: rows are read once and written once (the K - 1 tokens that a piece of a sequence shares with the next one a second time, from
-// L2).  A thread takes 16 bytes of channels (one channel where rows do not allow that) through a piece's tokens, the next ones on their way; inputs and
-// gradients that later tokens need stay in registers.
+// L2).  A thread takes four channels (one where rows are not whole numbers of four) through a piece's tokens, the next ones on their way; inputs and
+// gradients that later tokens need stay in registers.  (Eight channels of 16 bits, 16 bytes a lane, take 256 registers backwards: 188 us in place of 181, and forwards
+// no less.)
 #include "ring_recur.hpp"
 #include "ringattr.h"
 
@@ -126,8 +127,8 @@ __global__ __launch_bounds__(256) void ring_conv_fwd_kernel(RingConvArgs p, int 
 }
 
 // A token at a time, its input and gradient read KT tokens (or more) ahead.  Inputs and gradients of the last KT tokens go round in registers: a piece's token t is in
-// place t % KT, and so many tokens follow each other without a loop between them that places are known.  Bound by memory and by the vector instructions about half
-// each: 8 x 4096 tokens of 4096 channels, 4 taps, silu, bf16: 190 us, 805 MB at 4.2 TB/s (18 more with windows that move up by one a token).
+// place t % KT, and so many tokens follow each other without a loop between them that places are known.  Bound by memory, in part by its
+// latency: 8 x 4096 tokens of 4096 channels, 4 taps, silu, bf16: 181 us, 805 MB at 4.5 TB/s (18 more with windows that move up by one a token).
 template <typename T, int E, int KT, bool SILU>
 __global__ __launch_bounds__(256) void ring_conv_bwd_kernel(RingConvArgs p, int tx, int blocks) {
   constexpr int N = KT == 2 ? 4 : KT;    // tokens that follow each other
@@ -316,9 +317,8 @@ static int along(int C, int E) {         // threads along the channels
   return tx;
 }
 
-// Pieces are long beside the K - 1 tokens that they share, and short enough that every compute unit has two workgroups, which is what there are registers for
-// backwards (8 x 4096 tokens, 4096 channels, 4 taps, bf16, us forwards and with gradients by a piece's tokens: 32 111, 338; 64 108, 307; 128 105, 289; 192
-// 124, 333; 256 99, 289; 512 155, 438).
+// Pieces are long beside the K - 1 tokens that they share, up to 256, and short enough that every compute unit has two workgroups (8 x 4096 tokens, 4096 channels,
+// 4 taps, bf16, us forwards and with gradients by a piece's tokens: 64 111, 310; 128 103, 292; 256 102, 282; 512 102, 318).
 static void cut(RingConvArgs& p, int tx, int blocks) {
   const int subs = 256 / tx;
   p.seg_tokens = 256;
@@ -334,23 +334,17 @@ template <typename T, int E> static hipError_t launch(RingConvArgs p, bool back,
 #define RING_CONV(KT)                                                                             \
   if (back && p.act == kSilu) hipLaunchKernelGGL((ring_conv_bwd_kernel<T, E, KT, true>), grid, block, 0, st, p, tx, blocks); \
   else if (back) hipLaunchKernelGGL((ring_conv_bwd_kernel<T, E, KT, false>), grid, block, 0, st, p, tx, blocks); \
-  else hipLaunchKernelGGL((ring_conv_fwd_kernel<T, E, KT, 4>), grid, block, 0, st, p, tx, blocks)
+  else hipLaunchKernelGGL((ring_conv_fwd_kernel<T, E, KT, (E > 1 ? 8 : 4)>), grid, block, 0, st, p, tx, blocks)
   if (p.K == 2) { RING_CONV(2); }
   else if (p.K == 3) { RING_CONV(3); }
   else if (p.K == 4) { RING_CONV(4); }
-  else if constexpr (E < 8) { RING_CONV(8); }
+  else { RING_CONV(8); }
 #undef RING_CONV
   return hipGetLastError();
 }
 
-// (of 16 bits: eight channels a thread as long as their inputs, weights and sums have registers; one tap goes through the kernel for up to eight)
-static bool units_of_eight(int K) { return K >= 2 && K <= 4; }
-
 template <typename T> static hipError_t launch_wide(const RingConvArgs& p, bool back, hipStream_t st) {
-  if (!(p.wide && p.wide_out && p.wide_state)) return launch<T, 1>(p, back, st);
-  if constexpr (sizeof(T) == 2)
-    if (units_of_eight(p.K)) return launch<T, 8>(p, back, st);
-  return launch<T, 4>(p, back, st);
+  return p.wide && p.wide_out && p.wide_state ? launch<T, 4>(p, back, st) : launch<T, 1>(p, back, st);
 }
 
 static hipError_t launch_type(const RingConvArgs& p, int type, bool back, hipStream_t st) {
@@ -359,9 +353,9 @@ static hipError_t launch_type(const RingConvArgs& p, int type, bool back, hipStr
   return launch_wide<_Float16>(p, back, st);
 }
 
-// (rows that allow 16 bytes make fewer parts or as many)
-static int parts_of(int type, int B, int T, int C, int K, bool wide) {
-  const int E = wide ? (type == RINGATTR_F32 || !units_of_eight(K) ? 4 : 8) : 1, tx = along(C, E), blocks = (C + tx * E - 1) / (tx * E);
+// (rows of four channels make fewer parts or as many)
+static int parts_of(int B, int T, int C, bool wide) {
+  const int E = wide ? 4 : 1, tx = along(C, E), blocks = (C + tx * E - 1) / (tx * E);
   RingConvArgs p = {};
   p.B = B;
   p.T = T;
@@ -370,9 +364,9 @@ static int parts_of(int type, int B, int T, int C, int K, bool wide) {
   return p.nseg * B;
 }
 
-size_t ring_conv_bwd_bytes(int type, int B, int T, int C, int K, bool params) {
+size_t ring_conv_bwd_bytes(int B, int T, int C, int K, bool params) {
   if (!params) return 0;
-  const int a = parts_of(type, B, T, C, K, true), b = parts_of(type, B, T, C, K, false);
+  const int a = parts_of(B, T, C, true), b = parts_of(B, T, C, false);
   return (size_t)(a > b ? a : b) * C * (K + 1) * sizeof(float);
 }
 
@@ -381,7 +375,7 @@ hipError_t ring_conv_fwd(RingConvArgs p, int type, hipStream_t st) { return laun
 hipError_t ring_conv_bwd(RingConvArgs p, int type, hipStream_t st) {
   hipError_t e = launch_type(p, type, true, st);
   if (e != hipSuccess || !p.part) return e;
-  return ring_launch_sum_parts(RingSumArgs{p.part, parts_of(type, p.B, p.T, p.C, p.K, p.wide && p.wide_out && p.wide_state), p.K + 1, p.K, 1,
+  return ring_launch_sum_parts(RingSumArgs{p.part, parts_of(p.B, p.T, p.C, p.wide && p.wide_out && p.wide_state), p.K + 1, p.K, 1,
                                            (size_t)p.C * (p.K + 1), p.dw, {p.dbias, nullptr}}, st);
 }
 

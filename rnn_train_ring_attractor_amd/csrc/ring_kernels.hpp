@@ -483,7 +483,7 @@ struct RingConvStep {
   const unsigned char* active;
   int B, C, K, act;
 };
-size_t ring_conv_bwd_bytes(int type, int B, int T, int C, int K, bool params);
+size_t ring_conv_bwd_bytes(int B, int T, int C, int K, bool params);
 hipError_t ring_conv_fwd(RingConvArgs p, int type, hipStream_t st);
 hipError_t ring_conv_bwd(RingConvArgs p, int type, hipStream_t st);
 hipError_t ring_conv_step(const RingConvStep& p, int type, hipStream_t st);

@@ -1118,6 +1118,11 @@ static bool rows_wide(const void* p, const long long* strides, int per, int unit
 // Whether a chunk's rows lie behind one another, each as long as it is, within 32 bits of an address.
 static bool rows_apart(long long stride, int n) { return stride >= n && stride <= (1 << 22); }
 
+// Whether rows can be read and written four channels at a time.
+static bool rows_by_four(const void* p, const long long* strides, int C, int type) {
+  return !p || (C % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & (type == RINGATTR_F32 ? 15 : 7)) == 0 && (!strides || (strides[0] % 4 == 0 && strides[1] % 4 == 0)));
+}
+
 static RingRows rows_of_channels(const void* p, const long long* strides) { return RingRows{p, (long)strides[0], (long)strides[1]}; }
 
 static bool conv_shape(const char* who, int act, int type, int B, int T, int C, int K) {
@@ -1131,7 +1136,7 @@ static bool conv_shape(const char* who, int act, int type, int B, int T, int C, 
 
 size_t ringattr_causal_conv_bwd_workspace_bytes(int type, int batch_size, int seq_len, int channels, int taps, int weights) {
   if (!conv_shape("ringattr_causal_conv", RINGATTR_ACT_NONE, type, batch_size, seq_len, channels, taps)) return 0;
-  return ring_conv_bwd_bytes(type, batch_size, seq_len, channels, taps, weights != 0);
+  return ring_conv_bwd_bytes(batch_size, seq_len, channels, taps, weights != 0);
 }
 
 int ringattr_causal_conv_fwd(const void* x, const long long* strides, const void* weight, const void* bias, const void* initial_state,
@@ -1141,7 +1146,6 @@ int ringattr_causal_conv_fwd(const void* x, const long long* strides, const void
   if (!conv_shape(who, activation, type, batch_size, seq_len, channels, taps)) return RINGATTR_ERR_INVALID;
   if (!x || !strides || !weight || !y) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
   if (!aligned16(y) || !aligned16(final_state)) return fail(RINGATTR_ERR_INVALID, "%s: outputs must be 16-byte aligned", who);
-  const int unit = type == RINGATTR_F32 ? 4 : 8;
   RingConvArgs p = {};
   p.x = rows_of_channels(x, strides);
   p.w = (const float*)weight;
@@ -1155,9 +1159,9 @@ int ringattr_causal_conv_fwd(const void* x, const long long* strides, const void
   p.C = channels;
   p.K = taps;
   p.act = activation;
-  p.wide = rows_wide(x, strides, channels, unit);
-  p.wide_state = rows_wide(p.start, nullptr, channels, unit);
-  p.wide_out = channels % unit == 0;
+  p.wide = rows_by_four(x, strides, channels, type);
+  p.wide_state = rows_by_four(p.start, nullptr, channels, type);
+  p.wide_out = channels % 4 == 0;
   hipError_t e = ring_conv_fwd(p, type, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "causal convolution forward launch");
   return RINGATTR_OK;
@@ -1173,10 +1177,9 @@ int ringattr_causal_conv_bwd(const void* x, const void* grad_y, const long long*
   if (!aligned16(grad_x) || !aligned16(grad_initial_state) || !aligned16(workspace))
     return fail(RINGATTR_ERR_INVALID, "%s: outputs and workspace must be 16-byte aligned", who);
   const bool weights = grad_weight || grad_bias;
-  const size_t need = ring_conv_bwd_bytes(type, batch_size, seq_len, channels, taps, weights);
+  const size_t need = ring_conv_bwd_bytes(batch_size, seq_len, channels, taps, weights);
   if (need && (!workspace || workspace_bytes < need))
     return fail(RINGATTR_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
-  const int unit = type == RINGATTR_F32 ? 4 : 8;
   RingConvArgs p = {};
   p.x = rows_of_channels(x, strides);
   p.dy = rows_of_channels(grad_y, strides + 2);
@@ -1195,9 +1198,9 @@ int ringattr_causal_conv_bwd(const void* x, const void* grad_y, const long long*
   p.C = channels;
   p.K = taps;
   p.act = activation;
-  p.wide = rows_wide(x, strides, channels, unit) && rows_wide(grad_y, strides + 2, channels, unit);
-  p.wide_state = rows_wide(p.start, nullptr, channels, unit) && rows_wide(p.dend, nullptr, channels, unit);
-  p.wide_out = channels % unit == 0;
+  p.wide = rows_by_four(x, strides, channels, type) && rows_by_four(grad_y, strides + 2, channels, type);
+  p.wide_state = rows_by_four(p.start, nullptr, channels, type) && rows_by_four(p.dend, nullptr, channels, type);
+  p.wide_out = channels % 4 == 0;
   hipError_t e = ring_conv_bwd(p, type, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "causal convolution backward launch");
   return RINGATTR_OK;
