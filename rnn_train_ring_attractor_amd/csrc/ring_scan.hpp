@@ -102,10 +102,11 @@ template <typename T, int L, int NS> struct Shared {
 // Outputs (and the states kept for a backward), or what a segment adds to a state of zeros, or, backwards in time, to an adjoint of zeros.
 // The first four waves go through the tokens; the other four read and work out the next chunk's rows and finish the last one's outputs meanwhile.
 //
-// Bound by vector instructions: 6 slots of four cycles for a state of a token (a power takes two) and 2.9 for its share of the rows', which keep a unit's four
-// vector pipes busy to 97 percent by their counters; what decides is the one wave of a pipe that goes through the tokens (taking 6 percent of all
-// instructions off the other changed nothing).  Bf16, 16 states, gate: eight sequences of 2048 tokens of 2048 channels 142 us (270 MB: 51 at the
-// rate of a copy; 3.8 T states/s), one of 32768 tokens in 16 segments 190 for what they add, 7 between them and 270 for the outputs.
+// Bound by vector instructions: a power takes a pipe 8.5 cycles, as do exchanges of lanes; a multiplication or addition takes 4.5 of one wave, of which two waves' overlap.
+// A state of a token is a power and four of the others, and 2.4 instructions for its share of the rows'.  Their counters have the pipes busy to 97
+// percent at four cycles each; two workgroups a unit, where there are so many, are 4 percent faster than one.  Bf16, 16 states, gate: eight sequences of
+// 2048 tokens of 2048 channels 142 us (270 MB: 51 at the rate of a copy; 3.8 T states/s), one of 32768 tokens in 16 segments 190 for what they add,
+// 7 between them and 270 for the outputs.
 template <typename T, int NL, int NB, int MODE, bool WIDE>
 __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
   constexpr int CH = 64 / NB, L = kL, E = CH / 8, NS = 4 * NL * NB, PL = plane<CH, L>();
@@ -328,9 +329,10 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
 // The gradients.  Chunks of kSave tokens against the time: forwards through a chunk from the state kept in front of it, powers and states in
 // registers, then back.  A quad of lanes shares a channel: sums over its states cross the quad, sums over channels (of dB and dC) the 16 quads.
 //
-// Bound by the vector instructions of the wave that goes through the tokens, 19 for a state of a token: four on the way there, nine on the way back, six for
-// the sums across lanes; it starts one in 69 percent of the cycles that it could.  93 KB of LDS and 250 registers: one workgroup a unit.  Eight sequences of 2048
-// tokens of 2048 channels, 16 states, gate, bf16: 412 us (540 MB with the sums of dB and dC: 102 at the rate of a copy).
+// Bound by the wave of a pipe that goes through the tokens, which never waits for the others: 19 vector instructions for a state of a token (four on the way there,
+// nine on the way back, six for the sums across lanes), 4.5 cycles each and 8.5 for powers and exchanges, and 80 accesses to LDS a chunk.  Eight waves of
+// two states a lane have more of both and are slower (us of a training step 647 in place of 552).  93 KB of LDS and 250 registers: one workgroup a
+// unit.  Eight sequences of 2048 tokens of 2048 channels, 16 states, gate, bf16: 412 us (540 MB with the sums of dB and dC: 102 at the rate of a copy).
 template <typename T, int NL, int NB, bool WIDE>
 __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
   constexpr int CH = 64 / NB, L = kSave, E = CH / 16, NS = 4 * NL * NB, PL = plane<CH, L>(), CW = 4 / NB, R = 8 * NL;
