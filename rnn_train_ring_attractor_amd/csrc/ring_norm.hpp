@@ -420,7 +420,7 @@ inline int pow2(int n) {
   return p;
 }
 
-struct Plan { Lie lie; int V, I, threads; bool many; };
+struct Plan { Lie lie; int I, threads; bool many; };
 
 // Eight values a thread (four of 32 bits) up to 512 threads, whose weights stay in registers; then twice that with 512 threads; then 1024 threads, for rows of 8192
 // whose groups fill little more than half of their threads.  Us of a training step's norms, bf16, 67 million values: rows of 8192 as 512 threads of two
@@ -430,7 +430,6 @@ struct Plan { Lie lie; int V, I, threads; bool many; };
 inline Plan plan_of(int C, int group, int V) {
   Plan a = {};
   const int groups = C / group, units = (group + V - 1) / V;
-  a.V = V;
   a.many = groups > 1 && units <= 64;
   for (a.threads = 64; a.threads <= 1024; a.threads *= 2) {
     a.lie = {0, 0, 1, units, groups};

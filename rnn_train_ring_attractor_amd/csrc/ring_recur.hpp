@@ -77,14 +77,10 @@ template <typename T, int E> struct Row {
       for (int e = 0; e < E; ++e) v[e] = e < here ? p[e] : (T)0.f;
     }
   }
-  // The same without conditions: `here` of them (at least one) and copies of the last
-  template <bool WIDE> __device__ __forceinline__ void read(const T* p, int here) {
-    if constexpr (WIDE) {
-      load(p, true, E);
-    } else {
+  // One by one without conditions: `here` of them (at least one) and copies of the last
+  __device__ __forceinline__ void read(const T* p, int here) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = p[min(e, here - 1)];
-    }
+    for (int e = 0; e < E; ++e) v[e] = p[min(e, here - 1)];
   }
   // From and to a buffer, at a number of bytes
   __device__ __forceinline__ void fetch(__amdgpu_buffer_rsrc_t b, int at) {

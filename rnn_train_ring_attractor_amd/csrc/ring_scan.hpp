@@ -216,7 +216,7 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
   // Rows two chunks ahead: a chunk takes less time than a row from memory (one chunk ahead: 255 us in place of 168 for eight sequences of 2048 tokens, 2048
   // channels, before the rows were buffers).  Reads have no conditions, which the compiler could not count them by: what is not there is read from a place that is, and left out.
   const bool skip = p.D != nullptr;
-  struct In { Row<T, E> x, d, z, y; Shared<T, L, NS> B, C; } in[2];
+  struct In { Row<T, E> x, d, z; Shared<T, L, NS> B, C; } in[2];
   struct { Row<T, E> x, z; } now, before;
   const int tr = here > 0 ? here : at_.here, cw = here > 0 ? cr : at_.c0;
   const T *const dp = (const T*)p.delta.p + b * p.delta.sb, *const xp = (const T*)(REV ? p.dy.p : p.x.p) + b * (REV ? p.dy.sb : p.x.sb),
@@ -244,9 +244,9 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
       if (OUT) r.C.fetch(buffer_of(Cp + t0 * p.cst, p.cst, rows), Cw);
     } else {
       const long t = min(t0 + tl, end - 1);
-      r.d.template read<false>(dp + cw + t * p.delta.st, tr);
-      r.x.template read<false>(xp + cw + t * xt, tr);
-      if (OUT || REV) r.z.template read<false>(zp + cw + t * zt, tr);
+      r.d.read(dp + cw + t * p.delta.st, tr);
+      r.x.read(xp + cw + t * xt, tr);
+      if (OUT || REV) r.z.read(zp + cw + t * zt, tr);
       r.B.load(Bp, Bt, t0, end, p.N, tid);
       if (OUT) r.C.load(Cp, p.cst, t0, end, p.N, tid);
     }
@@ -536,10 +536,10 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
       r.C.fetch(buffer_of(Cp + t0 * p.cst, p.cst, rows), Cw);
     } else {
       const long t = min(t0 + tl, end - 1);
-      r.d.template read<false>(dp + cw + t * p.delta.st, tr);
-      r.x.template read<false>(xp + cw + t * p.x.st, tr);
-      r.z.template read<false>(zp + cw + t * zt, tr);
-      r.y.template read<false>(yp + cw + t * p.dy.st, tr);
+      r.d.read(dp + cw + t * p.delta.st, tr);
+      r.x.read(xp + cw + t * p.x.st, tr);
+      r.z.read(zp + cw + t * zt, tr);
+      r.y.read(yp + cw + t * p.dy.st, tr);
       r.B.load(Bp, p.bst, t0, end, p.N, tid);
       r.C.load(Cp, p.cst, t0, end, p.N, tid);
     }

@@ -1110,18 +1110,13 @@ static bool rows_shape(const char* who, int type, int B, int T, int C) {
   return true;
 }
 
-// Whether rows of channels can be read (or written) 16 bytes at a time; `per` channels are what belongs together.
-static bool rows_wide(const void* p, const long long* strides, int per, int unit) {
-  return !p || (per % unit == 0 && aligned16(p) && (!strides || (strides[0] % unit == 0 && strides[1] % unit == 0)));
+// Whether rows of channels can be read (or written) `unit` at a time, `bytes` or whole numbers of that; `per` channels are what belongs together.
+static bool rows_by(const void* p, const long long* strides, int per, int unit, int bytes) {
+  return !p || (per % unit == 0 && reinterpret_cast<uintptr_t>(p) % bytes == 0 && (!strides || (strides[0] % unit == 0 && strides[1] % unit == 0)));
 }
 
 // Whether a chunk's rows lie behind one another, each as long as it is, within 32 bits of an address.
 static bool rows_apart(long long stride, int n) { return stride >= n && stride <= (1 << 22); }
-
-// Whether rows can be read and written four channels at a time.
-static bool rows_by_four(const void* p, const long long* strides, int C, int type) {
-  return !p || (C % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & (type == RINGATTR_F32 ? 15 : 7)) == 0 && (!strides || (strides[0] % 4 == 0 && strides[1] % 4 == 0)));
-}
 
 static RingRows rows_of_channels(const void* p, const long long* strides) { return RingRows{p, (long)strides[0], (long)strides[1]}; }
 
@@ -1146,6 +1141,7 @@ int ringattr_causal_conv_fwd(const void* x, const long long* strides, const void
   if (!conv_shape(who, activation, type, batch_size, seq_len, channels, taps)) return RINGATTR_ERR_INVALID;
   if (!x || !strides || !weight || !y) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
   if (!aligned16(y) || !aligned16(final_state)) return fail(RINGATTR_ERR_INVALID, "%s: outputs must be 16-byte aligned", who);
+  const int bytes = type == RINGATTR_F32 ? 16 : 8;
   RingConvArgs p = {};
   p.x = rows_of_channels(x, strides);
   p.w = (const float*)weight;
@@ -1159,8 +1155,8 @@ int ringattr_causal_conv_fwd(const void* x, const long long* strides, const void
   p.C = channels;
   p.K = taps;
   p.act = activation;
-  p.wide = rows_by_four(x, strides, channels, type);
-  p.wide_state = rows_by_four(p.start, nullptr, channels, type);
+  p.wide = rows_by(x, strides, channels, 4, bytes);
+  p.wide_state = rows_by(p.start, nullptr, channels, 4, bytes);
   p.wide_out = channels % 4 == 0;
   hipError_t e = ring_conv_fwd(p, type, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "causal convolution forward launch");
@@ -1180,6 +1176,7 @@ int ringattr_causal_conv_bwd(const void* x, const void* grad_y, const long long*
   const size_t need = ring_conv_bwd_bytes(batch_size, seq_len, channels, taps, weights);
   if (need && (!workspace || workspace_bytes < need))
     return fail(RINGATTR_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
+  const int bytes = type == RINGATTR_F32 ? 16 : 8;
   RingConvArgs p = {};
   p.x = rows_of_channels(x, strides);
   p.dy = rows_of_channels(grad_y, strides + 2);
@@ -1198,8 +1195,8 @@ int ringattr_causal_conv_bwd(const void* x, const void* grad_y, const long long*
   p.C = channels;
   p.K = taps;
   p.act = activation;
-  p.wide = rows_by_four(x, strides, channels, type) && rows_by_four(grad_y, strides + 2, channels, type);
-  p.wide_state = rows_by_four(p.start, nullptr, channels, type) && rows_by_four(p.dend, nullptr, channels, type);
+  p.wide = rows_by(x, strides, channels, 4, bytes) && rows_by(grad_y, strides + 2, channels, 4, bytes);
+  p.wide_state = rows_by(p.start, nullptr, channels, 4, bytes) && rows_by(p.dend, nullptr, channels, 4, bytes);
   p.wide_out = channels % 4 == 0;
   hipError_t e = ring_conv_bwd(p, type, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "causal convolution backward launch");
@@ -1280,7 +1277,7 @@ static RingScanArgs scan_args(const RingScanShape& s, const void* x, const void*
   a.G = s.G;
   a.softplus = softplus ? 1 : 0;
   const int per = s.C / s.G;
-  a.wide = rows_wide(x, st, per, 8) && rows_wide(delta, st + 2, per, 8) && rows_wide(z, st + 4, per, 8) && rows_apart(st[1], s.C) &&
+  a.wide = rows_by(x, st, per, 8, 16) && rows_by(delta, st + 2, per, 8, 16) && rows_by(z, st + 4, per, 8, 16) && rows_apart(st[1], s.C) &&
            rows_apart(st[3], s.C) && (!z || rows_apart(st[5], s.C)) && rows_apart(st[7], s.N) && rows_apart(st[10], s.N);
   return a;
 }
@@ -1326,7 +1323,7 @@ int ringattr_selective_scan_bwd(const void* x, const void* delta, const void* z,
     return fail(RINGATTR_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
   RingScanArgs a = scan_args(s, x, delta, z, B, C, strides, A, D, delta_bias, lengths, softplus);
   a.dy = rows_of_channels(grad_y, strides + 12);
-  a.wide = a.wide && rows_wide(grad_y, strides + 12, channels / groups, 8) && rows_apart(strides[13], channels);
+  a.wide = a.wide && rows_by(grad_y, strides + 12, channels / groups, 8, 16) && rows_apart(strides[13], channels);
   a.states = (float*)const_cast<void*>(states_kept);
   a.s_in = (const float*)grad_final_state;
   a.s_out = (float*)grad_initial_state;
