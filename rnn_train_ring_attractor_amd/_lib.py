@@ -232,6 +232,11 @@ def pointer(t):
     return None if t is None else t.data_ptr()
 
 
+def empty_of(t):
+    """Memory for a result of t's shape and type, contiguous (the first way costs the host a third less)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def checked_lengths(lengths, B, T, device):
     """The tokens that count of each sequence of a padded batch, as the library takes them."""
     if lengths is None:

@@ -11,7 +11,7 @@ import torch
 from torch.autograd import Function
 
 from . import _lib
-from ._lib import SEQUENCE_TYPES, check_sequence_sizes, check_sequence_tensor, checked_parameter, pointer, resolved, rows_of
+from ._lib import SEQUENCE_TYPES, check_sequence_sizes, check_sequence_tensor, checked_parameter, empty_of, pointer, resolved, rows_of
 
 _Strides2, _Strides4 = ctypes.c_longlong * 2, ctypes.c_longlong * 4
 _ACTIVATIONS = {None: 0, "silu": 1}
@@ -37,7 +37,7 @@ def _forward(x, weight, bias, initial_state, lengths, act, want_state):
     B, T, C = x.shape
     K, dev = weight.shape[1], x.device
     with _lib.on_device(dev):
-        y = x.new_empty((B, T, C))
+        y = empty_of(x)
         state = x.new_empty((B, K - 1, C)) if want_state else None
         if B == 0 or T == 0:
             if want_state:
@@ -68,7 +68,7 @@ class CausalConvFunc(Function):
         K, dev = weight.shape[1], x.device
         lib, kind = _lib.load(), SEQUENCE_TYPES[x.dtype]
         with _lib.on_device(dev):
-            gx, gw, gb, g0 = (t.new_empty(t.shape) if t is not None and needed else None
+            gx, gw, gb, g0 = (empty_of(t) if t is not None and needed else None
                               for t, needed in zip((x, weight, bias, initial_state), ctx.needs_input_grad))
             gs = None if grad_state is None else resolved(grad_state).contiguous()
             if B == 0 or T == 0:

@@ -7,7 +7,7 @@ import torch
 from torch.autograd import Function
 
 from . import _lib
-from ._lib import SEQUENCE_TYPES, check_sequence_tensor, checked_parameter, pointer
+from ._lib import SEQUENCE_TYPES, check_sequence_tensor, checked_parameter, empty_of, pointer
 
 _Strides3, _Strides5 = ctypes.c_longlong * 3, ctypes.c_longlong * 5
 _KINDS = {"rms": 0, "layer": 1}
@@ -27,8 +27,8 @@ def _flat(t):
 def _forward(x, weight, gate, residual, scale, next_weight, group, eps, kind, act):
     C, dev = x.shape[-1], x.device
     with _lib.on_device(dev):
-        y = x.new_empty(x.shape)
-        n = x.new_empty(x.shape) if next_weight is not None else None
+        y = empty_of(x)
+        n = empty_of(x) if next_weight is not None else None
         if x.numel() == 0:
             return y, n
         (fx, sx), (fg, sg), (fr, sr) = _flat(x), _flat(gate), _flat(residual)
@@ -58,9 +58,9 @@ class NormGateFunc(Function):
         C, dev, need = x.shape[-1], x.device, ctx.needs_input_grad
         lib, code = _lib.load(), SEQUENCE_TYPES[x.dtype]
         with _lib.on_device(dev):
-            gx, gw, gg, gs, gn = (t.new_empty(t.shape) if t is not None and n else None
+            gx, gw, gg, gs, gn = (empty_of(t) if t is not None and n else None
                                   for t, n in zip((x, weight, gate, scale, next_weight), (*need[:3], *need[4:6])))
-            gr = x.new_empty(x.shape) if need[3] else None
+            gr = empty_of(x) if need[3] else None
             if grad_n is None and gn is not None:
                 gn.zero_()
             if x.numel() == 0 or (grad_y is None and grad_n is None):

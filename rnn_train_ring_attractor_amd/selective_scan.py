@@ -14,7 +14,7 @@ import torch
 from torch.autograd import Function
 
 from . import _lib
-from ._lib import SEQUENCE_TYPES, check_sequence_sizes, check_sequence_tensor, checked_parameter, pointer, resolved, rows_of
+from ._lib import SEQUENCE_TYPES, check_sequence_sizes, check_sequence_tensor, checked_parameter, empty_of, pointer, resolved, rows_of
 
 _Strides12, _Strides14, _Strides7 = ctypes.c_longlong * 12, ctypes.c_longlong * 14, ctypes.c_longlong * 7
 
@@ -51,7 +51,7 @@ def _forward(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths, softpl
     N, G, dev = A.shape[1], B.shape[2], x.device
     lib, sizes = _lib.load(), (SEQUENCE_TYPES[x.dtype], batch, T, channels, N, G)
     with _lib.on_device(dev):
-        y = x.new_empty((batch, T, channels))
+        y = empty_of(x)
         state = A.new_empty((batch, channels, N)) if want_state else None
         if batch == 0 or T == 0:
             if want_state:
@@ -87,7 +87,7 @@ class SelectiveScanFunc(Function):
         lib, dev, sizes = _lib.load(), x.device, (SEQUENCE_TYPES[x.dtype], batch, T, channels, A.shape[1], B.shape[2])
         need = ctx.needs_input_grad
         with _lib.on_device(dev):
-            gx, gd, gA, gB, gC, gD, gz, gb = (t.new_empty(t.shape) if t is not None and n else None
+            gx, gd, gA, gB, gC, gD, gz, gb = (empty_of(t) if t is not None and n else None
                                               for t, n in zip((x, delta, A, B, C, D, z, delta_bias), need))
             g0 = A.new_empty(ctx.start) if ctx.start is not None and need[8] else None
             gs = None if grad_state is None else resolved(grad_state).contiguous()
