@@ -331,7 +331,8 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
 //
 // Bound by the wave of a pipe that goes through the tokens, which never waits for the others: 19 vector instructions for a state of a token (four on the way there,
 // nine on the way back, six for the sums across lanes), 4.5 cycles each and 8.5 for powers and exchanges, and 80 accesses to LDS a chunk.  Eight waves of
-// two states a lane have more of both and are slower (us of a training step 647 in place of 552).  93 KB of LDS and 250 registers: one workgroup a
+// two states a lane have more of both and are slower (us of a training step 647 in place of 552).  Outputs in front of the gate, two more instructions and the sums, are
+// found only where its gradient is wanted (541 us without a gate, 513 so).  93 KB of LDS and 250 registers: one workgroup a
 // unit.  Eight sequences of 2048 tokens of 2048 channels, 16 states, gate, bf16: 412 us (540 MB with the sums of dB and dC: 102 at the rate of a copy).
 template <typename T, int NL, int NB, bool WIDE>
 __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
@@ -365,7 +366,8 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
     if (chunks > 0) kept(0);
     __syncthreads();
     const int r = lane >> 4, quad = lane >> 2 & 3;
-    auto chunk = [&](int k, auto whole) {
+    auto chunk = [&](int k, auto whole, auto gated) {      // gated: the outputs in front of the gate are wanted, for its gradient
+      constexpr bool GATED = decltype(gated)::value;
       const int t0 = begin(k), f = k & 1;
       float h[NL], hs[L][NL], as[L][NL], dAc[NL];
 #pragma unroll
@@ -451,7 +453,7 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
                 for (int n = 0; n < NL; ++n) dAc[n] = 0.f;
 #pragma unroll
             for (int n = 0; n < NL; ++n) {
-              y[i] = n == 0 ? Cn[n] * h[n] : fmaf(Cn[n], h[n], y[i]);
+              if constexpr (GATED) y[i] = n == 0 ? Cn[n] * h[n] : fmaf(Cn[n], h[n], y[i]);
               v[NL + n] = q4[i] * h[n];
               const float gn = fmaf(q4[i], Cn[n], G[n]);
               v[n] = gn * u4[i];
@@ -473,7 +475,7 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
         // over a quad, whose lane sub is left with token j + sub
         o_[j] = quad_sums(s1, sub);
         o_[NB * PL + j] = quad_sums(s2, sub);
-        o_[2 * NB * PL + j] = quad_sums(y, sub);
+        if constexpr (GATED) o_[2 * NB * PL + j] = quad_sums(y, sub);
         // over a row's quads
 #pragma unroll
         for (int m = 0; m < LEFT; ++m) r_[(j + m * 4 / LEFT) * R] = row_sums(val + 4 * m, quad);
@@ -484,8 +486,11 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
       __syncthreads();
     };
     int k = 0;
-    if (chunks > 0 && begin(0) + L > end) chunk(k++, std::false_type{});
-    for (; k < chunks; ++k) chunk(k, std::true_type{});
+    if (chunks > 0 && begin(0) + L > end) chunk(k++, std::false_type{}, std::true_type{});
+    if (p.dz)
+      for (; k < chunks; ++k) chunk(k, std::true_type{}, std::true_type{});
+    else
+      for (; k < chunks; ++k) chunk(k, std::true_type{}, std::false_type{});
     if (mine) {
       if (part) {
 #pragma unroll
@@ -582,15 +587,14 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
     const int t0 = begin(k), t = t0 + tl, f = k & 1;
     const float* const o_ = so[f] + at<L>(cl, tl);
     Row<T, E> ox, od, oz;
-    float s1[E], s2[E], y[E], dd[E];
+    float s1[E], s2[E], dd[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      s1[e] = s2[e] = y[e] = 0.f;
+      s1[e] = s2[e] = 0.f;
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         s1[e] += o_[i * PL + e * (L + 4)];
         s2[e] += o_[(NB + i) * PL + e * (L + 4)];
-        y[e] += o_[(2 * NB + i) * PL + e * (L + 4)];
       }
       dd[e] = fmaf(s1[e], (float)before.x.v[e], s2[e] * kLn2) * before.slope[e];
     }
@@ -603,10 +607,13 @@ __global__ __launch_bounds__(512) void ring_scan_bwd_kernel(RingScanArgs p) {
       dD[e] = counts ? fmaf(before.q[e], x, dD[e]) : dD[e];
       dbias[e] = counts ? dbias[e] + dd[e] : dbias[e];
     }
-    if (p.z.p)
+    if (p.dz)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float g = (float)before.y.v[e] * fmaf(D[e], (float)before.x.v[e], y[e]) * silu_slope((float)before.z.v[e], before.gate[e]);
+        float y = o_[2 * NB * PL + e * (L + 4)];
+#pragma unroll
+        for (int i = 1; i < NB; ++i) y += o_[(2 * NB + i) * PL + e * (L + 4)];
+        const float g = (float)before.y.v[e] * fmaf(D[e], (float)before.x.v[e], y) * silu_slope((float)before.z.v[e], before.gate[e]);
         oz.v[e] = (T)(t < end && e < here ? g : 0.f);
       }
     if constexpr (WIDE) {
