@@ -331,7 +331,7 @@ __global__ __launch_bounds__(512) void ring_scan_kernel(RingScanArgs p) {
 //
 // Bound by the wave of a pipe that goes through the tokens, which never waits for the others: 19 vector instructions for a state of a token (four on the way there,
 // nine on the way back, six for the sums across lanes), 4.5 cycles each and 8.5 for powers and exchanges, and 80 accesses to LDS a chunk.  Eight waves of
-// two states a lane have more of both and are slower (us of a training step 647 in place of 552).  Outputs in front of the gate, two more instructions and the sums, are
+// two states a lane have more of both and are slower (us of a training step 647 in place of 552).  Outputs in front of the gate, one more and the sums, are
 // found only where its gradient is wanted (541 us without a gate, 513 so).  93 KB of LDS and 250 registers: one workgroup a
 // unit.  Eight sequences of 2048 tokens of 2048 channels, 16 states, gate, bf16: 412 us (540 MB with the sums of dB and dC: 102 at the rate of a copy).
 template <typename T, int NL, int NB, bool WIDE>
