@@ -163,6 +163,34 @@ template <int CTRL> __device__ __forceinline__ float plus_dpp(float x) {
 }
 constexpr int kRor8 = 0x128, kUp4 = 0x104, kDown4 = 0x114, kXor1 = 0xB1, kXor2 = 0x4E;      // (up 4: the lane four further on)
 
+// Sums over parts in their order (RingSumArgs): a workgroup of 256 takes 256 / W columns; W threads share a column's parts and are added in their order
+constexpr int kWays = 8;
+inline int sum_ways(const RingSumArgs& p) { return p.parts >= 16 ? kWays : 1; }
+inline unsigned sum_blocks(const RingSumArgs& p) { return (unsigned)((p.n * sum_ways(p) + 255) / 256); }
+template <int W> __device__ __forceinline__ void sum_parts(const RingSumArgs& p, unsigned block, float* sums) {
+  constexpr int COLS = 256 / W;
+  const size_t i = (size_t)block * COLS + threadIdx.x % COLS;
+  const int w = threadIdx.x / COLS, each = (p.parts + W - 1) / W, end = min(p.parts, (w + 1) * each);
+  float sum = 0.f;
+  if (i < p.n)
+#pragma unroll 8
+    for (int k = w * each; k < end; ++k) sum += p.part[(size_t)k * p.n + i];
+  if constexpr (W > 1) {
+    sums[threadIdx.x] = sum;
+    __syncthreads();
+    if (w > 0) return;
+    for (int k = 1; k < W; ++k) sum += sums[k * COLS + threadIdx.x];
+  }
+  if (i >= p.n) return;
+  const size_t column = i / p.per;
+  const int k = (int)(i - column * p.per), more = k - (p.per - p.rest);
+  if (k < p.N) {
+    if (p.out) p.out[column * p.N + k] = sum;
+  } else if (more >= 0 && p.more[more]) {
+    p.more[more][column] = sum;
+  }
+}
+
 __device__ __forceinline__ int length_of(const int* lengths, int b, int T) { return lengths ? min(max(lengths[b], 0), T) : T; }
 
 }  // namespace ring_recur

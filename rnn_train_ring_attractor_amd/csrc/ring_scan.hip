@@ -94,13 +94,16 @@ hipError_t ring_scan_fwd(const RingScanShape& s, RingScanArgs a, void* ws, hipSt
   return e == hipSuccess ? launch_pass(s.type, a, RING_SCAN_OUTPUTS, st) : e;
 }
 
-// dB and dC [B,T,G,N] from the sums over the tiles of a group's channels, in their order; rows that do not count are zero.  Bound by memory (32 tiles of 16384
-// tokens, 16 states: 67 MB in 13 us, just written and in the last cache in part).
-template <typename T>
-__global__ __launch_bounds__(256) void ring_scan_share_kernel(const float* __restrict__ part, T* dB, T* dC, const int* lengths, int tiles, int B, int Tn, int G,
-                                                              int N, int NS) {
+// What parts become, in one launch.  The first `columns` workgroups: sums of the parameters' parts, bound by latency.  The others: dB and dC [B,T,G,N] from the sums over the
+// tiles of a group's channels, in their order; rows that do not count are zero; bound by memory (32 tiles of 16384 tokens, 16 states: 67 MB, just written and in the
+// last cache in part).  14 us there, 4 for 4 tiles of 3885 tokens (as two launches 18, 9).
+template <typename T, int W>
+__global__ __launch_bounds__(256) void ring_scan_join_kernel(const float* __restrict__ part, T* dB, T* dC, const int* lengths, int tiles, int B, int Tn, int G, int N,
+                                                             int NS, unsigned columns, RingSumArgs p) {
+  __shared__ float sums[256];
+  if (blockIdx.x < columns) return sum_parts<W>(p, blockIdx.x, sums);
   const size_t rows = (size_t)B * Tn * G, all = rows * 2 * NS;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
+  for (size_t i = (size_t)(blockIdx.x - columns) * 256 + threadIdx.x; i < all; i += (size_t)(gridDim.x - columns) * 256) {
     const size_t row = i / (2 * NS);
     const int k = (int)(i - row * 2 * NS), n = k % NS;
     T* out = k < NS ? dB : dC;
@@ -114,10 +117,18 @@ __global__ __launch_bounds__(256) void ring_scan_share_kernel(const float* __res
   }
 }
 
-template <typename T> static void launch_share(const RingScanShape& s, const RingScanArgs& a, const RingScanGrads& g, hipStream_t st) {
-  const size_t blocks = ((size_t)s.B * s.T * s.G * 2 * padded(s.N) + 255) / 256;
-  hipLaunchKernelGGL(ring_scan_share_kernel<T>, dim3((unsigned)(blocks < (1 << 22) ? blocks : 1 << 22)), dim3(256), 0, st, a.part_bc, (T*)g.B, (T*)g.C, a.lengths,
-                     tiles_of(s), s.B, s.T, s.G, s.N, padded(s.N));
+template <typename T> static hipError_t launch_join(const RingScanShape& s, const RingScanArgs& a, const RingScanGrads& g, int nseg, hipStream_t st) {
+  const int per = padded(s.N) + 2;
+  const RingSumArgs p = {a.part_a, nseg * s.B, per, s.N, 2, a.part_a ? (size_t)s.C * per : 0, g.A, {g.D, g.bias}};
+  const size_t blocks = a.part_bc ? ((size_t)s.B * s.T * s.G * 2 * padded(s.N) + 255) / 256 : 0;
+  const unsigned columns = sum_blocks(p);
+  const dim3 grid(columns + (unsigned)(blocks < (1 << 22) ? blocks : 1 << 22)), block(256);
+  if (grid.x == 0) return hipSuccess;
+  T *const dB = (T*)g.B, *const dC = (T*)g.C;
+  const int tiles = tiles_of(s), NS = padded(s.N);
+  if (sum_ways(p) > 1) hipLaunchKernelGGL((ring_scan_join_kernel<T, kWays>), grid, block, 0, st, a.part_bc, dB, dC, a.lengths, tiles, s.B, s.T, s.G, s.N, NS, columns, p);
+  else hipLaunchKernelGGL((ring_scan_join_kernel<T, 1>), grid, block, 0, st, a.part_bc, dB, dC, a.lengths, tiles, s.B, s.T, s.G, s.N, NS, columns, p);
+  return hipGetLastError();
 }
 
 hipError_t ring_scan_bwd(const RingScanShape& s, RingScanArgs a, const RingScanGrads& g, void* ws, hipStream_t st) {
@@ -132,15 +143,8 @@ hipError_t ring_scan_bwd(const RingScanShape& s, RingScanArgs a, const RingScanG
   hipError_t e = between(s, a, RING_SCAN_ADJOINT, st);
   if (e == hipSuccess) e = launch_pass(s.type, a, RING_SCAN_GRADIENTS, st);
   if (e != hipSuccess) return e;
-  if (a.part_bc) {
-    if (s.type == RINGATTR_F32) launch_share<float>(s, a, g, st);
-    else if (s.type == RINGATTR_BF16) launch_share<__bf16>(s, a, g, st);
-    else launch_share<_Float16>(s, a, g, st);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-  }
-  if (!a.part_a) return hipSuccess;
-  const int per = padded(s.N) + 2;
-  return ring_launch_sum_parts(RingSumArgs{a.part_a, nseg * s.B, per, s.N, 2, (size_t)s.C * per, g.A, {g.D, g.bias}}, st);
+  if (s.type == RINGATTR_F32) return launch_join<float>(s, a, g, nseg, st);
+  return s.type == RINGATTR_BF16 ? launch_join<__bf16>(s, a, g, nseg, st) : launch_join<_Float16>(s, a, g, nseg, st);
 }
 
 // A single token.  A lane takes V states of a channel, 2^log_lanes of them a channel; bound by the states, read and written once (bf16, 16 states, gate: 256
