@@ -52,8 +52,10 @@ hipError_t launch_pass(int type, const RingScanArgs& a, int mode, hipStream_t st
 
 }  // namespace
 
-// What the segments add to a state of zeros becomes the states behind them, in place; a segment's whole decay is the power of its sum of d.
-// A thread walks one state through them, four reads ahead: bound by latency (16 segments of 2048 channels of 16 states: 7 us; of 630 of 11, 5).
+// What the segments add to a state of zeros becomes the states behind them, in place; a segment's whole decay is the power of its sum of d.  Where that may be a power that 32
+// bits do not hold and its product with the state a number all the same, whole powers go into the exponent: zero and infinity stay what they are, as
+// they do under the tokens one by one.
+// A thread walks one state through them, a segment's reads behind the last one's write: bound by latency (16 segments of 2048 channels of 16 states: 7 us; of 630 of 11, 5).
 __global__ __launch_bounds__(256) void ring_scan_between_kernel(float* seg, const float* total, const float* A, const float* s_in, int B, int C, int N,
                                                                 int NS, int ns) {
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, rows = (size_t)B * C;
@@ -64,8 +66,10 @@ __global__ __launch_bounds__(256) void ring_scan_between_kernel(float* seg, cons
   float run = s_in && n < N ? s_in[row * N + n] : 0.f;
 #pragma unroll 4
   for (int u = 0; u < ns; ++u) {
-    const float local = seg[u * rows * NS + i], d = total[u * rows + row];
-    run = fmaf(__builtin_amdgcn_exp2f(d * A2), run, local);
+    const float local = seg[u * rows * NS + i], x = total[u * rows + row] * A2;
+    const bool far = fabsf(x) >= 126.f;
+    const float y = far ? __builtin_amdgcn_fmed3f(x, -1000.f, 1000.f) : x, whole = far ? truncf(y) : 0.f;
+    run = fmaf(__builtin_amdgcn_exp2f(y - whole), ldexpf(run, (int)whole), local);
     seg[u * rows * NS + i] = run;
   }
 }
