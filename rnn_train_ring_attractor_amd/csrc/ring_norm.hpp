@@ -60,6 +60,12 @@ template <int K> __device__ __forceinline__ void add_up(float (&v)[K], int n, Ro
   }
 }
 
+// Of a gate by itself NaN stays NaN, which FINE's clamped argument loses (silu multiplies by it besides)
+template <bool FINE> __device__ __forceinline__ float gate_sigmoid(float x) {
+  const float s = sigmoid<FINE>(x);
+  return FINE && x != x ? x : s;
+}
+
 // v times act(gate)
 template <typename T, int V> __device__ __forceinline__ void gate_of(float (&v)[V], const Row<T, V>& g, int act) {
   if (act == kSilu) {
@@ -67,7 +73,7 @@ template <typename T, int V> __device__ __forceinline__ void gate_of(float (&v)[
     for (int e = 0; e < V; ++e) v[e] *= silu<sizeof(T) == 4>((float)g.v[e]);
   } else if (act == kSigmoid) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] *= sigmoid<sizeof(T) == 4>((float)g.v[e]);
+    for (int e = 0; e < V; ++e) v[e] *= gate_sigmoid<sizeof(T) == 4>((float)g.v[e]);
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] *= (float)g.v[e];
@@ -280,7 +286,7 @@ __global__ __launch_bounds__(MOST) void ring_norm_bwd_kernel(RingNormArgs p, Lie
       for (int i = 0; i < I; ++i) {
         if (p.act != kIdentity)
 #pragma unroll
-          for (int e = 0; e < V; ++e) sig[i][e] = sigmoid<FINE>((float)now[i].g.v[e]);
+          for (int e = 0; e < V; ++e) sig[i][e] = gate_sigmoid<FINE>((float)now[i].g.v[e]);
         if (p.act == kSigmoid)
 #pragma unroll
           for (int e = 0; e < V; ++e) act[i][e] = sig[i][e];

@@ -22,7 +22,7 @@ template <bool FINE> __device__ __forceinline__ float exp_of(float x) {
 // x log2(e), rounded once
 __device__ __forceinline__ float times_log2e(float x) { return fmaf(x, kLog2e, x * kLog2eLow); }
 
-// 1 / (1 + e^-x)
+// 1 / (1 + e^-x)  (FINE, of NaN: a number; its users multiply by x as well, or look at it themselves)
 template <bool FINE> __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.f + exp_of<FINE>(FINE ? __builtin_amdgcn_fmed3f(-x, -87.f, 87.f) : -x));
 }

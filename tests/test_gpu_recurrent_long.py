@@ -18,6 +18,37 @@ def _code(kind):
 
 
 # ------------------------------------------------------------------------------------------------
+# What is not finite
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_norm_of_gates_that_are_not_finite(kind, gpu_device):
+    """NaN in a gate is NaN in y and, where the activation has a slope that depends on it, in the gate's own gradient, and the rest of the row is what it is without; a
+    sigmoid of an infinite gate is one or zero, and its gradient zero."""
+    dtype, C = TYPES[kind], 24
+    for act in ("silu", "sigmoid", None):
+        for value in (math.nan, math.inf, -math.inf):
+            if act != "sigmoid" and not math.isnan(value):
+                continue
+            print(f"[case] gate {value} {act} {kind}", flush=True)
+            p = norm_problem(59, (3,), C, dtype, next=False)
+            clean = run_norm(p, dtype, gpu_device, group=8, activation=act)
+            p["gate"][1, 5] = value
+            got = run_norm(p, dtype, gpu_device, group=8, activation=act)
+            rest = torch.ones(3, C, dtype=torch.bool, device=gpu_device)
+            rest[1, 5] = False
+            for n in ("y", "dgate"):
+                assert torch.equal(got[n][rest], clean[n][rest]), (n, act, value)
+                if math.isnan(value) and (n == "y" or act is not None):
+                    assert torch.isnan(got[n][1, 5]), (n, act)
+            if math.isnan(value):
+                assert torch.isnan(got["dx"][1, :8]).all() and torch.equal(got["dx"][1, 8:], clean["dx"][1, 8:])
+            else:
+                p["gate"][1, 5] = 1e4 * math.copysign(1, value)
+                want = run_norm(p, dtype, gpu_device, group=8, activation=act)
+                assert all(torch.allclose(got[n], want[n], rtol=0, atol=1e-30) for n in ("y", "dgate", "dx"))
+
+
+# ------------------------------------------------------------------------------------------------
 # States over the borders of segments
 # ------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("kind", list(TYPES))
