@@ -338,8 +338,8 @@ RINGATTR_API int ringattr_dropout(const void* x, const void* residual, void* y, 
  * that is not said to be fp32; parameters are fp32.  A tensor [B,T,C] is given by its address and its strides (batch, token, in elements; channels
  * are neighbours), outputs are contiguous.  lengths as above: outputs and gradients behind a length are zero and nothing there is read.
  * Outputs, kept states and workspaces start at 16 bytes, everything else at its own type's size.  Sequences and channels up to 2^20 and 16000000
- * together, 2^22 groups together, up to 2^30 tokens.  Sums over tokens, sequences and channels are
- * fp32, in a fixed order. */
+ * together, 2^22 groups together, up to 2^30 tokens; single tokens (_step): up to 2^20, with states (a power of two) 2^31
+ * together.  Sums over tokens, sequences and channels are fp32, in a fixed order. */
 #define RINGATTR_ACT_NONE 0
 #define RINGATTR_ACT_SILU 1
 #define RINGATTR_ACT_SIGMOID 2

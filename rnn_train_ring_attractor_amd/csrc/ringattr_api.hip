@@ -1096,15 +1096,28 @@ static bool known_activation(const char* who, int act, int most) {
   return false;
 }
 
+static bool rows_positive(const char* who, int type, int B, int T, int C) {
+  if (!known_type(who, type)) return false;
+  if (B > 0 && T > 0 && C > 0) return true;
+  fail(RINGATTR_ERR_INVALID, "%s: batch_size, seq_len, channels must be positive (got %d, %d, %d)", who, B, T, C);
+  return false;
+}
+
 // Workgroups are counted in one launch dimension and rows within a tensor in 64 bits.
 static bool rows_shape(const char* who, int type, int B, int T, int C) {
-  if (!known_type(who, type)) return false;
-  if (B <= 0 || T <= 0 || C <= 0) {
-    fail(RINGATTR_ERR_INVALID, "%s: batch_size, seq_len, channels must be positive (got %d, %d, %d)", who, B, T, C);
-    return false;
-  }
+  if (!rows_positive(who, type, B, T, C)) return false;
   if (B > (1 << 20) || C > (1 << 20) || (double)B * C > 1.6e7 || T > (1 << 30)) {
     fail(RINGATTR_ERR_INVALID, "%s: batch_size and channels up to 2^20, their product up to 16000000, seq_len up to 2^30 (got %d, %d, %d)", who, B, C, T);
+    return false;
+  }
+  return true;
+}
+
+// Single tokens: a thread for each state at most (`each`: a channel's, a power of two), up to 255 more a sequence: a launch counts fewer than 2^32
+static bool token_shape(const char* who, int type, int B, int C, int each) {
+  if (!rows_positive(who, type, B, 1, C)) return false;
+  if (B > (1 << 20) || C > (1 << 20) || (double)B * C * each > 2147483648.0) {
+    fail(RINGATTR_ERR_INVALID, "%s: batch_size and channels up to 2^20, their product with states (a power of two) up to 2^31 (got %d, %d, %d)", who, B, C, each);
     return false;
   }
   return true;
@@ -1120,13 +1133,17 @@ static bool rows_apart(long long stride, int n) { return stride >= n && stride <
 
 static RingRows rows_of_channels(const void* p, const long long* strides) { return RingRows{p, (long)strides[0], (long)strides[1]}; }
 
-static bool conv_shape(const char* who, int act, int type, int B, int T, int C, int K) {
-  if (!known_activation(who, act, RINGATTR_ACT_SILU) || !rows_shape(who, type, B, T, C)) return false;
+static bool conv_taps(const char* who, int act, int K) {
+  if (!known_activation(who, act, RINGATTR_ACT_SILU)) return false;
   if (K < 1 || K > RINGATTR_CONV_MAX_TAPS) {
     fail(RINGATTR_ERR_INVALID, "%s: taps between 1 and %d (got %d)", who, RINGATTR_CONV_MAX_TAPS, K);
     return false;
   }
   return true;
+}
+
+static bool conv_shape(const char* who, int act, int type, int B, int T, int C, int K) {
+  return conv_taps(who, act, K) && rows_shape(who, type, B, T, C);
 }
 
 size_t ringattr_causal_conv_bwd_workspace_bytes(int type, int batch_size, int seq_len, int channels, int taps, int weights) {
@@ -1206,7 +1223,7 @@ int ringattr_causal_conv_bwd(const void* x, const void* grad_y, const long long*
 int ringattr_causal_conv_step(const void* x, long long stride, const void* weight, const void* bias, void* state, const void* active, void* y,
                               int activation, int type, int batch_size, int channels, int taps, void* stream) {
   const char* who = "ringattr_causal_conv_step";
-  if (!conv_shape(who, activation, type, batch_size, 1, channels, taps)) return RINGATTR_ERR_INVALID;
+  if (!conv_taps(who, activation, taps) || !token_shape(who, type, batch_size, channels, 1)) return RINGATTR_ERR_INVALID;
   if (!x || !weight || (!state && taps > 1) || !y) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
   RingConvStep p = {x, (long)stride, (const float*)weight, (const float*)bias, state, y, (const unsigned char*)active, batch_size, channels, taps,
                     activation};
@@ -1215,8 +1232,7 @@ int ringattr_causal_conv_step(const void* x, long long stride, const void* weigh
   return RINGATTR_OK;
 }
 
-static bool scan_shape(const char* who, int type, int B, int T, int C, int N, int G, RingScanShape& s) {
-  if (!rows_shape(who, type, B, T, C)) return false;
+static bool scan_states(const char* who, int C, int N, int G) {
   if (N < 1 || N > RINGATTR_SCAN_MAX_STATES) {
     fail(RINGATTR_ERR_INVALID, "%s: states between 1 and %d (got %d)", who, RINGATTR_SCAN_MAX_STATES, N);
     return false;
@@ -1225,6 +1241,11 @@ static bool scan_shape(const char* who, int type, int B, int T, int C, int N, in
     fail(RINGATTR_ERR_INVALID, "%s: channels (%d) must be a multiple of groups (%d)", who, C, G);
     return false;
   }
+  return true;
+}
+
+static bool scan_shape(const char* who, int type, int B, int T, int C, int N, int G, RingScanShape& s) {
+  if (!rows_shape(who, type, B, T, C) || !scan_states(who, C, N, G)) return false;
   // (a workgroup of 512 threads for each group of a sequence and each 16 of its channels or more: a launch counts fewer than 2^32 threads)
   if ((double)B * G > (double)(1 << 22)) {
     fail(RINGATTR_ERR_INVALID, "%s: batch_size times groups up to 2^22 (got %d, %d)", who, B, G);
@@ -1340,8 +1361,10 @@ int ringattr_selective_scan_step(const void* x, const void* delta, const void* z
                                  const void* A, const void* D, const void* delta_bias, void* state, const void* active, void* y, int softplus,
                                  int type, int batch_size, int channels, int states, int groups, void* stream) {
   const char* who = "ringattr_selective_scan_step";
-  RingScanShape s;
-  if (!scan_shape(who, type, batch_size, 1, channels, states, groups, s)) return RINGATTR_ERR_INVALID;
+  int each = 1;
+  while (each < states && each < RINGATTR_SCAN_MAX_STATES) each *= 2;
+  if (!token_shape(who, type, batch_size, channels, each) || !scan_states(who, channels, states, groups)) return RINGATTR_ERR_INVALID;
+  const RingScanShape s = {batch_size, 1, channels, states, groups, type};
   if (!x || !delta || !B || !C || !strides || !A || !state || !y) return fail(RINGATTR_ERR_INVALID, "%s: null tensor pointer", who);
   RingScanStep a = {};
   a.x = x;

@@ -241,3 +241,23 @@ def test_scan_across_powers_that_no_float_holds(what, A, kind, gpu_device):
             a, b = got[n][0].double().cpu(), many[n][0].double().cpu()
             assert ((a - b).abs() <= torch.finfo(got[n].dtype).eps * b.abs() + 2 * (3 * T + 13 * total + 100) * 2.0 ** -24 * size[n][0] + 1e-37 + 1e-30 * (dtype == torch.float16))[
                 torch.isfinite(b)].all() and (torch.isfinite(a) == torch.isfinite(b)).all(), n
+
+
+# ------------------------------------------------------------------------------------------------
+# Single tokens of large batches
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("B,C,N,G", [(8192, 2048, 16, 1), (8192, 1024, 2, 1024), (16384, 2048, 33, 2)])
+def test_tokens_of_more_channels_than_sequences_take(B, C, N, G, gpu_device):
+    """More than 16000000 channels of all sequences, up to a thread count of 2^31: the bits of calls of 2048 sequences each."""
+    from rnn_train_ring_attractor_amd import causal_conv_step, selective_scan_step
+    gen = torch.Generator(device=gpu_device).manual_seed(67)
+    r = lambda *s: torch.randn(*s, generator=gen, device=gpu_device)
+    print(f"[case] tokens {B} {C} {N} {G}", flush=True)
+    with torch.no_grad():
+        x, Bm, A, w, bias, D = r(B, C).bfloat16(), r(B, G, N).bfloat16(), -r(C, N).exp(), r(C, 4), r(C), r(C)
+        for state, step in ((r(B, 3, C).bfloat16(), lambda at, s: causal_conv_step(x[at], w, s, bias=bias, activation="silu")),
+                            (r(B, C, N), lambda at, s: selective_scan_step(x[at], x[at], A, Bm[at], Bm[at], s, D=D, z=x[at], delta_bias=bias, softplus=True))):
+            parts, rows = [], state.clone()
+            for at in range(0, B, 2048):
+                parts.append(step(slice(at, at + 2048), rows[at:at + 2048]))
+            assert torch.equal(step(slice(None), state), torch.cat(parts)) and torch.equal(state, rows)

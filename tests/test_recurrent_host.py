@@ -122,3 +122,18 @@ def test_c_abi_refusals():
         assert bwd(**bad) == 1 and "gradient of" in _lib.last_error()
     need = lib.ringattr_norm_gate_bwd_workspace_bytes(*shape[2:], 1)
     assert need > 0 and lib.ringattr_norm_gate_bwd_workspace_bytes(*shape[2:], 0) == 0 and bwd(gw=p) == 2 and bwd(gw=p, ws=p, n=need - 1) == 2
+
+
+def test_c_abi_refusals_of_single_tokens():
+    """Sequences times channels times states (a power of two) end at 2^31, what a launch counts; sequences and channels at 2^20 each."""
+    lib = _lib.load()
+    buf = (ctypes.c_char * 512)()
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    st = (ctypes.c_longlong * 16)(*[8] * 16)
+    conv = lambda B, C: lib.ringattr_causal_conv_step(p, 8, p, None, p, None, p, 1, 1, B, C, 4, None)
+    scan = lambda B, C, N, G: lib.ringattr_selective_scan_step(p, p, None, p, p, st, p, None, None, p, None, p, 1, 1, B, C, N, G, None)
+    for call in (lambda: conv(1 << 12, (1 << 19) + 8), lambda: conv((1 << 20) + 1, 8), lambda: conv(8, (1 << 20) + 8), lambda: scan(1 << 14, 1 << 12, 33, 1),
+                 lambda: scan(1 << 16, (1 << 11) + 1, 16, 1), lambda: scan((1 << 20) + 1, 8, 1, 1)):
+        assert call() == 1 and "2^20" in _lib.last_error()
+    assert conv(0, 8) == 1 and scan(1, 0, 1, 1) == 1 and "positive" in _lib.last_error()
+    assert scan(1 << 13, 1 << 11, 65, 1) == 1 and scan(1 << 13, 1 << 11, 16, 3) == 1 and "multiple" in _lib.last_error()
