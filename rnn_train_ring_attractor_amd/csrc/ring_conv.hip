@@ -353,7 +353,7 @@ static hipError_t launch_type(const RingConvArgs& p, int type, bool back, hipStr
   return launch_wide<_Float16>(p, back, st);
 }
 
-// (rows of four channels make fewer parts or as many)
+// (of rows read four channels at a time and one; either may be more)
 static int parts_of(int B, int T, int C, bool wide) {
   const int E = wide ? 4 : 1, tx = along(C, E), blocks = (C + tx * E - 1) / (tx * E);
   RingConvArgs p = {};

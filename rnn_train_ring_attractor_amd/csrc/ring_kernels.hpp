@@ -472,7 +472,7 @@ struct RingConvArgs {
   void *y, *end, *dx, *dstart;           // null: not wanted
   float *dw, *dbias;
   float* part;                           // [parts,C,K + 1]
-  int B, T, C, K, act, seg_tokens, nseg, parts;
+  int B, T, C, K, act, seg_tokens, nseg;
   bool wide, wide_out, wide_state;
 };
 struct RingConvStep {

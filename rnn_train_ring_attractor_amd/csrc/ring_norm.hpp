@@ -20,7 +20,7 @@ enum { kIdentity = 0, kSilu = 1, kSigmoid = 2 };
 
 // How a row lies on threads: groups of `lanes` threads (a power of two), `slots` groups side by side (a power of two), `rows` rows a workgroup.  MANY: a thread
 // holds one unit of V values of each of I groups, else I units of one group.
-struct Lie { int lanes, slots, rows, units, groups; };
+struct Lie { int lanes, slots, rows, groups; };
 
 // Sums of K values over `n` neighbouring threads, a power of two, the same in each.  Across waves through one of two rooms by turns: who writes into a room
 // for the next but one sum has passed the barrier of the next one, which nobody reaches before this one is read.
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(1024) void ring_norm_fwd_kernel(RingNormArgs p, Lie
   __shared__ float rooms[kRoom];
   Room room = {rooms, 0};
   const Spot<V, I, MANY> at(l);
-  const Lie whole = {at.threads, 1, l.rows, 0, 1};
+  const Lie whole = {at.threads, 1, l.rows, 1};
   const long row = ((long)blockIdx.y * gridDim.x + blockIdx.x) * l.rows + at.row;
   const bool real = row < p.rows;
   bool there[I];
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(MOST) void ring_norm_bwd_kernel(RingNormArgs p, Lie
   Room room = {rooms, 0};
   extern __shared__ float sums[];        // [threads][V]: rows of a workgroup are added up
   const Spot<V, I, MANY> at(l);
-  const Lie whole = {at.threads, 1, l.rows, 0, 1};
+  const Lie whole = {at.threads, 1, l.rows, 1};
   struct Unit { Row<T, V> x, g, r, t, n; };          // of the row: x, gate, residual, gradients of y and n
   struct Weights { Row<float, V> w, s, n; } kept[KEEP ? I : 1];
   Unit next[I];
@@ -438,7 +438,7 @@ inline Plan plan_of(int C, int group, int V) {
   const int groups = C / group, units = (group + V - 1) / V;
   a.many = groups > 1 && units <= 64;
   for (a.threads = 64; a.threads <= 1024; a.threads *= 2) {
-    a.lie = {0, 0, 1, units, groups};
+    a.lie = {0, 0, 1, groups};
     if (a.many) {
       a.lie.lanes = pow2(units);
       a.lie.slots = a.threads / a.lie.lanes;
