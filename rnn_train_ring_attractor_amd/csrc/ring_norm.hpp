@@ -432,7 +432,8 @@ struct Plan { Lie lie; int I, threads; bool many; };
 // whose groups fill little more than half of their threads.  Us of a training step's norms, bf16, 67 million values: rows of 8192 as 512 threads of two
 // units 506, as 1024 of one 877; rows of 2047, value by value, as 256 threads of eight 600, as 1024 of two 1279; of 8191 as 512 of sixteen 3588, as 1024 of
 // eight 4115 (both spill registers); fp32, half as many, rows of 2048 as 512 threads of one unit 323, as 256 of two 353, of 8192 as 512 of four 630, as
-// 1024 of two 949.
+// 1024 of two 949.  Backwards every row over 4096 spills: 28 registers (bf16) and 240 to 317 (fp32) of whole units on 512 threads, 378 to 651 on 1024, 636 to 957 value by value.  A
+// training step's norms by the row's width 2048, 4096, 5120, 6144, 8192: bf16 334, 333, 581, 540, 507; fp32 319, 334, 715, 659, 623.
 inline Plan plan_of(int C, int group, int V) {
   Plan a = {};
   const int groups = C / group, units = (group + V - 1) / V;

@@ -16,7 +16,8 @@ int saved_of(const RingScanShape& s) { return (s.T + RingScanArgs::kSave - 1) / 
 
 // Segments that the tokens are cut into: none where every compute unit has a workgroup without, otherwise so many that each has two (us, bf16, 16 states, 2048
 // channels: one sequence of 32768 tokens by workgroups 256 472, 384 557, 512 424, 768 433; with gradients four of 2048 tokens, none 540, four
-// segments 396; eight, none 549, two 661).
+// segments 396; eight, none 549, two 661).  Measured on 16-bit rows of whole 16 bytes, whose outputs have two workgroups a unit; gradients, and outputs
+// of most other rows (at ring_scan_kernel), have one, and so many workgroups are two rounds there, a few more three.  Just over 256 without segments leave most units idle in a second round.
 int segments(const RingScanShape& s) {
   const long groups = (long)tiles_of(s) * s.G * s.B;
   const int units = (s.T + kChunk - 1) / kChunk;

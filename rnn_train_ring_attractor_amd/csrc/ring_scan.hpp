@@ -104,7 +104,9 @@ template <typename T, int L, int NS> struct Shared {
 //
 // Bound by vector instructions: a power takes a pipe 8.5 cycles, as do exchanges of lanes; a multiplication or addition takes 4.5 of one wave, of which two waves' overlap.
 // A state of a token is a power and four of the others, and 2.4 instructions for its share of the rows'.  Their counters have the pipes busy to 97
-// percent at four cycles each; two workgroups a unit, where there are so many, are 4 percent faster than one.  Bf16, 16 states, gate: eight sequences of
+// percent at four cycles each; two workgroups a unit, where there are so many and they fit, are 4 percent faster than one.  They fit where outputs take up to 128
+// registers: 16-bit rows of whole 16 bytes (107 to 119), such fp32 rows of over 16 states (119 to 125; 178 to 185 otherwise), rows value by value of over 32 states (120; 135 to
+// 206 otherwise).  Bf16, 16 states, gate: eight sequences of
 // 2048 tokens of 2048 channels 142 us (270 MB: 51 at the rate of a copy; 3.8 T states/s), one of 32768 tokens in 16 segments 190 for what they add,
 // 7 between them and 270 for the outputs.
 template <typename T, int NL, int NB, int MODE, bool WIDE>
