@@ -261,3 +261,36 @@ def test_tokens_of_more_channels_than_sequences_take(B, C, N, G, gpu_device):
             for at in range(0, B, 2048):
                 parts.append(step(slice(at, at + 2048), rows[at:at + 2048]))
             assert torch.equal(step(slice(None), state), torch.cat(parts)) and torch.equal(state, rows)
+
+
+# ------------------------------------------------------------------------------------------------
+# Rows that lie on each other
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("name", ["conv", "scan", "norm"])
+def test_rows_that_overlap_and_one_tensor_twice(name, kind, gpu_device):
+    """Inputs and gradients that are one token's values for all tokens, or windows that move up by eight values a token, the same memory in several places: the results of their
+    copies.  (Rows' results to the bit, each place's gradient by itself, as autograd adds them in an order of its own; a parameter's sums in another order, up to the counts above.)"""
+    from rnn_train_ring_attractor_amd import causal_conv_func, norm_gate_func, selective_scan_func
+    gen = torch.Generator(device=gpu_device).manual_seed(71)
+    B, T, C, N = 2, 75, 64, 16
+    r = lambda *s: torch.randn(*s, generator=gen, device=gpu_device)
+    w, A, D, n = r(C, 4), -r(C, N).exp(), r(C), r(C)
+    whole = lambda x: x
+    ops = {"conv": (lambda x, w, D: causal_conv_func(x, w, D, activation="silu"), (whole,), (w, D)),
+           "scan": (lambda x, d, z, Bm, Cm, A, D: selective_scan_func(x, d, A, Bm, Cm, D=D, z=z, softplus=True),
+                    (whole, whole, whole, lambda x: x[..., None, :N], lambda x: x[..., None, N:2 * N]), (A, D)),
+           "norm": (lambda x, g, e, n, D: norm_gate_func(x, n, gate=g, residual=e, scale=D), (whole, whole, whole), (n, D))}
+    call, places, params = ops[name]
+    flat = r(B * (8 * T + C)).to(TYPES[kind])
+    for what, x in (("one token", flat[:B * C].view(B, 1, C).expand(B, T, C)), ("windows", flat.as_strided((B, T, C), (8 * T + C, 8, 1))), ("one value", flat[:1].view(1, 1, 1).expand(B, T, C))):
+        print(f"[case] overlap {name} {kind} {what}", flush=True)
+        results = []
+        for lie in (x, x.contiguous()):
+            leaves = [*(of(lie).detach().requires_grad_(True) for of in places), *(p.clone().requires_grad_(True) for p in params)]
+            y = call(*leaves)
+            results.append((y.detach(), *torch.autograd.grad(y, leaves, lie)))
+        rows = 1 + len(places)
+        assert all(torch.equal(a, b) for a, b in zip(results[0][:rows], results[1][:rows])), what
+        for a, b in zip(results[0][rows:], results[1][rows:]):
+            assert torch.allclose(a, b, rtol=0, atol=2 * (B * T + 256) * 2.0 ** -24 * float((a.abs().max() + b.abs().max()) * 64)), what
